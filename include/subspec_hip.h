@@ -58,6 +58,9 @@ extern "C" {
  * (configs/exp_offloading/subspec_sd_qwen_7b.yaml:16-19). */
 #define SUBSPEC_MAX_TREE_NODES 512
 
+/* Most sequences of one batched step over a page pool */
+#define SUBSPEC_MAX_BATCH 4096
+
 int subspec_abi_version(void);
 const char* subspec_last_error(void);
 
@@ -274,6 +277,103 @@ int subspec_tree_attention_paged(const void* q, const void* kv_pool_layer, const
 int subspec_kv_compact_paged(void* pool, int64_t n_layers, int64_t max_pages, int64_t page_len, int64_t token_bytes,
                              const int32_t* page_indices, int64_t n_pages, int64_t offset, const int64_t* ctx,
                              const int32_t* count_dev, int32_t count_host, int32_t max_count, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * One step of a BATCH of sequences over one page pool: every sequence brings some new tokens (one when it decodes, a chunk
+ * of its prompt, the tokens of a draft, or none).  The pool's layout is that of the paged cache above; sequence b's row p lives in
+ * page block_table[b][p / page_len] at token p % page_len, and that row's SLOT is page * page_len + p % page_len.  The new tokens
+ * of all sequences lie one after the other ("packed"): those of sequence b are rows query_starts[b] .. query_starts[b + 1] - 1.
+ * Lengths, tables and starts are read on the device, so nothing here waits for the host and a captured step can be replayed.
+ *
+ * subspec_paged_batch_plan takes the pages the new rows need and says where each token's row goes.
+ * Replaces  KvCacheBatchPosition / getKvCacheBatchPosition and the per-request page lists of RequestKvCache.increment
+ *           specdecodes/models/utils/flashinfer/cache_manager.py:9-25,218-240,350-372 (host lists, copied to the device each step).
+ *
+ * kv_lens       device int32 [batch]  rows each sequence has cached
+ * new_lens      device int32 [batch]  rows it brings (0: none)
+ * free_pages    device int32 [free_capacity]: pages 0 .. *n_free - 1 of it are free, the last of them is taken first; left as it is
+ * n_free        device int32
+ * block_table   device int32, row b at b * table_stride, max_blocks columns.  Entries of the pages taken are written, in the order of
+ *               the sequences; all others are left as they are
+ * n_tokens      rows the token outputs hold (a captured step: the most it will see); rows behind the last token get position 0,
+ *               slot -1, sequence -1
+ * query_starts  device int32 [batch + 1];  total_lens  device int32 [batch]: kv_lens + new_lens
+ * positions     device int32 [n_tokens];   slots  device int64 [n_tokens];   sequences  device int32 [n_tokens]
+ * counts        device int32 [4]  {tokens, pages taken, pages still free, status}.  The pages taken are those that leave the
+ *               stack: the caller's next *n_free is counts[2].  status != 0 is a sum of SUBSPEC_PLAN_*: then nothing is taken, the
+ *               table is left as it is, total_lens = kv_lens, all query_starts are 0 and every slot is -1
+ * No output may overlap an input (total_lens and kv_lens, say).  Limits: 1 <= batch <= SUBSPEC_MAX_BATCH, page_len a power of two.
+ */
+#define SUBSPEC_PLAN_NEGATIVE 1 /* a length below zero */
+#define SUBSPEC_PLAN_TABLE 2    /* a sequence needs more than max_blocks pages */
+#define SUBSPEC_PLAN_PAGES 4    /* too few free pages (or *n_free beyond free_capacity) */
+#define SUBSPEC_PLAN_TOKENS 8   /* more than n_tokens new tokens */
+
+int subspec_paged_batch_plan(const int32_t* kv_lens, const int32_t* new_lens, int64_t batch, const int32_t* free_pages,
+                             const int32_t* n_free, int64_t free_capacity, int32_t* block_table, int64_t max_blocks,
+                             int64_t table_stride, int64_t page_len, int64_t n_tokens, int32_t* query_starts, int32_t* total_lens,
+                             int32_t* positions, int64_t* slots, int32_t* sequences, int32_t* counts, void* stream);
+
+/* The new tokens' K and V rows into one layer of the pool, each at its slot.
+ * Replaces  flashinfer.append_paged_kv_cache   specdecodes/models/utils/flashinfer/attention_wrapper.py:244-253
+ *
+ * k, v    device [n_tokens, n_kv_heads, head_dim] with token and head strides in elements (a slice of a fused projection's output);
+ *         the elements of a head are consecutive
+ * slots   device int64 [n_tokens]; a row whose slot lies outside [0, max_pages * page_len) is not written.  Slots are distinct (those of a
+ *         plan are): of two rows with one slot either may be left there, or pieces of both
+ * dtype   any; the rows are copied as they are
+ */
+int subspec_kv_append_paged(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                            int64_t v_head_stride, void* kv_pool_layer, int dtype, int64_t max_pages, int64_t page_len,
+                            int64_t n_kv_heads, int64_t head_dim, const int64_t* slots, int64_t n_tokens, void* stream);
+
+/* Attention of the new tokens over their sequences' cached rows, their own among them (append first):
+ * out[t, h] = softmax(scale * q[t, h] . k[j, h / group]) v[j, h / group] over the rows j that the token sees.  Token i of the n new ones of
+ * a sequence of kv_lens[b] rows is at position p = kv_lens[b] - n + i and sees j <= p; with a window w > 0 only j > p - w, and
+ * the first `sinks` rows.  A token that sees no row (p < 0) gets zeros.
+ * Replaces  flashinfer.BatchPrefillWithPagedKVCacheWrapper / BatchDecodeWithPagedKVCacheWrapper with a causal mask (modes "prefill" and
+ *           "decode")   specdecodes/models/utils/flashinfer/attention_wrapper.py:71-137,288-316
+ *
+ * q            device [n_tokens, n_q_heads, head_dim], bf16 / fp16, head_dim 64 or 128, with token and head strides in elements
+ *              (multiples of 8; a slice of a fused projection's output)
+ * block_table, query_starts, kv_lens   device, as the plan leaves them (kv_lens: its total_lens)
+ * max_new      no sequence brings more new tokens;  max_kv: no kv_lens is larger.  They lay out the launches and the workspace and may be larger
+ *              than what a call meets; tokens and rows beyond them are left out
+ * out          device [n_tokens, n_q_heads, head_dim]; rows behind query_starts[batch] are left as they were
+ * workspace    subspec_paged_attention_workspace bytes of the same sizes, 16-byte aligned
+ * Page numbers are clamped to the pool, so a bad table reads wrong rows and never leaves it.  Rows that no token of the call sees (those behind
+ * kv_lens, those a window has passed, other sequences' pages) have no influence, whatever they hold.  Among the rows of one
+ * call, an infinite or NaN VALUE row may reach tokens that do not see it, if they share a tile with one that does.
+ */
+size_t subspec_paged_attention_workspace(int64_t batch, int64_t n_tokens, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
+                                         int64_t max_new, int64_t max_kv, int64_t window, int64_t sinks);
+
+int subspec_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* kv_pool_layer, int64_t max_pages,
+                            int64_t page_len, const int32_t* block_table, int64_t max_blocks, int64_t table_stride,
+                            const int32_t* query_starts, const int32_t* kv_lens, void* out, int dtype, int64_t batch, int64_t n_tokens,
+                            int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim, int64_t max_new, int64_t max_kv, int64_t window,
+                            int64_t sinks, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * One token per row of logits, drawn after temperature, top-k, top-p and min-p from one given number per row.
+ * Entries are ordered by logit, larger first, equal ones by index, and entry j has the mass exp((l_j - l_max) / T).  Every filter keeps a
+ * prefix of that order: top-k the first k; top-p the entries with less than p times the mass of those k before them;
+ * min-p those with at least min_p times the first entry's mass.  The first entry always stays.  The draw is the first entry
+ * whose mass added to that of all before it exceeds u times the mass of what stays.  Masses are summed exactly, to 2^-42 of the largest.
+ * Replaces  TemperatureLogitsWarper, TopKLogitsWarper, TopPLogitsWarper (sort, cumsum, scatter over the vocabulary), softmax and multinomial
+ *           specdecodes/models/generators/base.py:42-64,116-132
+ *
+ * logits    device [rows, vocab] at row_stride elements, fp32 / fp16 / bf16, vocab <= 2^20.  NaN and -inf are never drawn; +inf
+ *           entries share all the mass
+ * uniforms  device float [rows] in [0, 1)
+ * temperatures, top_ks, top_ps, min_ps   device [rows] (float, int32, float, float) or NULL: then the scalar beside it, for every row.
+ *           T <= 0 takes the first largest; k <= 0, p >= 1 and min_p <= 0 filter nothing
+ * tokens    device int64 [rows], -1 where nothing can be drawn (no logit above -inf)
+ * probs     device float [rows]: the token's share of the mass that stays (0 where nothing can be drawn)
+ */
+int subspec_sample_filtered(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride, const float* uniforms,
+                            const float* temperatures, float temperature, const int32_t* top_ks, int32_t top_k, const float* top_ps,
+                            float top_p, const float* min_ps, float min_p, int64_t* tokens, float* probs, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Draft probabilities: out = softmax(round(logits / temperature)) over the last axis, in the logits

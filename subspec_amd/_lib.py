@@ -18,6 +18,8 @@ VERIFY_EXACT, VERIFY_LOSSY = 0, 1
 GATE_ENTROPY, GATE_PROB = 0, 1
 ENTROPY_GUARD, ENTROPY_ALWAYS = 0, 1
 MAX_TREE_NODES = 512
+MAX_BATCH = 4096
+PLAN_NEGATIVE, PLAN_TABLE, PLAN_PAGES, PLAN_TOKENS = 1, 2, 4, 8
 TREE_VERIFY_STATIC_MAX_ROWS = 2048
 
 _lib = None
@@ -70,6 +72,13 @@ _SIGNATURES = {
     "subspec_tree_attention_paged": (C.c_int, [_p, _p, _p, _i64, _i64, _i64, _p, C.c_int, _i64, _i64, _i64, _i64, _i64, _i64, _p,
                                                C.c_float, _p, _sz, _p]),
     "subspec_kv_compact_paged": (C.c_int, [_p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i32, _i32, _p]),
+    "subspec_paged_batch_plan": (C.c_int, [_p, _p, _i64, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p]),
+    "subspec_kv_append_paged": (C.c_int, [_p, _i64, _i64, _p, _i64, _i64, _p, C.c_int, _i64, _i64, _i64, _i64, _p, _i64, _p]),
+    "subspec_paged_attention_workspace": (_sz, [_i64] * 9),
+    "subspec_paged_attention": (C.c_int, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, C.c_int, _i64, _i64, _i64, _i64,
+                                          _i64, _i64, _i64, _i64, _i64, C.c_float, _p, _sz, _p]),
+    "subspec_sample_filtered": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, _p, _p, C.c_float, _p, _i32, _p, C.c_float, _p, C.c_float,
+                                          _p, _p, _p]),
     "subspec_softmax_temperature_workspace": (_sz, [_i64, _i64]),
     "subspec_softmax_temperature": (C.c_int, [_p, _p, C.c_int, _i64, _i64, C.c_float, _p, _sz, _p]),
     "subspec_temperature_warp": (C.c_int, [_p, _p, C.c_int, _i64, C.c_float, _p]),

@@ -409,6 +409,179 @@ def kv_compact_paged_(pool: torch.Tensor, page_indices: torch.Tensor, contexts: 
     return pool
 
 
+# ---------------------------------------------------------------------------------------------- a batch over one page pool
+_PLAN_OUT = (("query_starts", torch.int32), ("kv_lens", torch.int32), ("positions", torch.int32), ("slots", torch.int64),
+             ("sequences", torch.int32), ("counts", torch.int32))
+
+
+def _int32_vector(t: torch.Tensor, n: Optional[int], what: str) -> None:
+    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.numel() != n):
+        raise ValueError(f"{what} must be a contiguous int32 vector" + ("" if n is None else f" of {n} elements"))
+
+
+def _table_shape(block_table: torch.Tensor, batch: int):
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch or block_table.shape[1] < 1 \
+            or block_table.stride(1) != 1 or (batch > 1 and block_table.stride(0) < block_table.shape[1]):
+        raise ValueError(f"block_table must be int32 [{batch}, max_blocks] with consecutive columns")
+    return block_table.shape[1], max(block_table.stride(0), block_table.shape[1])
+
+
+def paged_batch_plan(kv_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor, n_free: torch.Tensor,
+                     block_table: torch.Tensor, page_len: int, n_tokens: int,
+                     out: Optional[Dict[str, torch.Tensor]] = None) -> Dict[str, torch.Tensor]:
+    """Pages and slots of one step of a batch over a page pool, on the device (no synchronisation): sequence b has ``kv_lens[b]``
+    rows cached and brings ``new_lens[b]`` more (int32 [batch] each).  The pages these need are taken from the end of the free
+    ones, ``free_pages[:n_free]`` (int32, ``n_free`` int32 of one element), and entered in ``block_table`` (int32 [batch, max_blocks], in
+    place).  ``n_tokens``: rows of the token outputs, at least the new rows of all sequences.
+
+    Returns device tensors: ``query_starts`` int32 [batch + 1] (the packed new tokens of sequence b are rows
+    ``query_starts[b]`` to ``query_starts[b + 1] - 1``), ``kv_lens`` int32 [batch] with the new rows, ``positions`` int32, ``slots`` int64 (row
+    of the pool) and ``sequences`` int32 [n_tokens] of every new token (0, -1 and -1 behind the last), ``counts`` int32 [4]: tokens,
+    pages taken, pages still free (the next call's ``n_free``), status.  A status other than 0 is a sum of ``_lib.PLAN_NEGATIVE``
+    (a length below zero), ``PLAN_TABLE`` (``max_blocks`` is too small), ``PLAN_PAGES`` (too few free pages) and ``PLAN_TOKENS`` (``n_tokens`` is too
+    small); then nothing is taken, the table is as it was and all slots are -1.  ``out``: the dictionary an earlier call of the same
+    sizes returned, written again (a captured step).  Replaces the host lists of
+    specdecodes/models/utils/flashinfer/cache_manager.py:218-240,350-372."""
+    dev = _require_gpu(kv_lens, new_lens, free_pages, n_free, block_table)
+    _int32_vector(kv_lens, None, "kv_lens")
+    batch, n_tokens = kv_lens.numel(), int(n_tokens)
+    _int32_vector(new_lens, batch, "new_lens")
+    _int32_vector(free_pages, None, "free_pages")
+    if n_free.dtype is not torch.int32 or n_free.numel() != 1:
+        raise ValueError("n_free must be an int32 tensor of one element")
+    max_blocks, stride = _table_shape(block_table, batch)
+    if n_tokens < 0:
+        raise ValueError("n_tokens must not be negative")
+    sizes = (batch + 1, batch, n_tokens, n_tokens, n_tokens, 4)
+    if out is None:
+        out = {key: torch.empty(n, dtype=dtype, device=dev) for (key, dtype), n in zip(_PLAN_OUT, sizes)}
+    else:
+        for (key, dtype), n in zip(_PLAN_OUT, sizes):
+            t = out[key]
+            if t.dtype is not dtype or t.shape != (n,) or t.device != dev or not t.is_contiguous():
+                raise ValueError(f"out[{key!r}] must be a contiguous {dtype} tensor of shape ({n},) on {dev}")
+        if out["kv_lens"].data_ptr() == kv_lens.data_ptr():
+            raise ValueError("out['kv_lens'] must not be kv_lens itself: every workgroup reads the old lengths")
+    code = L.lib().subspec_paged_batch_plan(
+        kv_lens.data_ptr(), new_lens.data_ptr(), batch, free_pages.data_ptr(), n_free.data_ptr(), free_pages.numel(),
+        block_table.data_ptr(), max_blocks, stride, int(page_len), n_tokens, out["query_starts"].data_ptr(), out["kv_lens"].data_ptr(),
+        out["positions"].data_ptr(), out["slots"].data_ptr(), out["sequences"].data_ptr(), out["counts"].data_ptr(), _stream(dev))
+    L.check(code, "subspec_paged_batch_plan")
+    return out
+
+
+def _pool_layer_shape(pool_layer: torch.Tensor):
+    if pool_layer.dim() != 5 or pool_layer.shape[1] != 2 or not pool_layer.is_contiguous():
+        raise ValueError("expected a contiguous pool layer [max_pages, 2, page_len, kv_heads, head_dim]")
+    return pool_layer.shape[0], pool_layer.shape[2], pool_layer.shape[3], pool_layer.shape[4]
+
+
+def kv_append_paged_(pool_layer: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
+    """In place: row ``slots[t]`` (page * page_len + token in the page) of one layer [max_pages, 2, page_len, kv_heads, head_dim] of a page pool
+    takes ``k[t]`` and ``v[t]`` [tokens, kv_heads, head_dim] (views of a fused projection's output are read where they are); rows whose
+    slot is negative or outside the pool are left out.  The slots are distinct, as a plan's are.  What ``flashinfer.append_paged_kv_cache``
+    does in the reference (specdecodes/models/utils/flashinfer/attention_wrapper.py:244-253)."""
+    dev = _require_gpu(pool_layer, k, v, slots)
+    max_pages, page_len, heads, D = _pool_layer_shape(pool_layer)
+    n = slots.numel()
+    if slots.dtype is not torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
+        raise ValueError("kv_append_paged_: slots must be a contiguous int64 vector")
+    if k.shape != (n, heads, D) or v.shape != (n, heads, D):
+        raise ValueError(f"kv_append_paged_: k and v must be [{n}, {heads}, {D}]")
+    if k.dtype != pool_layer.dtype or v.dtype != pool_layer.dtype:
+        raise ValueError("kv_append_paged_: k, v and the pool must share a dtype")
+    k, v = (t if t.stride(2) == 1 or D == 1 else t.contiguous() for t in (k, v))
+    code = L.lib().subspec_kv_append_paged(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                                           pool_layer.data_ptr(), _dtype_code(pool_layer), max_pages, page_len, heads, D,
+                                           slots.data_ptr(), n, _stream(dev))
+    L.check(code, "subspec_kv_append_paged")
+    return pool_layer
+
+
+def paged_attention(q: torch.Tensor, pool_layer: torch.Tensor, block_table: torch.Tensor, query_starts: torch.Tensor,
+                    kv_lens: torch.Tensor, max_new: int, max_kv: int, *, window: Optional[int] = None, sinks: int = 0,
+                    scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                    workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of a batch's packed new tokens ``q`` [tokens, Hq, D] (D 64 or 128, bf16 / fp16; a view of a fused projection's output is
+    read where it is) over their sequences' rows in ``pool_layer`` [max_pages, 2, page_len, Hkv, D], whose K / V are already there
+    (``kv_append_paged_``).  ``block_table``, ``query_starts`` and ``kv_lens`` as ``paged_batch_plan`` leaves them.  ``max_new`` and ``max_kv`` bound the
+    new tokens and the rows of any one sequence: they lay out the launch, need not be tight, and rows beyond them are left out.
+
+    ``window``: a token sees its own row and the ``window - 1`` before it (None or 0: all), and the first ``sinks`` rows besides.  A token that sees
+    no row gets zeros.  Returns [tokens, Hq * D]; rows behind the last sequence's are left as they were in ``out``.
+    Replaces the prefill and decode wrappers of specdecodes/models/utils/flashinfer/attention_wrapper.py:71-137."""
+    dev = _require_gpu(q, pool_layer, block_table, query_starts, kv_lens)
+    max_pages, page_len, Hkv, D = _pool_layer_shape(pool_layer)
+    if q.dim() != 3 or q.shape[2] != D or q.dtype != pool_layer.dtype:
+        raise ValueError("paged_attention: expected q [tokens, Hq, D] with the pool's head_dim and dtype")
+    T, Hq, _ = q.shape
+    _int32_vector(kv_lens, None, "kv_lens")
+    batch = kv_lens.numel()
+    _int32_vector(query_starts, batch + 1, "query_starts")
+    max_blocks, stride = _table_shape(block_table, batch)
+    if Hq < 1 or Hkv < 1 or Hq % Hkv:
+        raise ValueError(f"paged_attention: {Hq} query heads over {Hkv} KV heads")
+    max_new, max_kv, window, sinks = int(max_new), int(max_kv), 0 if window is None else int(window), int(sinks)
+    if max_new < 0 or max_kv < 0 or window < 0 or sinks < 0 or (sinks and not window):
+        raise ValueError("paged_attention: max_new, max_kv, window and sinks must not be negative, and sinks need a window")
+    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+    if out is None:
+        out = torch.empty((T, Hq * D), dtype=q.dtype, device=dev)
+    elif out.dtype != q.dtype or out.shape != (T, Hq * D) or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f"paged_attention: out must be a contiguous {q.dtype} tensor [{T}, {Hq * D}]")
+    lib = L.lib()
+    need = lib.subspec_paged_attention_workspace(batch, T, Hq, Hkv, D, max_new, max_kv, window, sinks)
+    if workspace is None and need > 256:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    code = lib.subspec_paged_attention(
+        q.data_ptr(), q.stride(0), q.stride(1), pool_layer.data_ptr(), max_pages, page_len, block_table.data_ptr(), max_blocks, stride,
+        query_starts.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), _dtype_code(q), batch, T, Hq, Hkv, D, max_new, max_kv, window, sinks,
+        float(D ** -0.5 if scale is None else scale), None if workspace is None else workspace.data_ptr(),
+        0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(dev))
+    L.check(code, "subspec_paged_attention")
+    return out
+
+
+def _per_row(value, rows: int, dtype: torch.dtype, dev: torch.device, what: str):
+    """(pointer, scalar) of a setting given for all rows or for each."""
+    if isinstance(value, torch.Tensor):
+        if value.dtype is not dtype or value.shape != (rows,) or not value.is_contiguous() or value.device != dev:
+            raise ValueError(f"sample_filtered: {what} must be a number or a contiguous {dtype} tensor of {rows} elements on {dev}")
+        return value.data_ptr(), 0
+    return None, value
+
+
+def sample_filtered(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One token per row of ``logits`` [rows, V] after temperature, top-k, top-p and min-p (in this order), from the given ``uniforms`` float32
+    [rows] in [0, 1).  Each setting is a number or a device tensor with one value a row (float32; ``top_k`` int32): ``temperature`` 0
+    takes the first largest logit, ``top_k`` 0, ``top_p`` 1 and ``min_p`` 0 filter nothing.  The token is the first, in falling order of the
+    logits (equal ones by index), whose probability added to all before it exceeds the uniform number.  Returns ``(tokens int64 [rows], probs float32
+    [rows])``: ``probs`` is the token's probability among those that stay; a row without a logit above -inf gives -1 and 0.  What the
+    warpers, the softmax and ``torch.multinomial`` of specdecodes/models/generators/base.py:42-64,116-132 do, without sorting the row."""
+    if logits.dim() != 2:
+        raise ValueError("sample_filtered: expected logits [rows, vocab]")
+    dev = _require_gpu(logits, uniforms)
+    rows, V = logits.shape
+    if uniforms.dtype is not torch.float32 or uniforms.shape != (rows,) or not uniforms.is_contiguous():
+        raise ValueError(f"sample_filtered: uniforms must be a contiguous float32 tensor of {rows} elements")
+    if logits.stride(1) != 1 and V > 1 or (rows > 1 and logits.stride(0) < V):
+        logits = logits.contiguous()
+    t_ptr, t = _per_row(temperature, rows, torch.float32, dev, "temperature")
+    k_ptr, k = _per_row(top_k, rows, torch.int32, dev, "top_k")
+    p_ptr, p = _per_row(top_p, rows, torch.float32, dev, "top_p")
+    m_ptr, m = _per_row(min_p, rows, torch.float32, dev, "min_p")
+    if t < 0 or p < 0 or m < 0 or k < 0:
+        raise ValueError("sample_filtered: temperature, top_k, top_p and min_p must not be negative")
+    tokens = torch.empty(rows, dtype=torch.int64, device=dev)
+    probs = torch.empty(rows, dtype=torch.float32, device=dev)
+    code = L.lib().subspec_sample_filtered(
+        logits.data_ptr(), _dtype_code(logits), rows, V, max(logits.stride(0), V), uniforms.data_ptr(), t_ptr, float(t), k_ptr,
+        min(int(k), (1 << 31) - 1), p_ptr, float(p), m_ptr, float(m), tokens.data_ptr(), probs.data_ptr(), _stream(dev))
+    L.check(code, "subspec_sample_filtered")
+    return tokens, probs
+
+
 def int4_linear(x: torch.Tensor, wq: torch.Tensor, sz: torch.Tensor, out_features: int,
                 bias: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x`` [..., K] (bf16 / fp16; 64 rows per pass over the weights, more rows are more passes) times the tiled int4 weight

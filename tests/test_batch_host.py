@@ -1,0 +1,98 @@
+"""What the batched entry points refuse, from the library's host code alone, and the oracle of the batch on small cases done by hand."""
+import pytest
+import torch
+
+from oracle import batch as ob
+from subspec_amd import _lib as L
+
+ANY = 4096                                                   # a non-null, aligned address that no refused call touches
+
+
+def _plan(**change):
+    a = dict(batch=2, capacity=8, max_blocks=4, stride=4, page_len=16, n_tokens=8, kv=ANY, counts=ANY)
+    a.update(change)
+    return L.lib().subspec_paged_batch_plan(a["kv"], ANY, a["batch"], ANY, ANY, a["capacity"], ANY, a["max_blocks"], a["stride"], a["page_len"],
+                                            a["n_tokens"], ANY, ANY, ANY, ANY, ANY, a["counts"], None)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(kv=None), -1), (dict(counts=None), -1), (dict(batch=0), -4), (dict(batch=L.MAX_BATCH + 1), -4), (dict(page_len=12), -1),
+    (dict(page_len=0), -1), (dict(max_blocks=0), -1), (dict(stride=3), -1), (dict(n_tokens=-1), -1), (dict(capacity=-1), -1)])
+def test_plan_refuses(change, code):
+    assert _plan(**change) == code and b"paged_batch_plan" in L.lib().subspec_last_error()
+
+
+def _append(**change):
+    a = dict(k=ANY, dtype=L.BF16, pages=4, page_len=16, heads=2, D=64, n=3, stride=128, slots=ANY)
+    a.update(change)
+    return L.lib().subspec_kv_append_paged(a["k"], a["stride"], 64, ANY, 128, 64, ANY, a["dtype"], a["pages"], a["page_len"], a["heads"], a["D"],
+                                           a["slots"], a["n"], None)
+
+
+@pytest.mark.parametrize("change", [dict(k=None), dict(slots=None), dict(dtype=9), dict(pages=0), dict(page_len=24), dict(heads=0), dict(D=0),
+                                    dict(n=-1), dict(stride=-128), dict(k=ANY + 1)])
+def test_append_refuses(change):
+    assert _append(**change) == -1 and b"kv_append_paged" in L.lib().subspec_last_error()
+
+
+def test_nothing_to_append_launches_nothing():
+    assert _append(n=0, k=None, slots=None) == 0
+
+
+def _attention(**change):
+    a = dict(q=ANY, qs=512, pages=4, page_len=16, max_blocks=4, stride=4, dtype=L.BF16, batch=2, n=4, hq=4, hkv=2, D=128, new=2, kv=64,
+             window=0, sinks=0, scale=0.1, ws=None, ws_bytes=0, out=ANY)
+    a.update(change)
+    return L.lib().subspec_paged_attention(a["q"], a["qs"], 128, ANY, a["pages"], a["page_len"], ANY, a["max_blocks"], a["stride"], ANY, ANY, a["out"],
+                                           a["dtype"], a["batch"], a["n"], a["hq"], a["hkv"], a["D"], a["new"], a["kv"], a["window"], a["sinks"],
+                                           a["scale"], a["ws"], a["ws_bytes"], None)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(q=None), -1), (dict(out=None), -1), (dict(q=ANY + 2), -1), (dict(qs=513), -1), (dict(dtype=L.F32), -1), (dict(D=96), -4), (dict(batch=0), -4),
+    (dict(hq=5), -1), (dict(hkv=0), -1), (dict(page_len=3), -1), (dict(stride=2), -1), (dict(n=-1), -1), (dict(new=-1), -1), (dict(kv=-1), -1),
+    (dict(window=-1), -1), (dict(sinks=3), -1), (dict(scale=0.0), -1), (dict(scale=float("nan")), -1), (dict(pages=0), -1)])
+def test_attention_refuses(change, code):
+    assert _attention(**change) == code and b"paged_attention" in L.lib().subspec_last_error()
+
+
+def test_attention_over_nothing_launches_nothing():
+    assert _attention(n=0, q=None) == 0 and _attention(new=0) == 0 and _attention(kv=0) == 0
+
+
+def _sample(**change):
+    a = dict(logits=ANY, dtype=L.BF16, rows=2, vocab=100, stride=100, u=ANY)
+    a.update(change)
+    return L.lib().subspec_sample_filtered(a["logits"], a["dtype"], a["rows"], a["vocab"], a["stride"], a["u"], None, 1.0, None, 0, None, 1.0, None,
+                                           0.0, ANY, ANY, None)
+
+
+@pytest.mark.parametrize("change,code", [(dict(logits=None), -1), (dict(u=None), -1), (dict(dtype=5), -1), (dict(vocab=0), -4),
+                                         (dict(vocab=(1 << 20) + 1, stride=1 << 21), -4), (dict(rows=-1), -4), (dict(stride=99), -1),
+                                         (dict(logits=ANY + 1), -1)])
+def test_sample_refuses(change, code):
+    assert _sample(**change) == code and b"sample_filtered" in L.lib().subspec_last_error()
+
+
+def test_oracle_plan_by_hand():
+    got = ob.plan([3, 0, 4], [2, 0, 1], [9, 8, 7], [[5, -1], [-1, -1], [6, -1]], 4, 5)
+    assert got["table"] == [[5, 7], [-1, -1], [6, 8]] and got["counts"] == [3, 2, 1, 0]
+    assert got["slots"] == [5 * 4 + 3, 7 * 4, 8 * 4, -1, -1] and got["sequences"] == [0, 0, 2, -1, -1]
+    assert got["positions"] == [3, 4, 4, 0, 0] and got["query_starts"] == [0, 2, 2, 3] and got["kv_lens"] == [5, 0, 5]
+
+
+def test_oracle_sample_by_hand():
+    x = torch.log(torch.tensor([0.1, 0.4, 0.3, 0.2], dtype=torch.float64))
+    assert [ob.sample(x, u)[0] for u in (0.0, 0.39, 0.41, 0.71, 0.91)] == [1, 1, 2, 3, 0]
+    assert ob.sample(x, 0.99, top_k=2)[0] == 2 and ob.sample(x, 0.99, top_p=0.35)[0] == 1 and ob.sample(x, 0.99, min_p=0.6)[0] == 2
+    assert abs(ob.sample(x, 0.5, top_k=2)[1] - 0.4 / 0.7) < 1e-12 or abs(ob.sample(x, 0.5, top_k=2)[1] - 0.3 / 0.7) < 1e-12
+
+
+def test_oracle_attention_window_by_hand():
+    pool = torch.zeros(3, 2, 2, 1, 2, dtype=torch.float64)
+    table = [[2, 0, 1]]
+    for j in range(6):                                        # equal scores: the average of the values seen
+        pool[table[0][j // 2], 1, j % 2] = float(1 << j)
+    q = torch.zeros(2, 1, 2, dtype=torch.float64)
+    out, _, _ = ob.attention(q, pool, table, [0, 2], [6], window=2, sinks=1)
+    assert out[0, 0, 0].item() == pytest.approx((1 + 8 + 16) / 3) and out[1, 0, 0].item() == pytest.approx((1 + 16 + 32) / 3)
