@@ -1,9 +1,28 @@
-// Attention of the new tokens of a batch of sequences over a page pool.
+// Attention of the new tokens of a batch of sequences over a page pool, for gfx950.
+//
+// The new tokens are packed; sequence b's are query_starts[b] .. query_starts[b + 1] - 1, and the row r = (token i of them) * group + head of
+// a KV head's query heads is a row of that KV head's products, so that all query heads of a group share a key's way out of memory.
+// Every length is read on the device; the host knows bounds only (max_new, max_kv) and lays out launches and workspace by them.
 #include "common.h"
+#include "dma.h"
 #include <algorithm>
 
 namespace subspec {
 
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+
+// How one of the kernels cuts its sequences: `rows` packed rows a tile, the keys in chunks; partial results [unit][chunk][rows][D], fp32,
+// with (reference, sum) of each row.
+struct PagedCut {
+  int rows, chunk_keys, chunks;
+  float* part_o;
+  float* part_ml;
+};
 struct PagedParams {
   const uint16_t* q;
   const uint16_t* pool;
@@ -13,8 +32,9 @@ struct PagedParams {
   uint16_t* out;
   int64_t q_token, q_head;                 // strides, elements
   int64_t table_stride, page_elems;        // page_elems: a page's K (V follows it)
-  int batch, n_tokens, hq, hkv, group, max_new, max_kv, window, sinks, page_shift, max_pages, max_blocks;
+  int batch, n_tokens, hq, hkv, group, head_dim, max_new, max_kv, window, sinks, page_shift, max_pages, max_blocks;
   float scale_log2;
+  PagedCut few;                            // sequences of at most few.rows rows a KV head (0 rows: none)
 };
 
 // keys a row at position pos sees: j <= pos, and with a window w only j > pos - w or j < sinks
@@ -22,6 +42,230 @@ __device__ __forceinline__ bool paged_sees(const PagedParams& p, int pos, int j)
   return j <= pos && (p.window == 0 || j > pos - p.window || j < p.sinks);
 }
 
+struct PagedSequence { int b, first, n, len; };
+__device__ __forceinline__ PagedSequence paged_sequence(const PagedParams& p, int b) {
+  PagedSequence s;
+  s.b = b;
+  s.first = min(max(p.starts[b], 0), p.n_tokens);
+  s.n = min(min(p.starts[b + 1], p.n_tokens) - s.first, p.max_new);
+  s.len = min(p.lens[b], p.max_kv);        // (max_kv is within the table: the host saw to it)
+  return s;
+}
+
+// The keys that rows at positions pos0 .. len - 1 see between them: [0, sinks) and [low, high), as one range of `length` virtual keys in
+// blocks of `block`: the first `skip` of them are keys 0 .., the others keys `start` .. (start and skip are multiples of the block).
+struct PagedSpan { int skip, start, low, length; };
+__device__ __forceinline__ PagedSpan paged_span(const PagedParams& p, int pos0, int high, int block) {
+  PagedSpan s;
+  s.low = p.window ? max(0, pos0 - p.window + 1) : 0;
+  s.start = s.low & -block;
+  s.skip = min((int)(((int64_t)p.sinks + block - 1) & -block), s.start);
+  s.length = max(0, s.skip + high - s.start);
+  return s;
+}
+__device__ __forceinline__ int paged_real(const PagedSpan& s, int v) { return v < s.skip ? v : v - s.skip + s.start; }
+__device__ __forceinline__ int paged_chunks(const PagedSpan& s, int chunk_keys) { return max(1, (s.length + chunk_keys - 1) / chunk_keys); }
+// Byte offset of virtual key v's K row of KV head 0.  A key inside a block that no row sees (between the sinks and the window) stands for
+// one that some row does: what it holds must not reach a product, not even multiplied by zero.
+__device__ __forceinline__ int64_t paged_row_bytes(const PagedParams& p, const PagedSequence& sq, const PagedSpan& s, int v) {
+  const int real = paged_real(s, v), j = real >= p.sinks && real < s.low ? s.low : real;
+  const int page = min(max(p.table[sq.b * p.table_stride + (j >> p.page_shift)], 0), p.max_pages - 1);
+  const int64_t row = ((int64_t)p.hkv * p.head_dim) * (j & ((1 << p.page_shift) - 1));
+  return 2 * ((int64_t)page * 2 * p.page_elems + row);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- few rows
+// Sequences whose new tokens make at most 16 ROWT rows a KV head (one token of up to 64 query heads, a handful of tokens of a few): the
+// call is the K / V rows' way out of memory, and everything is arranged for that.  A unit is (sequence, KV head, chunk of the keys) and ONE
+// wavefront: it has no barrier to meet anyone at, so nine or more of them share a compute unit and each waits for its own rows only.
+// Rows travel from memory straight into the wavefront's ring of LDS stages, 16 keys each, which the transposing reads of V need anyway;
+// a stage is asked for again as soon as it has been read.  S^T = K Q^T by 16x16x32 products, whose accumulator (four keys of one query a
+// lane) is, packed, the operand of the 16x16x16 products O^T = V^T P^T.
+// A row's probabilities are relative to a reference that follows its largest score by at most 2^8 (see kSlack), so that a stage without a
+// new maximum needs no step across lanes.  Rows of a stage: the 16-byte pieces are swapped (XOR) so that 16 rows' reads of one piece, and the
+// transposing reads of 8 rows' two pieces, cover all banks.
+constexpr int kFewKeys = 16;
+constexpr int kSegment = 256;             // keys whose row offsets are in LDS at a time
+constexpr float kSlack = 8.0f;            // 2^8 above the reference is within the range of fp16, and costs no bits of a float's
+
+template <int DT>
+__device__ __forceinline__ v4f mfma16x16x32(dec_u4 a, dec_u4 b, v4f c) {
+  if constexpr (DT == SUBSPEC_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+template <int DT>
+__device__ __forceinline__ v4f mfma16x16x16(uint2 a, uint2 b, v4f c) {
+  if constexpr (DT == SUBSPEC_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(v4s, a), __builtin_bit_cast(v4s, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(v4h, a), __builtin_bit_cast(v4h, b), c, 0, 0, 0);
+}
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+typedef __attribute__((address_space(3))) dec_u4 lds_u4;
+__device__ __forceinline__ uint2 lds_tr16(uint32_t address) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(uintptr_t)address));
+}
+__device__ __forceinline__ dec_u4 lds_16(uint32_t address) { return *(const lds_u4*)(uintptr_t)address; }
+__device__ __forceinline__ void dma16_from(uint32_t lds_base, const void* src) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_base), "v"(src) : "memory", "m0");
+}
+
+// where the stored piece of a row is, in pieces: K is read a piece of 16 rows at a time, V two pieces of 8 rows
+template <int D> __device__ __forceinline__ int few_k_swap(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+template <int D> __device__ __forceinline__ int few_v_swap(int row) { return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3); }
+
+template <int DT, int D, int ROWT, int STAGES>
+__global__ __launch_bounds__(64) void paged_few_kernel(PagedParams p) {
+  constexpr int kRowBytes = D * 2, kPieces = kRowBytes / 16, kRowsPerCopy = 64 / kPieces, kCopies = kFewKeys / kRowsPerCopy;
+  constexpr int kHalf = kFewKeys * kRowBytes, kStage = 2 * kHalf;
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[STAGES * kStage];
+  __shared__ int64_t row_at[kSegment];
+  const uint32_t unit = blockIdx.x;
+  const int kvh = (int)(unit % (uint32_t)p.hkv);
+  const uint32_t bc = unit / (uint32_t)p.hkv;
+  const int chunk = (int)(bc % (uint32_t)p.few.chunks), b = (int)(bc / (uint32_t)p.few.chunks);
+  const PagedSequence sq = paged_sequence(p, b);
+  const int rows = sq.n * p.group;
+  if (sq.n <= 0 || rows > p.few.rows) return;
+  const PagedSpan sp = paged_span(p, sq.len - sq.n, sq.len, kFewKeys);
+  const int chunks = paged_chunks(sp, p.few.chunk_keys);
+  if (chunk >= chunks) return;
+  const int lane = threadIdx.x, lq = lane & 15, lg = lane >> 4;
+  const int pos0 = sq.len - sq.n;
+
+  dec_u4 q[ROWT][D / 32];
+  int pos[ROWT];
+  int64_t out_at[ROWT];                                     // row (token, head) of the output
+#pragma unroll
+  for (int nt = 0; nt < ROWT; ++nt) {
+    const int r = nt * 16 + lq, i = r / p.group;
+    const bool ok = r < rows;
+    const int token = sq.first + (ok ? i : 0), head = kvh * p.group + (ok ? r - i * p.group : 0);
+    pos[nt] = ok ? pos0 + i : -1;
+    out_at[nt] = (int64_t)token * p.hq + head;
+    const uint16_t* src = p.q + token * p.q_token + head * p.q_head + lg * 8;
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ++ks) q[nt][ks] = ok ? *(const dec_u4*)(src + ks * 32) : dec_u4{0, 0, 0, 0};
+  }
+
+  v4f o[ROWT][D / 16];
+  float ref[ROWT], l[ROWT];                                  // ref in units of exp2's argument
+#pragma unroll
+  for (int nt = 0; nt < ROWT; ++nt) {
+    ref[nt] = -INFINITY;
+    l[nt] = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < D / 16; ++mt) o[nt][mt] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+  const int v_begin = chunk * p.few.chunk_keys, v_end = min(v_begin + p.few.chunk_keys, sp.length);
+  const uint32_t ring0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)ring;
+  const char* kbase = (const char*)(p.pool + kvh * D);
+  const int64_t v_bytes = p.page_elems * 2;
+  const int crow = lane / kPieces, cpiece = lane % kPieces;
+  const uint32_t koff = ring0 + lq * kRowBytes;
+  const uint32_t voff = ring0 + kHalf + (4 * lg + (lq >> 2)) * kRowBytes + (lq & 1) * 8;
+  const int kswap = few_k_swap<D>(lq), vswap = few_v_swap<D>(4 * lg + (lq >> 2)), vpiece = (lq >> 1) & 1;
+
+  for (int v0 = v_begin; v0 < v_end; v0 += kSegment) {
+    const int v1 = min(v0 + kSegment, v_end), stages = (v1 - v0 + kFewKeys - 1) / kFewKeys;
+#pragma unroll
+    for (int u = 0; u < kSegment / 64; ++u) {
+      const int v = v0 + u * 64 + lane;                     // past the end: the last row again, which nobody sees there
+      if (u * 64 < v1 - v0) row_at[u * 64 + lane] = paged_row_bytes(p, sq, sp, min(v, v1 - 1));
+    }
+    __builtin_amdgcn_s_waitcnt(0);                           // rows' offsets and the queries; from here on only copies are counted
+    auto request = [&](int st) {
+      const uint32_t at = ring0 + (uint32_t)(st % STAGES) * kStage;
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c) {
+        const int row = c * kRowsPerCopy + crow;
+        const char* src = kbase + row_at[st * kFewKeys + row];
+        dma16_from(at + c * 1024, src + ((cpiece ^ few_k_swap<D>(row)) << 4));
+        dma16_from(at + kHalf + c * 1024, src + v_bytes + ((cpiece ^ few_v_swap<D>(row)) << 4));
+      }
+    };
+    for (int st = 0; st < min(STAGES, stages); ++st) request(st);
+    for (int st = 0; st < stages; ++st) {
+      if (st + STAGES <= stages) wait_vmcnt<(STAGES - 1) * 2 * kCopies>();
+      else wait_vmcnt<0>();
+      const uint32_t at = (uint32_t)(st % STAGES) * kStage;
+      const int kb = paged_real(sp, v0 + st * kFewKeys);
+      v4f s[ROWT];
+#pragma unroll
+      for (int nt = 0; nt < ROWT; ++nt) s[nt] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < D / 32; ++ks) {
+        const dec_u4 a = lds_16(koff + at + (((ks * 4 + lg) ^ kswap) << 4));
+#pragma unroll
+        for (int nt = 0; nt < ROWT; ++nt) s[nt] = mfma16x16x32<DT>(a, q[nt][ks], s[nt]);
+      }
+      uint2 vt[D / 16];
+#pragma unroll
+      for (int mt = 0; mt < D / 16; ++mt) vt[mt] = lds_tr16(voff + at + (((mt * 2 + vpiece) ^ vswap) << 4));
+      const bool plain = kb + kFewKeys - 1 <= pos0 && (p.window == 0 || kb > sq.len - 1 - p.window || kb + kFewKeys <= p.sinks);
+      uint2 pb[ROWT];
+#pragma unroll
+      for (int nt = 0; nt < ROWT; ++nt) {
+        float x[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[r] = s[nt][r] * p.scale_log2;
+          if (!plain && !paged_sees(p, pos[nt], kb + 4 * lg + r)) x[r] = -INFINITY;
+        }
+        const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        if (__any(top > ref[nt] + kSlack)) {                 // (also where the reference is still -inf)
+          float m = fmaxf(top, __shfl_xor(top, 16, kWave));
+          m = fmaxf(m, __shfl_xor(m, 32, kWave));
+          const float next = m > ref[nt] + kSlack ? m : ref[nt];
+          const float alpha = next == ref[nt] ? 1.f : __builtin_amdgcn_exp2f(ref[nt] - next);
+          ref[nt] = next;
+          l[nt] *= alpha;
+#pragma unroll
+          for (int mt = 0; mt < D / 16; ++mt) o[nt][mt] *= alpha;
+        }
+        const float base = ref[nt] == -INFINITY ? 0.f : ref[nt];
+        float e[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          e[r] = __builtin_amdgcn_exp2f(x[r] - base);
+          l[nt] += e[r];
+        }
+        pb[nt] = make_uint2(pack2<DT>(e[0], e[1]), pack2<DT>(e[2], e[3]));
+      }
+#pragma unroll
+      for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < ROWT; ++nt) o[nt][mt] = mfma16x16x16<DT>(vt[mt], pb[nt], o[nt][mt]);
+      if (st + STAGES < stages) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the stage has been read
+        request(st + STAGES);
+      }
+    }
+  }
+
+#pragma unroll
+  for (int nt = 0; nt < ROWT; ++nt) {
+    float sum = l[nt] + __shfl_xor(l[nt], 16, kWave);
+    sum += __shfl_xor(sum, 32, kWave);
+    const int r = nt * 16 + lq;
+    if (r >= rows) continue;
+    if (chunks == 1) {
+      const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+      uint16_t* dst = p.out + out_at[nt] * D + lg * 4;
+#pragma unroll
+      for (int mt = 0; mt < D / 16; ++mt)
+        *(uint2*)(dst + mt * 16) = make_uint2(pack2<DT>(o[nt][mt][0] * inv, o[nt][mt][1] * inv), pack2<DT>(o[nt][mt][2] * inv, o[nt][mt][3] * inv));
+    } else {
+      const int64_t slot = (((int64_t)b * p.hkv + kvh) * p.few.chunks + chunk) * p.few.rows + r;
+      float* dst = p.few.part_o + slot * D + lg * 4;
+#pragma unroll
+      for (int mt = 0; mt < D / 16; ++mt) *(v4f*)(dst + mt * 16) = o[nt][mt];
+      if (lg == 0) *(v2f*)(p.few.part_ml + slot * 2) = v2f{ref[nt], sum};
+    }
+  }
+}
 // One workgroup per (token, query head): 256 keys at a time, a thread per key for the scores, then a thread per head dimension.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void paged_attention_row_kernel(PagedParams p) {
@@ -32,8 +276,8 @@ __global__ __launch_bounds__(256) void paged_attention_row_kernel(PagedParams p)
   while (b < p.batch && p.starts[b + 1] <= t) ++b;
   if (b == p.batch || p.starts[b] > t) return;
   const int first = p.starts[b], n = min(p.starts[b + 1] - first, p.max_new);
-  if (t - first >= n) return;
-  const int len = min(min(p.lens[b], p.max_kv), (int)min((int64_t)p.max_blocks << p.page_shift, (int64_t)INT32_MAX));
+  if (t - first >= n || n * p.group <= p.few.rows) return;
+  const int len = min(p.lens[b], p.max_kv);
   const int pos = len - n + t - first;
   for (int d = tid; d < D; d += 256) qs[d] = Elem<DT>::load(p.q, t * p.q_token + h * p.q_head + d);
   const int kvh = h / p.group;
@@ -70,13 +314,100 @@ __global__ __launch_bounds__(256) void paged_attention_row_kernel(PagedParams p)
   if (part == 0) Elem<DT>::store(p.out, ((int64_t)t * p.hq + h) * D + d, l > 0.f ? o / l : 0.f);
 }
 
+// ---------------------------------------------------------------------------------------------------------------- merge
+// out = sum_c 2^(ref_c - max ref) O_c / sum_c 2^(ref_c - max ref) l_c.  A wavefront a row: 256 / D chunks side by side, 16 bytes a lane, the
+// references and sums of 64 chunks in one load.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
+  constexpr int kLanes = D / 4, kSide = kWave / kLanes;
+  const int64_t id = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+  if (id >= (int64_t)p.n_tokens * p.hq) return;
+  const int t = (int)(id / p.hq), h = (int)(id - (int64_t)t * p.hq);
+  int lo = 0, hi = p.batch;                                  // the sequence with starts[lo] <= t < starts[lo + 1]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.starts[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  const PagedSequence sq = paged_sequence(p, lo);
+  const int i = t - sq.first;
+  if (i < 0 || i >= sq.n) return;
+  const int r = i * p.group + h % p.group, kvh = h / p.group;
+  if (sq.n * p.group > p.few.rows) return;
+  const PagedSpan sp = paged_span(p, sq.len - sq.n, sq.len, kFewKeys);
+  const int chunks = paged_chunks(sp, p.few.chunk_keys);
+  if (chunks == 1) return;                                   // complete already
+  const int64_t slot = ((int64_t)sq.b * p.hkv + kvh) * p.few.chunks * p.few.rows + r;
+  const int rows = p.few.rows;
+  const float* po = p.few.part_o;
+  const float* ml = p.few.part_ml;
+  const int lane = threadIdx.x & (kWave - 1), d4 = (lane % kLanes) * 4, side = lane / kLanes;
+  float top = -INFINITY;
+  for (int c = lane; c < chunks; c += kWave) top = fmaxf(top, ml[(slot + (int64_t)c * rows) * 2]);
+  top = wave_max(top);
+  const float base = top == -INFINITY ? 0.f : top;
+  v4f num = {0.f, 0.f, 0.f, 0.f};
+  float den = 0.f;
+#pragma unroll 8
+  for (int c = side; c < chunks; c += kSide) {
+    const int64_t at = slot + (int64_t)c * rows;
+    const v2f m = *(const v2f*)(ml + at * 2);
+    const v4f o = *(const v4f*)(po + at * D + d4);
+    const float w = __builtin_amdgcn_exp2f(m[0] - base);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) num[e] = fmaf(w, o[e], num[e]);
+    den = fmaf(w, m[1], den);
+  }
+#pragma unroll
+  for (int s = kLanes; s < kWave; s <<= 1) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) num[e] += __shfl_xor(num[e], s, kWave);
+    den += __shfl_xor(den, s, kWave);
+  }
+  if (side) return;
+  const float inv = den > 0.f ? 1.f / den : 0.f;
+  *(uint2*)(p.out + id * D + d4) = make_uint2(pack2<DT>(num[0] * inv, num[1] * inv), pack2<DT>(num[2] * inv, num[3] * inv));
+}
+
+// How a call is cut, from the bounds alone.  Keys of a row: at most max_kv, or a window's, its sinks and the row's fellow tokens'.
+struct PagedPlan { int few_rows, few_keys, few_chunks; size_t few_o, few_ml, bytes; };
+static PagedPlan paged_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64_t hkv, int64_t head_dim, int64_t max_new, int64_t max_kv,
+                            int64_t window, int64_t sinks) {
+  PagedPlan pl{};
+  const int64_t group = hq / hkv, most = max_new * group;
+  auto span = [&](int64_t tokens, int64_t block) {
+    return window ? std::min(max_kv, window + tokens + (sinks + block - 1) / block * block + block) : max_kv;
+  };
+  // one token's rows, or all of a short call's: 16, 32 or 64
+  const int64_t few = most <= 64 ? most : group;
+  pl.few_rows = few <= 16 ? 16 : few <= 32 ? 32 : few <= 64 ? 64 : 0;
+  if (pl.few_rows) {
+    const int64_t keys = std::max<int64_t>(1, span(pl.few_rows / group, kFewKeys)), units = batch * hkv;
+    int64_t per = (units * keys / 4096 + kFewKeys - 1) / kFewKeys * kFewKeys;
+    per = std::min<int64_t>(std::max<int64_t>(per, 64), kSegment);
+    while (per < keys && units * ((keys + per - 1) / per) * pl.few_rows > (1 << 21)) per *= 2;         // a gigabyte of partial results at 128 a head
+    pl.few_keys = (int)per;
+    pl.few_chunks = (int)((keys + per - 1) / per);
+    const size_t slots = (size_t)units * pl.few_chunks * pl.few_rows;
+    if (pl.few_chunks > 1) {
+      pl.few_o = align_up(slots * head_dim * sizeof(float), 256);
+      pl.few_ml = align_up(slots * 2 * sizeof(float), 256);
+    }
+  }
+  pl.bytes = 256 + pl.few_o + pl.few_ml;
+  return pl;
+}
+
 }  // namespace subspec
 
 using namespace subspec;
 
 extern "C" size_t subspec_paged_attention_workspace(int64_t batch, int64_t n_tokens, int64_t n_q_heads, int64_t n_kv_heads,
                                                     int64_t head_dim, int64_t max_new, int64_t max_kv, int64_t window, int64_t sinks) {
-  return 256;
+  if (batch < 1 || batch > SUBSPEC_MAX_BATCH || n_kv_heads < 1 || n_q_heads < n_kv_heads || n_q_heads % n_kv_heads || n_q_heads > 1024 || max_kv < 0 ||
+      max_new < 0 || window < 0 || sinks < 0 || head_dim < 1 || head_dim > 1024)
+    return 256;
+  return paged_plan(batch, n_tokens, n_q_heads, n_kv_heads, head_dim, std::min(max_new, n_tokens), max_kv, window, sinks).bytes;
 }
 
 extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* kv_pool_layer,
@@ -111,25 +442,43 @@ extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, in
   if ((uintptr_t)q % 16 || (uintptr_t)kv_pool_layer % 16 || (uintptr_t)out % 16 || q_token_stride % 8 || q_head_stride % 8 ||
       q_token_stride < 0 || q_head_stride < 0)
     SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: q, the pool and out must be 16-byte aligned, q's strides multiples of 8 elements", what);
+  max_new = std::min(max_new, n_tokens);
+  const PagedPlan pl = paged_plan(batch, n_tokens, n_q_heads, n_kv_heads, head_dim, max_new, max_kv, window, sinks);
+  if (pl.bytes > 256 && (!workspace || workspace_bytes < pl.bytes))
+    SUBSPEC_FAIL(SUBSPEC_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the %zu required", what, workspace_bytes, pl.bytes);
+  if ((uintptr_t)workspace % 16) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
   PagedParams p;
   p.q = (const uint16_t*)q; p.pool = (const uint16_t*)kv_pool_layer; p.table = block_table; p.starts = query_starts; p.lens = kv_lens;
   p.out = (uint16_t*)out;
   p.q_token = q_token_stride; p.q_head = q_head_stride; p.table_stride = table_stride;
   p.page_elems = page_len * n_kv_heads * head_dim;
   p.batch = (int)batch; p.n_tokens = (int)n_tokens; p.hq = (int)n_q_heads; p.hkv = (int)n_kv_heads; p.group = (int)(n_q_heads / n_kv_heads);
-  p.max_new = (int)std::min<int64_t>(max_new, n_tokens); p.max_kv = (int)max_kv;
+  p.head_dim = (int)head_dim; p.max_new = (int)max_new; p.max_kv = (int)std::min(max_kv, max_blocks * page_len);
   p.window = (int)std::min<int64_t>(window, 1ll << 30); p.sinks = (int)std::min<int64_t>(sinks, 1ll << 30);
   p.page_shift = 0;
   while ((1ll << p.page_shift) < page_len) ++p.page_shift;
   p.max_pages = (int)max_pages; p.max_blocks = (int)max_blocks;
   p.scale_log2 = scale * kLog2e;
-  const dim3 grid((unsigned)n_tokens, (unsigned)n_q_heads);
+  p.few = PagedCut{pl.few_rows, pl.few_keys, pl.few_chunks, (float*)workspace, (float*)((char*)workspace + pl.few_o)};
   hipStream_t st = (hipStream_t)stream;
-#define SUBSPEC_PAGED(DT, D) hipLaunchKernelGGL((paged_attention_row_kernel<DT, D>), grid, dim3(256), 0, st, p)
-  DominantKernelTimer timer(st);
+  const bool others = max_new * p.group > pl.few_rows;      // sequences of more rows may be there
+  const int64_t few_units = batch * n_kv_heads * pl.few_chunks;
+#define SUBSPEC_PAGED_FEW(DT, D, ROWT) hipLaunchKernelGGL((paged_few_kernel<DT, D, ROWT, 2>), dim3((unsigned)few_units), dim3(64), 0, st, p)
+#define SUBSPEC_PAGED(DT, D)                                                                                                           \
+  do {                                                                                                                                 \
+    DominantKernelTimer timer(st);                                                                                                     \
+    if (pl.few_rows == 16) SUBSPEC_PAGED_FEW(DT, D, 1);                                                                                \
+    else if (pl.few_rows == 32) SUBSPEC_PAGED_FEW(DT, D, 2);                                                                           \
+    else if (pl.few_rows == 64) SUBSPEC_PAGED_FEW(DT, D, 4);                                                                           \
+    if (others)                                                                                                                        \
+      hipLaunchKernelGGL((paged_attention_row_kernel<DT, D>), dim3((unsigned)n_tokens, (unsigned)n_q_heads), dim3(256), 0, st, p);     \
+    if (pl.few_chunks > 1)                                                                                                             \
+      hipLaunchKernelGGL((paged_merge_kernel<DT, D>), dim3((unsigned)((n_tokens * n_q_heads + 3) / 4)), dim3(256), 0, st, p);          \
+  } while (0)
   if (dtype == SUBSPEC_BF16) { if (head_dim == 128) SUBSPEC_PAGED(SUBSPEC_BF16, 128); else SUBSPEC_PAGED(SUBSPEC_BF16, 64); }
   else { if (head_dim == 128) SUBSPEC_PAGED(SUBSPEC_F16, 128); else SUBSPEC_PAGED(SUBSPEC_F16, 64); }
 #undef SUBSPEC_PAGED
+#undef SUBSPEC_PAGED_FEW
   SUBSPEC_CHECK_HIP(hipGetLastError());
   return SUBSPEC_OK;
 }

@@ -153,4 +153,5 @@ def test_attention(dtype, Hq, Hkv, D, lens, page_len, window, sinks):
     got = got.double().cpu().view(want.shape)
     tol = _tolerance(want, weight, worst, dtype, max(kv), float(pool.nan_to_num(0.0).abs().max()), D)
     off = (got - want).abs()
-    assert torch.isfinite(got).all() and (off <= tol).all(), (off / tol).max().item()
+    assert torch.isfinite(got).all().item()
+    assert (off / tol).max().item() <= 1.0
