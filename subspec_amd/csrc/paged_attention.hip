@@ -3,76 +3,10 @@
 // The new tokens are packed; sequence b's are query_starts[b] .. query_starts[b + 1] - 1, and the row r = (token i of them) * group + head of
 // a KV head's query heads is a row of that KV head's products, so that all query heads of a group share a key's way out of memory.
 // Every length is read on the device; the host knows bounds only (max_new, max_kv) and lays out launches and workspace by them.
-#include "common.h"
-#include "dma.h"
+#include "paged.h"
 #include <algorithm>
 
 namespace subspec {
-
-typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef _Float16 v4h __attribute__((ext_vector_type(4)));
-typedef short v4s __attribute__((ext_vector_type(4)));
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef float v2f __attribute__((ext_vector_type(2)));
-
-// How one of the kernels cuts its sequences: `rows` packed rows a tile, the keys in chunks; partial results [unit][chunk][rows][D], fp32,
-// with (reference, sum) of each row.
-struct PagedCut {
-  int rows, chunk_keys, chunks;
-  float* part_o;
-  float* part_ml;
-};
-struct PagedParams {
-  const uint16_t* q;
-  const uint16_t* pool;
-  const int32_t* table;
-  const int32_t* starts;
-  const int32_t* lens;
-  uint16_t* out;
-  int64_t q_token, q_head;                 // strides, elements
-  int64_t table_stride, page_elems;        // page_elems: a page's K (V follows it)
-  int batch, n_tokens, hq, hkv, group, head_dim, max_new, max_kv, window, sinks, page_shift, max_pages, max_blocks;
-  float scale_log2;
-  PagedCut few;                            // sequences of at most few.rows rows a KV head (0 rows: none)
-};
-
-// keys a row at position pos sees: j <= pos, and with a window w only j > pos - w or j < sinks
-__device__ __forceinline__ bool paged_sees(const PagedParams& p, int pos, int j) {
-  return j <= pos && (p.window == 0 || j > pos - p.window || j < p.sinks);
-}
-
-struct PagedSequence { int b, first, n, len; };
-__device__ __forceinline__ PagedSequence paged_sequence(const PagedParams& p, int b) {
-  PagedSequence s;
-  s.b = b;
-  s.first = min(max(p.starts[b], 0), p.n_tokens);
-  s.n = min(min(p.starts[b + 1], p.n_tokens) - s.first, p.max_new);
-  s.len = min(p.lens[b], p.max_kv);        // (max_kv is within the table: the host saw to it)
-  return s;
-}
-
-// The keys that rows at positions pos0 .. len - 1 see between them: [0, sinks) and [low, high), as one range of `length` virtual keys in
-// blocks of `block`: the first `skip` of them are keys 0 .., the others keys `start` .. (start and skip are multiples of the block).
-struct PagedSpan { int skip, start, low, length; };
-__device__ __forceinline__ PagedSpan paged_span(const PagedParams& p, int pos0, int high, int block) {
-  PagedSpan s;
-  s.low = p.window ? max(0, pos0 - p.window + 1) : 0;
-  s.start = s.low & -block;
-  s.skip = min((int)(((int64_t)p.sinks + block - 1) & -block), s.start);
-  s.length = max(0, s.skip + high - s.start);
-  return s;
-}
-__device__ __forceinline__ int paged_real(const PagedSpan& s, int v) { return v < s.skip ? v : v - s.skip + s.start; }
-__device__ __forceinline__ int paged_chunks(const PagedSpan& s, int chunk_keys) { return max(1, (s.length + chunk_keys - 1) / chunk_keys); }
-// Byte offset of virtual key v's K row of KV head 0.  A key inside a block that no row sees (between the sinks and the window) stands for
-// one that some row does: what it holds must not reach a product, not even multiplied by zero.
-__device__ __forceinline__ int64_t paged_row_bytes(const PagedParams& p, const PagedSequence& sq, const PagedSpan& s, int v) {
-  const int real = paged_real(s, v), j = real >= p.sinks && real < s.low ? s.low : real;
-  const int page = min(max(p.table[sq.b * p.table_stride + (j >> p.page_shift)], 0), p.max_pages - 1);
-  const int64_t row = ((int64_t)p.hkv * p.head_dim) * (j & ((1 << p.page_shift) - 1));
-  return 2 * ((int64_t)page * 2 * p.page_elems + row);
-}
 
 // ---------------------------------------------------------------------------------------------------------------- few rows
 // Sequences whose new tokens make at most 16 ROWT rows a KV head (one token of up to 64 query heads, a handful of tokens of a few): the
@@ -86,31 +20,6 @@ __device__ __forceinline__ int64_t paged_row_bytes(const PagedParams& p, const P
 // transposing reads of 8 rows' two pieces, cover all banks.
 constexpr int kFewKeys = 16;
 constexpr int kSegment = 256;             // keys whose row offsets are in LDS at a time
-constexpr float kSlack = 8.0f;            // 2^8 above the reference is within the range of fp16, and costs no bits of a float's
-
-template <int DT>
-__device__ __forceinline__ v4f mfma16x16x32(dec_u4 a, dec_u4 b, v4f c) {
-  if constexpr (DT == SUBSPEC_BF16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
-}
-template <int DT>
-__device__ __forceinline__ v4f mfma16x16x16(uint2 a, uint2 b, v4f c) {
-  if constexpr (DT == SUBSPEC_BF16)
-    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(v4s, a), __builtin_bit_cast(v4s, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(v4h, a), __builtin_bit_cast(v4h, b), c, 0, 0, 0);
-}
-typedef __attribute__((address_space(3))) v4s lds_v4s;
-typedef __attribute__((address_space(3))) dec_u4 lds_u4;
-__device__ __forceinline__ uint2 lds_tr16(uint32_t address) {
-  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(uintptr_t)address));
-}
-__device__ __forceinline__ dec_u4 lds_16(uint32_t address) { return *(const lds_u4*)(uintptr_t)address; }
-__device__ __forceinline__ void dma16_from(uint32_t lds_base, const void* src) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_base), "v"(src) : "memory", "m0");
-}
 
 // where the stored piece of a row is, in pieces: K is read a piece of 16 rows at a time, V two pieces of 8 rows
 template <int D> __device__ __forceinline__ int few_k_swap(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
@@ -266,54 +175,6 @@ __global__ __launch_bounds__(64) void paged_few_kernel(PagedParams p) {
     }
   }
 }
-// One workgroup per (token, query head): 256 keys at a time, a thread per key for the scores, then a thread per head dimension.
-template <int DT, int D>
-__global__ __launch_bounds__(256) void paged_attention_row_kernel(PagedParams p) {
-  __shared__ float qs[D], prob[256], scratch[4], half[D];
-  __shared__ int64_t row_at[256];
-  const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-  int b = 0;
-  while (b < p.batch && p.starts[b + 1] <= t) ++b;
-  if (b == p.batch || p.starts[b] > t) return;
-  const int first = p.starts[b], n = min(p.starts[b + 1] - first, p.max_new);
-  if (t - first >= n || n * p.group <= p.few.rows) return;
-  const int len = min(p.lens[b], p.max_kv);
-  const int pos = len - n + t - first;
-  for (int d = tid; d < D; d += 256) qs[d] = Elem<DT>::load(p.q, t * p.q_token + h * p.q_head + d);
-  const int kvh = h / p.group;
-  float m = -INFINITY, l = 0.f, o = 0.f;
-  const int d = tid % D, part = tid / D;
-  for (int j0 = 0; j0 <= pos; j0 += 256) {
-    const int j = j0 + tid;
-    float s = -INFINITY;
-    __syncthreads();
-    if (paged_sees(p, pos, j)) {
-      const int page = min(max(p.table[b * p.table_stride + (j >> p.page_shift)], 0), p.max_pages - 1);
-      const int64_t at = (int64_t)page * 2 * p.page_elems + ((int64_t)(j & ((1 << p.page_shift) - 1)) * p.hkv + kvh) * D;
-      row_at[tid] = at;
-      s = 0.f;
-      for (int i = 0; i < D; ++i) s = fmaf(qs[i], Elem<DT>::load(p.pool, at + i), s);
-      s *= p.scale_log2;
-    }
-    const float mx = fmaxf(m, block_max<256>(s, scratch));
-    const float e = s == -INFINITY ? 0.f : exp2f(s - mx);
-    prob[tid] = e;
-    const float alpha = m == -INFINITY ? 0.f : exp2f(m - mx);
-    l = l * alpha + block_sum<256>(e, scratch);
-    o *= alpha;
-    m = mx;
-    for (int i = part; i < 256; i += 256 / D)
-      if (prob[i] > 0.f) o = fmaf(prob[i], Elem<DT>::load(p.pool, row_at[i] + p.page_elems + d), o);
-  }
-  for (int w = 1; w < 256 / D; ++w) {
-    __syncthreads();
-    if (part == w) half[d] = o;
-    __syncthreads();
-    if (part == 0) o += half[d];
-  }
-  if (part == 0) Elem<DT>::store(p.out, ((int64_t)t * p.hq + h) * D + d, l > 0.f ? o / l : 0.f);
-}
-
 // ---------------------------------------------------------------------------------------------------------------- merge
 // out = sum_c 2^(ref_c - max ref) O_c / sum_c 2^(ref_c - max ref) l_c.  A wavefront a row: 256 / D chunks side by side, 16 bytes a lane, the
 // references and sums of 64 chunks in one load.
@@ -370,16 +231,16 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
 }
 
 // How a call is cut, from the bounds alone.  Keys of a row: at most max_kv, or a window's, its sinks and the row's fellow tokens'.
-struct PagedPlan { int few_rows, few_keys, few_chunks; size_t few_o, few_ml, bytes; };
-static PagedPlan paged_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64_t hkv, int64_t head_dim, int64_t max_new, int64_t max_kv,
-                            int64_t window, int64_t sinks) {
+struct PagedPlan { int few_rows, few_keys, few_chunks, tile_keys, tile_chunks; int64_t tiles; size_t few_o, few_ml, tile_o, tile_ml, bytes; };
+static PagedPlan paged_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64_t hkv, int64_t head_dim, int64_t page_len, int64_t max_new,
+                            int64_t max_kv, int64_t window, int64_t sinks) {
   PagedPlan pl{};
   const int64_t group = hq / hkv, most = max_new * group;
   auto span = [&](int64_t tokens, int64_t block) {
     return window ? std::min(max_kv, window + tokens + (sinks + block - 1) / block * block + block) : max_kv;
   };
-  // one token's rows, or all of a short call's: 16, 32 or 64
-  const int64_t few = most <= 64 ? most : group;
+  // one token's rows, or all of a short call's: 16, 32 or 64; none where the only sequence may bring more
+  const int64_t few = most <= 64 ? most : batch > 1 ? group : 65;
   pl.few_rows = few <= 16 ? 16 : few <= 32 ? 32 : few <= 64 ? 64 : 0;
   if (pl.few_rows) {
     const int64_t keys = std::max<int64_t>(1, span(pl.few_rows / group, kFewKeys)), units = batch * hkv;
@@ -394,7 +255,32 @@ static PagedPlan paged_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64_t
       pl.few_ml = align_up(slots * 2 * sizeof(float), 256);
     }
   }
-  pl.bytes = 256 + pl.few_o + pl.few_ml;
+  if (most > pl.few_rows) {
+    pl.tiles = n_tokens * group / kTileRows + batch;
+    const int64_t keys = std::max<int64_t>(1, span(std::min(max_new, kTileRows / group + 2), kTileKeys)), blocks = (keys + kTileKeys - 1) / kTileKeys;
+    // Tiles that all tokens make if none is left part empty: a compute unit takes one workgroup at a time, whose start and end cost about
+    // three blocks, and a chunk's partial results about two more.
+    const int64_t units = (n_tokens * group + kTileRows - 1) / kTileRows * hkv;
+    int64_t chunks = 1, best = INT64_MAX;
+    for (int64_t c = 1; c <= std::min<int64_t>(blocks, 64); ++c) {
+      const int64_t per = (blocks + c - 1) / c, used = (blocks + per - 1) / per, cost = (units * used + 255) / 256 * (per + 3 + (used > 1 ? 2 : 0));
+      if (used == c && cost < best) {
+        best = cost;
+        chunks = c;
+      }
+    }
+    while (chunks > 1 && pl.tiles * hkv * chunks > (1 << 13)) --chunks;                  // a gigabyte of partial results at 128 a head
+    int64_t per = (blocks + chunks - 1) / chunks * kTileKeys;
+    per = std::min(per, (kTilePages - 64) * page_len);                                   // its page numbers are in LDS (two more than the keys')
+    pl.tile_keys = (int)per;
+    pl.tile_chunks = (int)((keys + per - 1) / per);
+    const size_t slots = (size_t)pl.tiles * hkv * pl.tile_chunks * kTileRows;
+    if (pl.tile_chunks > 1) {
+      pl.tile_o = align_up(slots * head_dim * sizeof(float), 256);
+      pl.tile_ml = align_up(slots * 2 * sizeof(float), 256);
+    }
+  }
+  pl.bytes = 256 + pl.few_o + pl.few_ml + pl.tile_o + pl.tile_ml;
   return pl;
 }
 
@@ -403,11 +289,12 @@ static PagedPlan paged_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64_t
 using namespace subspec;
 
 extern "C" size_t subspec_paged_attention_workspace(int64_t batch, int64_t n_tokens, int64_t n_q_heads, int64_t n_kv_heads,
-                                                    int64_t head_dim, int64_t max_new, int64_t max_kv, int64_t window, int64_t sinks) {
+                                                    int64_t head_dim, int64_t page_len, int64_t max_new, int64_t max_kv,
+                                                    int64_t window, int64_t sinks) {
   if (batch < 1 || batch > SUBSPEC_MAX_BATCH || n_kv_heads < 1 || n_q_heads < n_kv_heads || n_q_heads % n_kv_heads || n_q_heads > 1024 || max_kv < 0 ||
-      max_new < 0 || window < 0 || sinks < 0 || head_dim < 1 || head_dim > 1024)
+      n_tokens < 1 || page_len < 1 || page_len > (1 << 20) || max_new < 0 || window < 0 || sinks < 0 || head_dim < 1 || head_dim > 1024)
     return 256;
-  return paged_plan(batch, n_tokens, n_q_heads, n_kv_heads, head_dim, std::min(max_new, n_tokens), max_kv, window, sinks).bytes;
+  return paged_plan(batch, n_tokens, n_q_heads, n_kv_heads, head_dim, page_len, std::min(max_new, n_tokens), max_kv, window, sinks).bytes;
 }
 
 extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* kv_pool_layer,
@@ -443,7 +330,7 @@ extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, in
       q_token_stride < 0 || q_head_stride < 0)
     SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: q, the pool and out must be 16-byte aligned, q's strides multiples of 8 elements", what);
   max_new = std::min(max_new, n_tokens);
-  const PagedPlan pl = paged_plan(batch, n_tokens, n_q_heads, n_kv_heads, head_dim, max_new, max_kv, window, sinks);
+  const PagedPlan pl = paged_plan(batch, n_tokens, n_q_heads, n_kv_heads, head_dim, page_len, max_new, max_kv, window, sinks);
   if (pl.bytes > 256 && (!workspace || workspace_bytes < pl.bytes))
     SUBSPEC_FAIL(SUBSPEC_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the %zu required", what, workspace_bytes, pl.bytes);
   if ((uintptr_t)workspace % 16) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
@@ -459,10 +346,16 @@ extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, in
   while ((1ll << p.page_shift) < page_len) ++p.page_shift;
   p.max_pages = (int)max_pages; p.max_blocks = (int)max_blocks;
   p.scale_log2 = scale * kLog2e;
-  p.few = PagedCut{pl.few_rows, pl.few_keys, pl.few_chunks, (float*)workspace, (float*)((char*)workspace + pl.few_o)};
+  char* ws = (char*)workspace;
+  p.few = PagedCut{pl.few_rows, pl.few_keys, pl.few_chunks, (float*)ws, (float*)(ws + pl.few_o)};
+  ws += pl.few_o + pl.few_ml;
+  p.tile = PagedCut{kTileRows, pl.tile_keys, pl.tile_chunks, (float*)ws, (float*)(ws + pl.tile_o)};
+  p.tiles = (int)pl.tiles;
   hipStream_t st = (hipStream_t)stream;
-  const bool others = max_new * p.group > pl.few_rows;      // sequences of more rows may be there
-  const int64_t few_units = batch * n_kv_heads * pl.few_chunks;
+  const int64_t few_units = batch * n_kv_heads * pl.few_chunks, tile_units = pl.tiles * n_kv_heads * pl.tile_chunks;
+  if (few_units > INT32_MAX || tile_units > INT32_MAX || n_tokens * n_q_heads > (1ll << 32))
+    SUBSPEC_FAIL(SUBSPEC_ERR_LIMIT, "%s: too large (%lld tokens of %lld heads, %lld sequences)", what, (long long)n_tokens, (long long)n_q_heads,
+                 (long long)batch);
 #define SUBSPEC_PAGED_FEW(DT, D, ROWT) hipLaunchKernelGGL((paged_few_kernel<DT, D, ROWT, 2>), dim3((unsigned)few_units), dim3(64), 0, st, p)
 #define SUBSPEC_PAGED(DT, D)                                                                                                           \
   do {                                                                                                                                 \
@@ -470,13 +363,22 @@ extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, in
     if (pl.few_rows == 16) SUBSPEC_PAGED_FEW(DT, D, 1);                                                                                \
     else if (pl.few_rows == 32) SUBSPEC_PAGED_FEW(DT, D, 2);                                                                           \
     else if (pl.few_rows == 64) SUBSPEC_PAGED_FEW(DT, D, 4);                                                                           \
-    if (others)                                                                                                                        \
-      hipLaunchKernelGGL((paged_attention_row_kernel<DT, D>), dim3((unsigned)n_tokens, (unsigned)n_q_heads), dim3(256), 0, st, p);     \
     if (pl.few_chunks > 1)                                                                                                             \
       hipLaunchKernelGGL((paged_merge_kernel<DT, D>), dim3((unsigned)((n_tokens * n_q_heads + 3) / 4)), dim3(256), 0, st, p);          \
   } while (0)
-  if (dtype == SUBSPEC_BF16) { if (head_dim == 128) SUBSPEC_PAGED(SUBSPEC_BF16, 128); else SUBSPEC_PAGED(SUBSPEC_BF16, 64); }
-  else { if (head_dim == 128) SUBSPEC_PAGED(SUBSPEC_F16, 128); else SUBSPEC_PAGED(SUBSPEC_F16, 64); }
+  if (pl.tiles) {
+    if (!pl.few_rows) {
+      DominantKernelTimer timer(st);
+      launch_paged_tile(p, dtype, st);
+    } else {
+      launch_paged_tile(p, dtype, st);
+    }
+    if (pl.tile_chunks > 1) launch_paged_tile_merge(p, dtype, st);
+  }
+  if (pl.few_rows) {
+    if (dtype == SUBSPEC_BF16) { if (head_dim == 128) SUBSPEC_PAGED(SUBSPEC_BF16, 128); else SUBSPEC_PAGED(SUBSPEC_BF16, 64); }
+    else { if (head_dim == 128) SUBSPEC_PAGED(SUBSPEC_F16, 128); else SUBSPEC_PAGED(SUBSPEC_F16, 64); }
+  }
 #undef SUBSPEC_PAGED
 #undef SUBSPEC_PAGED_FEW
   SUBSPEC_CHECK_HIP(hipGetLastError());

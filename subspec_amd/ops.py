@@ -531,7 +531,7 @@ def paged_attention(q: torch.Tensor, pool_layer: torch.Tensor, block_table: torc
     elif out.dtype != q.dtype or out.shape != (T, Hq * D) or not out.is_contiguous() or out.device != dev:
         raise ValueError(f"paged_attention: out must be a contiguous {q.dtype} tensor [{T}, {Hq * D}]")
     lib = L.lib()
-    need = lib.subspec_paged_attention_workspace(batch, T, Hq, Hkv, D, max_new, max_kv, window, sinks)
+    need = lib.subspec_paged_attention_workspace(batch, T, Hq, Hkv, D, page_len, max_new, max_kv, window, sinks)
     if workspace is None and need > 256:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     code = lib.subspec_paged_attention(
