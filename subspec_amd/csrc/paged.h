@@ -7,7 +7,6 @@ namespace subspec {
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
@@ -81,19 +80,15 @@ __device__ __forceinline__ v4f mfma16x16x32(dec_u4 a, dec_u4 b, v4f c) {
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
-template <int DT>
-__device__ __forceinline__ v4f mfma16x16x16(uint2 a, uint2 b, v4f c) {
-  if constexpr (DT == SUBSPEC_BF16)
-    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(v4s, a), __builtin_bit_cast(v4s, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(v4h, a), __builtin_bit_cast(v4h, b), c, 0, 0, 0);
-}
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 typedef __attribute__((address_space(3))) dec_u4 lds_u4;
 __device__ __forceinline__ uint2 lds_tr16(uint32_t address) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(uintptr_t)address));
 }
 __device__ __forceinline__ dec_u4 lds_16(uint32_t address) { return *(const lds_u4*)(uintptr_t)address; }
+__device__ __forceinline__ void dma16_nt(uint32_t lds_base, const void* src) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds_base), "v"(src) : "memory", "m0");
+}
 __device__ __forceinline__ void dma16_from(uint32_t lds_base, const void* src) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_base), "v"(src) : "memory", "m0");
 }

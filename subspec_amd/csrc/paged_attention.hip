@@ -5,31 +5,35 @@
 // Every length is read on the device; the host knows bounds only (max_new, max_kv) and lays out launches and workspace by them.
 #include "paged.h"
 #include <algorithm>
+#include <cmath>
 
 namespace subspec {
 
 // ---------------------------------------------------------------------------------------------------------------- few rows
 // Sequences whose new tokens make at most 16 ROWT rows a KV head (one token of up to 64 query heads, a handful of tokens of a few): the
 // call is the K / V rows' way out of memory, and everything is arranged for that.  A unit is (sequence, KV head, chunk of the keys) and ONE
-// wavefront: it has no barrier to meet anyone at, so nine or more of them share a compute unit and each waits for its own rows only.
-// Rows travel from memory straight into the wavefront's ring of LDS stages, 16 keys each, which the transposing reads of V need anyway;
-// a stage is asked for again as soon as it has been read.  S^T = K Q^T by 16x16x32 products, whose accumulator (four keys of one query a
-// lane) is, packed, the operand of the 16x16x16 products O^T = V^T P^T.
+// wavefront: it has no barrier to meet anyone at, so four of them share a compute unit and each waits for its own rows only.  Rows
+// travel from memory straight into the wavefront's ring of LDS stages, 32 keys each, which the transposing reads of V need anyway; a stage is
+// asked for again as soon as it has been read.  The rows are read once and copied as streaming data: 64 tokens of up to 4096 rows, 28 : 4
+// heads, 348 MB: 70.8 us against 79.6, 16 of up to 32768 rows, 32 : 8, 1.3 GB: 243 against 262 (5.5 TB/s; a large copy reaches 5.2 here).
+// S^T = K Q^T and O^T = V^T P^T by 16x16x32 products: the two accumulators of a stage (eight keys of one query a lane) are, packed, the
+// operand of the second, with its keys taken in the same order from V.
 // A row's probabilities are relative to a reference that follows its largest score by at most 2^8 (see kSlack), so that a stage without a
 // new maximum needs no step across lanes.  Rows of a stage: the 16-byte pieces are swapped (XOR) so that 16 rows' reads of one piece, and the
 // transposing reads of 8 rows' two pieces, cover all banks.
-constexpr int kFewKeys = 16;
-constexpr int kSegment = 256;             // keys whose row offsets are in LDS at a time
+constexpr int kFewKeys = 32;
+constexpr int kFewStages = 2;
+constexpr int kSegment = 512;             // keys whose row offsets are in LDS at a time
 
 // where the stored piece of a row is, in pieces: K is read a piece of 16 rows at a time, V two pieces of 8 rows
 template <int D> __device__ __forceinline__ int few_k_swap(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
 template <int D> __device__ __forceinline__ int few_v_swap(int row) { return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3); }
 
-template <int DT, int D, int ROWT, int STAGES>
+template <int DT, int D, int ROWT>
 __global__ __launch_bounds__(64) void paged_few_kernel(PagedParams p) {
   constexpr int kRowBytes = D * 2, kPieces = kRowBytes / 16, kRowsPerCopy = 64 / kPieces, kCopies = kFewKeys / kRowsPerCopy;
   constexpr int kHalf = kFewKeys * kRowBytes, kStage = 2 * kHalf;
-  __shared__ __attribute__((aligned(1024))) uint8_t ring[STAGES * kStage];
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[kFewStages * kStage];
   __shared__ int64_t row_at[kSegment];
   const uint32_t unit = blockIdx.x;
   const int kvh = (int)(unit % (uint32_t)p.hkv);
@@ -85,45 +89,62 @@ __global__ __launch_bounds__(64) void paged_few_kernel(PagedParams p) {
       if (u * 64 < v1 - v0) row_at[u * 64 + lane] = paged_row_bytes(p, sq, sp, min(v, v1 - 1));
     }
     __builtin_amdgcn_s_waitcnt(0);                           // rows' offsets and the queries; from here on only copies are counted
+    int64_t from[kCopies];                                   // of the copies to be asked for next: read together, well before their use
+    auto look_up = [&](int st) {
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c) from[c] = row_at[st * kFewKeys + c * kRowsPerCopy + crow];
+    };
     auto request = [&](int st) {
-      const uint32_t at = ring0 + (uint32_t)(st % STAGES) * kStage;
+      const uint32_t at = ring0 + (uint32_t)(st % kFewStages) * kStage;
 #pragma unroll
       for (int c = 0; c < kCopies; ++c) {
         const int row = c * kRowsPerCopy + crow;
-        const char* src = kbase + row_at[st * kFewKeys + row];
-        dma16_from(at + c * 1024, src + ((cpiece ^ few_k_swap<D>(row)) << 4));
-        dma16_from(at + kHalf + c * 1024, src + v_bytes + ((cpiece ^ few_v_swap<D>(row)) << 4));
+        const char* src = kbase + from[c];
+        dma16_nt(at + c * 1024, src + ((cpiece ^ few_k_swap<D>(row)) << 4));
+        dma16_nt(at + kHalf + c * 1024, src + v_bytes + ((cpiece ^ few_v_swap<D>(row)) << 4));
       }
     };
-    for (int st = 0; st < min(STAGES, stages); ++st) request(st);
+    for (int st = 0; st < min(kFewStages, stages); ++st) {
+      look_up(st);
+      request(st);
+    }
     for (int st = 0; st < stages; ++st) {
-      if (st + STAGES <= stages) wait_vmcnt<(STAGES - 1) * 2 * kCopies>();
+      if (st + kFewStages <= stages) wait_vmcnt<(kFewStages - 1) * 2 * kCopies>();
       else wait_vmcnt<0>();
-      const uint32_t at = (uint32_t)(st % STAGES) * kStage;
+      look_up(min(st + kFewStages, stages - 1));
+      const uint32_t at = (uint32_t)(st % kFewStages) * kStage;
       const int kb = paged_real(sp, v0 + st * kFewKeys);
-      v4f s[ROWT];
+      v4f s[ROWT][2];
 #pragma unroll
-      for (int nt = 0; nt < ROWT; ++nt) s[nt] = v4f{0.f, 0.f, 0.f, 0.f};
+      for (int nt = 0; nt < ROWT; ++nt) s[nt][0] = s[nt][1] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int ks = 0; ks < D / 32; ++ks) {
-        const dec_u4 a = lds_16(koff + at + (((ks * 4 + lg) ^ kswap) << 4));
+      for (int ks = 0; ks < D / 32; ++ks)
 #pragma unroll
-        for (int nt = 0; nt < ROWT; ++nt) s[nt] = mfma16x16x32<DT>(a, q[nt][ks], s[nt]);
+        for (int t = 0; t < 2; ++t) {
+          const dec_u4 a = lds_16(koff + at + t * 16 * kRowBytes + (((ks * 4 + lg) ^ kswap) << 4));
+#pragma unroll
+          for (int nt = 0; nt < ROWT; ++nt) s[nt][t] = mfma16x16x32<DT>(a, q[nt][ks], s[nt][t]);
+        }
+      dec_u4 vt[D / 16];
+#pragma unroll
+      for (int mt = 0; mt < D / 16; ++mt) {
+        const uint32_t va = voff + at + (((mt * 2 + vpiece) ^ vswap) << 4);
+        const uint2 lo = lds_tr16(va), hi = lds_tr16(va + 16 * kRowBytes);
+        vt[mt] = dec_u4{lo.x, lo.y, hi.x, hi.y};
       }
-      uint2 vt[D / 16];
-#pragma unroll
-      for (int mt = 0; mt < D / 16; ++mt) vt[mt] = lds_tr16(voff + at + (((mt * 2 + vpiece) ^ vswap) << 4));
       const bool plain = kb + kFewKeys - 1 <= pos0 && (p.window == 0 || kb > sq.len - 1 - p.window || kb + kFewKeys <= p.sinks);
-      uint2 pb[ROWT];
+      dec_u4 pb[ROWT];
 #pragma unroll
       for (int nt = 0; nt < ROWT; ++nt) {
-        float x[4];
+        float x[8];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          x[r] = s[nt][r] * p.scale_log2;
-          if (!plain && !paged_sees(p, pos[nt], kb + 4 * lg + r)) x[r] = -INFINITY;
+        for (int r = 0; r < 8; ++r) x[r] = s[nt][r >> 2][r & 3] * p.scale_log2;
+        if (!plain) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (!paged_sees(p, pos[nt], kb + (r >> 2) * 16 + 4 * lg + (r & 3))) x[r] = -INFINITY;
         }
-        const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
         if (__any(top > ref[nt] + kSlack)) {                 // (also where the reference is still -inf)
           float m = fmaxf(top, __shfl_xor(top, 16, kWave));
           m = fmaxf(m, __shfl_xor(m, 32, kWave));
@@ -135,21 +156,19 @@ __global__ __launch_bounds__(64) void paged_few_kernel(PagedParams p) {
           for (int mt = 0; mt < D / 16; ++mt) o[nt][mt] *= alpha;
         }
         const float base = ref[nt] == -INFINITY ? 0.f : ref[nt];
-        float e[4];
+        float e[8];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          e[r] = __builtin_amdgcn_exp2f(x[r] - base);
-          l[nt] += e[r];
-        }
-        pb[nt] = make_uint2(pack2<DT>(e[0], e[1]), pack2<DT>(e[2], e[3]));
+        for (int r = 0; r < 8; ++r) e[r] = __builtin_amdgcn_exp2f(x[r] - base);
+        l[nt] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+        pb[nt] = pack8<DT>(e);
       }
 #pragma unroll
       for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
-        for (int nt = 0; nt < ROWT; ++nt) o[nt][mt] = mfma16x16x16<DT>(vt[mt], pb[nt], o[nt][mt]);
-      if (st + STAGES < stages) {
+        for (int nt = 0; nt < ROWT; ++nt) o[nt][mt] = mfma16x16x32<DT>(vt[mt], pb[nt], o[nt][mt]);
+      if (st + kFewStages < stages) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the stage has been read
-        request(st + STAGES);
+        request(st + kFewStages);
       }
     }
   }
@@ -176,14 +195,19 @@ __global__ __launch_bounds__(64) void paged_few_kernel(PagedParams p) {
   }
 }
 // ---------------------------------------------------------------------------------------------------------------- merge
-// out = sum_c 2^(ref_c - max ref) O_c / sum_c 2^(ref_c - max ref) l_c.  A wavefront a row: 256 / D chunks side by side, 16 bytes a lane, the
-// references and sums of 64 chunks in one load.
-template <int DT, int D>
+// out = sum_c 2^(ref_c - max ref) O_c / sum_c 2^(ref_c - max ref) l_c, a row of WAVES wavefronts: the chunks' weights go through LDS,
+// kMergeWeights of them at a time, then every kLanes lanes take the chunks in turn, 16 bytes of their row a lane.
+constexpr int kMergeWeights = 1024;
+template <int DT, int D, int WAVES>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
-  constexpr int kLanes = D / 4, kSide = kWave / kLanes;
-  const int64_t id = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
-  if (id >= (int64_t)p.n_tokens * p.hq) return;
-  const int t = (int)(id / p.hq), h = (int)(id - (int64_t)t * p.hq);
+  constexpr int kLanes = D / 4, kSide = WAVES * kWave / kLanes, kTeams = 4 / WAVES, kThreads = WAVES * kWave;
+  __shared__ float weight[kTeams][kMergeWeights / kTeams];
+  __shared__ __attribute__((aligned(16))) float part[kTeams][WAVES][D + 4];
+  __shared__ float tops[4];
+  const int team = threadIdx.x / kThreads, tid = threadIdx.x % kThreads, wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+  const int64_t id = (int64_t)blockIdx.x * kTeams + team;
+  bool mine = id < (int64_t)p.n_tokens * p.hq;
+  const int t = mine ? (int)(id / p.hq) : 0, h = mine ? (int)(id - (int64_t)t * p.hq) : 0;
   int lo = 0, hi = p.batch;                                  // the sequence with starts[lo] <= t < starts[lo + 1]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -191,41 +215,65 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
     else hi = mid;
   }
   const PagedSequence sq = paged_sequence(p, lo);
-  const int i = t - sq.first;
-  if (i < 0 || i >= sq.n) return;
-  const int r = i * p.group + h % p.group, kvh = h / p.group;
-  if (sq.n * p.group > p.few.rows) return;
-  const PagedSpan sp = paged_span(p, sq.len - sq.n, sq.len, kFewKeys);
-  const int chunks = paged_chunks(sp, p.few.chunk_keys);
-  if (chunks == 1) return;                                   // complete already
-  const int64_t slot = ((int64_t)sq.b * p.hkv + kvh) * p.few.chunks * p.few.rows + r;
-  const int rows = p.few.rows;
-  const float* po = p.few.part_o;
-  const float* ml = p.few.part_ml;
-  const int lane = threadIdx.x & (kWave - 1), d4 = (lane % kLanes) * 4, side = lane / kLanes;
+  const int i = t - sq.first, rows = p.few.rows;
+  mine = mine && i >= 0 && i < sq.n && sq.n * p.group <= rows;
+  int chunks = 1;
+  if (mine) chunks = paged_chunks(paged_span(p, sq.len - sq.n, sq.len, kFewKeys), p.few.chunk_keys);
+  mine = mine && chunks > 1;                                 // (one chunk: complete already)
+  if (WAVES == 4 && !mine) return;                           // (the whole workgroup)
+  const int64_t slot = ((int64_t)sq.b * p.hkv + h / p.group) * p.few.chunks * rows + i * p.group + h % p.group;
+  const float* ml = p.few.part_ml + slot * 2;
+  const int d4 = (tid % kLanes) * 4, side = tid / kLanes;
+  const float* po = p.few.part_o + slot * D + d4;
   float top = -INFINITY;
-  for (int c = lane; c < chunks; c += kWave) top = fmaxf(top, ml[(slot + (int64_t)c * rows) * 2]);
+  if (mine)
+    for (int c = tid; c < chunks; c += kThreads) top = fmaxf(top, ml[(int64_t)c * rows * 2]);
   top = wave_max(top);
+  if constexpr (WAVES == 4) {
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  }
   const float base = top == -INFINITY ? 0.f : top;
   v4f num = {0.f, 0.f, 0.f, 0.f};
   float den = 0.f;
+  constexpr int kAtOnce = kMergeWeights / kTeams;
+  for (int c0 = 0; mine && c0 < chunks; c0 += kAtOnce) {     // (uniform in a team)
+    const int some = min(kAtOnce, chunks - c0);
+    for (int c = tid; c < some; c += kThreads) {
+      const v2f m = *(const v2f*)(ml + (int64_t)(c0 + c) * rows * 2);
+      const float w = __builtin_amdgcn_exp2f(m[0] - base);
+      weight[team][c] = w;
+      den = fmaf(w, m[1], den);
+    }
+    if constexpr (WAVES == 4) __syncthreads();
+    else __builtin_amdgcn_wave_barrier();
 #pragma unroll 8
-  for (int c = side; c < chunks; c += kSide) {
-    const int64_t at = slot + (int64_t)c * rows;
-    const v2f m = *(const v2f*)(ml + at * 2);
-    const v4f o = *(const v4f*)(po + at * D + d4);
-    const float w = __builtin_amdgcn_exp2f(m[0] - base);
+    for (int c = side; c < some; c += kSide) {
+      const v4f o = *(const v4f*)(po + (int64_t)(c0 + c) * rows * D);
+      const float w = weight[team][c];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) num[e] = fmaf(w, o[e], num[e]);
-    den = fmaf(w, m[1], den);
+      for (int e = 0; e < 4; ++e) num[e] = fmaf(w, o[e], num[e]);
+    }
+    if constexpr (WAVES == 4) __syncthreads();
+    else __builtin_amdgcn_wave_barrier();
   }
+  den = wave_sum(den);
 #pragma unroll
-  for (int s = kLanes; s < kWave; s <<= 1) {
+  for (int s = kLanes; s < kWave; s <<= 1)
 #pragma unroll
     for (int e = 0; e < 4; ++e) num[e] += __shfl_xor(num[e], s, kWave);
-    den += __shfl_xor(den, s, kWave);
+  if constexpr (WAVES == 4) {
+    if (lane < kLanes) *(v4f*)&part[0][wave][d4] = num;
+    if (lane == 0) part[0][wave][D] = den;
+    __syncthreads();
+    if (wave != 0 || lane >= kLanes) return;
+    for (int w = 1; w < WAVES; ++w) {
+      num += *(const v4f*)&part[0][w][d4];
+      den += part[0][w][D];
+    }
   }
-  if (side) return;
+  if (!mine || lane >= kLanes) return;
   const float inv = den > 0.f ? 1.f / den : 0.f;
   *(uint2*)(p.out + id * D + d4) = make_uint2(pack2<DT>(num[0] * inv, num[1] * inv), pack2<DT>(num[2] * inv, num[3] * inv));
 }
@@ -244,8 +292,12 @@ static PagedPlan paged_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64_t
   pl.few_rows = few <= 16 ? 16 : few <= 32 ? 32 : few <= 64 ? 64 : 0;
   if (pl.few_rows) {
     const int64_t keys = std::max<int64_t>(1, span(pl.few_rows / group, kFewKeys)), units = batch * hkv;
-    int64_t per = (units * keys / 4096 + kFewKeys - 1) / kFewKeys * kFewKeys;
-    per = std::min<int64_t>(std::max<int64_t>(per, 64), kSegment);
+    // A unit's stage takes 0.5 to 0.65 us however deep its ring (16 copies and the products of 32 keys, one after the other), so short calls
+    // want short chunks; a partial result costs the merge as much as 7 keys of 28 : 4 heads, so long ones want long ones.  Both launches,
+    // chunks of 64 / 128 / 256 / 384 / 512 keys, us: one token of 1000 rows, 32 : 8 heads of 64: 8.2 9.4 11.8 14.5 17.2; of 32768, 28 : 4:
+    // 41 27.5 22.5 22.5 21.5; 32 tokens of 1000: 18 15.8 15.6 18 19.8; 64 of 4096: 95 87 87 79 85
+    int64_t per = ((int64_t)(0.65 * std::sqrt((double)units * (double)keys)) + kFewKeys - 1) / kFewKeys * kFewKeys;
+    per = std::min<int64_t>(std::max<int64_t>(per, 64), 384);
     while (per < keys && units * ((keys + per - 1) / per) * pl.few_rows > (1 << 21)) per *= 2;         // a gigabyte of partial results at 128 a head
     pl.few_keys = (int)per;
     pl.few_chunks = (int)((keys + per - 1) / per);
@@ -353,18 +405,20 @@ extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, in
   p.tiles = (int)pl.tiles;
   hipStream_t st = (hipStream_t)stream;
   const int64_t few_units = batch * n_kv_heads * pl.few_chunks, tile_units = pl.tiles * n_kv_heads * pl.tile_chunks;
-  if (few_units > INT32_MAX || tile_units > INT32_MAX || n_tokens * n_q_heads > (1ll << 32))
+  if (few_units > INT32_MAX || tile_units > INT32_MAX || n_tokens * n_q_heads > INT32_MAX)
     SUBSPEC_FAIL(SUBSPEC_ERR_LIMIT, "%s: too large (%lld tokens of %lld heads, %lld sequences)", what, (long long)n_tokens, (long long)n_q_heads,
                  (long long)batch);
-#define SUBSPEC_PAGED_FEW(DT, D, ROWT) hipLaunchKernelGGL((paged_few_kernel<DT, D, ROWT, 2>), dim3((unsigned)few_units), dim3(64), 0, st, p)
+#define SUBSPEC_PAGED_FEW(DT, D, ROWT) hipLaunchKernelGGL((paged_few_kernel<DT, D, ROWT>), dim3((unsigned)few_units), dim3(64), 0, st, p)
 #define SUBSPEC_PAGED(DT, D)                                                                                                           \
   do {                                                                                                                                 \
     DominantKernelTimer timer(st);                                                                                                     \
     if (pl.few_rows == 16) SUBSPEC_PAGED_FEW(DT, D, 1);                                                                                \
     else if (pl.few_rows == 32) SUBSPEC_PAGED_FEW(DT, D, 2);                                                                           \
     else if (pl.few_rows == 64) SUBSPEC_PAGED_FEW(DT, D, 4);                                                                           \
-    if (pl.few_chunks > 1)                                                                                                             \
-      hipLaunchKernelGGL((paged_merge_kernel<DT, D>), dim3((unsigned)((n_tokens * n_q_heads + 3) / 4)), dim3(256), 0, st, p);          \
+    if (pl.few_chunks > 12)                                                                                                            \
+      hipLaunchKernelGGL((paged_merge_kernel<DT, D, 4>), dim3((unsigned)(n_tokens * n_q_heads)), dim3(256), 0, st, p);                 \
+    else if (pl.few_chunks > 1)                                                                                                        \
+      hipLaunchKernelGGL((paged_merge_kernel<DT, D, 1>), dim3((unsigned)((n_tokens * n_q_heads + 3) / 4)), dim3(256), 0, st, p);       \
   } while (0)
   if (pl.tiles) {
     if (!pl.few_rows) {
