@@ -370,10 +370,14 @@ int subspec_paged_attention(const void* q, int64_t q_token_stride, int64_t q_hea
  *           T <= 0 takes the first largest; k <= 0, p >= 1 and min_p <= 0 filter nothing
  * tokens    device int64 [rows], -1 where nothing can be drawn (no logit above -inf)
  * probs     device float [rows]: the token's share of the mass that stays (0 where nothing can be drawn)
+ * workspace subspec_sample_filtered_workspace bytes, 16-byte aligned (NULL where that is 256): few long rows are cut into slices
  */
+size_t subspec_sample_filtered_workspace(int64_t rows, int64_t vocab);
+
 int subspec_sample_filtered(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride, const float* uniforms,
                             const float* temperatures, float temperature, const int32_t* top_ks, int32_t top_k, const float* top_ps,
-                            float top_p, const float* min_ps, float min_p, int64_t* tokens, float* probs, void* stream);
+                            float top_p, const float* min_ps, float min_p, void* workspace, size_t workspace_bytes, int64_t* tokens, float* probs,
+                            void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Draft probabilities: out = softmax(round(logits / temperature)) over the last axis, in the logits

@@ -77,8 +77,9 @@ _SIGNATURES = {
     "subspec_paged_attention_workspace": (_sz, [_i64] * 10),
     "subspec_paged_attention": (C.c_int, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, C.c_int, _i64, _i64, _i64, _i64,
                                           _i64, _i64, _i64, _i64, _i64, C.c_float, _p, _sz, _p]),
+    "subspec_sample_filtered_workspace": (_sz, [_i64, _i64]),
     "subspec_sample_filtered": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, _p, _p, C.c_float, _p, _i32, _p, C.c_float, _p, C.c_float,
-                                          _p, _p, _p]),
+                                          _p, _sz, _p, _p, _p]),
     "subspec_softmax_temperature_workspace": (_sz, [_i64, _i64]),
     "subspec_softmax_temperature": (C.c_int, [_p, _p, C.c_int, _i64, _i64, C.c_float, _p, _sz, _p]),
     "subspec_temperature_warp": (C.c_int, [_p, _p, C.c_int, _i64, C.c_float, _p]),

@@ -30,6 +30,7 @@ struct PagedParams {
   int batch, n_tokens, hq, hkv, group, head_dim, max_new, max_kv, window, sinks, page_shift, max_pages, max_blocks;
   float scale_log2;
   PagedCut few;                            // sequences of at most few.rows rows a KV head (0 rows: none)
+  int few_most;                            // rows a KV head that one of them can have
   PagedCut tile;                           // the others
   int tiles;                               // tiles of a KV head that the launch has room for
 };

@@ -205,23 +205,16 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
   __shared__ __attribute__((aligned(16))) float part[kTeams][WAVES][D + 4];
   __shared__ float tops[4];
   const int team = threadIdx.x / kThreads, tid = threadIdx.x % kThreads, wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
-  const int64_t id = (int64_t)blockIdx.x * kTeams + team;
-  bool mine = id < (int64_t)p.n_tokens * p.hq;
-  const int t = mine ? (int)(id / p.hq) : 0, h = mine ? (int)(id - (int64_t)t * p.hq) : 0;
-  int lo = 0, hi = p.batch;                                  // the sequence with starts[lo] <= t < starts[lo + 1]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.starts[mid] <= t) lo = mid;
-    else hi = mid;
-  }
-  const PagedSequence sq = paged_sequence(p, lo);
-  const int i = t - sq.first, rows = p.few.rows;
-  mine = mine && i >= 0 && i < sq.n && sq.n * p.group <= rows;
+  const int64_t id = (int64_t)blockIdx.x * kTeams + team;    // (sequence, KV head, row)
+  const int r = (int)(id % p.few_most), bk = (int)(id / p.few_most), kvh = bk % p.hkv, rows = p.few.rows;
+  bool mine = bk / p.hkv < p.batch;
+  const PagedSequence sq = paged_sequence(p, mine ? bk / p.hkv : 0);
+  mine = mine && r < sq.n * p.group && sq.n * p.group <= rows;
   int chunks = 1;
   if (mine) chunks = paged_chunks(paged_span(p, sq.len - sq.n, sq.len, kFewKeys), p.few.chunk_keys);
   mine = mine && chunks > 1;                                 // (one chunk: complete already)
   if (WAVES == 4 && !mine) return;                           // (the whole workgroup)
-  const int64_t slot = ((int64_t)sq.b * p.hkv + h / p.group) * p.few.chunks * rows + i * p.group + h % p.group;
+  const int64_t slot = (int64_t)bk * p.few.chunks * rows + r;
   const float* ml = p.few.part_ml + slot * 2;
   const int d4 = (tid % kLanes) * 4, side = tid / kLanes;
   const float* po = p.few.part_o + slot * D + d4;
@@ -275,7 +268,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
   }
   if (!mine || lane >= kLanes) return;
   const float inv = den > 0.f ? 1.f / den : 0.f;
-  *(uint2*)(p.out + id * D + d4) = make_uint2(pack2<DT>(num[0] * inv, num[1] * inv), pack2<DT>(num[2] * inv, num[3] * inv));
+  *(uint2*)(p.out + ((int64_t)(sq.first + r / p.group) * p.hq + kvh * p.group + r % p.group) * D + d4) =
+      make_uint2(pack2<DT>(num[0] * inv, num[1] * inv), pack2<DT>(num[2] * inv, num[3] * inv));
 }
 
 // How a call is cut, from the bounds alone.  Keys of a row: at most max_kv, or a window's, its sinks and the row's fellow tokens'.
@@ -403,9 +397,11 @@ extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, in
   ws += pl.few_o + pl.few_ml;
   p.tile = PagedCut{kTileRows, pl.tile_keys, pl.tile_chunks, (float*)ws, (float*)(ws + pl.tile_o)};
   p.tiles = (int)pl.tiles;
+  p.few_most = (int)std::max<int64_t>(1, std::min<int64_t>(pl.few_rows, max_new * p.group));
   hipStream_t st = (hipStream_t)stream;
+  const int64_t merge_rows = batch * n_kv_heads * p.few_most;
   const int64_t few_units = batch * n_kv_heads * pl.few_chunks, tile_units = pl.tiles * n_kv_heads * pl.tile_chunks;
-  if (few_units > INT32_MAX || tile_units > INT32_MAX || n_tokens * n_q_heads > INT32_MAX)
+  if (few_units > INT32_MAX || tile_units * 8 > INT32_MAX || merge_rows > INT32_MAX)
     SUBSPEC_FAIL(SUBSPEC_ERR_LIMIT, "%s: too large (%lld tokens of %lld heads, %lld sequences)", what, (long long)n_tokens, (long long)n_q_heads,
                  (long long)batch);
 #define SUBSPEC_PAGED_FEW(DT, D, ROWT) hipLaunchKernelGGL((paged_few_kernel<DT, D, ROWT>), dim3((unsigned)few_units), dim3(64), 0, st, p)
@@ -416,9 +412,9 @@ extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, in
     else if (pl.few_rows == 32) SUBSPEC_PAGED_FEW(DT, D, 2);                                                                           \
     else if (pl.few_rows == 64) SUBSPEC_PAGED_FEW(DT, D, 4);                                                                           \
     if (pl.few_chunks > 12)                                                                                                            \
-      hipLaunchKernelGGL((paged_merge_kernel<DT, D, 4>), dim3((unsigned)(n_tokens * n_q_heads)), dim3(256), 0, st, p);                 \
+      hipLaunchKernelGGL((paged_merge_kernel<DT, D, 4>), dim3((unsigned)merge_rows), dim3(256), 0, st, p);                              \
     else if (pl.few_chunks > 1)                                                                                                        \
-      hipLaunchKernelGGL((paged_merge_kernel<DT, D, 1>), dim3((unsigned)((n_tokens * n_q_heads + 3) / 4)), dim3(256), 0, st, p);       \
+      hipLaunchKernelGGL((paged_merge_kernel<DT, D, 1>), dim3((unsigned)((merge_rows + 3) / 4)), dim3(256), 0, st, p);                  \
   } while (0)
   if (pl.tiles) {
     if (!pl.few_rows) {

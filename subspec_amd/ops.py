@@ -575,9 +575,13 @@ def sample_filtered(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.
         raise ValueError("sample_filtered: temperature, top_k, top_p and min_p must not be negative")
     tokens = torch.empty(rows, dtype=torch.int64, device=dev)
     probs = torch.empty(rows, dtype=torch.float32, device=dev)
-    code = L.lib().subspec_sample_filtered(
+    lib = L.lib()
+    need = lib.subspec_sample_filtered_workspace(rows, V)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 256 else None
+    code = lib.subspec_sample_filtered(
         logits.data_ptr(), _dtype_code(logits), rows, V, max(logits.stride(0), V), uniforms.data_ptr(), t_ptr, float(t), k_ptr,
-        min(int(k), (1 << 31) - 1), p_ptr, float(p), m_ptr, float(m), tokens.data_ptr(), probs.data_ptr(), _stream(dev))
+        min(int(k), (1 << 31) - 1), p_ptr, float(p), m_ptr, float(m), None if ws is None else ws.data_ptr(), need,
+        tokens.data_ptr(), probs.data_ptr(), _stream(dev))
     L.check(code, "subspec_sample_filtered")
     return tokens, probs
 

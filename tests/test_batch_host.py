@@ -61,15 +61,15 @@ def test_attention_over_nothing_launches_nothing():
 
 
 def _sample(**change):
-    a = dict(logits=ANY, dtype=L.BF16, rows=2, vocab=100, stride=100, u=ANY)
+    a = dict(logits=ANY, dtype=L.BF16, rows=2, vocab=100, stride=100, u=ANY, ws=None)
     a.update(change)
     return L.lib().subspec_sample_filtered(a["logits"], a["dtype"], a["rows"], a["vocab"], a["stride"], a["u"], None, 1.0, None, 0, None, 1.0, None,
-                                           0.0, ANY, ANY, None)
+                                           0.0, a["ws"], 0, ANY, ANY, None)
 
 
 @pytest.mark.parametrize("change,code", [(dict(logits=None), -1), (dict(u=None), -1), (dict(dtype=5), -1), (dict(vocab=0), -4),
                                          (dict(vocab=(1 << 20) + 1, stride=1 << 21), -4), (dict(rows=-1), -4), (dict(stride=99), -1),
-                                         (dict(logits=ANY + 1), -1)])
+                                         (dict(logits=ANY + 1), -1), (dict(vocab=50000, stride=50000), -2), (dict(ws=ANY + 8), -1)])
 def test_sample_refuses(change, code):
     assert _sample(**change) == code and b"sample_filtered" in L.lib().subspec_last_error()
 
