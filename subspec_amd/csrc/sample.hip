@@ -38,90 +38,90 @@ struct SampleArgs {
 };
 
 // What a row is drawn with.
-struct RowRule { double inv_t; float inv_tf; bool greedy; int k; double p, min_p, u; };
+struct RowRule { double inv_t_log2e; float inv_t; bool greedy; int k; double p, min_p, u; };
 __device__ __forceinline__ RowRule row_rule(const SampleArgs& a, int row) {
   RowRule r;
   const float t = a.temperatures ? a.temperatures[row] : a.temperature;
   const int k = a.top_ks ? a.top_ks[row] : a.top_k;
   const float p = a.top_ps ? a.top_ps[row] : a.top_p, q = a.min_ps ? a.min_ps[row] : a.min_p, u = a.uniforms[row];
-  r.greedy = !(t > 0.f);
-  r.inv_t = r.greedy ? 1.0 : 1.0 / (double)t;
-  r.inv_tf = (float)r.inv_t;
+  r.greedy = !(t >= 1.17549435e-38f);                    // (below the smallest normal number 1 / T is infinite)
+  const double inv_t = r.greedy ? 1.0 : 1.0 / (double)t;
+  r.inv_t_log2e = inv_t * 1.44269504088896340736;
+  r.inv_t = (float)inv_t;
   r.k = r.greedy ? 1 : k <= 0 ? INT32_MAX : k;
   r.p = p < 1.f ? (double)p : 1.0;                       // (a NaN filters nothing)
   r.min_p = q > 0.f ? fmin((double)q, 1.0) : 0.0;
   r.u = u > 0.f ? (double)u : 0.0;
   return r;
 }
+// The largest logit, and whether only entries that equal it have mass (T = 0, or it is infinite).
+struct RowTop { float value; double wide; bool only; };
+__device__ __forceinline__ RowTop row_top_of(float top, const RowRule& r) { return RowTop{top, (double)top, r.greedy || top == INFINITY}; }
 
-// 2^x for x <= 0 times 2^42, rounded to a whole number: x = n + f, |f| <= 1/2, the Taylor series of e^(f ln 2) to the tenth power
-// (remainder (ln 2 / 2)^11 / 11! = 2.2e-13 of the value).
+// 2^f * 2^42 for |f| <= 1/2: the Taylor series of e^(f ln 2) to the tenth power, its coefficients ln^k 2 / k! (remainder (ln 2 / 2)^11 / 11! =
+// 2.2e-13 of the value).  (The three-operand instruction by hand: the compiler takes the two-operand one and copies each coefficient first.)
+__device__ __forceinline__ double fma_s(double a, double b, double c) {
+  double d;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
+  return d;
+}
 __device__ __forceinline__ double exp2_part(double f) {
-  const double y = f * 0.69314718055994530942;
-  double s = 1.0 / 3628800.0;
-  s = fma(s, y, 1.0 / 362880.0);
-  s = fma(s, y, 1.0 / 40320.0);
-  s = fma(s, y, 1.0 / 5040.0);
-  s = fma(s, y, 1.0 / 720.0);
-  s = fma(s, y, 1.0 / 120.0);
-  s = fma(s, y, 1.0 / 24.0);
-  s = fma(s, y, 1.0 / 6.0);
-  s = fma(s, y, 0.5);
-  s = fma(s, y, 1.0);
-  return fma(s, y, 1.0);
+  constexpr double k = (double)(1ull << kMassBits);
+  double s = fma_s(f, 7.0549116208011233e-9 * k, 1.0178086009239699e-7 * k);
+  s = fma_s(s, f, 1.3215486790144309e-6 * k);
+  s = fma_s(s, f, 1.5252733804059841e-5 * k);
+  s = fma_s(s, f, 1.5403530393381610e-4 * k);
+  s = fma_s(s, f, 1.3333558146428443e-3 * k);
+  s = fma_s(s, f, 9.6181291076284772e-3 * k);
+  s = fma_s(s, f, 5.5504108664821580e-2 * k);
+  s = fma_s(s, f, 2.4022650695910072e-1 * k);
+  s = fma_s(s, f, 6.9314718055994531e-1 * k);
+  return fma_s(s, f, k);
 }
-// How far entry l is below the largest in units of T, in 32 bits: what the bins go by (falls as l rises, so bins keep the order; kReach or more,
-// or NaN: no mass).  With T = 0 only entries that equal the largest are near.
-__device__ __forceinline__ float entry_distance(float l, float top, const RowRule& r) {
-  if (l == top) return 0.f;
-  return r.greedy ? INFINITY : (top - l) * r.inv_tf;
+// How far entry l is below the largest in units of T, in 32 bits: what the bins go by (falls as l rises, so bins keep the order).  Entries at kReach
+// and beyond, and NaN, have no mass and no bin.
+__device__ __forceinline__ float entry_distance(float l, const RowTop& top, const RowRule& r) {
+  if (top.only) return l == top.value ? 0.f : INFINITY;
+  return (top.value - l) * r.inv_t;
 }
-__device__ __forceinline__ int bin_of(float d) { return min((int)(d * (kBins / kReach)), kBins - 1); }
-// The mass of an entry less than about kReach below the largest, in units of 2^-42 and before rounding.
-__device__ __forceinline__ double entry_mass(float l, float top, const RowRule& r) {
-  const double x = l == top ? 0.0 : ((double)l - (double)top) * r.inv_t * 1.44269504088896340736, n = rint(x);
-  return ldexp(exp2_part(x - n), (int)n + kMassBits);
+__device__ __forceinline__ int bin_of(float d) { return (int)(d * (0.999999f * kBins / kReach)); }      // (below kBins, rounding or not)
+// The mass of an entry less than kReach below the largest, in units of 2^-42 and before rounding.
+__device__ __forceinline__ double entry_mass(float l, const RowTop& top, const RowRule& r) {
+  if (top.only) return (double)(1ull << kMassBits);
+  const double x = ((double)l - top.wide) * r.inv_t_log2e, n = rint(x);
+  return ldexp(exp2_part(x - n), (int)n);
 }
-__device__ __forceinline__ uint64_t whole(double m) { return (uint64_t)rint(m); }
-// f(bin, mass before rounding, mass) for an entry that has any
-template <typename F>
-__device__ __forceinline__ void with_mass(float l, float top, const RowRule& r, F f) {
-  const float d = entry_distance(l, top, r);
-  if (!(d < kReach)) return;
-  const double m = entry_mass(l, top, r);
-  const uint64_t w = whole(m);
-  if (w != 0) f(bin_of(d), m, w);
-}
-// larger logits first, then lower indexes: ascending 64-bit keys
+// ... rounded (to even): below 2^52 a sum with 2^52 has no bits behind the point
+__device__ __forceinline__ uint64_t whole(double m) { return (uint64_t)__double_as_longlong(m + 4503599627370496.0) & 0xfffffffffffffull; }
+
+// Larger logits first, then lower indexes, as ascending keys: the bits of the value that its type has (a bf16's or fp16's float is zero behind
+// them), turned round, and 20 bits of the index.
+template <int DT> constexpr int kDropped = DT == SUBSPEC_F32 ? 0 : DT == SUBSPEC_F16 ? 13 : 16;
+template <int DT> constexpr int kKeyBits = 52 - kDropped<DT>;
+template <int DT>
 __device__ __forceinline__ uint64_t order_key(float l, int i) {
   uint32_t b = __float_as_uint(l == 0.f ? 0.f : l);      // (-0 is 0)
-  b = b >> 31 ? b : ~b & 0x7fffffffu;                     // larger first: positive values below, negative ones with the sign bit above
-  return (uint64_t)b << 32 | (uint32_t)i;
+  b = b >> 31 ? b : ~b & 0x7fffffffu;                     // positive values below, negative ones with the sign bit above
+  return (uint64_t)(b >> kDropped<DT>) << 20 | (uint32_t)i;
 }
+template <int DT>
 __device__ __forceinline__ float key_logit(uint64_t key) {
-  const uint32_t b = (uint32_t)(key >> 32);
-  return __uint_as_float(b >> 31 ? b : ~b & 0x7fffffffu);
+  const uint32_t b = (uint32_t)(key >> 20) << kDropped<DT>;
+  return __uint_as_float(b >> 31 ? b : ~(b | ((1u << kDropped<DT>) - 1)) & 0x7fffffffu);
 }
 
 struct Hist {
   uint64_t mass[kBins];            // a bin's own, or inclusive sums after scan_bins
   uint32_t count[kBins];
 };
-struct Candidates {
-  uint64_t key[kCandidates];
-  uint64_t upto[kCandidates];      // inclusive mass over the ordered candidates
-};
-struct SampleShared {
-  Hist bins;
-  union {
-    Candidates c;
-    Hist digits;                   // a search without candidates
-  };
+// What a search works with.
+struct Search {
+  Hist digits;
   uint64_t wave_mass[kSampleThreads / kWave];
   uint32_t wave_count[kSampleThreads / kWave];
-  float scratch[kSampleThreads / kWave];
-  unsigned long long min_p_mass;
-  int n_candidates;
+  uint64_t list[kWave];
+  uint64_t key, upto;              // its answer
+  int n;
 };
 
 __device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {      // inclusive
@@ -183,62 +183,125 @@ __device__ __forceinline__ void clear_hist(Hist& h) {
   }
 }
 
-// first bin whose inclusive mass (count) exceeds t, which one does (uniform; every thread searches)
-__device__ __forceinline__ int bin_at(const Hist& h, bool by_count, uint64_t t) {
-  int lo = 0, hi = kBins - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if ((by_count ? (uint64_t)h.count[mid] : h.mass[mid]) > t) hi = mid;
-    else lo = mid + 1;
+// First index below n at which `over` holds (it then holds behind it too); n if nowhere.  64 probes at a time: two or three trips to LDS where
+// halving takes ten to twelve.  (Every wavefront searches for itself; all its lanes are active.)
+template <typename F>
+__device__ __forceinline__ int first_over(int n, F over) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int lo = 0, hi = n;                                         // the answer lies in [lo, hi]
+  while (hi > lo) {
+    const int step = (hi - lo + kWave - 1) / kWave, at = lo + (lane + 1) * step - 1;        // the last of the lane's stretch
+    const uint64_t hit = __ballot(at >= hi || over(min(at, hi - 1)));
+    const int f = hit ? __ffsll((unsigned long long)hit) - 1 : kWave;
+    if (step == 1) return min(lo + f, hi);
+    hi = min(lo + (f + 1) * step - 1, hi);                    // (its last one is over, or there is none: the answer is at most there)
+    lo = min(lo + f * step, hi);
   }
   return lo;
 }
+// first bin whose inclusive mass (count) exceeds t, which one does
+__device__ __forceinline__ int bin_at(const Hist& h, bool by_count, uint64_t t) {
+  return min(first_over(kBins, [&](int i) { return (by_count ? (uint64_t)h.count[i] : h.mass[i]) > t; }), kBins - 1);
+}
 
-// f(logit, index) for a workgroup's part of a row: 16 bytes a load between the row's aligned addresses, four of them in flight a thread (one
-// in flight is 16 KB a compute unit, which a round trip of a microsecond turns into 16 GB/s)
+// A workgroup's part [i0, i1) of a row: pieces of 16 bytes between the row's aligned addresses, and the ragged ends, less than a piece each.
+template <int DT>
+struct Part {
+  static constexpr int kVec = 16 / Elem<DT>::kBytes;
+  const void* row;
+  const dec_u4* src;
+  int i0, i1, first, pieces, rest;
+  __device__ __forceinline__ Part(const void* r, int b, int e) : row(r), i0(b), i1(e) {
+    const size_t address = (size_t)(uintptr_t)row + (size_t)i0 * Elem<DT>::kBytes;
+    first = min(i0 + (int)((16 - address % 16) % 16) / Elem<DT>::kBytes, i1);
+    pieces = (i1 - first) / kVec;
+    rest = first + pieces * kVec;
+    src = (const dec_u4*)((const char*)row + (size_t)first * Elem<DT>::kBytes);
+  }
+  __device__ __forceinline__ dec_u4 piece(int p) const {                  // (past the end: the last one again)
+    return pieces > 0 ? src[min(p, pieces - 1)] : dec_u4{0, 0, 0, 0};
+  }
+  template <int THREADS, typename F>
+  __device__ __forceinline__ void ends(F f) const {
+#pragma unroll 1
+    for (int e = threadIdx.x; e < first - i0 + i1 - rest; e += THREADS) {
+      const int i = e < first - i0 ? i0 + e : rest + e - (first - i0);
+      f(Elem<DT>::load(row, i), i);
+    }
+  }
+};
+// f(logit, index) for a part of a row, the next pieces asked for before the last are worked on.  One copy of f in the code (two for pairs of 16-bit
+// logits): it is long, and a slice takes few turns.
 template <int DT, int THREADS, typename F>
 __device__ __forceinline__ void each_entry(const void* row, int i0, int i1, F f) {
-  constexpr int kVec = 16 / Elem<DT>::kBytes, kFlight = 4;
-  const int tid = threadIdx.x;
-  const size_t address = (size_t)(uintptr_t)row + (size_t)i0 * Elem<DT>::kBytes;
-  const int first = min(i0 + (int)((16 - address % 16) % 16) / Elem<DT>::kBytes, i1);
-  const int pieces = (i1 - first) / kVec, rest = first + pieces * kVec;
-  if (i0 + tid < first) f(Elem<DT>::load(row, i0 + tid), i0 + tid);
-  const dec_u4* src = (const dec_u4*)((const char*)row + (size_t)first * Elem<DT>::kBytes);
-  for (int p0 = tid; p0 < pieces; p0 += kFlight * THREADS) {
+  const Part<DT> part(row, i0, i1);
+  dec_u4 next[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) next[u] = part.piece(threadIdx.x + u * THREADS);
+#pragma unroll 1
+  for (int p = threadIdx.x; p < part.pieces; p += THREADS) {
+    dec_u4 v = next[0];
+    next[0] = next[1];
+    next[1] = part.piece(p + 2 * THREADS);
+#pragma unroll 1
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t bits = v[0];
+      v = dec_u4{v[1], v[2], v[3], bits};
+      if constexpr (DT == SUBSPEC_F32) {
+        f(__uint_as_float(bits), part.first + p * 4 + j);
+      } else {
+        float x[2];
+        unpack2<DT>(bits, x);
+        f(x[0], part.first + p * 8 + 2 * j);
+        f(x[1], part.first + p * 8 + 2 * j + 1);
+      }
+    }
+  }
+  part.template ends<THREADS>(f);
+}
+// The largest of a part of a row (a thread's own)
+__device__ __forceinline__ float larger(float m, float l) { return l > m ? l : m; }      // a NaN never is
+template <int DT, int THREADS>
+__device__ __forceinline__ float part_top(const void* row, int i0, int i1) {
+  constexpr int kFlight = 4;
+  const Part<DT> part(row, i0, i1);
+  float top = -INFINITY;
+  for (int p0 = threadIdx.x; p0 < part.pieces; p0 += kFlight * THREADS) {
     dec_u4 v[kFlight];
 #pragma unroll
-    for (int u = 0; u < kFlight; ++u) v[u] = src[min(p0 + u * THREADS, pieces - 1)];
+    for (int u = 0; u < kFlight; ++u) v[u] = part.piece(p0 + u * THREADS);
 #pragma unroll
     for (int u = 0; u < kFlight; ++u) {
-      const int p = p0 + u * THREADS, at = first + p * kVec;
-      if (p >= pieces) break;
       if constexpr (DT == SUBSPEC_F32) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f(__uint_as_float(v[u][e]), at + e);
+        for (int e = 0; e < 4; ++e) top = larger(top, __uint_as_float(v[u][e]));
       } else {
         float x[8];
         unpack8<DT>(v[u], x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f(x[e], at + e);
+        for (int e = 0; e < 8; ++e) top = larger(top, x[e]);
       }
     }
   }
-  if (rest + tid < i1) f(Elem<DT>::load(row, rest + tid), rest + tid);
+  part.template ends<THREADS>([&](float l, int) { top = larger(top, l); });
+  return top;
 }
 
 // The bins of a part of a row, and the mass that min-p keeps of it (a thread's own, returned).  Counts are wanted with a top-k only.
 template <int DT, int THREADS>
-__device__ __forceinline__ uint64_t fill_bins(Hist& h, const void* row, int i0, int i1, int vocab, float top, const RowRule& r) {
+__device__ __forceinline__ uint64_t fill_bins(Hist& h, const void* row, int i0, int i1, int vocab, const RowTop& top, const RowRule& r) {
   const double least = r.min_p * (double)(1ull << kMassBits);
-  const bool counted = r.k < vocab;
+  const bool counted = r.k < vocab, sorted_out = r.min_p > 0.0;
   uint64_t kept = 0;
   each_entry<DT, THREADS>(row, i0, i1, [&](float l, int) {
-    with_mass(l, top, r, [&](int bin, double m, uint64_t w) {
-      atomicAdd((unsigned long long*)&h.mass[bin], (unsigned long long)w);
-      if (counted) atomicAdd(&h.count[bin], 1u);
-      if (!(m < least)) kept += w;
-    });
+    const float d = entry_distance(l, top, r);
+    if (!(d < kReach)) return;
+    const double m = entry_mass(l, top, r);
+    const uint64_t w = whole(m);
+    const int bin = bin_of(d);
+    atomicAdd((unsigned long long*)&h.mass[bin], (unsigned long long)w);
+    if (counted) atomicAdd(&h.count[bin], 1u);
+    if (sorted_out) kept += m < least ? 0 : w;
   });
   return kept;
 }
@@ -252,7 +315,7 @@ __device__ __forceinline__ uint64_t draw_goal(double u, uint64_t z) {
   const uint64_t t = (uint64_t)(u * (double)z);
   return z > 0 ? min(t, z - 1) : 0;
 }
-__device__ __forceinline__ BinRanges bin_ranges(const Hist& h, uint64_t min_p_mass, const RowRule& r) {
+__device__ __forceinline__ BinRanges bin_ranges(const Hist& h, uint64_t min_p_mass, const RowRule& r) {      // (min_p_mass counts with a min-p only)
   BinRanges g;
   uint64_t z_lo = h.mass[kBins - 1], z_hi = z_lo;
   g.by_k = (uint32_t)r.k < h.count[kBins - 1];
@@ -270,8 +333,10 @@ __device__ __forceinline__ BinRanges bin_ranges(const Hist& h, uint64_t min_p_ma
     z_lo = below(h, g.lo[1]) + 1;
     z_hi = h.mass[g.hi[1]];
   }
-  z_lo = min(z_lo, min_p_mass);
-  z_hi = min(z_hi, min_p_mass);
+  if (r.min_p > 0.0) {
+    z_lo = min(z_lo, min_p_mass);
+    z_hi = min(z_hi, min_p_mass);
+  }
   g.lo[2] = bin_at(h, false, draw_goal(r.u, z_lo));
   g.hi[2] = bin_at(h, false, draw_goal(r.u, z_hi));
   return g;
@@ -280,131 +345,155 @@ __device__ __forceinline__ bool in_ranges(const BinRanges& g, int b) {
   return (b >= g.lo[0] && b <= g.hi[0]) || (b >= g.lo[1] && b <= g.hi[1]) || (b >= g.lo[2] && b <= g.hi[2]);
 }
 
-// The entries of those bins in a part of a row; *n counts them, `most` of them are kept.
+// The entries of those bins in a part of a row; *n counts them, `most` of them are kept.  Few are, so a piece is first looked over in 32 bits:
+// within a bin of one of the ranges, |top - l - centre| <= width, nine instructions an entry (a NaN, and infinities among them, passes).
 template <int DT, int THREADS>
-__device__ __forceinline__ void gather(uint64_t* keys, int most, int* n, const void* row, int i0, int i1, float top, const RowRule& r,
+__device__ __forceinline__ void gather(uint64_t* keys, int most, int* n, const void* row, int i0, int i1, const RowTop& top, const RowRule& r,
                                        const BinRanges& g) {
-  each_entry<DT, THREADS>(row, i0, i1, [&](float l, int i) {
+  float centre[3], width[3];
+  const float bin = kReach / kBins / r.inv_t;                             // width of a bin in logits
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    centre[k] = 0.5f * (float)(g.lo[k] + g.hi[k] + 1) * bin;
+    width[k] = g.lo[k] > g.hi[k] ? -1.f : (0.5f * (float)(g.hi[k] - g.lo[k] + 1) + 1.f) * bin;
+  }
+  auto near = [&](float l) {
+    const float x = top.value - l;
+    return !(fabsf(x - centre[0]) > width[0]) || !(fabsf(x - centre[1]) > width[1]) || !(fabsf(x - centre[2]) > width[2]);
+  };
+  auto take = [&](float l, int i) {
     const float d = entry_distance(l, top, r);
-    if (!(d < kReach) || !in_ranges(g, bin_of(d)) || whole(entry_mass(l, top, r)) == 0) return;
+    if (!(d < kReach) || !in_ranges(g, bin_of(d))) return;
     const int at = atomicAdd(n, 1);
-    if (at < most) keys[at] = order_key(l, i);
-  });
-}
-
-// The candidates in order, with the inclusive sums of their masses (all threads; ends with a barrier).
-__device__ void order_candidates(SampleShared& s, int n, float top, const RowRule& r) {
-  const int tid = threadIdx.x, wave = tid / kWave, lane = tid & (kWave - 1);
-  int size = kWave;
-  while (size < n) size <<= 1;
-  for (int i = tid; i < size; i += kSampleThreads)
-    if (i >= n) s.c.key[i] = ~0ull;
-  __syncthreads();
-  for (int span = 2; span <= size; span <<= 1) {             // bitonic
-    for (int step = span >> 1; step > 0; step >>= 1) {
-      for (int i = tid; i < size / 2; i += kSampleThreads) {
-        const int lo = (i & (step - 1)) | (i & ~(step - 1)) << 1, hi = lo | step;
-        const uint64_t a = s.c.key[lo], b = s.c.key[hi];
-        if ((a > b) == ((lo & span) == 0)) {
-          s.c.key[lo] = b;
-          s.c.key[hi] = a;
-        }
-      }
-      __syncthreads();
+    if (at < most) keys[at] = order_key<DT>(l, i);
+  };
+  constexpr int kVec = 16 / Elem<DT>::kBytes;
+  const Part<DT> part(row, i0, i1);
+  dec_u4 next[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) next[u] = part.piece(threadIdx.x + u * THREADS);
+#pragma unroll 1
+  for (int p = threadIdx.x; p < part.pieces; p += THREADS) {
+    dec_u4 v = next[0];
+    next[0] = next[1];
+    next[1] = part.piece(p + 2 * THREADS);
+    float x[kVec];
+    if constexpr (DT == SUBSPEC_F32) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(v[e]);
+    } else {
+      unpack8<DT>(v, x);
+    }
+    uint32_t hits = 0;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) hits |= (near(x[e]) ? 1u : 0u) << e;
+    if (top.only) hits = (1u << kVec) - 1;
+    while (hits) {                                                        // (one turn for most wavefronts that have any)
+      const int e = __ffs(hits) - 1;
+      hits &= hits - 1;
+      float l = x[0];
+#pragma unroll
+      for (int k = 1; k < kVec; ++k) l = e == k ? x[k] : l;
+      take(l, part.first + p * kVec + e);
     }
   }
-  uint64_t before = 0;
-  for (int i0 = 0; i0 < n; i0 += kSampleThreads) {
-    const int i = i0 + tid;
-    const uint64_t w = wave_scan_u64(i < n ? whole(entry_mass(key_logit(s.c.key[i]), top, r)) : 0);
-    if (lane == kWave - 1) s.wave_mass[wave] = w;
-    __syncthreads();
-    uint64_t base = before;
-    for (int v = 0; v < kSampleThreads / kWave; ++v) {
-      if (v < wave) base += s.wave_mass[v];
-      before += s.wave_mass[v];
-    }
-    if (i < n) s.c.upto[i] = base + w;
-    __syncthreads();
-  }
+  part.template ends<THREADS>(take);
 }
 
-// The first entry in order whose rank (by_count) or inclusive mass exceeds t: its key, and the inclusive mass there.  (uniform)
+// The first entry in order whose rank (by_count) or inclusive mass exceeds t: its key, and the inclusive mass there.  `each` hands its argument
+// the keys among which the entries of that bin are (all threads; ends with a barrier).  While more than 64 are left, the next ten bits of the
+// keys tell them apart by a histogram like the bins'; 64 are put in order by one wavefront.
 struct Found { uint64_t key, upto; };
-__device__ Found find_ordered(const SampleShared& s, int n, bool by_count, uint64_t t, float top, const RowRule& r) {
-  const int b = bin_at(s.bins, by_count, t);
-  int lo = 0, hi = n;                                         // first candidate of bin b
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (bin_of(entry_distance(key_logit(s.c.key[mid]), top, r)) >= b) hi = mid;
-    else lo = mid + 1;
-  }
-  const uint64_t passed = below(s.bins, b) - (lo > 0 ? s.c.upto[lo - 1] : 0);        // mass before the bin that is not in the list
-  if (by_count) {
-    lo = min(lo + (int)(t - (b > 0 ? s.bins.count[b - 1] : 0)), n - 1);
-  } else {
-    hi = n - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (s.c.upto[mid] + passed > t) hi = mid;
-      else lo = mid + 1;
+template <int DT, int THREADS, typename Each>
+__device__ Found find_entry(Search& s, const Hist& bins, bool by_count, uint64_t t, const RowTop& top, const RowRule& r, int most, Each each) {
+  const int b = bin_at(bins, by_count, t);
+  uint64_t prefix = 0, upto = below(bins, b);
+  t -= by_count ? (uint64_t)(b > 0 ? bins.count[b - 1] : 0) : upto;
+  // the keys of a bin (and of its neighbours, for what rounding there is) agree in their leading bits
+  const float wide = kReach / kBins / r.inv_t;
+  const uint64_t first = order_key<DT>(top.only ? top.value : top.value - (float)(b - 1) * wide, 0);
+  const uint64_t last = order_key<DT>(top.only ? top.value : top.value - (float)(b + 2) * wide, (1 << 20) - 1);
+  int shift = 64 - __clzll((long long)((first ^ last) | 1));
+  prefix = last >> shift << shift;
+  int left = most <= kWave ? 0 : most;                        // at most how many there are (0: look)
+  auto mine = [&](uint64_t key) { return (key ^ prefix) >> shift == 0 && bin_of(entry_distance(key_logit<DT>(key), top, r)) == b; };
+  for (;;) {
+    if (left <= kWave) {
+      if (threadIdx.x == 0) s.n = 0;
+      __syncthreads();
+      each([&](uint64_t key) {
+        if (!mine(key)) return;
+        const int at = atomicAdd(&s.n, 1);
+        if (at < kWave) s.list[at] = key;
+      });
+      __syncthreads();
+      left = s.n;
+      if (left <= kWave) break;
     }
-  }
-  return Found{s.c.key[lo], s.c.upto[lo] + passed};
-}
-
-// The same over the whole row, for bins that hold more entries than the list (thousands of equal logits): digit by digit of the
-// order's key, a pass over the row for each.
-template <int DT>
-__device__ Found find_in_row(SampleShared& s, const void* row, int vocab, bool by_count, uint64_t t, float top, const RowRule& r) {
-  const int b = bin_at(s.bins, by_count, t);
-  t -= by_count ? (uint64_t)(b > 0 ? s.bins.count[b - 1] : 0) : below(s.bins, b);
-  uint64_t prefix = 0, upto = below(s.bins, b);
-  const int shifts[6] = {54, 44, 34, 32, 10, 0}, widths[6] = {10, 10, 10, 2, 10, 10};        // 32 bits of the logit, 20 of the index
-  for (int level = 0; level < 6; ++level) {
-    const int shift = shifts[level], width = widths[level];
+    clear_hist<THREADS>(s.digits);
     __syncthreads();
-    clear_hist<kSampleThreads>(s.digits);
-    __syncthreads();
-    each_entry<DT, kSampleThreads>(row, 0, vocab, [&](float l, int i) {
-      const float d = entry_distance(l, top, r);
-      if (!(d < kReach) || bin_of(d) != b) return;
-      const uint64_t key = order_key(l, i);
-      if (level > 0 && ((key ^ prefix) >> (shift + width)) != 0) return;
-      const uint64_t m = whole(entry_mass(l, top, r));
-      if (m == 0) return;
-      const int digit = (int)(key >> shift) & ((1 << width) - 1);
-      atomicAdd((unsigned long long*)&s.digits.mass[digit], (unsigned long long)m);
+    const int width = min(10, shift), next = shift - width;
+    each([&](uint64_t key) {
+      if (!mine(key)) return;
+      const int digit = (int)(key >> next) & ((1 << width) - 1);
+      atomicAdd((unsigned long long*)&s.digits.mass[digit], (unsigned long long)whole(entry_mass(key_logit<DT>(key), top, r)));
       atomicAdd(&s.digits.count[digit], 1u);
     });
     __syncthreads();
-    scan_bins<kSampleThreads>(s.digits, s.wave_mass, s.wave_count);
+    scan_bins<THREADS>(s.digits, s.wave_mass, s.wave_count);
     const int digit = bin_at(s.digits, by_count, t);
-    t -= by_count ? (uint64_t)(digit > 0 ? s.digits.count[digit - 1] : 0) : below(s.digits, digit);
-    upto += level == 5 ? s.digits.mass[digit] : below(s.digits, digit);
-    prefix |= (uint64_t)digit << shift;
+    const uint32_t ahead = digit > 0 ? s.digits.count[digit - 1] : 0;
+    left = (int)(s.digits.count[digit] - ahead);
+    t -= by_count ? (uint64_t)ahead : below(s.digits, digit);
+    upto += below(s.digits, digit);
+    prefix |= (uint64_t)digit << next;
+    shift = next;
+    __syncthreads();
+  }
+  if (threadIdx.x < kWave) {
+    const int lane = threadIdx.x;
+    uint64_t k = lane < left ? s.list[lane] : ~0ull;
+    for (int span = 2; span / 2 < left; span <<= 1) {         // bitonic, over as many lanes as there are entries
+      for (int step = span >> 1; step > 0; step >>= 1) {
+        const uint64_t other = __shfl_xor((unsigned long long)k, step, kWave);
+        k = ((lane & step) == 0) == ((lane & span) == 0) ? min(k, other) : max(k, other);
+      }
+    }
+    const uint64_t sum = wave_scan_u64(lane < left ? whole(entry_mass(key_logit<DT>(k), top, r)) : 0);
+    const uint64_t over = __ballot(lane < left && (by_count ? (uint64_t)lane : sum) >= t + (by_count ? 0 : 1));
+    if (lane == (over ? __ffsll((unsigned long long)over) - 1 : max(left - 1, 0))) {
+      s.key = k;
+      s.upto = upto + sum;
+    }
   }
   __syncthreads();
-  return Found{prefix, upto};
+  return Found{s.key, s.upto};
 }
 
-// The row's token from the scanned bins and, where they fit, the candidates (n > kCandidates: they do not).
-template <int DT>
-__device__ void draw_row(SampleShared& s, const SampleArgs& a, int row_index, const void* row, float top, const RowRule& r, bool by_k, bool by_p,
-                         uint64_t min_p_mass, int n) {
-  const bool listed = n <= kCandidates;
-  if (listed) order_candidates(s, n, top, r);
-  auto find = [&](bool by_count, uint64_t t) {
-    return listed ? find_ordered(s, n, by_count, t, top, r) : find_in_row<DT>(s, row, a.vocab, by_count, t, top, r);
-  };
-  uint64_t z = s.bins.mass[kBins - 1];
-  if (by_k) z = find(true, (uint32_t)r.k - 1).upto;
-  if (by_p) z = find(false, top_p_goal(r.p, z)).upto;
-  z = min(z, min_p_mass);
-  const Found drawn = find(false, draw_goal(r.u, z));
+// The row's token from the scanned bins and the candidates (`n` of them, or more than `most`: then from the row itself).
+template <int DT, int THREADS>
+__device__ void draw_row(Search& s, const Hist& bins, const uint64_t* keys, int n, int most, const SampleArgs& a, int row_index, const void* row,
+                         const RowTop& top, const RowRule& r, bool by_k, bool by_p, uint64_t min_p_mass) {
+  uint64_t z = bins.mass[kBins - 1];
+  Found found{};
+#pragma unroll 1
+  for (int which = by_k ? 0 : by_p ? 1 : 2; which < 3; which += which == 0 && !by_p ? 2 : 1) {       // (one copy of the search in the code)
+    if (which == 2 && r.min_p > 0.0) z = min(z, min_p_mass);
+    const uint64_t t = which == 0 ? (uint32_t)r.k - 1 : which == 1 ? top_p_goal(r.p, z) : draw_goal(r.u, z);
+    found = find_entry<DT, THREADS>(s, bins, which == 0, t, top, r, n <= most ? n : a.vocab, [&](auto f) {
+      if (n <= most) {
+        for (int i = threadIdx.x; i < n; i += THREADS) f(keys[i]);
+      } else {
+        each_entry<DT, THREADS>(row, 0, a.vocab, [&](float l, int i) {
+          if (entry_distance(l, top, r) < kReach) f(order_key<DT>(l, i));
+        });
+      }
+    });
+    if (which < 2) z = found.upto;
+  }
   if (threadIdx.x == 0) {
-    a.tokens[row_index] = (int64_t)(uint32_t)drawn.key;
-    a.probs[row_index] = (float)(entry_mass(key_logit(drawn.key), top, r) / (double)z);
+    a.tokens[row_index] = (int64_t)(found.key & 0xfffff);
+    a.probs[row_index] = (float)(entry_mass(key_logit<DT>(found.key), top, r) / (double)z);
   }
 }
 __device__ __forceinline__ void nothing_to_draw(const SampleArgs& a, int row_index) {
@@ -414,7 +503,6 @@ __device__ __forceinline__ void nothing_to_draw(const SampleArgs& a, int row_ind
   }
 }
 
-__device__ __forceinline__ float larger(float m, float l) { return l > m ? l : m; }      // a NaN never is
 template <int DT>
 __device__ __forceinline__ const void* row_of(const SampleArgs& a, int row_index) {
   return (const char*)a.logits + (int64_t)row_index * a.row_stride * Elem<DT>::kBytes;
@@ -423,28 +511,31 @@ __device__ __forceinline__ const void* row_of(const SampleArgs& a, int row_index
 // One workgroup a row, the row read three times: the largest, the bins, the entries of the bins that matter.
 template <int DT>
 __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a) {
-  __shared__ SampleShared s;
+  __shared__ Hist bins;
+  __shared__ Search s;
+  __shared__ uint64_t keys[kCandidates];
+  __shared__ float scratch[kSampleThreads / kWave];
+  __shared__ unsigned long long min_p_mass;
+  __shared__ int n;
   const int row_index = blockIdx.x;
   const void* row = row_of<DT>(a, row_index);
   const RowRule r = row_rule(a, row_index);
-  float top = -INFINITY;
-  each_entry<DT, kSampleThreads>(row, 0, a.vocab, [&](float l, int) { top = larger(top, l); });
-  top = block_max<kSampleThreads>(top, s.scratch);
-  if (top == -INFINITY) return nothing_to_draw(a, row_index);              // (uniform)
-  clear_hist<kSampleThreads>(s.bins);
+  const RowTop top = row_top_of(block_max<kSampleThreads>(part_top<DT, kSampleThreads>(row, 0, a.vocab), scratch), r);
+  if (top.value == -INFINITY) return nothing_to_draw(a, row_index);              // (uniform)
+  clear_hist<kSampleThreads>(bins);
   if (threadIdx.x == 0) {
-    s.min_p_mass = 0;
-    s.n_candidates = 0;
+    min_p_mass = 0;
+    n = 0;
   }
   __syncthreads();
-  const uint64_t kept = wave_scan_u64(fill_bins<DT, kSampleThreads>(s.bins, row, 0, a.vocab, a.vocab, top, r));
-  if ((threadIdx.x & (kWave - 1)) == kWave - 1) atomicAdd(&s.min_p_mass, (unsigned long long)kept);
+  const uint64_t kept = wave_scan_u64(fill_bins<DT, kSampleThreads>(bins, row, 0, a.vocab, a.vocab, top, r));
+  if ((threadIdx.x & (kWave - 1)) == kWave - 1) atomicAdd(&min_p_mass, (unsigned long long)kept);
   __syncthreads();
-  scan_bins<kSampleThreads>(s.bins, s.wave_mass, s.wave_count);
-  const BinRanges g = bin_ranges(s.bins, s.min_p_mass, r);
-  gather<DT, kSampleThreads>(s.c.key, kCandidates, &s.n_candidates, row, 0, a.vocab, top, r, g);
+  scan_bins<kSampleThreads>(bins, s.wave_mass, s.wave_count);
+  const BinRanges g = bin_ranges(bins, min_p_mass, r);
+  gather<DT, kSampleThreads>(keys, kCandidates, &n, row, 0, a.vocab, top, r, g);
   __syncthreads();
-  draw_row<DT>(s, a, row_index, row, top, r, g.by_k, g.by_p, s.min_p_mass, s.n_candidates);
+  draw_row<DT, kSampleThreads>(s, bins, keys, n, kCandidates, a, row_index, row, top, r, g.by_k, g.by_p, min_p_mass);
 }
 
 // Few long rows: a row is cut into slices so that all compute units have a part of one, and the steps are launches: the slices' largest; their
@@ -477,10 +568,8 @@ template <int DT>
 __global__ __launch_bounds__(kSliceThreads) void sample_top_kernel(SampleArgs a, SliceArgs c) {
   __shared__ float scratch[kSliceThreads / kWave];
   const int row_index = blockIdx.x / c.count, slice = blockIdx.x % c.count;
-  float top = -INFINITY;
-  each_entry<DT, kSliceThreads>(row_of<DT>(a, row_index), slice * c.length, min((slice + 1) * c.length, a.vocab),
-                                [&](float l, int) { top = larger(top, l); });
-  top = block_max<kSliceThreads>(top, scratch);
+  const float top = block_max<kSliceThreads>(
+      part_top<DT, kSliceThreads>(row_of<DT>(a, row_index), slice * c.length, min((slice + 1) * c.length, a.vocab)), scratch);
   if (threadIdx.x == 0) c.slices[blockIdx.x].top = top;
 }
 
@@ -493,7 +582,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_bins_kernel(SampleArgs a
   clear_hist<kSliceThreads>(h);
   if (threadIdx.x == 0) min_p_mass = 0;
   const RowRule r = row_rule(a, row_index);
-  const float top = row_top<kSliceThreads>(c, row_index, scratch);          // (its barriers also stand between the clearing and the sums)
+  const RowTop top = row_top_of(row_top<kSliceThreads>(c, row_index, scratch), r);          // (its barriers also stand between the clearing and the sums)
   const uint64_t kept = wave_scan_u64(fill_bins<DT, kSliceThreads>(h, row_of<DT>(a, row_index), slice * c.length,
                                                                    min((slice + 1) * c.length, a.vocab), a.vocab, top, r));
   if ((threadIdx.x & (kWave - 1)) == kWave - 1) atomicAdd(&min_p_mass, (unsigned long long)kept);
@@ -517,21 +606,33 @@ __global__ __launch_bounds__(kSliceThreads) void sample_gather_kernel(SampleArgs
   if (threadIdx.x == 0) n = 0;
   const RowRule r = row_rule(a, row_index);
   const SliceRecord* of = c.slices + (int64_t)row_index * c.count;
-  const float top = row_top<kSliceThreads>(c, row_index, scratch);
-  if (top == -INFINITY) return;                                             // (uniform) the last launch says so
-  for (int i = threadIdx.x; i < kBins; i += kSliceThreads) {
-    uint64_t m = 0;
-    uint32_t k = 0;
-#pragma unroll 8
-    for (int j = 0; j < c.count; ++j) {
-      m += of[j].bins.mass[i];
-      k += of[j].bins.count[i];
-    }
-    h.mass[i] = m;
-    h.count[i] = k;
+  const int lane = threadIdx.x & (kWave - 1);
+  uint64_t kept = lane < c.count ? of[lane].min_p_mass : 0;                                  // (at most 32 slices)
+  const RowTop top = row_top_of(row_top<kSliceThreads>(c, row_index, scratch), r);
+  if (top.value == -INFINITY) return;                                             // (uniform) the last launch says so
+  static_assert(kBins == 2 * kSliceThreads, "a thread adds up two bins");
+  const int i2 = threadIdx.x * 2;
+  uint64_t m0 = 0, m1 = 0;
+#pragma unroll 16
+  for (int j = 0; j < c.count; ++j) {
+    const ulonglong2 m = *(const ulonglong2*)&of[j].bins.mass[i2];
+    m0 += m.x;
+    m1 += m.y;
   }
-  uint64_t kept = 0;
-  for (int j = 0; j < c.count; ++j) kept += of[j].min_p_mass;
+  h.mass[i2] = m0;
+  h.mass[i2 + 1] = m1;
+  uint32_t k0 = 0, k1 = 0;
+  if (r.k < a.vocab) {
+#pragma unroll 16
+    for (int j = 0; j < c.count; ++j) {
+      const uint2 k = *(const uint2*)&of[j].bins.count[i2];
+      k0 += k.x;
+      k1 += k.y;
+    }
+  }
+  h.count[i2] = k0;
+  h.count[i2 + 1] = k1;
+  kept = __shfl((unsigned long long)wave_scan_u64(kept), kWave - 1, kWave);
   __syncthreads();
   scan_bins<kSliceThreads>(h, wave_mass, wave_count);
   const BinRanges g = bin_ranges(h, kept, r);
@@ -554,37 +655,42 @@ __global__ __launch_bounds__(kSliceThreads) void sample_gather_kernel(SampleArgs
 }
 
 template <int DT>
-__global__ __launch_bounds__(kSampleThreads) void sample_draw_kernel(SampleArgs a, SliceArgs c) {
-  __shared__ SampleShared s;
+__global__ __launch_bounds__(kSliceThreads) void sample_draw_kernel(SampleArgs a, SliceArgs c) {
+  __shared__ Hist bins;
+  __shared__ Search s;
+  __shared__ uint64_t keys[kCandidates];
+  __shared__ float scratch[kSliceThreads / kWave];
   const int row_index = blockIdx.x;
   const RowRule r = row_rule(a, row_index);
   const SliceRecord* of = c.slices + (int64_t)row_index * c.count;
-  const float top = row_top<kSampleThreads>(c, row_index, s.scratch);
-  if (top == -INFINITY) return nothing_to_draw(a, row_index);               // (uniform)
   const RowRecord& rec = c.rows[row_index];
-  for (int i = threadIdx.x; i < kBins; i += kSampleThreads) {
-    s.bins.mass[i] = rec.bins.mass[i];
-    s.bins.count[i] = rec.bins.count[i];
-  }
-  int n = 0;
-  bool whole_list = true;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
-  for (int j = 0; j < c.count; ++j) {                                       // a wavefront a slice
-    const int some = of[j].n_candidates;
-    whole_list = whole_list && some <= kSliceCandidates && n + some <= kCandidates;
-    if (whole_list && j % (kSampleThreads / kWave) == wave)
-      for (int i = lane; i < some; i += kWave) s.c.key[n + i] = of[j].key[i];
-    n += some;
+  const int some = lane < c.count ? of[lane].n_candidates : 0;                               // (at most 32 slices)
+  const RowTop top = row_top_of(row_top<kSliceThreads>(c, row_index, scratch), r);
+  if (top.value == -INFINITY) return nothing_to_draw(a, row_index);               // (uniform)
+  for (int i = threadIdx.x; i < kBins; i += kSliceThreads) {
+    bins.mass[i] = rec.bins.mass[i];
+    bins.count[i] = rec.bins.count[i];
+  }
+  const int upto = (int)wave_scan_u32((uint32_t)some), n = __shfl(upto, kWave - 1, kWave);
+  const bool all = !__any(some > kSliceCandidates) && n <= kCandidates;
+  if (all) {
+    for (int j = wave; j < c.count; j += kSliceThreads / kWave) {                            // a wavefront a slice
+      const int to = __shfl(upto, j, kWave), len = __shfl(some, j, kWave);
+      for (int i = lane; i < len; i += kWave) keys[to - len + i] = of[j].key[i];
+    }
   }
   __syncthreads();
-  draw_row<DT>(s, a, row_index, row_of<DT>(a, row_index), top, r, rec.by_k, rec.by_p, rec.min_p_mass, whole_list ? n : kCandidates + 1);
+  draw_row<DT, kSliceThreads>(s, bins, keys, all ? n : 1, all ? kCandidates : 0, a, row_index, row_of<DT>(a, row_index), top, r, rec.by_k, rec.by_p,
+                              rec.min_p_mass);
 }
 
-// Slices a row is cut into: as many as give every compute unit two, of 4096 entries and more, 32 at most (each adds up the bins of all); 1:
-// the row stays whole, which is one launch in the place of four.
+// Slices a row is cut into; 1: the row stays whole, which is one launch in the place of four.  More slices shorten the two passes over the row, but
+// each adds up the bins of all for itself.  1 / 4 / 8 / 16 / 32 slices, us: one row of 152064 fp32 93 55 41 34 33, 16 rows bf16 88 54 45 40 46, 64 90 58 58
+// 59 78, 128 94 76 81 89 124, 256 100 109 124 140 213; one row of 32000 31 29 28 26 -, 64 38 36 43 48 -; one of 16384 21 24 24 - -.
 static int sample_slices(int64_t rows, int64_t vocab) {
-  if (vocab < 16384 || rows >= 512) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / rows, 32), vocab / 4096));
+  if (vocab < 24576 || rows >= 192) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / rows, 16), vocab / (rows <= 8 ? 2048 : 8192)));
 }
 
 }  // namespace subspec
@@ -634,7 +740,7 @@ extern "C" int subspec_sample_filtered(const void* logits, int dtype, int64_t ro
         hipLaunchKernelGGL(sample_bins_kernel<DT>, slices, dim3(kSliceThreads), 0, st, a, c);                              \
       }                                                                                                                    \
       hipLaunchKernelGGL(sample_gather_kernel<DT>, slices, dim3(kSliceThreads), 0, st, a, c);                              \
-      hipLaunchKernelGGL(sample_draw_kernel<DT>, grid, dim3(kSampleThreads), 0, st, a, c);                                 \
+      hipLaunchKernelGGL(sample_draw_kernel<DT>, grid, dim3(kSliceThreads), 0, st, a, c);                                  \
     }                                                                                                                      \
   } while (0)
   if (dtype == SUBSPEC_F32) SUBSPEC_SAMPLE(SUBSPEC_F32);
