@@ -39,17 +39,17 @@ template <int D> struct TileShape {
   static __device__ __forceinline__ int v_swap(int row) { return D == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1); }
 };
 
-// The copies of a wavefront's rows of one block, lane addresses and the rows' place in the stage.
-template <int D> struct TileCopy {
-  const char* k[TileShape<D>::kCopies];
-  const char* v[TileShape<D>::kCopies];
-  uint32_t at;                                                         // K; V kVRing behind
+// The copies of a wavefront's eight rows of one block.  In one page: a scalar address and the lane's offset in the rows.  (The address comes out of
+// scalar instructions and has its five wait states behind them.)
+struct TileCopy {
+  const char* k;                                                       // the first row's K
+  const char* v;
+  uint32_t at;                                                         // place in the stage; V's is kVRing behind
+  int block;                                                           // of the chunk
+  bool one_page;
 };
-template <int D>
-__device__ __forceinline__ void issue_copy(const TileCopy<D>& cp, int c) {
-  constexpr int n = TileShape<D>::kCopies;
-  if (c < n) dma16_from(cp.at + c * 1024, cp.k[c < n ? c : 0]);
-  else dma16_from(cp.at + TileShape<D>::kVRing + (c - n) * 1024, cp.v[c >= n ? c - n : 0]);
+__device__ __forceinline__ void dma16_row(uint32_t lds_base, uint32_t offset, const char* base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_base), "v"(offset), "s"(base) : "memory", "m0");
 }
 template <int D>
 __device__ __forceinline__ void wait_block() { wait_vmcnt<2 * TileShape<D>::kCopies>(); }     // all but the newest block's copies
@@ -72,11 +72,12 @@ __device__ __forceinline__ dec_u4 load_step(int k, const uint32_t (&kaddr)[D / 1
   }
   return lds_16(kaddr[j >> 1] + (uint32_t)((j & 1) * 32 * S::kRowBytes));
 }
-template <int DT, int D, int MODE>
-__device__ __forceinline__ void matrix_phase(const TileAddress& ad, const TileCopy<D>& cp, bool copy, v16f (&o)[D / 32], v16f (&s)[2],
-                                             const v16f& cinit, const dec_u4 (&pb)[4], const dec_u4 (&q)[D / 16]) {
+// between(k) is what else the phase does behind step k.
+template <int DT, int D, int MODE, typename Between>
+__device__ __forceinline__ void matrix_phase(const TileAddress& ad, v16f (&o)[D / 32], v16f (&s)[2], const v16f& cinit, const dec_u4 (&pb)[4],
+                                             const dec_u4 (&q)[D / 16], Between between) {
   using S = TileShape<D>;
-  constexpr int kOne = 2 * S::kKSteps, kSteps = MODE == 2 ? 2 * kOne : kOne, kAhead = 4, kEach = kSteps / (2 * S::kCopies);
+  constexpr int kOne = 2 * S::kKSteps, kSteps = MODE == 2 ? 2 * kOne : kOne, kAhead = 4;
   __builtin_amdgcn_s_setprio(1);                                       // the wavefront that multiplies goes first
   uint32_t kaddr[S::kKSteps], vaddr[S::kDTiles];
   if (MODE != 1) {
@@ -103,7 +104,7 @@ __device__ __forceinline__ void matrix_phase(const TileAddress& ad, const TileCo
     }
     __builtin_amdgcn_sched_barrier(0);
     if (k + kAhead < kSteps) ring[k % kAhead] = load_step<D, MODE>(k + kAhead, kaddr, vaddr);
-    if (k % kEach == 1 && copy) issue_copy<D>(cp, k / kEach);          // (uniform)
+    between(k, kSteps);
     __builtin_amdgcn_sched_barrier(0);
   }
   __builtin_amdgcn_s_setprio(0);
@@ -254,47 +255,77 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int64_t tok_bytes = (int64_t)p.hkv * S::kRowBytes, page_bytes = p.page_elems * 2;
   const char* kbase = (const char*)(p.pool + kvh * D);
   const int tok_mask = (1 << p.page_shift) - 1;
-  // lane offsets of the wavefront's copies inside a page whose rows are wave * 8 ..
-  uint32_t kpiece[S::kCopies], vpiece[S::kCopies];
+  // lane offsets of the wavefront's copies from its first row's
+  uint32_t kfrom[S::kCopies], vfrom[S::kCopies];
 #pragma unroll
   for (int c = 0; c < S::kCopies; ++c) {
-    const int in = wave * 8 + c * S::kRowsPerCopy + crow;
-    kpiece[c] = (uint32_t)((cpiece ^ S::k_swap(in)) << 4);
-    vpiece[c] = (uint32_t)((cpiece ^ S::v_swap(in)) << 4);
+    const int in = c * S::kRowsPerCopy + crow;
+    kfrom[c] = (uint32_t)(in * (int)tok_bytes) + (uint32_t)((cpiece ^ S::k_swap(wave * 8 + in)) << 4);
+    vfrom[c] = (uint32_t)(in * (int)tok_bytes) + (uint32_t)((cpiece ^ S::v_swap(wave * 8 + in)) << 4);
   }
-  TileCopy<D> cp;
-  // block J of the chunk -> stage J % 4; blocks past the last repeat it (every wavefront's count of copies is the same on every path)
+  TileCopy cp;
+  int asked = 0;
+  // The next copies are those of block J -> stage J % 4; blocks past the last repeat it (every wavefront's count of copies is the same on every
+  // path).  ask() reads the page number that plan() uses a few products later.
+  auto place = [&](int J, int* v, int* j, int* shift) {
+    *v = v0 + min(J, nb - 1) * kTileKeys + wave * 8;                   // the wavefront's eight keys
+    *j = paged_real(sp, *v);
+    *shift = *v < sp.skip ? -base1 : count1 - base2;                   // page number of key j: pages[(j >> page_shift) + shift]
+  };
+  auto ask = [&](int J) {
+    int v, j, shift;
+    place(J, &v, &j, &shift);
+    asked = pages[(j >> p.page_shift) + shift];
+  };
   auto plan = [&](int J) {
-    const int Jc = min(J, nb - 1);
-    const int v = v0 + Jc * kTileKeys + wave * 8, j = paged_real(sp, v);          // the wavefront's eight keys
-    const int shift = v < sp.skip ? -base1 : count1 - base2;                      // page number of key j: pages[(j >> page_shift) + shift]
+    int v, j, shift;
+    place(J, &v, &j, &shift);
+    cp.block = J;
     cp.at = lds0 + (uint32_t)(J & (kStages - 1)) * S::kHalf + (uint32_t)(wave * 8 * S::kRowBytes);
-    if (p.page_shift >= 3 && j + 7 <= tp.pos_hi && (j >= sp.low || j + 7 < p.sinks)) {
-      const int page = __builtin_amdgcn_readfirstlane(pages[(j >> p.page_shift) + shift]);
-      const char* at = kbase + (int64_t)page * 2 * page_bytes + (j & tok_mask) * tok_bytes;
+    cp.one_page = p.page_shift >= 3 && j + 7 <= tp.pos_hi && (j >= sp.low || j + 7 < p.sinks);
+    cp.k = kbase + (int64_t)__builtin_amdgcn_readfirstlane(asked) * 2 * page_bytes + (j & tok_mask) * tok_bytes;
+    cp.v = cp.k + page_bytes;
+  };
+  auto copy_one = [&](int c) {                                         // c: K's, then V's
+    if (c < S::kCopies) dma16_row(cp.at + c * 1024, kfrom[c < S::kCopies ? c : 0], cp.k);
+    else dma16_row(cp.at + S::kVRing + (c - S::kCopies) * 1024, vfrom[c < S::kCopies ? 0 : c - S::kCopies], cp.v);
+  };
+  // small pages, the end of the keys, the gap: row by row.  A key that no row sees stands for one that some row does, what it holds must not reach
+  // a product, not even multiplied by zero.
+  auto copy_rows = [&]() {
+    int v, j, shift;
+    place(cp.block, &v, &j, &shift);
+    int self = lane;
+    asm volatile("" : "+v"(self));                                     // (what follows from the lane is worked out here, not kept for the whole loop)
+    const int crow = self / S::kPieces, cpiece = self % S::kPieces;
 #pragma unroll
-      for (int c = 0; c < S::kCopies; ++c) {
-        const int64_t in = (c * S::kRowsPerCopy + crow) * tok_bytes;
-        cp.k[c] = at + (in + kpiece[c]);
-        cp.v[c] = at + page_bytes + (in + vpiece[c]);
-      }
-    } else {
-      // small pages, the end of the keys, the gap: a key that no row sees stands for one that some row does, what it holds must not reach
-      // a product, not even multiplied by zero
-#pragma unroll
-      for (int c = 0; c < S::kCopies; ++c) {
-        int key = j + c * S::kRowsPerCopy + crow;
-        if (v < sp.skip) key = min(key, p.sinks - 1);
-        else key = min(key >= p.sinks ? max(key, sp.low) : key, tp.pos_hi);
-        const char* at = kbase + (int64_t)pages[(key >> p.page_shift) + shift] * 2 * page_bytes + (key & tok_mask) * tok_bytes;
-        cp.k[c] = at + kpiece[c];
-        cp.v[c] = at + page_bytes + vpiece[c];
-      }
+    for (int c = 0; c < S::kCopies; ++c) {
+      const int in = c * S::kRowsPerCopy + crow;
+      int key = j + in;
+      if (v < sp.skip) key = min(key, p.sinks - 1);
+      else key = min(key >= p.sinks ? max(key, sp.low) : key, tp.pos_hi);
+      const char* at = kbase + (int64_t)pages[(key >> p.page_shift) + shift] * 2 * page_bytes + (key & tok_mask) * tok_bytes;
+      dma16_from(cp.at + c * 1024, at + ((cpiece ^ S::k_swap(wave * 8 + in)) << 4));
+      dma16_from(cp.at + S::kVRing + c * 1024, at + page_bytes + ((cpiece ^ S::v_swap(wave * 8 + in)) << 4));
     }
   };
-  auto issue_all = [&]() {
+  auto copy_all = [&]() {
+    if (cp.one_page) {
 #pragma unroll
-    for (int c = 0; c < 2 * S::kCopies; ++c) issue_copy<D>(cp, c);
+      for (int c = 0; c < 2 * S::kCopies; ++c) copy_one(c);
+    } else {
+      copy_rows();
+    }
+  };
+  // behind step k of an M phase: a copy every so many steps, then what the next ones need
+  auto between = [&](int J, int k, int steps) {
+    const int each = steps / (2 * S::kCopies);
+    if (k % each == 1 && cp.one_page) copy_one(k / each);
+    if (k == 2) ask(J);
+    if (k == steps - each + 2) {
+      if (!cp.one_page) copy_rows();
+      plan(J);
+    }
   };
   // operand addresses inside a stage.  K: key 32 t + lr, piece 2 ks + g.  V^T: of 16 lanes, lane i supplies the 8 bytes of key 4 g + i / 4 at
   // d = 32 dt + 16 h + 4 (i % 4)
@@ -315,19 +346,24 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
 
   if (nb > 0) {
+    ask(0);
     plan(0);
-    issue_all();
+    copy_all();
+    ask(1);
     plan(1);
-    issue_all();
+    copy_all();
+    ask(2);
+    plan(2);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (second) __syncthreads();
-    plan(2);
     if (live) {
       stages(0);
-      matrix_phase<DT, D, 0>(ad, cp, true, o, s, cinit, pb, q);
+      matrix_phase<DT, D, 0>(ad, o, s, cinit, pb, q, [&](int k, int steps) { between(3, k, steps); });
     } else {
-      issue_all();
+      copy_all();
+      ask(3);
+      plan(3);
     }
     if (second) wait_block<D>();
     __syncthreads();
@@ -335,12 +371,13 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if (!second) wait_block<D>();
     __syncthreads();
     for (int i = 1; i < nb; ++i) {
-      plan(i + 2);
       if (live) {
         stages(i);
-        matrix_phase<DT, D, 2>(ad, cp, true, o, s, cinit, pb, q);
+        matrix_phase<DT, D, 2>(ad, o, s, cinit, pb, q, [&](int k, int steps) { between(i + 3, k, steps); });
       } else {
-        issue_all();
+        copy_all();
+        ask(i + 3);
+        plan(i + 3);
       }
       if (second) wait_block<D>();
       __syncthreads();
@@ -350,7 +387,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     if (live) {
       stages(nb);
-      matrix_phase<DT, D, 1>(ad, cp, false, o, s, cinit, pb, q);
+      matrix_phase<DT, D, 1>(ad, o, s, cinit, pb, q, [](int, int) {});
     }
     __syncthreads();
     if (!second) __syncthreads();

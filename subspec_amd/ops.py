@@ -454,7 +454,11 @@ def paged_batch_plan(kv_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: 
         raise ValueError("n_tokens must not be negative")
     sizes = (batch + 1, batch, n_tokens, n_tokens, n_tokens, 4)
     if out is None:
-        out = {key: torch.empty(n, dtype=dtype, device=dev) for (key, dtype), n in zip(_PLAN_OUT, sizes)}
+        # one allocation: six of them took 8 of the call's 17 us
+        slots, starts, lens, positions, sequences, counts = torch.empty(
+            4 * n_tokens + 2 * batch + 5, dtype=torch.int32, device=dev).split_with_sizes((2 * n_tokens, *sizes[:3], n_tokens, 4))
+        out = {"query_starts": starts, "kv_lens": lens, "positions": positions, "slots": slots.view(torch.int64), "sequences": sequences,
+               "counts": counts}
     else:
         for (key, dtype), n in zip(_PLAN_OUT, sizes):
             t = out[key]
