@@ -272,6 +272,26 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
       make_uint2(pack2<DT>(num[0] * inv, num[1] * inv), pack2<DT>(num[2] * inv, num[3] * inv));
 }
 
+// Chunks of `blocks` key blocks each for `units` (tile, KV head) pairs.  In blocks (1.6 us): a compute unit takes one workgroup at a time, whose start and
+// end cost about three; a launch for the merge two and 0.4 for every chunk that it adds up; a chunk's partial results, 128 KB out and back, a
+// thirtieth.  Both launches at 1 / 2 / 3 / 4 / 5 / 8 / 16 chunks, 28 : 4 heads, us: 512 tokens behind 4096 rows (56 pairs, 72 blocks) 121 73 56 50 69 62 88,
+// 33 behind 7967 (4, 125) 199 107 - 60 51 38 29, 2048 behind 6144 (224, 128) 221 243 241 247 249 298 414, four of 200 behind 2800, 32 : 8 heads (72, 47)
+// 86 58 52 60 62 68 -.
+static int64_t paged_tile_chunks(int64_t blocks, int64_t units) {
+  double best = 1e30;
+  int64_t chunks = 1;
+  for (int64_t c = 1; c <= std::min<int64_t>(blocks, 32); ++c) {
+    const int64_t per = (blocks + c - 1) / c;
+    if ((blocks + per - 1) / per != c) continue;
+    const double cost = (double)((units * c + 255) / 256) * (double)(per + 3) + (c > 1 ? 2 + 0.4 * (double)c + (double)(units * c) / 30 : 0);
+    if (cost < best) {
+      best = cost;
+      chunks = c;
+    }
+  }
+  return chunks;
+}
+
 // How a call is cut, from the bounds alone.  Keys of a row: at most max_kv, or a window's, its sinks and the row's fellow tokens'.
 struct PagedPlan { int few_rows, few_keys, few_chunks, tile_keys, tile_chunks; int64_t tiles; size_t few_o, few_ml, tile_o, tile_ml, bytes; };
 static PagedPlan paged_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64_t hkv, int64_t head_dim, int64_t page_len, int64_t max_new,
@@ -304,17 +324,7 @@ static PagedPlan paged_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64_t
   if (most > pl.few_rows) {
     pl.tiles = n_tokens * group / kTileRows + batch;
     const int64_t keys = std::max<int64_t>(1, span(std::min(max_new, kTileRows / group + 2), kTileKeys)), blocks = (keys + kTileKeys - 1) / kTileKeys;
-    // Tiles that all tokens make if none is left part empty: a compute unit takes one workgroup at a time, whose start and end cost about
-    // three blocks, and a chunk's partial results about two more.
-    const int64_t units = (n_tokens * group + kTileRows - 1) / kTileRows * hkv;
-    int64_t chunks = 1, best = INT64_MAX;
-    for (int64_t c = 1; c <= std::min<int64_t>(blocks, 64); ++c) {
-      const int64_t per = (blocks + c - 1) / c, used = (blocks + per - 1) / per, cost = (units * used + 255) / 256 * (per + 3 + (used > 1 ? 2 : 0));
-      if (used == c && cost < best) {
-        best = cost;
-        chunks = c;
-      }
-    }
+    int64_t chunks = paged_tile_chunks(blocks, (n_tokens * group + kTileRows - 1) / kTileRows * hkv);      // (tiles of all tokens, none part empty)
     while (chunks > 1 && pl.tiles * hkv * chunks > (1 << 13)) --chunks;                  // a gigabyte of partial results at 128 a head
     int64_t per = (blocks + chunks - 1) / chunks * kTileKeys;
     per = std::min(per, (kTilePages - 64) * page_len);                                   // its page numbers are in LDS (two more than the keys')

@@ -200,11 +200,11 @@ template <int DT, int D>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_tile_kernel(PagedParams p) {
   using S = TileShape<D>;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kLds];
-  // KV heads fastest: workgroups are dealt to the XCDs in turn, so that those of a KV head meet in the same L2s; the last tiles first, whose
-  // rows see the most keys
+  // KV heads fastest: workgroups are dealt to the XCDs in turn, so that those of a KV head meet in the same L2s.  The longest first: whole chunks
+  // before what is left over behind them, the last tiles, whose rows see the most keys, before the first.
   const int kvh = (int)(blockIdx.x % (uint32_t)p.hkv);
   const uint32_t rest = blockIdx.x / (uint32_t)p.hkv;
-  const int chunk = (int)(rest % (uint32_t)p.tile.chunks), u = p.tiles - 1 - (int)(rest / (uint32_t)p.tile.chunks);
+  const int chunk = (int)(rest / (uint32_t)p.tiles), u = p.tiles - 1 - (int)(rest % (uint32_t)p.tiles);
   TilePlace tp;
   if (!tile_place(p, u, &tp)) return;
   const PagedSpan sp = paged_span(p, tp.pos_lo, max(tp.pos_hi + 1, 0), kTileKeys);
