@@ -44,6 +44,21 @@ def _stream(dev: torch.device) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _call(dev: torch.device, name: str, *args) -> None:
+    """The library's ``name`` with the tensors' device current: a launch on a default stream goes to the current device."""
+    fn = getattr(L.lib(), name)
+    if _current_device() == dev.index:
+        code = fn(*args)
+    else:
+        with torch.cuda.device(dev):
+            code = fn(*args)
+    if code != 0:
+        L.check(code, name)
+
+
 _METHODS = {"exact": L.VERIFY_EXACT, "lossy": L.VERIFY_LOSSY}
 _GATES = {"entropy": L.GATE_ENTROPY, "prob": L.GATE_PROB}
 _VERIFY_OUT = (("tokens", "n", torch.int64), ("contexts", "n", torch.int64), ("counts", "counts", torch.int32),
@@ -466,11 +481,10 @@ def paged_batch_plan(kv_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: 
                 raise ValueError(f"out[{key!r}] must be a contiguous {dtype} tensor of shape ({n},) on {dev}")
         if out["kv_lens"].data_ptr() == kv_lens.data_ptr():
             raise ValueError("out['kv_lens'] must not be kv_lens itself: every workgroup reads the old lengths")
-    code = L.lib().subspec_paged_batch_plan(
-        kv_lens.data_ptr(), new_lens.data_ptr(), batch, free_pages.data_ptr(), n_free.data_ptr(), free_pages.numel(),
-        block_table.data_ptr(), max_blocks, stride, int(page_len), n_tokens, out["query_starts"].data_ptr(), out["kv_lens"].data_ptr(),
-        out["positions"].data_ptr(), out["slots"].data_ptr(), out["sequences"].data_ptr(), out["counts"].data_ptr(), _stream(dev))
-    L.check(code, "subspec_paged_batch_plan")
+    _call(dev, "subspec_paged_batch_plan", kv_lens.data_ptr(), new_lens.data_ptr(), batch, free_pages.data_ptr(), n_free.data_ptr(),
+          free_pages.numel(), block_table.data_ptr(), max_blocks, stride, int(page_len), n_tokens,
+          out["query_starts"].data_ptr(), out["kv_lens"].data_ptr(), out["positions"].data_ptr(), out["slots"].data_ptr(),
+          out["sequences"].data_ptr(), out["counts"].data_ptr(), _stream(dev))
     return out
 
 
@@ -495,10 +509,8 @@ def kv_append_paged_(pool_layer: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if k.dtype != pool_layer.dtype or v.dtype != pool_layer.dtype:
         raise ValueError("kv_append_paged_: k, v and the pool must share a dtype")
     k, v = (t if t.stride(2) == 1 or D == 1 else t.contiguous() for t in (k, v))
-    code = L.lib().subspec_kv_append_paged(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                                           pool_layer.data_ptr(), _dtype_code(pool_layer), max_pages, page_len, heads, D,
-                                           slots.data_ptr(), n, _stream(dev))
-    L.check(code, "subspec_kv_append_paged")
+    _call(dev, "subspec_kv_append_paged", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+          pool_layer.data_ptr(), _dtype_code(pool_layer), max_pages, page_len, heads, D, slots.data_ptr(), n, _stream(dev))
     return pool_layer
 
 
@@ -534,16 +546,16 @@ def paged_attention(q: torch.Tensor, pool_layer: torch.Tensor, block_table: torc
         out = torch.empty((T, Hq * D), dtype=q.dtype, device=dev)
     elif out.dtype != q.dtype or out.shape != (T, Hq * D) or not out.is_contiguous() or out.device != dev:
         raise ValueError(f"paged_attention: out must be a contiguous {q.dtype} tensor [{T}, {Hq * D}]")
-    lib = L.lib()
-    need = lib.subspec_paged_attention_workspace(batch, T, Hq, Hkv, D, page_len, max_new, max_kv, window, sinks)
+    if workspace is not None:
+        _require_gpu(q, workspace)
+    need = L.lib().subspec_paged_attention_workspace(batch, T, Hq, Hkv, D, page_len, max_new, max_kv, window, sinks)
     if workspace is None and need > 256:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    code = lib.subspec_paged_attention(
-        q.data_ptr(), q.stride(0), q.stride(1), pool_layer.data_ptr(), max_pages, page_len, block_table.data_ptr(), max_blocks, stride,
-        query_starts.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), _dtype_code(q), batch, T, Hq, Hkv, D, max_new, max_kv, window, sinks,
-        float(D ** -0.5 if scale is None else scale), None if workspace is None else workspace.data_ptr(),
-        0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(dev))
-    L.check(code, "subspec_paged_attention")
+    _call(dev, "subspec_paged_attention", q.data_ptr(), q.stride(0), q.stride(1), pool_layer.data_ptr(), max_pages, page_len,
+          block_table.data_ptr(), max_blocks, stride, query_starts.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), _dtype_code(q), batch, T,
+          Hq, Hkv, D, max_new, max_kv, window, sinks, float(D ** -0.5 if scale is None else scale),
+          None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel() * workspace.element_size(),
+          _stream(dev))
     return out
 
 
@@ -579,14 +591,11 @@ def sample_filtered(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.
         raise ValueError("sample_filtered: temperature, top_k, top_p and min_p must not be negative")
     tokens = torch.empty(rows, dtype=torch.int64, device=dev)
     probs = torch.empty(rows, dtype=torch.float32, device=dev)
-    lib = L.lib()
-    need = lib.subspec_sample_filtered_workspace(rows, V)
+    need = L.lib().subspec_sample_filtered_workspace(rows, V)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 256 else None
-    code = lib.subspec_sample_filtered(
-        logits.data_ptr(), _dtype_code(logits), rows, V, max(logits.stride(0), V), uniforms.data_ptr(), t_ptr, float(t), k_ptr,
-        min(int(k), (1 << 31) - 1), p_ptr, float(p), m_ptr, float(m), None if ws is None else ws.data_ptr(), need,
-        tokens.data_ptr(), probs.data_ptr(), _stream(dev))
-    L.check(code, "subspec_sample_filtered")
+    _call(dev, "subspec_sample_filtered", logits.data_ptr(), _dtype_code(logits), rows, V, max(logits.stride(0), V), uniforms.data_ptr(),
+          t_ptr, float(t), k_ptr, min(int(k), (1 << 31) - 1), p_ptr, float(p), m_ptr, float(m), None if ws is None else ws.data_ptr(), need,
+          tokens.data_ptr(), probs.data_ptr(), _stream(dev))
     return tokens, probs
 
 

@@ -15,7 +15,7 @@ Page bookkeeping is host-side Python, as in the reference.
 from __future__ import annotations
 
 import math
-from typing import List, Optional
+from typing import Dict, List, Optional, Sequence
 
 import torch
 
@@ -164,6 +164,83 @@ class RequestKvCache:
         table = self.page_table(max(0, offset + max(int(beam_idx.numel()), num_new_tokens) - self.kv_len))
         self.kvCachePool.reorder_cache_with_offset(beam_idx, offset, num_new_tokens, page_indices=table)
         self._set_len(offset + int(beam_idx.size(0)), allow_growth=False)
+
+
+class KvBatch:
+    """Several sequences over one ``KvCachePool``, a step at a time: what the reference's per-request page lists and
+    ``KvCacheBatchPosition`` (:9-25,218-240,350-372) are for its batched wrappers, with the page tables, the free pages and the lengths on
+    the device.  ``step`` hands out pages and slots for the new tokens of every sequence, then each layer's ``append`` and ``attention``
+    go through them:
+
+        plan = batch.step([1, 1, 130, 0])          # two sequences decode, one brings a chunk of its prompt, one rests
+        batch.append(layer, k, v)                  # k, v [tokens, kv_heads, head_dim], the sequences' new tokens one after the other
+        out = batch.attention(layer, q)            # q [tokens, heads, head_dim] -> [tokens, heads * head_dim]
+
+    The host keeps the lengths too, so running out of pages or of table columns is an error before anything is launched, and nothing waits
+    for the device."""
+
+    def __init__(self, pool: KvCachePool, max_batch: int, max_len: int, num_pages: Optional[int] = None):
+        self.pool, self.page_len, self.max_len = pool, pool.page_len, int(max_len)
+        self.pages = pool.allocate(int(pool.num_free_pages()) if num_pages is None else int(num_pages))
+        self.num_free = len(self.pages)
+        self.lens: List[int] = [0] * int(max_batch)
+        dev = pool.device
+        self.free_pages = torch.tensor(self.pages, dtype=torch.int32, device=dev)
+        self.n_free = torch.tensor([self.num_free], dtype=torch.int32, device=dev)
+        self.kv_lens = torch.zeros(int(max_batch), dtype=torch.int32, device=dev)
+        self.block_table = torch.full((int(max_batch), max(1, self._pages(self.max_len))), -1, dtype=torch.int32, device=dev)
+        self.plan: Optional[Dict[str, torch.Tensor]] = None
+        self.max_new = self.max_kv = 0
+
+    def _pages(self, rows: int) -> int:
+        return (rows + self.page_len - 1) // self.page_len
+
+    def step(self, new_lens: Sequence[int], n_tokens: Optional[int] = None) -> Dict[str, torch.Tensor]:
+        """Pages and slots for ``new_lens[b]`` new tokens of every sequence; returns the plan (``ops.paged_batch_plan``).  ``n_tokens``: rows of
+        its token outputs, default the new tokens of all sequences."""
+        new = [int(n) for n in new_lens]
+        if len(new) != len(self.lens) or min(new) < 0:
+            raise ValueError(f"expected {len(self.lens)} numbers of new tokens, none below zero")
+        total = [a + b for a, b in zip(self.lens, new)]
+        if max(total) > self.max_len:
+            raise ValueError(f"a sequence of {max(total)} rows is longer than the {self.max_len} of this batch")
+        taken = sum(self._pages(t) - self._pages(a) for a, t in zip(self.lens, total))
+        if taken > self.num_free:
+            raise ValueError(f"Out of available cache pages: asked {taken}, only {self.num_free} free pages")
+        rows = sum(new) if n_tokens is None else int(n_tokens)
+        if rows < sum(new):
+            raise ValueError(f"n_tokens={rows} is less than the {sum(new)} new tokens")
+        fresh = torch.tensor(new, dtype=torch.int32, device=self.pool.device)
+        self.plan = ops.paged_batch_plan(self.kv_lens, fresh, self.free_pages, self.n_free, self.block_table, self.page_len, rows)
+        self.kv_lens, self.n_free = self.plan["kv_lens"], self.plan["counts"][2:3]
+        self.lens, self.num_free = total, self.num_free - taken
+        self.max_new, self.max_kv = max(new), max(total)
+        return self.plan
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        ops.kv_append_paged_(self.pool.cache_data[layer], k, v, self.plan["slots"])
+
+    def attention(self, layer: int, q: torch.Tensor, window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return ops.paged_attention(q, self.pool.cache_data[layer], self.block_table, self.plan["query_starts"], self.kv_lens, self.max_new,
+                                   self.max_kv, window=window, sinks=sinks, scale=scale, out=out)
+
+    def release(self, index: int) -> None:
+        """Sequence ``index`` is done: its pages are free again and its place is empty."""
+        n = self._pages(self.lens[index])
+        self.free_pages = self.free_pages.clone()             # (a step on another stream may still read the old ones)
+        self.free_pages[self.num_free:self.num_free + n] = self.block_table[index, :n]
+        self.num_free += n
+        self.lens[index] = 0
+        self.n_free = torch.full_like(self.n_free, self.num_free)
+        self.kv_lens = self.kv_lens.clone()
+        self.kv_lens[index] = 0
+
+    def close(self) -> None:
+        """All pages go back to the pool."""
+        self.pool.deallocate(self.pages)
+        self.pages, self.num_free, self.lens = [], 0, [0] * len(self.lens)
+        self.n_free, self.kv_lens = torch.zeros_like(self.n_free), torch.zeros_like(self.kv_lens)
 
 
 class PagedKVCache:

@@ -96,3 +96,36 @@ def test_oracle_attention_window_by_hand():
     q = torch.zeros(2, 1, 2, dtype=torch.float64)
     out, _, _ = ob.attention(q, pool, table, [0, 2], [6], window=2, sinks=1)
     assert out[0, 0, 0].item() == pytest.approx((1 + 8 + 16) / 3) and out[1, 0, 0].item() == pytest.approx((1 + 16 + 32) / 3)
+
+
+def test_a_batch_refuses_before_anything_is_launched():
+    from subspec_amd.paged_cache import KvBatch, KvCachePool
+    pool = KvCachePool(max_pages=8, num_layers=1, num_heads=2, head_dim=64, page_len=4, dtype=torch.bfloat16, device="cpu")
+    batch = KvBatch(pool, 2, 40, num_pages=5)
+    assert int(pool.num_free_pages()) == 3 and batch.block_table.shape == (2, 10)
+    for bad in ([1], [1, -1], [41, 0], [12, 9]):              # a place missing, below zero, longer than the batch allows, six pages
+        with pytest.raises(ValueError):
+            batch.step(bad)
+    with pytest.raises(ValueError):
+        batch.step([3, 3], n_tokens=5)
+    assert batch.lens == [0, 0] and batch.num_free == 5
+    with pytest.raises(L.SubspecHipError):                     # the device work itself has no CPU fallback
+        batch.step([3, 3])
+    assert batch.lens == [0, 0] and batch.num_free == 5
+    batch.close()
+    assert int(pool.num_free_pages()) == 8
+
+
+@pytest.mark.parametrize("hq,hkv,D", [(28, 4, 128), (32, 32, 128), (14, 2, 64), (64, 1, 128)])
+def test_attention_workspace_holds_a_gigabyte_of_partials_at_most(hq, hkv, D):
+    size = L.lib().subspec_paged_attention_workspace
+    for batch, tokens, new in [(1, 1, 1), (64, 64, 1), (4096, 4096, 1), (1, 4096, 4096), (4096, 60000, 3000), (300, 5000, 40)]:
+        for kv in (1, 100, 4096, 131072, 1 << 20):
+            for page_len in (1, 16):
+                n = size(batch, tokens, hq, hkv, D, page_len, new, kv, 0, 0)
+                most = (1 << 30) + (1 << 26)
+                tiles = tokens * (hq // hkv) // 256 + batch
+                # pages of one row cut the keys at 4032 whatever it costs
+                cut = tiles * hkv * -(-kv // 4032) * 256 * (D + 2) * 4 if page_len == 1 and new * (hq // hkv) > 16 else 0
+                assert 256 <= n <= most * 2 + cut
+    assert size(1, 1, hq, hkv, D, 16, 1, 64, 0, 0) == 256       # one chunk: nothing to keep

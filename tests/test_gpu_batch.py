@@ -155,3 +155,254 @@ def test_attention(dtype, Hq, Hkv, D, lens, page_len, window, sinks):
     off = (got - want).abs()
     assert torch.isfinite(got).all().item()
     assert (off / tol).max().item() <= 1.0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_bounds_need_not_be_tight_and_rows_behind_the_last_sequence_stay(dtype):
+    g = torch.Generator().manual_seed(11)
+    lens = [(77, 1), (40, 40), (3, 5), (0, 0)]                             # the third brings more rows than it has: its first two see none
+    q, pool, table, starts, kv = _batch(g, lens, 16, 7, 1, 128, dtype)
+    q = torch.cat([q, torch.full((9, 7, 128), float("nan"), dtype=dtype)])
+    want, weight, worst = ob.attention(q, pool, table, starts, kv)
+    out = torch.full((q.shape[0], 7 * 128), 5.0, dtype=dtype, device=DEV)
+    got = ops.paged_attention(q.to(DEV), pool.to(DEV), _i32(table), _i32(starts), _i32(kv), 1000, 5 * 16 + 3000, out=out)
+    assert got.data_ptr() == out.data_ptr() and out[-9:].eq(5.0).all()
+    tol = _tolerance(want, weight, worst, dtype, max(kv), float(pool.nan_to_num(0.0).abs().max()), 128)[:-9]
+    off = (got.double().cpu().view(want.shape) - want).abs()[:-9]
+    assert (off / tol).max().item() <= 1.0 and got[starts[2]:starts[2] + 2].eq(0).all()
+    # bounds below what is there leave rows out and stay inside every tensor
+    cut = ops.paged_attention(q.to(DEV), pool.to(DEV), _i32(table), _i32(starts), _i32(kv), 2, 20, out=torch.full_like(out, 6.0))
+    assert cut[starts[1] + 2:starts[2]].eq(6.0).all() and cut[-9:].eq(6.0).all()
+
+
+def test_attention_reads_strided_queries_and_clamps_bad_tables():
+    g = torch.Generator().manual_seed(12)
+    lens = [(50, 1), (30, 12)]
+    q, pool, table, starts, kv = _batch(g, lens, 8, 4, 2, 64, torch.float16)
+    args = (pool.to(DEV), _i32(table), _i32(starts), _i32(kv), 12, 50)
+    plain = ops.paged_attention(q.to(DEV), *args)
+    fused = torch.zeros(q.shape[0], 8, 64, dtype=torch.float16)
+    fused[:, 2:6] = q
+    assert torch.equal(ops.paged_attention(fused.to(DEV)[:, 2:6], *args), plain)
+    assert torch.equal(ops.paged_attention(q.transpose(0, 1).contiguous().to(DEV).transpose(0, 1), *args), plain)
+    odd = torch.zeros(q.shape[0], 4 * 64 + 1, dtype=torch.float16)
+    odd[:, 1:] = q.reshape(q.shape[0], -1)
+    assert torch.equal(ops.paged_attention(odd.to(DEV)[:, 1:].view(-1, 4, 64), *args), plain)
+    wide = torch.cat([_i32(table), _i32([[-5] * 3] * 2)], 1)[:, :len(table[0])]     # a view with a longer row stride
+    assert torch.equal(ops.paged_attention(q.to(DEV), pool.to(DEV), wide, *args[2:]), plain)
+    bad = _i32([[(1 << 30) if i % 2 else -9 for i in range(len(table[0]))]] * 2)    # numbers outside the pool: other rows, no fault
+    assert ops.paged_attention(q.to(DEV), pool.nan_to_num(0.0).to(DEV), bad, *args[2:]).isfinite().all()
+
+
+def test_argument_errors():
+    pool = torch.zeros(6, 2, 16, 2, 128, dtype=torch.bfloat16, device=DEV)
+    q = torch.zeros(3, 4, 128, dtype=torch.bfloat16, device=DEV)
+    table, starts, lens = _i32([[0, 1]]), _i32([0, 3]), _i32([20])
+    ops.paged_attention(q, pool, table, starts, lens, 3, 32)
+    for bad in [dict(q=q.float()), dict(q=q[:, :3]), dict(q=q[:, :, :64]), dict(table=table.long()), dict(table=table[0]), dict(starts=_i32([0])),
+                dict(lens=lens.long()), dict(max_new=-1), dict(window=-3), dict(sinks=4), dict(out=q.view(3, -1).float()),
+                dict(pool=pool[:, :1]), dict(workspace=torch.zeros(16, dtype=torch.uint8, device=DEV), max_kv=4096), dict(scale=0.0)]:
+        a = dict(q=q, pool=pool, table=table, starts=starts, lens=lens, max_new=3, max_kv=32)
+        a.update(bad)
+        with pytest.raises((ValueError, L.SubspecHipError)):
+            ops.paged_attention(a.pop("q"), a.pop("pool"), a.pop("table"), a.pop("starts"), a.pop("lens"), a.pop("max_new"), a.pop("max_kv"), **a)
+    k = torch.zeros(3, 2, 128, dtype=torch.bfloat16, device=DEV)
+    slots = torch.arange(3, device=DEV)
+    for bad in [(pool, k.float(), k, slots), (pool, k[:2], k, slots), (pool, k, k, slots.int()), (pool[0], k, k, slots)]:
+        with pytest.raises(ValueError):
+            ops.kv_append_paged_(*bad)
+    one = _i32([1])
+    for bad in [(lens.long(), one, one, one, table), (lens, _i32([1, 1]), one, one, table), (lens, one, one, _i32([1, 1]), table),
+                (lens, one, one, one, table.t())]:
+        with pytest.raises(ValueError):
+            ops.paged_batch_plan(*bad, 16, 4)
+    with pytest.raises(ValueError):
+        ops.paged_batch_plan(lens, one, one, one, table, 12, 4)
+    with pytest.raises(ValueError):
+        ops.sample_filtered(torch.zeros(2, 8, device=DEV), torch.zeros(3, device=DEV))
+    with pytest.raises(ValueError):
+        ops.sample_filtered(torch.zeros(2, 8, device=DEV), torch.zeros(2, device=DEV), temperature=-1.0)
+    with pytest.raises(ValueError):
+        ops.sample_filtered(torch.zeros(2, 8, device=DEV), torch.zeros(2, device=DEV), top_k=torch.zeros(2, device=DEV))
+    with pytest.raises(L.SubspecHipError):
+        ops.kv_append_paged_(pool.cpu(), k.cpu(), k.cpu(), slots.cpu())
+
+
+# ------------------------------------------------------------------------------------------------ a run of them together
+def _dense(q, k, v, window, sinks):
+    """float64 causal attention of the last q.shape[0] rows of one sequence."""
+    n, total = q.shape[0], k.shape[0]
+    pool, table = torch.stack([k, v], 1).unsqueeze(0).transpose(1, 2), [[0]]
+    return ob.attention(q, pool, table, [0, n], [total], window, sinks)
+
+
+@pytest.mark.parametrize("page_len,window,sinks", [(16, 0, 0), (4, 20, 3)])
+def test_steps_of_a_batch(page_len, window, sinks):
+    """Prompts in chunks, single tokens, a sequence that rests, one that ends and one that takes its place, over two layers: every
+    step's attention against the sequence's own rows in float64, and the tokens drawn from its outputs."""
+    from subspec_amd.paged_cache import KvBatch, KvCachePool
+    g = torch.Generator().manual_seed(20 + page_len)
+    Hq, Hkv, D, dtype = 8, 2, 128, torch.bfloat16
+    pool = KvCachePool(max_pages=600 // page_len + 8, num_layers=2, num_heads=Hkv, head_dim=D, page_len=page_len, dtype=dtype, device=DEV)
+    pool.cache_data.fill_(float("nan"))
+    pool.allocate(3)
+    batch = KvBatch(pool, 3, 400)
+    head = torch.randn(200, Hq * D, generator=g) * 0.1
+    rows = [[[] for _ in range(3)] for _ in range(2)]
+    for new, end in [([40, 0, 7], None), ([1, 90, 1], None), ([1, 1, 33], None), ([0, 1, 1], 1), ([1, 65, 1], None), ([1, 1, 1], None)]:
+        plan = batch.step(new, n_tokens=sum(new) + 2)
+        T = sum(new)
+        for layer in range(2):
+            qkv = torch.randn(T + 2, Hq + 2 * Hkv, D, generator=g).to(dtype)
+            dev = qkv.to(DEV)
+            batch.append(layer, dev[:, Hq:Hq + Hkv], dev[:, Hq + Hkv:])
+            out = batch.attention(layer, dev[:, :Hq], window=window, sinks=sinks, out=torch.zeros(T + 2, Hq * D, dtype=dtype, device=DEV))
+            first = 0
+            for b, n in enumerate(new):
+                rows[layer][b] += list(qkv[first:first + n, Hq:].view(n, 2, Hkv, D))
+                if n:
+                    kv = torch.stack(rows[layer][b])
+                    want, weight, worst = _dense(qkv[first:first + n, :Hq], kv[:, 0], kv[:, 1], window, sinks)
+                    got = out[first:first + n].double().cpu().view(want.shape)
+                    tol = _tolerance(want, weight, worst, dtype, kv.shape[0], float(kv.abs().max()), D)
+                    assert ((got - want).abs() / tol).max().item() <= 1.0, (new, b, layer)
+                first += n
+            assert out[T:].eq(0).all()
+        last = plan["query_starts"][1:].long().clamp(min=1) - 1
+        logits = (out[last].float() @ head.t().contiguous().to(DEV)).to(dtype)
+        u = torch.rand(3, generator=g)
+        tokens, _ = ops.sample_filtered(logits, u.to(DEV), 0.9, 50, 0.9, 0.01)
+        f = lambda x: float(torch.tensor(x, dtype=torch.float32))
+        assert tokens.tolist() == [ob.sample(logits[b].cpu(), float(u[b]), f(0.9), 50, f(0.9), f(0.01))[0] for b in range(3)]
+        assert plan["counts"][3].item() == 0 and plan["counts"][2].item() == batch.num_free and batch.kv_lens.tolist() == batch.lens
+        if end is not None:
+            batch.release(end)
+            for layer in range(2):
+                rows[layer][end] = []
+    with pytest.raises(ValueError):
+        batch.step([400, 0, 0])
+    batch.close()
+    assert int(pool.num_free_pages()) == pool.max_pages - 3
+
+
+def test_a_captured_step_replays_as_the_batch_grows():
+    """Plan, append, attention (single tokens and a longer call) and sampling in one graph; between the replays other work runs, the
+    lengths move on the device, and every replay equals the eager calls."""
+    g = torch.Generator().manual_seed(31)
+    B, Hq, Hkv, D, P, cap = 5, 8, 2, 128, 16, 64
+    dtype = torch.bfloat16
+    pool = torch.randn(B * cap // P * 4, 2, P, Hkv, D, generator=g).to(dtype).to(DEV)
+    table = torch.full((B, cap * 4 // P), -1, dtype=torch.int32, device=DEV)
+    free = torch.randperm(pool.shape[0], generator=g).to(torch.int32).to(DEV)
+    state = dict(lens=_i32([0] * B), new=_i32([1] * B), n_free=_i32([pool.shape[0]]), qkv=torch.zeros(B + 12, Hq + 2 * Hkv, D, dtype=dtype, device=DEV),
+                 u=torch.zeros(B, device=DEV))
+    head = (torch.randn(Hq * D, 20000, generator=g) * 0.2).to(dtype).to(DEV)
+
+    def step(s, pool, table, plan=None):
+        plan = ops.paged_batch_plan(s["lens"], s["new"], free, s["n_free"], table, P, B + 12, out=plan)
+        ops.kv_append_paged_(pool, s["qkv"][:, Hq:Hq + Hkv], s["qkv"][:, Hq + Hkv:], plan["slots"])
+        args = (s["qkv"][:, :Hq], pool, table, plan["query_starts"], plan["kv_lens"])
+        out = ops.paged_attention(*args, 12, cap * 4, out=torch.zeros(B + 12, Hq * D, dtype=dtype, device=DEV))
+        near = ops.paged_attention(*args, 12, cap * 4, window=9, sinks=2, out=torch.zeros(B + 12, Hq * D, dtype=dtype, device=DEV))
+        tokens, probs = ops.sample_filtered(out[:B] @ head, s["u"], 0.8, 40, 0.95, 0.01)
+        return plan, out, near, tokens, probs
+
+    step({k: v.clone() for k, v in state.items()}, pool.clone(), table.clone())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(state, pool, table)
+        state["lens"].copy_(captured[0]["kv_lens"])
+        state["n_free"].copy_(captured[0]["counts"][2:3])
+    state["lens"].zero_()
+    state["n_free"].fill_(pool.shape[0])
+    for i, new in enumerate([[3, 1, 2, 5, 1], [1] * 5, [0, 12, 1, 0, 1], [1] * 5, [1, 1, 13, 0, 2]]):
+        state["new"].copy_(_i32(new))
+        state["qkv"].copy_(torch.randn(state["qkv"].shape, generator=g).to(dtype))
+        state["u"].copy_(torch.rand(B, generator=g))
+        mine = {k: v.clone() for k, v in state.items()}
+        want = step(mine, pool_copy := pool.clone(), table_copy := table.clone())
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        if max(new) <= 12:                                    # (the bound that the step is captured for)
+            for a, b in zip(want[1:], captured[1:]):
+                assert torch.equal(a, b), i
+        for key, value in want[0].items():
+            assert torch.equal(value, captured[0][key]), (i, key)
+        assert torch.equal(pool, pool_copy) and torch.equal(table, table_copy)
+        (torch.randn(1000, 1000, device=DEV) @ torch.randn(1000, 1000, device=DEV)).sum().item()
+
+
+def test_calls_on_two_streams_at_once():
+    g = torch.Generator().manual_seed(41)
+    jobs = []
+    for lens in ([(900, 1)] * 6, [(300, 120), (200, 1)]):
+        q, pool, table, starts, kv = _batch(g, lens, 16, 8, 2, 128, torch.bfloat16)
+        jobs.append((q.to(DEV), pool.to(DEV), _i32(table), _i32(starts), _i32(kv), max(n for _, n in lens), max(kv)))
+    logits = torch.randn(6, 40000, generator=g).to(DEV)
+    u = torch.rand(6, generator=g).to(DEV)
+    alone = [ops.paged_attention(*j) for j in jobs] + [ops.sample_filtered(logits, u, 1.0, 0, 0.9)[0]]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    results = [[], [], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                results[i].append(ops.paged_attention(*jobs[i]) if i < 2 else ops.sample_filtered(logits, u, 1.0, 0, 0.9)[0])
+    torch.cuda.synchronize()
+    for want, got in zip(alone, results):
+        assert all(torch.equal(want, x) for x in got)
+
+
+def test_long_offsets():
+    """Pool offsets beyond 2^31 elements: the pages of a sequence lie at both ends of a pool of 2.4 billion elements."""
+    P, Hkv, D = 256, 8, 128
+    pages = 4600                                               # 2 * 256 * 8 * 128 elements a page
+    pool = torch.empty(pages, 2, P, Hkv, D, dtype=torch.bfloat16, device=DEV)
+    assert pool.numel() > (1 << 31)
+    g = torch.Generator().manual_seed(51)
+    own = [pages - 1, 0, pages - 2, 4100]
+    k, v = (torch.randn(1000, Hkv, D, generator=g).to(torch.bfloat16) for _ in range(2))
+    slots = torch.tensor([own[j // P] * P + j % P for j in range(1000)])
+    ops.kv_append_paged_(pool, k.to(DEV), v.to(DEV), slots.to(DEV))
+    for n in (1, 40):
+        q = torch.randn(n, 16, D, generator=g).to(torch.bfloat16)
+        want, weight, worst = ob.attention(q, torch.stack([k, v], 1).unsqueeze(0).transpose(1, 2), [[0]], [0, n], [1000])
+        got = ops.paged_attention(q.to(DEV), pool, _i32([own]), _i32([0, n]), _i32([1000]), n, 1000).double().cpu().view(want.shape)
+        tol = _tolerance(want, weight, worst, torch.bfloat16, 1000, float(v.abs().max()), D)
+        assert ((got - want).abs() / tol).max().item() <= 1.0
+
+
+def test_pages_of_one_row_over_a_long_sequence():
+    """More page numbers than a chunk's share of LDS holds: the keys are cut for them."""
+    g = torch.Generator().manual_seed(61)
+    lens = [(9000, 70)]
+    q, pool, table, starts, kv = _batch(g, lens, 1, 7, 1, 64, torch.float16)
+    want, weight, worst = ob.attention(q, pool, table, starts, kv)
+    got = ops.paged_attention(q.to(DEV), pool.to(DEV), _i32(table), _i32(starts), _i32(kv), 70, 9000).double().cpu().view(want.shape)
+    tol = _tolerance(want, weight, worst, torch.float16, 9000, float(pool.nan_to_num(0.0).abs().max()), 64)
+    assert ((got - want).abs() / tol).max().item() <= 1.0
+
+
+def test_thousands_of_sequences_under_a_large_bound():
+    """So many (sequence, KV head) pairs that the partial results of key chunks would not fit: every pair takes its keys in one piece."""
+    g = torch.Generator().manual_seed(62)
+    B, H, D, P, long = 4096, 32, 64, 16, 1500
+    n_pages = B + long // P + 1
+    pool = torch.randn(n_pages, 2, P, H, D, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV, dtype=torch.bfloat16)
+    table = torch.full((B, 70000 // P), -1, dtype=torch.int32)
+    table[:, 0] = torch.arange(B)
+    table[17, 1:long // P + 1] = torch.arange(B, B + long // P)
+    lens = torch.ones(B, dtype=torch.int32)
+    lens[17], lens[99] = long, 0
+    q = torch.randn(B, H, D, generator=g).to(torch.bfloat16)
+    got = ops.paged_attention(q.to(DEV), pool, table.to(DEV), torch.arange(B + 1, dtype=torch.int32, device=DEV), lens.to(DEV), 1, 70000).view(B, H, D)
+    one = torch.ones(B, dtype=torch.bool)
+    one[17] = one[99] = False
+    assert torch.equal(got[one.to(DEV)], pool[:B, 1, 0][one.to(DEV)])          # one key: its value, weight 1
+    assert got[99].eq(0).all()                                                 # no key
+    rows = table[17, :long // P + 1].tolist()
+    want, weight, worst = ob.attention(q[17:18], pool[rows].cpu(), [list(range(len(rows)))], [0, 1], [long])
+    tol = _tolerance(want, weight, worst, torch.bfloat16, long, float(pool.abs().max()), D)
+    assert ((got[17:18].double().cpu() - want).abs() / tol).max().item() <= 1.0
