@@ -346,7 +346,7 @@ int subspec_kv_append_paged(const void* k, int64_t k_token_stride, int64_t k_hea
  * call, an infinite or NaN VALUE row may reach tokens that do not see it, if they share a tile with one that does.
  */
 size_t subspec_paged_attention_workspace(int64_t batch, int64_t n_tokens, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
-                                         int64_t page_len, int64_t max_new, int64_t max_kv, int64_t window, int64_t sinks);
+                                         int64_t max_new, int64_t max_kv, int64_t window, int64_t sinks);
 
 int subspec_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* kv_pool_layer, int64_t max_pages,
                             int64_t page_len, const int32_t* block_table, int64_t max_blocks, int64_t table_stride,

@@ -74,7 +74,7 @@ _SIGNATURES = {
     "subspec_kv_compact_paged": (C.c_int, [_p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i32, _i32, _p]),
     "subspec_paged_batch_plan": (C.c_int, [_p, _p, _i64, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p]),
     "subspec_kv_append_paged": (C.c_int, [_p, _i64, _i64, _p, _i64, _i64, _p, C.c_int, _i64, _i64, _i64, _i64, _p, _i64, _p]),
-    "subspec_paged_attention_workspace": (_sz, [_i64] * 10),
+    "subspec_paged_attention_workspace": (_sz, [_i64] * 9),
     "subspec_paged_attention": (C.c_int, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, C.c_int, _i64, _i64, _i64, _i64,
                                           _i64, _i64, _i64, _i64, _i64, C.c_float, _p, _sz, _p]),
     "subspec_sample_filtered_workspace": (_sz, [_i64, _i64]),

@@ -294,8 +294,8 @@ static int64_t paged_tile_chunks(int64_t blocks, int64_t units) {
 
 // How a call is cut, from the bounds alone.  Keys of a row: at most max_kv, or a window's, its sinks and the row's fellow tokens'.
 struct PagedPlan { int few_rows, few_keys, few_chunks, tile_keys, tile_chunks; int64_t tiles; size_t few_o, few_ml, tile_o, tile_ml, bytes; };
-static PagedPlan paged_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64_t hkv, int64_t head_dim, int64_t page_len, int64_t max_new,
-                            int64_t max_kv, int64_t window, int64_t sinks) {
+static PagedPlan paged_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64_t hkv, int64_t head_dim, int64_t max_new, int64_t max_kv,
+                            int64_t window, int64_t sinks) {
   PagedPlan pl{};
   const int64_t group = hq / hkv, most = max_new * group;
   auto span = [&](int64_t tokens, int64_t block) {
@@ -326,8 +326,7 @@ static PagedPlan paged_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64_t
     const int64_t keys = std::max<int64_t>(1, span(std::min(max_new, kTileRows / group + 2), kTileKeys)), blocks = (keys + kTileKeys - 1) / kTileKeys;
     int64_t chunks = paged_tile_chunks(blocks, (n_tokens * group + kTileRows - 1) / kTileRows * hkv);      // (tiles of all tokens, none part empty)
     while (chunks > 1 && pl.tiles * hkv * chunks > (1 << 13)) --chunks;                  // a gigabyte of partial results at 128 a head
-    int64_t per = (blocks + chunks - 1) / chunks * kTileKeys;
-    per = std::min(per, (kTilePages - 64) * page_len);                                   // its page numbers are in LDS (two more than the keys')
+    const int64_t per = (blocks + chunks - 1) / chunks * kTileKeys;
     pl.tile_keys = (int)per;
     pl.tile_chunks = (int)((keys + per - 1) / per);
     const size_t slots = (size_t)pl.tiles * hkv * pl.tile_chunks * kTileRows;
@@ -345,12 +344,12 @@ static PagedPlan paged_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64_t
 using namespace subspec;
 
 extern "C" size_t subspec_paged_attention_workspace(int64_t batch, int64_t n_tokens, int64_t n_q_heads, int64_t n_kv_heads,
-                                                    int64_t head_dim, int64_t page_len, int64_t max_new, int64_t max_kv,
-                                                    int64_t window, int64_t sinks) {
+                                                    int64_t head_dim, int64_t max_new, int64_t max_kv, int64_t window,
+                                                    int64_t sinks) {
   if (batch < 1 || batch > SUBSPEC_MAX_BATCH || n_kv_heads < 1 || n_q_heads < n_kv_heads || n_q_heads % n_kv_heads || n_q_heads > 1024 || max_kv < 0 ||
-      n_tokens < 1 || page_len < 1 || page_len > (1 << 20) || max_new < 0 || window < 0 || sinks < 0 || head_dim < 1 || head_dim > 1024)
+      n_tokens < 1 || max_new < 0 || window < 0 || sinks < 0 || head_dim < 1 || head_dim > 1024)
     return 256;
-  return paged_plan(batch, n_tokens, n_q_heads, n_kv_heads, head_dim, page_len, std::min(max_new, n_tokens), max_kv, window, sinks).bytes;
+  return paged_plan(batch, n_tokens, n_q_heads, n_kv_heads, head_dim, std::min(max_new, n_tokens), max_kv, window, sinks).bytes;
 }
 
 extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* kv_pool_layer,
@@ -386,7 +385,7 @@ extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, in
       q_token_stride < 0 || q_head_stride < 0)
     SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: q, the pool and out must be 16-byte aligned, q's strides multiples of 8 elements", what);
   max_new = std::min(max_new, n_tokens);
-  const PagedPlan pl = paged_plan(batch, n_tokens, n_q_heads, n_kv_heads, head_dim, page_len, max_new, max_kv, window, sinks);
+  const PagedPlan pl = paged_plan(batch, n_tokens, n_q_heads, n_kv_heads, head_dim, max_new, max_kv, window, sinks);
   if (pl.bytes > 256 && (!workspace || workspace_bytes < pl.bytes))
     SUBSPEC_FAIL(SUBSPEC_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the %zu required", what, workspace_bytes, pl.bytes);
   if ((uintptr_t)workspace % 16) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: workspace must be 16-byte aligned", what);

@@ -210,7 +210,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const PagedSpan sp = paged_span(p, tp.pos_lo, max(tp.pos_hi + 1, 0), kTileKeys);
   const int chunks = paged_chunks(sp, p.tile.chunk_keys);
   if (chunk >= chunks) return;
-  const int v0 = chunk * p.tile.chunk_keys, nkeys = min(p.tile.chunk_keys, sp.length - v0), nb = (nkeys + kTileKeys - 1) / kTileKeys;
+  const int v_begin = chunk * p.tile.chunk_keys, v_end = min(v_begin + p.tile.chunk_keys, sp.length);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, g = lane >> 5;
@@ -221,17 +221,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int token = tp.sq.first + (row_ok ? r / p.group : 0), head = kvh * p.group + (row_ok ? r % p.group : 0);
   const int wave_lo = pos0 + wrow / p.group, wave_hi = pos0 + (min(tp.rows, wrow + 32) - 1) / p.group;
 
-  // ---- the chunk's page numbers: those of its keys before the gap between sinks and window, then those behind it
-  int* pages = (int*)(lds + S::kPages);
-  const int split = min(max(sp.skip - v0, 0), nkeys);                  // keys of the first kind
-  const int base1 = v0 >> p.page_shift, count1 = split > 0 ? ((v0 + split - 1) >> p.page_shift) - base1 + 1 : 0;
-  const int real2 = paged_real(sp, v0 + split), base2 = real2 >> p.page_shift;
-  const int count2 = split < nkeys ? ((real2 + nkeys - split - 1) >> p.page_shift) - base2 + 1 : 0;
-  const int32_t* table = p.table + tp.sq.b * p.table_stride;
-  for (int e = tid; e < count1 + count2; e += 512) {
-    const int page = table[e < count1 ? base1 + e : base2 + e - count1];
-    pages[e] = min(max(page, 0), p.max_pages - 1);
-  }
   dec_u4 q[D / 16];
   {
     const uint16_t* src = p.q + token * p.q_token + head * p.q_head + g * 8;
@@ -247,8 +236,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
   dec_u4 pb[4] = {};
   TileRow row{row_ok ? pos0 + r / p.group : -1, 0.f, 0.f, false};
-  __builtin_amdgcn_s_waitcnt(0);                                       // queries and page numbers; from here on only copies are counted
-  __syncthreads();
 
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
   const int crow = lane / S::kPieces, cpiece = lane % S::kPieces;
@@ -265,6 +252,22 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
   TileCopy cp;
   int asked = 0;
+  // A stretch of the chunk: as many keys as there is room for page numbers (all of them but where pages hold a row or two).  pages[]: those of the
+  // keys before the gap between sinks and window, then those behind it.
+  int* pages = (int*)(lds + S::kPages);
+  const int64_t stretch = (int64_t)(kTilePages - 64) << p.page_shift;
+  int v0 = v_begin, nb = 0, base1 = 0, count1 = 0, base2 = 0;
+  auto load_pages = [&](int nkeys) {
+    const int split = min(max(sp.skip - v0, 0), nkeys);                // keys before the gap
+    const int real2 = paged_real(sp, v0 + split);
+    nb = (nkeys + kTileKeys - 1) / kTileKeys;
+    base1 = v0 >> p.page_shift;
+    count1 = split > 0 ? ((v0 + split - 1) >> p.page_shift) - base1 + 1 : 0;
+    base2 = real2 >> p.page_shift;
+    const int count2 = split < nkeys ? ((real2 + nkeys - split - 1) >> p.page_shift) - base2 + 1 : 0;
+    const int32_t* table = p.table + tp.sq.b * p.table_stride;
+    for (int e = tid; e < count1 + count2; e += 512) pages[e] = min(max(table[e < count1 ? base1 + e : base2 + e - count1], 0), p.max_pages - 1);
+  };
   // The next copies are those of block J -> stage J % 4; blocks past the last repeat it (every wavefront's count of copies is the same on every
   // path).  ask() reads the page number that plan() uses a few products later.
   auto place = [&](int J, int* v, int* j, int* shift) {
@@ -345,7 +348,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     softmax_phase<DT, D>(p, kb, plain, g, row, s, o, cinit, pb);
   };
 
-  if (nb > 0) {
+  for (; v0 < v_end; v0 = (int)min((int64_t)v_end, v0 + stretch)) {
+    load_pages((int)min((int64_t)(v_end - v0), stretch));
+    __builtin_amdgcn_s_waitcnt(0);                                     // page numbers (and queries); from here on only copies are counted
+    __syncthreads();
     ask(0);
     plan(0);
     copy_all();
@@ -391,7 +397,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     __syncthreads();
     if (!second) __syncthreads();
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                   // no copy may be on its way into LDS when the workgroup ends
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                   // no copy may be on its way into LDS when the workgroup ends, or begins anew
+    __syncthreads();
   }
 
   const float l = row.l + __shfl_xor(row.l, 32, kWave);

@@ -548,7 +548,7 @@ def paged_attention(q: torch.Tensor, pool_layer: torch.Tensor, block_table: torc
         raise ValueError(f"paged_attention: out must be a contiguous {q.dtype} tensor [{T}, {Hq * D}]")
     if workspace is not None:
         _require_gpu(q, workspace)
-    need = L.lib().subspec_paged_attention_workspace(batch, T, Hq, Hkv, D, page_len, max_new, max_kv, window, sinks)
+    need = L.lib().subspec_paged_attention_workspace(batch, T, Hq, Hkv, D, max_new, max_kv, window, sinks)
     if workspace is None and need > 256:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     _call(dev, "subspec_paged_attention", q.data_ptr(), q.stride(0), q.stride(1), pool_layer.data_ptr(), max_pages, page_len,

@@ -120,12 +120,6 @@ def test_a_batch_refuses_before_anything_is_launched():
 def test_attention_workspace_holds_a_gigabyte_of_partials_at_most(hq, hkv, D):
     size = L.lib().subspec_paged_attention_workspace
     for batch, tokens, new in [(1, 1, 1), (64, 64, 1), (4096, 4096, 1), (1, 4096, 4096), (4096, 60000, 3000), (300, 5000, 40)]:
-        for kv in (1, 100, 4096, 131072, 1 << 20):
-            for page_len in (1, 16):
-                n = size(batch, tokens, hq, hkv, D, page_len, new, kv, 0, 0)
-                most = (1 << 30) + (1 << 26)
-                tiles = tokens * (hq // hkv) // 256 + batch
-                # pages of one row cut the keys at 4032 whatever it costs
-                cut = tiles * hkv * -(-kv // 4032) * 256 * (D + 2) * 4 if page_len == 1 and new * (hq // hkv) > 16 else 0
-                assert 256 <= n <= most * 2 + cut
-    assert size(1, 1, hq, hkv, D, 16, 1, 64, 0, 0) == 256       # one chunk: nothing to keep
+        for kv in (1, 100, 4096, 131072, 1 << 20):            # (those of short calls and of long ones: a gigabyte each, and the sums' share)
+            assert 256 <= size(batch, tokens, hq, hkv, D, new, kv, 0, 0) <= (2 << 30) * 1.02
+    assert size(1, 1, hq, hkv, D, 1, 64, 0, 0) == 256       # one chunk: nothing to keep
