@@ -208,19 +208,21 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
   const int64_t id = (int64_t)blockIdx.x * kTeams + team;    // (sequence, KV head, row)
   const int r = (int)(id % p.few_most), bk = (int)(id / p.few_most), kvh = bk % p.hkv, rows = p.few.rows;
   bool mine = bk / p.hkv < p.batch;
+  const int64_t slot = (int64_t)bk * p.few.chunks * rows + r;
+  const float* ml = p.few.part_ml + slot * 2;
+  // the first chunks' references and sums, on their way before it is known how many chunks there are
+  const v2f early = mine && tid < p.few.chunks ? *(const v2f*)(ml + (int64_t)tid * rows * 2) : v2f{-INFINITY, 0.f};
   const PagedSequence sq = paged_sequence(p, mine ? bk / p.hkv : 0);
   mine = mine && r < sq.n * p.group && sq.n * p.group <= rows;
   int chunks = 1;
   if (mine) chunks = paged_chunks(paged_span(p, sq.len - sq.n, sq.len, kFewKeys), p.few.chunk_keys);
   mine = mine && chunks > 1;                                 // (one chunk: complete already)
   if (WAVES == 4 && !mine) return;                           // (the whole workgroup)
-  const int64_t slot = (int64_t)bk * p.few.chunks * rows + r;
-  const float* ml = p.few.part_ml + slot * 2;
   const int d4 = (tid % kLanes) * 4, side = tid / kLanes;
   const float* po = p.few.part_o + slot * D + d4;
-  float top = -INFINITY;
+  float top = tid < chunks ? early[0] : -INFINITY;
   if (mine)
-    for (int c = tid; c < chunks; c += kThreads) top = fmaxf(top, ml[(int64_t)c * rows * 2]);
+    for (int c = tid + kThreads; c < chunks; c += kThreads) top = fmaxf(top, ml[(int64_t)c * rows * 2]);
   top = wave_max(top);
   if constexpr (WAVES == 4) {
     if (lane == 0) tops[wave] = top;
@@ -234,7 +236,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
   for (int c0 = 0; mine && c0 < chunks; c0 += kAtOnce) {     // (uniform in a team)
     const int some = min(kAtOnce, chunks - c0);
     for (int c = tid; c < some; c += kThreads) {
-      const v2f m = *(const v2f*)(ml + (int64_t)(c0 + c) * rows * 2);
+      const v2f m = c0 + c < kThreads ? early : *(const v2f*)(ml + (int64_t)(c0 + c) * rows * 2);
       const float w = __builtin_amdgcn_exp2f(m[0] - base);
       weight[team][c] = w;
       den = fmaf(w, m[1], den);
