@@ -59,25 +59,34 @@ struct RowTop { float value; double wide; bool only; };
 __device__ __forceinline__ RowTop row_top_of(float top, const RowRule& r) { return RowTop{top, (double)top, r.greedy || top == INFINITY}; }
 
 // 2^f * 2^42 for |f| <= 1/2: the Taylor series of e^(f ln 2) to the tenth power, its coefficients ln^k 2 / k! (remainder (ln 2 / 2)^11 / 11! =
-// 2.2e-13 of the value).  (The three-operand instruction by hand: the compiler takes the two-operand one and copies each coefficient first.)
-__device__ __forceinline__ double fma_s(double a, double b, double c) {
-  double d;
-  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
-  return d;
-}
-__device__ __forceinline__ double exp2_part(double f) {
-  constexpr double k = (double)(1ull << kMassBits);
-  double s = fma_s(f, 7.0549116208011233e-9 * k, 1.0178086009239699e-7 * k);
-  s = fma_s(s, f, 1.3215486790144309e-6 * k);
-  s = fma_s(s, f, 1.5252733804059841e-5 * k);
-  s = fma_s(s, f, 1.5403530393381610e-4 * k);
-  s = fma_s(s, f, 1.3333558146428443e-3 * k);
-  s = fma_s(s, f, 9.6181291076284772e-3 * k);
-  s = fma_s(s, f, 5.5504108664821580e-2 * k);
-  s = fma_s(s, f, 2.4022650695910072e-1 * k);
-  s = fma_s(s, f, 6.9314718055994531e-1 * k);
-  return fma_s(s, f, k);
-}
+// 2.2e-13 of the value).  (They are held in registers of the wavefront: left to itself the compiler copies each into the result before it adds.)
+struct Series {
+  double c[11];
+  __device__ __forceinline__ Series() {
+    constexpr double of[11] = {1.0,
+                               6.9314718055994531e-1,
+                               2.4022650695910072e-1,
+                               5.5504108664821580e-2,
+                               9.6181291076284772e-3,
+                               1.3333558146428443e-3,
+                               1.5403530393381610e-4,
+                               1.5252733804059841e-5,
+                               1.3215486790144309e-6,
+                               1.0178086009239699e-7,
+                               7.0549116208011233e-9};
+#pragma unroll
+    for (int i = 0; i < 11; ++i) {
+      c[i] = of[i] * (double)(1ull << kMassBits);
+      asm("" : "+v"(c[i]));
+    }
+  }
+  __device__ __forceinline__ double operator()(double f) const {
+    double s = c[10];
+#pragma unroll
+    for (int i = 9; i >= 0; --i) s = fma(s, f, c[i]);
+    return s;
+  }
+};
 // How far entry l is below the largest in units of T, in 32 bits: what the bins go by (falls as l rises, so bins keep the order).  Entries at kReach
 // and beyond, and NaN, have no mass and no bin.
 __device__ __forceinline__ float entry_distance(float l, const RowTop& top, const RowRule& r) {
@@ -86,7 +95,7 @@ __device__ __forceinline__ float entry_distance(float l, const RowTop& top, cons
 }
 __device__ __forceinline__ int bin_of(float d) { return (int)(d * (0.999999f * kBins / kReach)); }      // (below kBins, rounding or not)
 // The mass of an entry less than kReach below the largest, in units of 2^-42 and before rounding.
-__device__ __forceinline__ double entry_mass(float l, const RowTop& top, const RowRule& r) {
+__device__ __forceinline__ double entry_mass(float l, const RowTop& top, const RowRule& r, const Series& exp2_part) {
   if (top.only) return (double)(1ull << kMassBits);
   const double x = ((double)l - top.wide) * r.inv_t_log2e, n = rint(x);
   return ldexp(exp2_part(x - n), (int)n);
@@ -292,11 +301,12 @@ template <int DT, int THREADS>
 __device__ __forceinline__ uint64_t fill_bins(Hist& h, const void* row, int i0, int i1, int vocab, const RowTop& top, const RowRule& r) {
   const double least = r.min_p * (double)(1ull << kMassBits);
   const bool counted = r.k < vocab, sorted_out = r.min_p > 0.0;
+  const Series series;
   uint64_t kept = 0;
   each_entry<DT, THREADS>(row, i0, i1, [&](float l, int) {
     const float d = entry_distance(l, top, r);
     if (!(d < kReach)) return;
-    const double m = entry_mass(l, top, r);
+    const double m = entry_mass(l, top, r, series);
     const uint64_t w = whole(m);
     const int bin = bin_of(d);
     atomicAdd((unsigned long long*)&h.mass[bin], (unsigned long long)w);
@@ -406,6 +416,7 @@ __device__ __forceinline__ void gather(uint64_t* keys, int most, int* n, const v
 struct Found { uint64_t key, upto; };
 template <int DT, int THREADS, typename Each>
 __device__ Found find_entry(Search& s, const Hist& bins, bool by_count, uint64_t t, const RowTop& top, const RowRule& r, int most, Each each) {
+  const Series series;
   const int b = bin_at(bins, by_count, t);
   uint64_t prefix = 0, upto = below(bins, b);
   t -= by_count ? (uint64_t)(b > 0 ? bins.count[b - 1] : 0) : upto;
@@ -436,7 +447,7 @@ __device__ Found find_entry(Search& s, const Hist& bins, bool by_count, uint64_t
     each([&](uint64_t key) {
       if (!mine(key)) return;
       const int digit = (int)(key >> next) & ((1 << width) - 1);
-      atomicAdd((unsigned long long*)&s.digits.mass[digit], (unsigned long long)whole(entry_mass(key_logit<DT>(key), top, r)));
+      atomicAdd((unsigned long long*)&s.digits.mass[digit], (unsigned long long)whole(entry_mass(key_logit<DT>(key), top, r, series)));
       atomicAdd(&s.digits.count[digit], 1u);
     });
     __syncthreads();
@@ -459,7 +470,7 @@ __device__ Found find_entry(Search& s, const Hist& bins, bool by_count, uint64_t
         k = ((lane & step) == 0) == ((lane & span) == 0) ? min(k, other) : max(k, other);
       }
     }
-    const uint64_t sum = wave_scan_u64(lane < left ? whole(entry_mass(key_logit<DT>(k), top, r)) : 0);
+    const uint64_t sum = wave_scan_u64(lane < left ? whole(entry_mass(key_logit<DT>(k), top, r, series)) : 0);
     const uint64_t over = __ballot(lane < left && (by_count ? (uint64_t)lane : sum) >= t + (by_count ? 0 : 1));
     if (lane == (over ? __ffsll((unsigned long long)over) - 1 : max(left - 1, 0))) {
       s.key = k;
@@ -493,7 +504,7 @@ __device__ void draw_row(Search& s, const Hist& bins, const uint64_t* keys, int 
   }
   if (threadIdx.x == 0) {
     a.tokens[row_index] = (int64_t)(found.key & 0xfffff);
-    a.probs[row_index] = (float)(entry_mass(key_logit<DT>(found.key), top, r) / (double)z);
+    a.probs[row_index] = (float)(entry_mass(key_logit<DT>(found.key), top, r, Series()) / (double)z);
   }
 }
 __device__ __forceinline__ void nothing_to_draw(const SampleArgs& a, int row_index) {
