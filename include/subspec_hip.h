@@ -305,7 +305,7 @@ int subspec_kv_compact_paged(void* pool, int64_t n_layers, int64_t max_pages, in
  * No output may overlap an input (total_lens and kv_lens, say).  Limits: 1 <= batch <= SUBSPEC_MAX_BATCH, page_len a power of two.
  */
 #define SUBSPEC_PLAN_NEGATIVE 1 /* a length below zero */
-#define SUBSPEC_PLAN_TABLE 2    /* a sequence needs more than max_blocks pages */
+#define SUBSPEC_PLAN_TABLE 2    /* a sequence needs more than max_blocks pages (or 2^31 rows) */
 #define SUBSPEC_PLAN_PAGES 4    /* too few free pages (or *n_free beyond free_capacity) */
 #define SUBSPEC_PLAN_TOKENS 8   /* more than n_tokens new tokens */
 
@@ -338,7 +338,7 @@ int subspec_kv_append_paged(const void* k, int64_t k_token_stride, int64_t k_hea
  *              (multiples of 8; a slice of a fused projection's output)
  * block_table, query_starts, kv_lens   device, as the plan leaves them (kv_lens: its total_lens)
  * max_new      no sequence brings more new tokens;  max_kv: no kv_lens is larger.  They lay out the launches and the workspace and may be larger
- *              than what a call meets; tokens and rows beyond them are left out
+ *              than what a call meets; tokens and rows beyond them are left out (either 0: nothing is written)
  * out          device [n_tokens, n_q_heads, head_dim]; rows behind query_starts[batch] are left as they were
  * workspace    subspec_paged_attention_workspace bytes of the same sizes, 16-byte aligned
  * Page numbers are clamped to the pool, so a bad table reads wrong rows and never leaves it.  Rows that no token of the call sees (those behind

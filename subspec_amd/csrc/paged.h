@@ -27,7 +27,7 @@ struct PagedParams {
   uint16_t* out;
   int64_t q_token, q_head;                 // strides, elements
   int64_t table_stride, page_elems;        // page_elems: a page's K (V follows it)
-  int batch, n_tokens, hq, hkv, group, head_dim, max_new, max_kv, window, sinks, page_shift, max_pages, max_blocks;
+  int batch, n_tokens, hq, hkv, group, head_dim, max_new, max_kv, window, sinks, page_shift, max_pages;
   float scale_log2;
   PagedCut few;                            // sequences of at most few.rows rows a KV head (0 rows: none)
   int few_most;                            // rows a KV head that one of them can have

@@ -341,6 +341,37 @@ static PagedPlan paged_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64_t
   return pl;
 }
 
+template <int DT, int D>
+static void launch_few_of(const PagedParams& p, int tiles, unsigned units, hipStream_t st) {
+  if (tiles == 1) hipLaunchKernelGGL((paged_few_kernel<DT, D, 1>), dim3(units), dim3(64), 0, st, p);
+  else if (tiles == 2) hipLaunchKernelGGL((paged_few_kernel<DT, D, 2>), dim3(units), dim3(64), 0, st, p);
+  else hipLaunchKernelGGL((paged_few_kernel<DT, D, 4>), dim3(units), dim3(64), 0, st, p);
+}
+static void launch_few(const PagedParams& p, int tiles, int dtype, unsigned units, hipStream_t st) {
+  if (dtype == SUBSPEC_BF16) {
+    if (p.head_dim == 128) launch_few_of<SUBSPEC_BF16, 128>(p, tiles, units, st);
+    else launch_few_of<SUBSPEC_BF16, 64>(p, tiles, units, st);
+  } else {
+    if (p.head_dim == 128) launch_few_of<SUBSPEC_F16, 128>(p, tiles, units, st);
+    else launch_few_of<SUBSPEC_F16, 64>(p, tiles, units, st);
+  }
+}
+// A workgroup a row where there are many chunks to add up, a wavefront a row where there are few.
+template <int DT, int D>
+static void launch_few_merge_of(const PagedParams& p, int64_t rows, hipStream_t st) {
+  if (p.few.chunks > 12) hipLaunchKernelGGL((paged_merge_kernel<DT, D, 4>), dim3((unsigned)rows), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((paged_merge_kernel<DT, D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
+}
+static void launch_few_merge(const PagedParams& p, int dtype, int64_t rows, hipStream_t st) {
+  if (dtype == SUBSPEC_BF16) {
+    if (p.head_dim == 128) launch_few_merge_of<SUBSPEC_BF16, 128>(p, rows, st);
+    else launch_few_merge_of<SUBSPEC_BF16, 64>(p, rows, st);
+  } else {
+    if (p.head_dim == 128) launch_few_merge_of<SUBSPEC_F16, 128>(p, rows, st);
+    else launch_few_merge_of<SUBSPEC_F16, 64>(p, rows, st);
+  }
+}
+
 }  // namespace subspec
 
 using namespace subspec;
@@ -401,7 +432,7 @@ extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, in
   p.window = (int)std::min<int64_t>(window, 1ll << 30); p.sinks = (int)std::min<int64_t>(sinks, 1ll << 30);
   p.page_shift = 0;
   while ((1ll << p.page_shift) < page_len) ++p.page_shift;
-  p.max_pages = (int)max_pages; p.max_blocks = (int)max_blocks;
+  p.max_pages = (int)max_pages;
   p.scale_log2 = scale * kLog2e;
   char* ws = (char*)workspace;
   p.few = PagedCut{pl.few_rows, pl.few_keys, pl.few_chunks, (float*)ws, (float*)(ws + pl.few_o)};
@@ -415,33 +446,22 @@ extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, in
   if (few_units > INT32_MAX || tile_units * 8 > INT32_MAX || merge_rows > INT32_MAX)
     SUBSPEC_FAIL(SUBSPEC_ERR_LIMIT, "%s: too large (%lld tokens of %lld heads, %lld sequences)", what, (long long)n_tokens, (long long)n_q_heads,
                  (long long)batch);
-#define SUBSPEC_PAGED_FEW(DT, D, ROWT) hipLaunchKernelGGL((paged_few_kernel<DT, D, ROWT>), dim3((unsigned)few_units), dim3(64), 0, st, p)
-#define SUBSPEC_PAGED(DT, D)                                                                                                           \
-  do {                                                                                                                                 \
-    DominantKernelTimer timer(st);                                                                                                     \
-    if (pl.few_rows == 16) SUBSPEC_PAGED_FEW(DT, D, 1);                                                                                \
-    else if (pl.few_rows == 32) SUBSPEC_PAGED_FEW(DT, D, 2);                                                                           \
-    else if (pl.few_rows == 64) SUBSPEC_PAGED_FEW(DT, D, 4);                                                                           \
-    if (pl.few_chunks > 12)                                                                                                            \
-      hipLaunchKernelGGL((paged_merge_kernel<DT, D, 4>), dim3((unsigned)merge_rows), dim3(256), 0, st, p);                              \
-    else if (pl.few_chunks > 1)                                                                                                        \
-      hipLaunchKernelGGL((paged_merge_kernel<DT, D, 1>), dim3((unsigned)((merge_rows + 3) / 4)), dim3(256), 0, st, p);                  \
-  } while (0)
   if (pl.tiles) {
-    if (!pl.few_rows) {
+    {
       DominantKernelTimer timer(st);
-      launch_paged_tile(p, dtype, st);
-    } else {
       launch_paged_tile(p, dtype, st);
     }
     if (pl.tile_chunks > 1) launch_paged_tile_merge(p, dtype, st);
   }
   if (pl.few_rows) {
-    if (dtype == SUBSPEC_BF16) { if (head_dim == 128) SUBSPEC_PAGED(SUBSPEC_BF16, 128); else SUBSPEC_PAGED(SUBSPEC_BF16, 64); }
-    else { if (head_dim == 128) SUBSPEC_PAGED(SUBSPEC_F16, 128); else SUBSPEC_PAGED(SUBSPEC_F16, 64); }
+    if (pl.tiles) {
+      launch_few(p, pl.few_rows / 16, dtype, (unsigned)few_units, st);
+    } else {
+      DominantKernelTimer timer(st);
+      launch_few(p, pl.few_rows / 16, dtype, (unsigned)few_units, st);
+    }
+    if (pl.few_chunks > 1) launch_few_merge(p, dtype, merge_rows, st);
   }
-#undef SUBSPEC_PAGED
-#undef SUBSPEC_PAGED_FEW
   SUBSPEC_CHECK_HIP(hipGetLastError());
   return SUBSPEC_OK;
 }

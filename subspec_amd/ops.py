@@ -434,6 +434,13 @@ def _int32_vector(t: torch.Tensor, n: Optional[int], what: str) -> None:
         raise ValueError(f"{what} must be a contiguous int32 vector" + ("" if n is None else f" of {n} elements"))
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors' first-to-last elements share bytes."""
+    def end(t):
+        return t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < end(b) and b.data_ptr() < end(a)
+
+
 def _table_shape(block_table: torch.Tensor, batch: int):
     if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch or block_table.shape[1] < 1 \
             or block_table.stride(1) != 1 or (batch > 1 and block_table.stride(0) < block_table.shape[1]):
@@ -479,8 +486,9 @@ def paged_batch_plan(kv_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: 
             t = out[key]
             if t.dtype is not dtype or t.shape != (n,) or t.device != dev or not t.is_contiguous():
                 raise ValueError(f"out[{key!r}] must be a contiguous {dtype} tensor of shape ({n},) on {dev}")
-        if out["kv_lens"].data_ptr() == kv_lens.data_ptr():
-            raise ValueError("out['kv_lens'] must not be kv_lens itself: every workgroup reads the old lengths")
+            for name, given in (("kv_lens", kv_lens), ("new_lens", new_lens), ("free_pages", free_pages), ("n_free", n_free), ("block_table", block_table)):
+                if _overlap(t, given):
+                    raise ValueError(f"out[{key!r}] overlaps {name}: every workgroup reads the inputs while another writes the outputs")
     _call(dev, "subspec_paged_batch_plan", kv_lens.data_ptr(), new_lens.data_ptr(), batch, free_pages.data_ptr(), n_free.data_ptr(),
           free_pages.numel(), block_table.data_ptr(), max_blocks, stride, int(page_len), n_tokens,
           out["query_starts"].data_ptr(), out["kv_lens"].data_ptr(), out["positions"].data_ptr(), out["slots"].data_ptr(),
@@ -548,6 +556,8 @@ def paged_attention(q: torch.Tensor, pool_layer: torch.Tensor, block_table: torc
         raise ValueError(f"paged_attention: out must be a contiguous {q.dtype} tensor [{T}, {Hq * D}]")
     if workspace is not None:
         _require_gpu(q, workspace)
+        if not workspace.is_contiguous():
+            raise ValueError("paged_attention: the workspace must be contiguous")
     need = L.lib().subspec_paged_attention_workspace(batch, T, Hq, Hkv, D, max_new, max_kv, window, sinks)
     if workspace is None and need > 256:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)

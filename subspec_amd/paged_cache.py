@@ -19,7 +19,7 @@ from typing import Dict, List, Optional, Sequence
 
 import torch
 
-from . import ops
+from . import _lib as L, ops
 
 
 class KvCachePool:
@@ -180,6 +180,8 @@ class KvBatch:
     for the device."""
 
     def __init__(self, pool: KvCachePool, max_batch: int, max_len: int, num_pages: Optional[int] = None):
+        if not 1 <= int(max_batch) <= L.MAX_BATCH:
+            raise ValueError(f"max_batch={max_batch} outside [1, {L.MAX_BATCH}]")
         self.pool, self.page_len, self.max_len = pool, pool.page_len, int(max_len)
         self.pages = pool.allocate(int(pool.num_free_pages()) if num_pages is None else int(num_pages))
         self.num_free = len(self.pages)
@@ -210,7 +212,8 @@ class KvBatch:
         rows = sum(new) if n_tokens is None else int(n_tokens)
         if rows < sum(new):
             raise ValueError(f"n_tokens={rows} is less than the {sum(new)} new tokens")
-        fresh = torch.tensor(new, dtype=torch.int32, device=self.pool.device)
+        # (from pinned memory: a copy from pageable memory would wait for everything the stream has to do)
+        fresh = torch.tensor(new, dtype=torch.int32, pin_memory=self.pool.device.type == "cuda").to(self.pool.device, non_blocking=True)
         self.plan = ops.paged_batch_plan(self.kv_lens, fresh, self.free_pages, self.n_free, self.block_table, self.page_len, rows)
         self.kv_lens, self.n_free = self.plan["kv_lens"], self.plan["counts"][2:3]
         self.lens, self.num_free = total, self.num_free - taken
@@ -234,7 +237,7 @@ class KvBatch:
         self.lens[index] = 0
         self.n_free = torch.full_like(self.n_free, self.num_free)
         self.kv_lens = self.kv_lens.clone()
-        self.kv_lens[index] = 0
+        self.kv_lens[index].zero_()                            # (an assignment of a number would wait for the device)
 
     def close(self) -> None:
         """All pages go back to the pool."""

@@ -114,6 +114,10 @@ def test_a_batch_refuses_before_anything_is_launched():
     assert batch.lens == [0, 0] and batch.num_free == 5
     batch.close()
     assert int(pool.num_free_pages()) == 8
+    for places in (0, L.MAX_BATCH + 1):
+        with pytest.raises(ValueError):
+            KvBatch(pool, places, 40)
+    assert int(pool.num_free_pages()) == 8
 
 
 @pytest.mark.parametrize("hq,hkv,D", [(28, 4, 128), (32, 32, 128), (14, 2, 64), (64, 1, 128)])

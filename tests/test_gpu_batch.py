@@ -334,6 +334,38 @@ def test_a_captured_step_replays_as_the_batch_grows():
         (torch.randn(1000, 1000, device=DEV) @ torch.randn(1000, 1000, device=DEV)).sum().item()
 
 
+def test_a_step_does_not_wait_for_the_device():
+    from subspec_amd.paged_cache import KvBatch, KvCachePool
+    pool = KvCachePool(max_pages=8, num_layers=1, num_heads=2, head_dim=64, page_len=16, dtype=torch.bfloat16, device=DEV)
+    batch = KvBatch(pool, 2, 64)
+    k = torch.randn(5, 2, 64, device=DEV).to(torch.bfloat16)
+    before = torch.cuda.get_sync_debug_mode()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        with pytest.raises(RuntimeError):
+            torch.ones(1, device=DEV).item()                   # (what the mode reports)
+        batch.step([3, 2])
+        batch.append(0, k, k)
+        batch.attention(0, k)
+        batch.release(1)
+        batch.step([1, 4])
+    finally:
+        torch.cuda.set_sync_debug_mode(before)
+    assert batch.plan["counts"].tolist() == [5, 1, 6, 0] and batch.kv_lens.tolist() == [4, 4]
+
+
+def test_a_plan_is_not_written_over_its_inputs():
+    table, one = _i32([[0, -1]]), _i32([1])
+    plan = ops.paged_batch_plan(_i32([3]), one, _i32([5, 6]), _i32([2]), table, 16, 4)
+    for change in (dict(kv=plan["kv_lens"]), dict(n_free=plan["counts"][2:3]), dict(new=plan["positions"][1:2]), dict(free=plan["sequences"])):
+        a = dict(kv=_i32([3]), new=one, free=_i32([5, 6]), n_free=_i32([2]))
+        a.update(change)
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.paged_batch_plan(a["kv"], a["new"], a["free"], a["n_free"], table, 16, 4, out=plan)
+    ops.paged_batch_plan(_i32([4]), one, _i32([5, 6]), _i32([2]), table, 16, 4, out=plan)
+    assert plan["kv_lens"].tolist() == [5] and plan["slots"].tolist() == [4, -1, -1, -1]
+
+
 def test_calls_on_two_streams_at_once():
     g = torch.Generator().manual_seed(41)
     jobs = []
@@ -375,7 +407,7 @@ def test_long_offsets():
 
 
 def test_pages_of_one_row_over_a_long_sequence():
-    """More page numbers than a chunk's share of LDS holds: the keys are cut for them."""
+    """More page numbers than LDS has room for: a chunk's keys are taken in stretches."""
     g = torch.Generator().manual_seed(61)
     lens = [(9000, 70)]
     q, pool, table, starts, kv = _batch(g, lens, 1, 7, 1, 64, torch.float16)
