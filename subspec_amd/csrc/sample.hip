@@ -10,6 +10,8 @@
 // order in which wavefronts add them, 2^20 entries stay below 2^62, and what rounds to zero (less than 2^-43 of the largest) is drawn with a
 // probability below 2^-23 even if a million such entries are there.  In fp32 the sum over a flat row of 150000 entries is off by more
 // than the step between two of them.
+// One row of 152064 fp32: 30 us, four dependent launches of 3 + 9 + 11 + 9; 64 rows bf16 (19.5 MB): 57, the exponentials in 64 bits 19 of them,
+// the sums of the slices' bins and the second pass 20, the search among the candidates 15.
 #include "common.h"
 #include <algorithm>
 
