@@ -294,6 +294,10 @@ static int64_t paged_tile_chunks(int64_t blocks, int64_t units) {
   return chunks;
 }
 
+// No key behind this many rows is read (max_kv), so a window or sinks beyond it say no more than it does: the plan and the kernels both take the smaller
+// number (the plan's sums with a window of 2^63 - 1 would wrap).
+constexpr int64_t kMostRows = 1ll << 30;
+
 // How a call is cut, from the bounds alone.  Keys of a row: at most max_kv, or a window's, its sinks and the row's fellow tokens'.
 struct PagedPlan { int few_rows, few_keys, few_chunks, tile_keys, tile_chunks; int64_t tiles; size_t few_o, few_ml, tile_o, tile_ml, bytes; };
 static PagedPlan paged_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64_t hkv, int64_t head_dim, int64_t max_new, int64_t max_kv,
@@ -380,9 +384,10 @@ extern "C" size_t subspec_paged_attention_workspace(int64_t batch, int64_t n_tok
                                                     int64_t head_dim, int64_t max_new, int64_t max_kv, int64_t window,
                                                     int64_t sinks) {
   if (batch < 1 || batch > SUBSPEC_MAX_BATCH || n_kv_heads < 1 || n_q_heads < n_kv_heads || n_q_heads % n_kv_heads || n_q_heads > 1024 || max_kv < 0 ||
-      n_tokens < 1 || max_new < 0 || window < 0 || sinks < 0 || head_dim < 1 || head_dim > 1024)
+      max_kv > kMostRows || n_tokens < 1 || n_tokens > (1ll << 30) || max_new < 0 || window < 0 || sinks < 0 || head_dim < 1 || head_dim > 1024)
     return 256;
-  return paged_plan(batch, n_tokens, n_q_heads, n_kv_heads, head_dim, std::min(max_new, n_tokens), max_kv, window, sinks).bytes;
+  return paged_plan(batch, n_tokens, n_q_heads, n_kv_heads, head_dim, std::min(max_new, n_tokens), max_kv, std::min(window, kMostRows),
+                    std::min(sinks, kMostRows)).bytes;
 }
 
 extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* kv_pool_layer,
@@ -396,7 +401,7 @@ extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, in
     SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: dtype %d not supported (bf16 / fp16 only)", what, dtype);
   if (head_dim != 64 && head_dim != 128)
     SUBSPEC_FAIL(SUBSPEC_ERR_LIMIT, "%s: head_dim=%lld (built for 64 and 128)", what, (long long)head_dim);
-  if (n_tokens < 0 || n_tokens > (1ll << 30) || max_new < 0 || max_kv < 0 || max_kv > (1ll << 30))
+  if (n_tokens < 0 || n_tokens > (1ll << 30) || max_new < 0 || max_kv < 0 || max_kv > kMostRows)
     SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: n_tokens=%lld max_new=%lld max_kv=%lld", what, (long long)n_tokens, (long long)max_new,
                  (long long)max_kv);
   if (batch < 1 || batch > SUBSPEC_MAX_BATCH)
@@ -418,6 +423,8 @@ extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, in
       q_token_stride < 0 || q_head_stride < 0)
     SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: q, the pool and out must be 16-byte aligned, q's strides multiples of 8 elements", what);
   max_new = std::min(max_new, n_tokens);
+  window = std::min(window, kMostRows);
+  sinks = std::min(sinks, kMostRows);
   const PagedPlan pl = paged_plan(batch, n_tokens, n_q_heads, n_kv_heads, head_dim, max_new, max_kv, window, sinks);
   if (pl.bytes > 256 && (!workspace || workspace_bytes < pl.bytes))
     SUBSPEC_FAIL(SUBSPEC_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the %zu required", what, workspace_bytes, pl.bytes);
@@ -429,7 +436,7 @@ extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, in
   p.page_elems = page_len * n_kv_heads * head_dim;
   p.batch = (int)batch; p.n_tokens = (int)n_tokens; p.hq = (int)n_q_heads; p.hkv = (int)n_kv_heads; p.group = (int)(n_q_heads / n_kv_heads);
   p.head_dim = (int)head_dim; p.max_new = (int)max_new; p.max_kv = (int)std::min(max_kv, max_blocks * page_len);
-  p.window = (int)std::min<int64_t>(window, 1ll << 30); p.sinks = (int)std::min<int64_t>(sinks, 1ll << 30);
+  p.window = (int)window; p.sinks = (int)sinks;
   p.page_shift = 0;
   while ((1ll << p.page_shift) < page_len) ++p.page_shift;
   p.max_pages = (int)max_pages;

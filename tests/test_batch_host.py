@@ -127,3 +127,16 @@ def test_attention_workspace_holds_a_gigabyte_of_partials_at_most(hq, hkv, D):
         for kv in (1, 100, 4096, 131072, 1 << 20):            # (those of short calls and of long ones: a gigabyte each, and the sums' share)
             assert 256 <= size(batch, tokens, hq, hkv, D, new, kv, 0, 0) <= (2 << 30) * 1.02
     assert size(1, 1, hq, hkv, D, 1, 64, 0, 0) == 256       # one chunk: nothing to keep
+
+
+@pytest.mark.parametrize("tokens,new", [(1, 1), (300, 300)])
+def test_a_window_or_sinks_beyond_any_sequence_are_planned_like_a_large_one(tokens, new):
+    """The largest int64, as a caller without a window may write it: the same chunks and workspace as any window that no sequence fills."""
+    size = lambda window, sinks, kv=32768: L.lib().subspec_paged_attention_workspace(1, tokens, 28, 4, 128, new, kv, window, sinks)
+    for huge in ((1 << 31) - 1, 1 << 31, 1 << 40, (1 << 62) - 1, (1 << 63) - 200, (1 << 63) - 1):
+        assert size(huge, 0) == size(1 << 30, 0) == size(0, 0) > 256
+        assert size(1024, huge) == size(1024, 1 << 30) == size(0, 0)
+        assert size(huge, huge) == size(0, 0)
+        assert _attention(n=tokens, new=new, hq=28, hkv=4, qs=28 * 128, kv=32768, window=huge, sinks=huge) == -2       # the same workspace is asked for
+    for kv in ((1 << 30) + 1, (1 << 63) - 1):                   # (the call refuses these rows: nothing to keep)
+        assert size(0, 0, kv) == 256 and _attention(kv=kv) == -1

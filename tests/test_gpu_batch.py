@@ -438,3 +438,14 @@ def test_thousands_of_sequences_under_a_large_bound():
     want, weight, worst = ob.attention(q[17:18], pool[rows].cpu(), [list(range(len(rows)))], [0, 1], [long])
     tol = _tolerance(want, weight, worst, torch.bfloat16, long, float(pool.abs().max()), D)
     assert ((got[17:18].double().cpu() - want).abs() / tol).max().item() <= 1.0
+
+
+@pytest.mark.parametrize("lens", [[(900, 1), (300, 2)], [(700, 130), (64, 1)]], ids=str)
+def test_a_window_beyond_any_sequence_is_none(lens):
+    g = torch.Generator().manual_seed(63)
+    q, pool, table, starts, kv = _batch(g, lens, 16, 8, 2, 128, torch.bfloat16)
+    args = (q.to(DEV), pool.to(DEV), _i32(table), _i32(starts), _i32(kv), max(n for _, n in lens), max(kv))
+    plain = ops.paged_attention(*args)
+    for window, sinks in [((1 << 63) - 1, 0), ((1 << 63) - 1, (1 << 63) - 1), (7, (1 << 63) - 1), (1 << 31, 5)]:
+        print("window", window, sinks, flush=True)
+        assert torch.equal(ops.paged_attention(*args, window=window, sinks=sinks), plain)
