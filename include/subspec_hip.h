@@ -338,7 +338,9 @@ int subspec_kv_append_paged(const void* k, int64_t k_token_stride, int64_t k_hea
  *              (multiples of 8; a slice of a fused projection's output)
  * block_table, query_starts, kv_lens   device, as the plan leaves them (kv_lens: its total_lens)
  * max_new      no sequence brings more new tokens;  max_kv: no kv_lens is larger.  They lay out the launches and the workspace and may be larger
- *              than what a call meets; tokens and rows beyond them are left out (either 0: nothing is written)
+ *              than what a call meets.  Of a sequence that exceeds them the tokens from max_new on are left out (their rows of out stay
+ *              as they were) and the cached rows from max_kv on are not seen; positions are those above, p = kv_lens[b] - n + i with
+ *              the sequence's own n (either bound 0: nothing is written)
  * out          device [n_tokens, n_q_heads, head_dim]; rows behind query_starts[batch] are left as they were
  * workspace    subspec_paged_attention_workspace bytes of the same sizes, 16-byte aligned
  * Page numbers are clamped to the pool, so a bad table reads wrong rows and never leaves it.  Rows that no token of the call sees (those behind

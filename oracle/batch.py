@@ -27,9 +27,9 @@ def plan(kv_lens, new_lens, free_pages, block_table, page_len, n_tokens):
                 counts=[starts[-1], taken, len(stack), 0])
 
 
-def attention(q, pool_layer, block_table, query_starts, kv_lens, window=0, sinks=0, scale=None):
+def attention(q, pool_layer, block_table, query_starts, kv_lens, window=0, sinks=0, scale=None, max_kv=None):
     """(out, weight) float64 [tokens, Hq, D]: ``weight`` is the same average over |v|, what the rounding of a probability acts on; and the
-    largest sum of |q_d k_d| times the scale, what the rounding of a score acts on."""
+    largest sum of |q_d k_d| times the scale, what the rounding of a score acts on.  ``max_kv``: rows from it on are not seen."""
     T, Hq, D = q.shape
     P, Hkv = pool_layer.shape[2], pool_layer.shape[3]
     scale = D ** -0.5 if scale is None else scale
@@ -44,12 +44,16 @@ def attention(q, pool_layer, block_table, query_starts, kv_lens, window=0, sinks
         seen = j <= p
         if window:
             seen &= (j > p - window) | (j < sinks)
+        if max_kv is not None:
+            seen &= j < max_kv
         some = seen.any(1)
+        if not some.any():
+            continue
         for h in range(Hq):
             k, v, rows = kv[:, 0, h // (Hq // Hkv)], kv[:, 1, h // (Hq // Hkv)], q[first:first + n, h].double()[some]
             a = torch.softmax((rows @ k.t() * scale).masked_fill(~seen[some], -math.inf), 1)
             size = (rows.abs() @ k.abs().t()).masked_fill(~seen[some], 0.0)
-            worst = max([worst] + [float(size.max()) * scale] * bool(some.any()))
+            worst = max(worst, float(size.max()) * scale)
             out[first:first + n, h][some], weight[first:first + n, h][some] = a @ v, a @ v.abs()
     return out, weight, worst
 

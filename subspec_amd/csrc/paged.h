@@ -35,30 +35,40 @@ struct PagedParams {
   int tiles;                               // tiles of a KV head that the launch has room for
 };
 
-// keys a row at position pos sees: j <= pos, and with a window w only j > pos - w or j < sinks
-__device__ __forceinline__ bool paged_sees(const PagedParams& p, int pos, int j) {
-  return j <= pos && (p.window == 0 || j > pos - p.window || j < p.sinks);
-}
-
-struct PagedSequence { int b, first, n, len; };
+// A sequence's tokens that the call computes, `n` from `first` on, the position of the first of them, and the keys that there are.  The bounds max_new
+// and max_kv leave tokens and keys out; they move no position, so pos0 comes from the lengths as they are.  (No token of a sequence can be more
+// than 2^30 behind its first: below -2^30 a position is as good as there.)
+struct PagedSequence { int b, first, n, pos0, len; };
 __device__ __forceinline__ PagedSequence paged_sequence(const PagedParams& p, int b) {
   PagedSequence s;
   s.b = b;
+  const int end = p.starts[b + 1], rows = max(p.lens[b], 0);
   s.first = min(max(p.starts[b], 0), p.n_tokens);
-  s.n = min(min(p.starts[b + 1], p.n_tokens) - s.first, p.max_new);
-  s.len = max(min(p.lens[b], p.max_kv), 0);        // (max_kv is within the table: the host saw to it)
+  s.n = min(min(end, p.n_tokens) - s.first, p.max_new);
+  s.pos0 = (int)max((int64_t)rows - ((int64_t)end - s.first), -(1ll << 30));
+  s.len = min(rows, p.max_kv);                     // (max_kv is within the table: the host saw to it)
   return s;
 }
+// keys a row at position pos (-1: none) sees: j <= pos, and with a window w only j > pos - w or j < sinks
+__device__ __forceinline__ bool paged_sees(const PagedParams& p, int len, int pos, int j) {
+  return j <= min(pos, len - 1) && (p.window == 0 || j > pos - p.window || j < p.sinks);
+}
 
-// The keys that rows at positions pos0 .. len - 1 see between them: [0, sinks) and [low, high), as one range of `length` virtual keys in
-// blocks of `block`: the first `skip` of them are keys 0 .., the others keys `start` .. (start and skip are multiples of the block).
-struct PagedSpan { int skip, start, low, length; };
-__device__ __forceinline__ PagedSpan paged_span(const PagedParams& p, int pos0, int high, int block) {
+// The keys that rows at positions pos_lo .. pos_hi see between them: [0, sinks) and [low, high), as one range of `length` virtual keys in
+// blocks of `block`: the first `skip` of them are keys 0 .., the others keys `start` .. (start and skip are multiples of the block).  Where all windows
+// begin behind the last key there are the sinks alone, keys [0, high).
+struct PagedSpan { int skip, start, low, high, length; };
+__device__ __forceinline__ PagedSpan paged_span(const PagedParams& p, int len, int pos_lo, int pos_hi, int block) {
   PagedSpan s;
-  s.low = p.window ? max(0, pos0 - p.window + 1) : 0;
+  s.low = p.window ? max(0, max(pos_lo, 0) - p.window + 1) : 0;
+  s.high = max(0, min(pos_hi + 1, len));
+  if (s.low >= s.high) {
+    s.low = 0;
+    if (p.window) s.high = min(s.high, p.sinks);
+  }
   s.start = s.low & -block;
   s.skip = min((int)(((int64_t)p.sinks + block - 1) & -block), s.start);
-  s.length = max(0, s.skip + high - s.start);
+  s.length = s.skip + s.high - s.start;
   return s;
 }
 __device__ __forceinline__ int paged_real(const PagedSpan& s, int v) { return v < s.skip ? v : v - s.skip + s.start; }

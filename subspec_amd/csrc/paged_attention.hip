@@ -42,11 +42,10 @@ __global__ __launch_bounds__(64) void paged_few_kernel(PagedParams p) {
   const PagedSequence sq = paged_sequence(p, b);
   const int rows = sq.n * p.group;
   if (sq.n <= 0 || rows > p.few.rows) return;
-  const PagedSpan sp = paged_span(p, sq.len - sq.n, sq.len, kFewKeys);
+  const PagedSpan sp = paged_span(p, sq.len, sq.pos0, sq.pos0 + sq.n - 1, kFewKeys);
   const int chunks = paged_chunks(sp, p.few.chunk_keys);
   if (chunk >= chunks) return;
   const int lane = threadIdx.x, lq = lane & 15, lg = lane >> 4;
-  const int pos0 = sq.len - sq.n;
 
   dec_u4 q[ROWT][D / 32];
   int pos[ROWT];
@@ -56,7 +55,7 @@ __global__ __launch_bounds__(64) void paged_few_kernel(PagedParams p) {
     const int r = nt * 16 + lq, i = r / p.group;
     const bool ok = r < rows;
     const int token = sq.first + (ok ? i : 0), head = kvh * p.group + (ok ? r - i * p.group : 0);
-    pos[nt] = ok ? pos0 + i : -1;
+    pos[nt] = ok ? max(sq.pos0 + i, -1) : -1;
     out_at[nt] = (int64_t)token * p.hq + head;
     const uint16_t* src = p.q + token * p.q_token + head * p.q_head + lg * 8;
 #pragma unroll
@@ -132,7 +131,8 @@ __global__ __launch_bounds__(64) void paged_few_kernel(PagedParams p) {
         const uint2 lo = lds_tr16(va), hi = lds_tr16(va + 16 * kRowBytes);
         vt[mt] = dec_u4{lo.x, lo.y, hi.x, hi.y};
       }
-      const bool plain = kb + kFewKeys - 1 <= pos0 && (p.window == 0 || kb > sq.len - 1 - p.window || kb + kFewKeys <= p.sinks);
+      const bool plain = kb + kFewKeys - 1 <= min(sq.pos0, sq.len - 1) &&
+                         (p.window == 0 || kb > sq.pos0 + sq.n - 1 - p.window || kb + kFewKeys <= p.sinks);
       dec_u4 pb[ROWT];
 #pragma unroll
       for (int nt = 0; nt < ROWT; ++nt) {
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(64) void paged_few_kernel(PagedParams p) {
         if (!plain) {
 #pragma unroll
           for (int r = 0; r < 8; ++r)
-            if (!paged_sees(p, pos[nt], kb + (r >> 2) * 16 + 4 * lg + (r & 3))) x[r] = -INFINITY;
+            if (!paged_sees(p, sq.len, pos[nt], kb + (r >> 2) * 16 + 4 * lg + (r & 3))) x[r] = -INFINITY;
         }
         const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
         if (__any(top > ref[nt] + kSlack)) {                 // (also where the reference is still -inf)
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
   const PagedSequence sq = paged_sequence(p, mine ? bk / p.hkv : 0);
   mine = mine && r < sq.n * p.group && sq.n * p.group <= rows;
   int chunks = 1;
-  if (mine) chunks = paged_chunks(paged_span(p, sq.len - sq.n, sq.len, kFewKeys), p.few.chunk_keys);
+  if (mine) chunks = paged_chunks(paged_span(p, sq.len, sq.pos0, sq.pos0 + sq.n - 1, kFewKeys), p.few.chunk_keys);
   mine = mine && chunks > 1;                                 // (one chunk: complete already)
   if (WAVES == 4 && !mine) return;                           // (the whole workgroup)
   const int d4 = (tid % kLanes) * 4, side = tid / kLanes;

@@ -125,9 +125,9 @@ __device__ __forceinline__ float max_halves(float x) {                 // of lan
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 struct TileRow { int pos; float ref, l; bool have; };
-// keys kb .. kb + 63 that a row at `pos` sees, as bits
-__device__ __forceinline__ uint64_t seen_bits(const PagedParams& p, int pos, int kb) {
-  const int left = pos - kb;
+// keys kb .. kb + 63 that a row at `pos` sees of `len`, as bits (paged_sees)
+__device__ __forceinline__ uint64_t seen_bits(const PagedParams& p, int len, int pos, int kb) {
+  const int left = min(pos, len - 1) - kb;
   uint64_t bits = left < 0 ? 0ull : left >= 63 ? ~0ull : (2ull << left) - 1ull;
   if (p.window) {
     const int low = pos - p.window + 1 - kb, first = p.sinks - kb;
@@ -138,10 +138,10 @@ __device__ __forceinline__ uint64_t seen_bits(const PagedParams& p, int pos, int
   return bits;
 }
 template <int DT, int D>
-__device__ __forceinline__ void softmax_phase(const PagedParams& p, int kb, bool plain, int g, TileRow& row, v16f (&s)[2], v16f (&o)[D / 32],
+__device__ __forceinline__ void softmax_phase(const PagedParams& p, int len, int kb, bool plain, int g, TileRow& row, v16f (&s)[2], v16f (&o)[D / 32],
                                               v16f& cinit, dec_u4 (&pb)[4]) {
   if (!plain) {
-    const uint64_t bits = seen_bits(p, row.pos, kb);
+    const uint64_t bits = seen_bits(p, len, row.pos, kb);
     const uint32_t half[2] = {(uint32_t)bits >> (4 * g), (uint32_t)(bits >> 32) >> (4 * g)};
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -193,9 +193,8 @@ __device__ __forceinline__ bool tile_place(const PagedParams& p, int u, TilePlac
   t->row0 = t->tile * kTileRows;
   if (t->sq.n <= 0 || t->rows <= p.few.rows || t->row0 >= t->rows) return false;
   t->row1 = min(t->rows, t->row0 + kTileRows);
-  const int pos0 = t->sq.len - t->sq.n;
-  t->pos_lo = pos0 + t->row0 / p.group;
-  t->pos_hi = pos0 + (t->row1 - 1) / p.group;
+  t->pos_lo = t->sq.pos0 + t->row0 / p.group;
+  t->pos_hi = t->sq.pos0 + (t->row1 - 1) / p.group;
   return true;
 }
 
@@ -210,7 +209,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int chunk = (int)(rest / (uint32_t)p.tiles), u = p.tiles - 1 - (int)(rest % (uint32_t)p.tiles);
   TilePlace tp;
   if (!tile_place(p, u, &tp)) return;
-  const PagedSpan sp = paged_span(p, tp.pos_lo, max(tp.pos_hi + 1, 0), kTileKeys);
+  const PagedSpan sp = paged_span(p, tp.sq.len, tp.pos_lo, tp.pos_hi, kTileKeys);
   const int chunks = paged_chunks(sp, p.tile.chunk_keys);
   if (chunk >= chunks) return;
   const int v_begin = chunk * p.tile.chunk_keys, v_end = min(v_begin + p.tile.chunk_keys, sp.length);
@@ -220,7 +219,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int wrow = tp.row0 + wave * 32, r = wrow + lr;                 // packed rows of the sequence
   const bool live = wrow < tp.rows, row_ok = r < tp.rows;
   const bool second = wave >= 4;                                       // the second wavefront of its SIMD
-  const int pos0 = tp.sq.len - tp.sq.n;
+  const int pos0 = tp.sq.pos0, len = tp.sq.len;
   const int token = tp.sq.first + (row_ok ? r / p.group : 0), head = kvh * p.group + (row_ok ? r % p.group : 0);
   const int wave_lo = pos0 + wrow / p.group, wave_hi = pos0 + (min(tp.rows, wrow + 32) - 1) / p.group;
 
@@ -238,7 +237,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     s[0][i] = s[1][i] = cinit[i] = 0.f;
   }
   dec_u4 pb[4] = {};
-  TileRow row{row_ok ? pos0 + r / p.group : -1, 0.f, 0.f, false};
+  TileRow row{row_ok ? max(pos0 + r / p.group, -1) : -1, 0.f, 0.f, false};
 
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
   const int crow = lane / S::kPieces, cpiece = lane % S::kPieces;
@@ -288,7 +287,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     place(J, &v, &j, &shift);
     cp.block = J;
     cp.at = lds0 + (uint32_t)(J & (kStages - 1)) * S::kHalf + (uint32_t)(wave * 8 * S::kRowBytes);
-    cp.one_page = p.page_shift >= 3 && j + 7 <= tp.pos_hi && (j >= sp.low || j + 7 < p.sinks);
+    cp.one_page = p.page_shift >= 3 && j + 7 < sp.high && (j >= sp.low || j + 7 < p.sinks);
     cp.k = kbase + (int64_t)__builtin_amdgcn_readfirstlane(asked) * 2 * page_bytes + (j & tok_mask) * tok_bytes;
     cp.v = cp.k + page_bytes;
   };
@@ -309,7 +308,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       const int in = c * S::kRowsPerCopy + crow;
       int key = j + in;
       if (v < sp.skip) key = min(key, p.sinks - 1);
-      else key = min(key >= p.sinks ? max(key, sp.low) : key, tp.pos_hi);
+      else key = min(key >= p.sinks ? max(key, sp.low) : key, sp.high - 1);
       const char* at = kbase + (int64_t)pages[(key >> p.page_shift) + shift] * 2 * page_bytes + (key & tok_mask) * tok_bytes;
       dma16_from(cp.at + c * 1024, at + ((cpiece ^ S::k_swap(wave * 8 + in)) << 4));
       dma16_from(cp.at + S::kVRing + c * 1024, at + page_bytes + ((cpiece ^ S::v_swap(wave * 8 + in)) << 4));
@@ -347,8 +346,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
   auto softmax = [&](int i) {
     const int kb = paged_real(sp, v0 + i * kTileKeys);
-    const bool plain = kb + kTileKeys - 1 <= wave_lo && (p.window == 0 || kb > wave_hi - p.window || kb + kTileKeys <= p.sinks);
-    softmax_phase<DT, D>(p, kb, plain, g, row, s, o, cinit, pb);
+    const bool plain = kb + kTileKeys - 1 <= min(wave_lo, len - 1) && (p.window == 0 || kb > wave_hi - p.window || kb + kTileKeys <= p.sinks);
+    softmax_phase<DT, D>(p, len, kb, plain, g, row, s, o, cinit, pb);
   };
 
   for (; v0 < v_end; v0 = (int)min((int64_t)v_end, v0 + stretch)) {
@@ -439,7 +438,7 @@ __global__ __launch_bounds__(256) void paged_tile_merge_kernel(PagedParams p) {
   const int lane = threadIdx.x & 63, lr = lane & 31, g = lane >> 5, piece = blockIdx.y * 4 + threadIdx.x / 64;
   const int r = tp.row0 + wave * 32 + lr;
   if (tp.row0 + wave * 32 >= tp.rows) return;
-  const PagedSpan sp = paged_span(p, tp.pos_lo, max(tp.pos_hi + 1, 0), kTileKeys);
+  const PagedSpan sp = paged_span(p, tp.sq.len, tp.pos_lo, tp.pos_hi, kTileKeys);
   const int chunks = paged_chunks(sp, p.tile.chunk_keys);
   if (chunks == 1 || r >= tp.rows) return;
   const int64_t slot = (((int64_t)u * p.hkv + kvh) * p.tile.chunks) * 8 + wave;

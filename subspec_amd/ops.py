@@ -529,7 +529,9 @@ def paged_attention(q: torch.Tensor, pool_layer: torch.Tensor, block_table: torc
     """Causal attention of a batch's packed new tokens ``q`` [tokens, Hq, D] (D 64 or 128, bf16 / fp16; a view of a fused projection's output is
     read where it is) over their sequences' rows in ``pool_layer`` [max_pages, 2, page_len, Hkv, D], whose K / V are already there
     (``kv_append_paged_``).  ``block_table``, ``query_starts`` and ``kv_lens`` as ``paged_batch_plan`` leaves them.  ``max_new`` and ``max_kv`` bound the
-    new tokens and the rows of any one sequence: they lay out the launch, need not be tight, and rows beyond them are left out.
+    new tokens and the rows of any one sequence: they lay out the launch and need not be tight.  Of a sequence that exceeds them the
+    tokens from ``max_new`` on are left as they were in ``out`` and the cached rows from ``max_kv`` on are not seen (a bound of 0: nothing is
+    written); what the other tokens see stays what their positions say.
 
     ``window``: a token sees its own row and the ``window - 1`` before it (None or 0: all), and the first ``sinks`` rows besides.  A token that sees
     no row gets zeros.  Returns [tokens, Hq * D]; rows behind the last sequence's are left as they were in ``out``.

@@ -449,3 +449,34 @@ def test_a_window_beyond_any_sequence_is_none(lens):
     for window, sinks in [((1 << 63) - 1, 0), ((1 << 63) - 1, (1 << 63) - 1), (7, (1 << 63) - 1), (1 << 31, 5)]:
         print("window", window, sinks, flush=True)
         assert torch.equal(ops.paged_attention(*args, window=window, sinks=sinks), plain)
+
+
+CUT = [[(40, 40)], [(13, 13), (1, 1)], [(100, 13), (90, 90), (30, 1)], [(900, 60), (700, 3), (900, 1), (5, 9)], [(3, 50), (2000, 300)]]
+
+
+@pytest.mark.parametrize("dtype,Hq,Hkv,D", [(torch.bfloat16, 7, 1, 128), (torch.float16, 4, 2, 64)])
+@pytest.mark.parametrize("lens", CUT, ids=str)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (33, 0), (33, 5), (64, 70), (500, 3)])
+def test_bounds_leave_tokens_and_rows_out_and_move_no_position(dtype, Hq, Hkv, D, lens, window, sinks):
+    """max_new and max_kv below what a sequence brings: tokens from max_new on stay as they were, rows from max_kv on are not seen (and
+    hold NaN here), and every other token sees what its position says, from either kernel and where its window begins behind max_kv."""
+    g = torch.Generator().manual_seed(sum(t for t, _ in lens) + Hq + window)
+    q, pool, table, starts, kv = _batch(g, lens, 16, Hq, Hkv, D, dtype)
+    before = pool.clone()
+    most_new, most_kv = max(n for _, n in lens), max(kv)
+    for max_new, max_kv in [(most_new, 20), (1, most_kv), (2, 20), (12, most_kv), (12, 64), (most_new, max(1, most_kv - 70)), (50, 333), (most_new, 1)]:
+        print("cut", dtype, Hq, lens, window, sinks, max_new, max_kv, flush=True)
+        pool.copy_(before)
+        for b, t in enumerate(kv):
+            for j in range(max_kv, t):
+                pool[table[b][j // 16], :, j % 16] = float("nan")
+        want, weight, worst = ob.attention(q, before, table, starts, kv, window, sinks, max_kv=max_kv)
+        out = torch.full((q.shape[0], Hq * D), 6.0, dtype=dtype, device=DEV)
+        ops.paged_attention(q.to(DEV), pool.to(DEV), _i32(table), _i32(starts), _i32(kv), max_new, max_kv, window=window, sinks=sinks, out=out)
+        got = out.double().cpu().view(want.shape)
+        tol = _tolerance(want, weight, worst, dtype, max(kv), float(before.nan_to_num(0.0).abs().max()), D)
+        for b, (_, n) in enumerate(lens):
+            kept = slice(starts[b], starts[b] + min(n, max_new))
+            assert torch.isfinite(got[kept]).all().item(), (b, max_new, max_kv)
+            assert ((got[kept] - want[kept]).abs() / tol[kept]).max().item() <= 1.0, (b, max_new, max_kv)
+            assert got[kept.stop:starts[b + 1]].eq(6.0).all(), (b, max_new, max_kv)
