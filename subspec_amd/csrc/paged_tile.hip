@@ -185,13 +185,15 @@ __device__ __forceinline__ void softmax_phase(const PagedParams& p, int len, int
   row.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
+// Where tile u lies, and whether it has rows.  A tile before the first sequence's (tokens before starts[0]: nobody's), like one behind the last of its
+// sequence, has none.
 struct TilePlace { PagedSequence sq; int tile, rows, row0, row1, pos_lo, pos_hi; };
 __device__ __forceinline__ bool tile_place(const PagedParams& p, int u, TilePlace* t) {
   t->sq = paged_sequence(p, __builtin_amdgcn_readfirstlane(paged_tile_owner(p, u)));
   t->tile = u - paged_first_tile(p, t->sq.b);
   t->rows = t->sq.n * p.group;
   t->row0 = t->tile * kTileRows;
-  if (t->sq.n <= 0 || t->rows <= p.few.rows || t->row0 >= t->rows) return false;
+  if (t->sq.n <= 0 || t->rows <= p.few.rows || t->tile < 0 || t->row0 >= t->rows) return false;
   t->row1 = min(t->rows, t->row0 + kTileRows);
   t->pos_lo = t->sq.pos0 + t->row0 / p.group;
   t->pos_hi = t->sq.pos0 + (t->row1 - 1) / p.group;

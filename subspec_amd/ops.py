@@ -534,7 +534,8 @@ def paged_attention(q: torch.Tensor, pool_layer: torch.Tensor, block_table: torc
     written); what the other tokens see stays what their positions say.
 
     ``window``: a token sees its own row and the ``window - 1`` before it (None or 0: all), and the first ``sinks`` rows besides.  A token that sees
-    no row gets zeros.  Returns [tokens, Hq * D]; rows behind the last sequence's are left as they were in ``out``.
+    no row gets zeros.  Returns [tokens, Hq * D]; rows before the first sequence's (``query_starts`` of a part of a batch) and behind
+    the last one's are left as they were in ``out``.
     Replaces the prefill and decode wrappers of specdecodes/models/utils/flashinfer/attention_wrapper.py:71-137."""
     dev = _require_gpu(q, pool_layer, block_table, query_starts, kv_lens)
     max_pages, page_len, Hkv, D = _pool_layer_shape(pool_layer)

@@ -480,3 +480,23 @@ def test_bounds_leave_tokens_and_rows_out_and_move_no_position(dtype, Hq, Hkv, D
             assert torch.isfinite(got[kept]).all().item(), (b, max_new, max_kv)
             assert ((got[kept] - want[kept]).abs() / tol[kept]).max().item() <= 1.0, (b, max_new, max_kv)
             assert got[kept.stop:starts[b + 1]].eq(6.0).all(), (b, max_new, max_kv)
+
+
+@pytest.mark.parametrize("lens", [[(700, 130), (64, 1)], [(500, 40), (300, 300), (41, 41)], [(90, 1), (33, 1)]], ids=str)
+@pytest.mark.parametrize("before", [5, 37, 100, 1000])
+def test_rows_before_the_first_sequence_stay(lens, before):
+    """The last sequences of a batch alone, through views of its lengths, starts and table: the tokens of the others are not theirs."""
+    print("rows before", lens, before, flush=True)
+    g = torch.Generator().manual_seed(before + len(lens))
+    Hq, Hkv, D, dtype = 14, 2, 128, torch.bfloat16
+    q, pool, table, starts, kv = _batch(g, lens, 16, Hq, Hkv, D, dtype)
+    want, weight, worst = ob.attention(q, pool, table, starts, kv)
+    room = torch.randn(before, Hq, D, generator=g).to(dtype)
+    starts_all = _i32([0, 0] + [s + before for s in starts])                     # two others before them
+    out = torch.full((before + q.shape[0], Hq * D), 6.0, dtype=dtype, device=DEV)
+    lens_all = _i32([50, 60] + kv)
+    table_all = _i32([[0] * len(table[0])] * 2 + table)
+    ops.paged_attention(torch.cat([room, q]).to(DEV), pool.to(DEV), table_all[2:], starts_all[2:], lens_all[2:], max(n for _, n in lens), max(kv), out=out)
+    assert out[:before].eq(6.0).all()
+    tol = _tolerance(want, weight, worst, dtype, max(kv), float(pool.nan_to_num(0.0).abs().max()), D)
+    assert ((out[before:].double().cpu().view(want.shape) - want).abs() / tol).max().item() <= 1.0
