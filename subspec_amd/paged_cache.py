@@ -220,12 +220,17 @@ class KvBatch:
         self.max_new, self.max_kv = max(new), max(total)
         return self.plan
 
+    def _current(self) -> Dict[str, torch.Tensor]:
+        if self.plan is None:
+            raise ValueError("no step to append to or attend in: step() comes first, and nothing comes after close()")
+        return self.plan
+
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
-        ops.kv_append_paged_(self.pool.cache_data[layer], k, v, self.plan["slots"])
+        ops.kv_append_paged_(self.pool.cache_data[layer], k, v, self._current()["slots"])
 
     def attention(self, layer: int, q: torch.Tensor, window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None,
                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        return ops.paged_attention(q, self.pool.cache_data[layer], self.block_table, self.plan["query_starts"], self.kv_lens, self.max_new,
+        return ops.paged_attention(q, self.pool.cache_data[layer], self.block_table, self._current()["query_starts"], self.kv_lens, self.max_new,
                                    self.max_kv, window=window, sinks=sinks, scale=scale, out=out)
 
     def release(self, index: int) -> None:
@@ -240,8 +245,9 @@ class KvBatch:
         self.kv_lens[index].zero_()                            # (an assignment of a number would wait for the device)
 
     def close(self) -> None:
-        """All pages go back to the pool."""
+        """All pages go back to the pool, which may hand them to anyone: the last step's plan, whose slots lie in them, goes with them."""
         self.pool.deallocate(self.pages)
+        self.plan = None
         self.pages, self.num_free, self.lens = [], 0, [0] * len(self.lens)
         self.n_free, self.kv_lens = torch.zeros_like(self.n_free), torch.zeros_like(self.kv_lens)
 

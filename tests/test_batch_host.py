@@ -140,3 +140,36 @@ def test_a_window_or_sinks_beyond_any_sequence_are_planned_like_a_large_one(toke
         assert _attention(n=tokens, new=new, hq=28, hkv=4, qs=28 * 128, kv=32768, window=huge, sinks=huge) == -2       # the same workspace is asked for
     for kv in ((1 << 30) + 1, (1 << 63) - 1):                   # (the call refuses these rows: nothing to keep)
         assert size(0, 0, kv) == 256 and _attention(kv=kv) == -1
+
+
+def _cpu_batch(places=2, pages=8):
+    from subspec_amd.paged_cache import KvBatch, KvCachePool
+    pool = KvCachePool(max_pages=pages, num_layers=1, num_heads=2, head_dim=64, page_len=4, dtype=torch.bfloat16, device="cpu")
+    return pool, KvBatch(pool, places, 40)
+
+
+def test_nothing_is_appended_without_a_step_or_after_close(monkeypatch):
+    """The pages of a closed batch belong to whoever asks the pool next: the last plan's slots must not reach an append."""
+    from subspec_amd import ops
+    calls = []
+    monkeypatch.setattr(ops, "kv_append_paged_", lambda *a, **k: calls.append("append"))
+    monkeypatch.setattr(ops, "paged_attention", lambda *a, **k: calls.append("attention"))
+    pool, batch = _cpu_batch()
+    k, q = torch.zeros(2, 2, 64, dtype=torch.bfloat16), torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+
+    def refused():
+        with pytest.raises(ValueError, match="step"):
+            batch.append(0, k, k)
+        with pytest.raises(ValueError, match="step"):
+            batch.attention(0, q)
+
+    refused()
+    batch.plan = dict(slots=torch.arange(2), query_starts=torch.tensor([0, 1, 2], dtype=torch.int32), kv_lens=torch.tensor([1, 1], dtype=torch.int32))
+    batch.append(0, k, k)
+    batch.attention(0, q)
+    assert calls == ["append", "attention"]
+    batch.close()
+    assert int(pool.num_free_pages()) == 8
+    refused()
+    batch.close()                                              # a second time does nothing
+    assert int(pool.num_free_pages()) == 8 and calls == ["append", "attention"]
