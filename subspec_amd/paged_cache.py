@@ -230,11 +230,13 @@ class KvBatch:
 
     def attention(self, layer: int, q: torch.Tensor, window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None,
                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        return ops.paged_attention(q, self.pool.cache_data[layer], self.block_table, self._current()["query_starts"], self.kv_lens, self.max_new,
+        plan = self._current()                                 # (its lengths, not self.kv_lens: those may already lack a released sequence)
+        return ops.paged_attention(q, self.pool.cache_data[layer], self.block_table, plan["query_starts"], plan["kv_lens"], self.max_new,
                                    self.max_kv, window=window, sinks=sinks, scale=scale, out=out)
 
     def release(self, index: int) -> None:
-        """Sequence ``index`` is done: its pages are free again and its place is empty."""
+        """Sequence ``index`` is done: its pages are free again and its place is empty, from the next ``step`` on.  Until then nobody gets the pages,
+        so the layers that the present step has left still append to them and read them."""
         n = self._pages(self.lens[index])
         self.free_pages = self.free_pages.clone()             # (a step on another stream may still read the old ones)
         self.free_pages[self.num_free:self.num_free + n] = self.block_table[index, :n]

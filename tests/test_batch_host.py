@@ -173,3 +173,17 @@ def test_nothing_is_appended_without_a_step_or_after_close(monkeypatch):
     refused()
     batch.close()                                              # a second time does nothing
     assert int(pool.num_free_pages()) == 8 and calls == ["append", "attention"]
+
+
+def test_a_release_between_layers_leaves_the_step_its_lengths(monkeypatch):
+    from subspec_amd import ops
+    seen = []
+    monkeypatch.setattr(ops, "paged_attention", lambda q, pool, table, starts, lens, *a, **k: seen.append((starts.tolist(), lens.tolist())))
+    pool, batch = _cpu_batch()
+    lens = torch.tensor([9, 5], dtype=torch.int32)
+    batch.plan = dict(slots=torch.arange(3), query_starts=torch.tensor([0, 2, 3], dtype=torch.int32), kv_lens=lens)
+    batch.kv_lens, batch.lens, batch.num_free = lens, [9, 5], 3
+    batch.attention(0, torch.zeros(3, 4, 64))
+    batch.release(0)
+    batch.attention(0, torch.zeros(3, 4, 64))
+    assert seen == [([0, 2, 3], [9, 5])] * 2 and batch.kv_lens.tolist() == [0, 5] and batch.lens == [0, 5]

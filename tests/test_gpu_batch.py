@@ -500,3 +500,29 @@ def test_rows_before_the_first_sequence_stay(lens, before):
     assert out[:before].eq(6.0).all()
     tol = _tolerance(want, weight, worst, dtype, max(kv), float(pool.nan_to_num(0.0).abs().max()), D)
     assert ((out[before:].double().cpu().view(want.shape) - want).abs() / tol).max().item() <= 1.0
+
+
+def test_a_sequence_released_between_layers_is_computed_to_the_step_s_end():
+    from subspec_amd.paged_cache import KvBatch, KvCachePool
+    g = torch.Generator().manual_seed(71)
+    Hq, Hkv, D, dtype = 8, 2, 64, torch.float16
+    pool = KvCachePool(max_pages=20, num_layers=2, num_heads=Hkv, head_dim=D, page_len=8, dtype=dtype, device=DEV)
+    batch = KvBatch(pool, 3, 60)
+    qkv = torch.randn(2, 50, Hq + 2 * Hkv, D, generator=g).to(dtype).to(DEV)
+    rows = [0, 21, 22, 50]
+    batch.step([21, 1, 28])
+    outs = []
+    for layer in range(2):
+        batch.append(layer, qkv[layer, :, Hq:Hq + Hkv], qkv[layer, :, Hq + Hkv:])
+        outs.append(batch.attention(layer, qkv[layer, :, :Hq]))
+        if layer == 0:
+            batch.release(0)
+    for layer, out in enumerate(outs):
+        for b in range(3):
+            one = qkv[layer, rows[b]:rows[b + 1]].cpu()
+            want, weight, worst = _dense(one[:, :Hq], one[:, Hq:Hq + Hkv], one[:, Hq + Hkv:], 0, 0)
+            tol = _tolerance(want, weight, worst, dtype, len(one), float(one.abs().max()), D)
+            got = out[rows[b]:rows[b + 1]].double().cpu().view(want.shape)
+            assert ((got - want).abs() / tol).max().item() <= 1.0, (layer, b)
+    batch.step([0, 1, 1])                                      # the place is empty, its three pages are free
+    assert batch.plan["kv_lens"].tolist() == [0, 2, 29] and batch.plan["counts"].tolist() == [2, 0, 15, 0]
