@@ -177,7 +177,9 @@ class KvBatch:
         out = batch.attention(layer, q)            # q [tokens, heads, head_dim] -> [tokens, heads * head_dim]
 
     The host keeps the lengths too, so running out of pages or of table columns is an error before anything is launched, and nothing waits
-    for the device."""
+    for the device.  That is also why ``step`` and ``release`` cannot be part of a captured graph, whose replays would move no host length (and
+    would copy new lengths out of host memory long given back): a captured step calls the operators with ``out=`` itself.  Sequences grow
+    and end; none is shortened."""
 
     def __init__(self, pool: KvCachePool, max_batch: int, max_len: int, num_pages: Optional[int] = None):
         if not 1 <= int(max_batch) <= L.MAX_BATCH:
@@ -197,9 +199,14 @@ class KvBatch:
     def _pages(self, rows: int) -> int:
         return (rows + self.page_len - 1) // self.page_len
 
+    def _not_captured(self, what: str) -> None:
+        if self.pool.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise ValueError(f"KvBatch.{what} keeps lengths on the host and cannot be captured into a graph")
+
     def step(self, new_lens: Sequence[int], n_tokens: Optional[int] = None) -> Dict[str, torch.Tensor]:
         """Pages and slots for ``new_lens[b]`` new tokens of every sequence; returns the plan (``ops.paged_batch_plan``).  ``n_tokens``: rows of
         its token outputs, default the new tokens of all sequences."""
+        self._not_captured("step")
         new = [int(n) for n in new_lens]
         if len(new) != len(self.lens) or min(new) < 0:
             raise ValueError(f"expected {len(self.lens)} numbers of new tokens, none below zero")
@@ -237,6 +244,7 @@ class KvBatch:
     def release(self, index: int) -> None:
         """Sequence ``index`` is done: its pages are free again and its place is empty, from the next ``step`` on.  Until then nobody gets the pages,
         so the layers that the present step has left still append to them and read them."""
+        self._not_captured("release")
         n = self._pages(self.lens[index])
         self.free_pages = self.free_pages.clone()             # (a step on another stream may still read the old ones)
         self.free_pages[self.num_free:self.num_free + n] = self.block_table[index, :n]

@@ -541,3 +541,35 @@ def test_a_plan_into_an_earlier_one_s_outputs_looks_at_every_tensor_once(monkeyp
     alone = len(asked)
     again = ops.paged_batch_plan(*args, out=plan)
     assert again is plan and alone == 11 and len(asked) - alone <= 2 * alone
+
+
+def test_a_batch_refuses_to_be_captured_and_its_layers_can_be():
+    from subspec_amd.paged_cache import KvBatch, KvCachePool
+    g = torch.Generator().manual_seed(72)
+    pool = KvCachePool(max_pages=8, num_layers=1, num_heads=2, head_dim=64, page_len=16, dtype=torch.bfloat16, device=DEV)
+    batch = KvBatch(pool, 2, 64)
+    qkv = torch.randn(5, 8, 64, generator=g).to(torch.bfloat16).to(DEV)
+    batch.step([3, 2])
+
+    def layer():
+        batch.append(0, qkv[:, 4:6], qkv[:, 6:])
+        return batch.attention(0, qkv[:, :4])
+
+    layer()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(ValueError, match="captured"):
+            batch.step([1, 1])
+        with pytest.raises(ValueError, match="captured"):
+            batch.release(0)
+        out = layer()
+    assert batch.lens == [3, 2] and batch.num_free == 6
+    for i in range(3):
+        qkv.copy_(torch.randn(5, 8, 64, generator=g).to(torch.bfloat16))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(layer(), out), i
+        (torch.randn(500, 500, device=DEV) @ torch.randn(500, 500, device=DEV)).sum().item()
+    batch.step([1, 1])
+    assert batch.plan["kv_lens"].tolist() == [4, 3]
