@@ -361,7 +361,8 @@ int subspec_paged_attention(const void* q, int64_t q_token_stride, int64_t q_hea
  * Entries are ordered by logit, larger first, equal ones by index, and entry j has the mass exp((l_j - l_max) / T).  Every filter keeps a
  * prefix of that order: top-k the first k; top-p the entries with less than p times the mass of those k before them;
  * min-p those with at least min_p times the first entry's mass.  The first entry always stays.  The draw is the first entry
- * whose mass added to that of all before it exceeds u times the mass of what stays.  Masses are summed exactly, to 2^-42 of the largest.
+ * whose mass added to that of all before it exceeds u times the mass of what stays.  Masses are whole multiples of 2^-42 of the largest, each
+ * within 0.54 of that unit, and are summed exactly.
  * Replaces  TemperatureLogitsWarper, TopKLogitsWarper, TopPLogitsWarper (sort, cumsum, scatter over the vocabulary), softmax and multinomial
  *           specdecodes/models/generators/base.py:42-64,116-132
  *

@@ -6,13 +6,14 @@
 // So a row needs no sort: it needs the entry at a rank (top-k) and twice the entry at a mass (top-p, the draw).  A histogram of
 // (l_max - l) / T with counts and masses says in which bin each of the three lies; the entries of those bins alone are put in order.
 //
-// Masses are whole numbers, round(m * 2^42), of an exponential evaluated in 64 bits: their sums are exact and do not depend on the
-// order in which wavefronts add them, 2^20 entries stay below 2^62, and what rounds to zero (less than 2^-43 of the largest) is drawn with a
+// Masses are whole numbers, m * 2^42 rounded, of an exponential evaluated in 64 bits (within 0.54 of such a unit, see mass_series.h): their sums are
+// exact and do not depend on the order in which wavefronts add them, 2^20 entries stay below 2^62, and what rounds to zero (less than 2^-43 of the largest) is drawn with a
 // probability below 2^-23 even if a million such entries are there.  In fp32 the sum over a flat row of 150000 entries is off by more
 // than the step between two of them.
 // One row of 152064 fp32: 30 us, four dependent launches of 3 + 9 + 11 + 9; 64 rows bf16 (19.5 MB): 57, the exponentials in 64 bits 19 of them,
 // the sums of the slices' bins and the second pass 20, the search among the candidates 15.
 #include "common.h"
+#include "mass_series.h"
 #include <algorithm>
 
 namespace subspec {
@@ -20,7 +21,6 @@ namespace subspec {
 constexpr int kSampleThreads = 1024;      // of a workgroup that has a whole row
 constexpr int kSliceThreads = 512;        // ... a slice of one
 constexpr int kBins = 1024;
-constexpr int kMassBits = 42;
 constexpr float kReach = 29.9f;           // 43 ln 2 = 29.81: masses beyond round to zero
 constexpr int kCandidates = 4096;
 constexpr int kSliceCandidates = 1024;
@@ -60,34 +60,19 @@ __device__ __forceinline__ RowRule row_rule(const SampleArgs& a, int row) {
 struct RowTop { float value; double wide; bool only; };
 __device__ __forceinline__ RowTop row_top_of(float top, const RowRule& r) { return RowTop{top, (double)top, r.greedy || top == INFINITY}; }
 
-// 2^f * 2^42 for |f| <= 1/2: the Taylor series of e^(f ln 2) to the tenth power, its coefficients ln^k 2 / k! (remainder (ln 2 / 2)^11 / 11! =
-// 2.2e-13 of the value).  (They are held in registers of the wavefront: left to itself the compiler copies each into the result before it adds.)
+// 2^f * 2^42 for |f| <= 1/2.  (The coefficients are held in registers of the wavefront: left to itself the compiler copies each into the result before
+// it adds.)
 struct Series {
-  double c[11];
+  double c[kSeriesTerms];
   __device__ __forceinline__ Series() {
-    constexpr double of[11] = {1.0,
-                               6.9314718055994531e-1,
-                               2.4022650695910072e-1,
-                               5.5504108664821580e-2,
-                               9.6181291076284772e-3,
-                               1.3333558146428443e-3,
-                               1.5403530393381610e-4,
-                               1.5252733804059841e-5,
-                               1.3215486790144309e-6,
-                               1.0178086009239699e-7,
-                               7.0549116208011233e-9};
+    constexpr SeriesTable of = series_table();
 #pragma unroll
-    for (int i = 0; i < 11; ++i) {
-      c[i] = of[i] * (double)(1ull << kMassBits);
+    for (int i = 0; i < kSeriesTerms; ++i) {
+      c[i] = of.c[i];
       asm("" : "+v"(c[i]));
     }
   }
-  __device__ __forceinline__ double operator()(double f) const {
-    double s = c[10];
-#pragma unroll
-    for (int i = 9; i >= 0; --i) s = fma(s, f, c[i]);
-    return s;
-  }
+  __device__ __forceinline__ double operator()(double f) const { return series_value(c, f); }
 };
 // How far entry l is below the largest in units of T, in 32 bits: what the bins go by (falls as l rises, so bins keep the order).  Entries at kReach
 // and beyond, and NaN, have no mass and no bin.
