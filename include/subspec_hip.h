@@ -343,6 +343,7 @@ int subspec_kv_append_paged(const void* k, int64_t k_token_stride, int64_t k_hea
  *              the sequence's own n (either bound 0: nothing is written)
  * out          device [n_tokens, n_q_heads, head_dim]; rows before query_starts[0] and from query_starts[batch] on are left as they were
  * workspace    subspec_paged_attention_workspace bytes of the same sizes, 16-byte aligned
+ * Limits: 1 <= batch <= SUBSPEC_MAX_BATCH, n_q_heads <= 1024, max_kv and n_tokens <= 2^30, min(max_new, n_tokens) * group < 2^31 - 256.
  * Page numbers are clamped to the pool, so a bad table reads wrong rows and never leaves it.  Rows that no token of the call sees (those behind
  * kv_lens, those a window has passed, other sequences' pages) have no influence, whatever they hold.  Among the rows of one
  * call, an infinite or NaN VALUE row may reach tokens that do not see it, if they share a tile with one that does.

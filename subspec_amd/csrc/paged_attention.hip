@@ -423,6 +423,9 @@ extern "C" int subspec_paged_attention(const void* q, int64_t q_token_stride, in
       q_token_stride < 0 || q_head_stride < 0)
     SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: q, the pool and out must be 16-byte aligned, q's strides multiples of 8 elements", what);
   max_new = std::min(max_new, n_tokens);
+  if (max_new * (n_q_heads / n_kv_heads) > INT32_MAX - kTileRows)        // (the kernels number a sequence's rows of a KV head in 32 bits)
+    SUBSPEC_FAIL(SUBSPEC_ERR_LIMIT, "%s: %lld tokens of %lld query heads a KV head in one sequence", what, (long long)max_new,
+                 (long long)(n_q_heads / n_kv_heads));
   window = std::min(window, kMostRows);
   sinks = std::min(sinks, kMostRows);
   const PagedPlan pl = paged_plan(batch, n_tokens, n_q_heads, n_kv_heads, head_dim, max_new, max_kv, window, sinks);

@@ -187,3 +187,10 @@ def test_a_release_between_layers_leaves_the_step_its_lengths(monkeypatch):
     batch.release(0)
     batch.attention(0, torch.zeros(3, 4, 64))
     assert seen == [([0, 2, 3], [9, 5])] * 2 and batch.kv_lens.tolist() == [0, 5] and batch.lens == [0, 5]
+
+
+def test_a_sequence_of_more_rows_than_32_bits_number_is_refused():
+    """(token, query head of a KV head) rows: 2^30 tokens of 4 heads a KV head, though q may be an expanded view of a few."""
+    assert _attention(n=1 << 30, new=1 << 30, hq=8, hkv=2, kv=64) == -4 and b"tokens of 4 query heads" in L.lib().subspec_last_error()
+    assert _attention(n=1 << 30, new=(1 << 29) - 65, hq=8, hkv=2, kv=640) == -2                        # (the workspace is looked at next)
+    assert _attention(n=1 << 30, new=1 << 29, hq=8, hkv=2, kv=640) == -4
