@@ -341,7 +341,9 @@ int subspec_kv_append_paged(const void* k, int64_t k_token_stride, int64_t k_hea
  *              than what a call meets.  Of a sequence that exceeds them the tokens from max_new on are left out (their rows of out stay
  *              as they were) and the cached rows from max_kv on are not seen; positions are those above, p = kv_lens[b] - n + i with
  *              the sequence's own n (either bound 0: nothing is written)
- * out          device [n_tokens, n_q_heads, head_dim]; rows before query_starts[0] and from query_starts[batch] on are left as they were
+ * out          device [n_tokens, n_q_heads, head_dim]; rows before query_starts[0] and from query_starts[batch] on are left as they were.
+ *              It may be q itself where that is contiguous (every row is read before it is written, by the same workgroup or by an earlier
+ *              launch); otherwise it overlaps no input
  * workspace    subspec_paged_attention_workspace bytes of the same sizes, 16-byte aligned
  * Limits: 1 <= batch <= SUBSPEC_MAX_BATCH, n_q_heads <= 1024, max_kv and n_tokens <= 2^30, min(max_new, n_tokens) * group < 2^31 - 256.
  * Page numbers are clamped to the pool, so a bad table reads wrong rows and never leaves it.  Rows that no token of the call sees (those behind

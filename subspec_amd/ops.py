@@ -542,7 +542,7 @@ def paged_attention(q: torch.Tensor, pool_layer: torch.Tensor, block_table: torc
 
     ``window``: a token sees its own row and the ``window - 1`` before it (None or 0: all), and the first ``sinks`` rows besides.  A token that sees
     no row gets zeros.  Returns [tokens, Hq * D]; rows before the first sequence's (``query_starts`` of a part of a batch) and behind
-    the last one's are left as they were in ``out``.
+    the last one's are left as they were in ``out``, which may be a contiguous ``q`` itself and otherwise overlaps no input.
     Replaces the prefill and decode wrappers of specdecodes/models/utils/flashinfer/attention_wrapper.py:71-137."""
     dev = _require_gpu(q, pool_layer, block_table, query_starts, kv_lens)
     max_pages, page_len, Hkv, D = _pool_layer_shape(pool_layer)
@@ -564,6 +564,12 @@ def paged_attention(q: torch.Tensor, pool_layer: torch.Tensor, block_table: torc
         out = torch.empty((T, Hq * D), dtype=q.dtype, device=dev)
     elif out.dtype != q.dtype or out.shape != (T, Hq * D) or not out.is_contiguous() or out.device != dev:
         raise ValueError(f"paged_attention: out must be a contiguous {q.dtype} tensor [{T}, {Hq * D}]")
+    else:
+        begin, end = _extent(out)
+        for name, given in (("q", q), ("the pool", pool_layer)):
+            first, last = _extent(given)
+            if begin < last and first < end and not (given is q and begin == first and q.is_contiguous()):
+                raise ValueError(f"paged_attention: out overlaps {name}, which other workgroups still read")
     if workspace is not None:
         _require_gpu(q, workspace)
         if not workspace.is_contiguous():

@@ -573,3 +573,21 @@ def test_a_batch_refuses_to_be_captured_and_its_layers_can_be():
         (torch.randn(500, 500, device=DEV) @ torch.randn(500, 500, device=DEV)).sum().item()
     batch.step([1, 1])
     assert batch.plan["kv_lens"].tolist() == [4, 3]
+
+
+@pytest.mark.parametrize("lens", [[(900, 1)] * 5, [(60, 1), (33, 4)], [(700, 130), (64, 1)], [(60, 40), (300, 200), (41, 1)]], ids=str)
+def test_the_output_may_be_the_queries_themselves_and_nothing_else_that_is_read(lens):
+    g = torch.Generator().manual_seed(73)
+    q, pool, table, starts, kv = _batch(g, lens, 16, 8, 2, 128, torch.bfloat16, spare=40)
+    pool, most = pool.to(DEV), (max(n for _, n in lens), max(kv))
+    plain = ops.paged_attention(q.to(DEV), pool, _i32(table), _i32(starts), _i32(kv), *most)
+    own = q.to(DEV)
+    got = ops.paged_attention(own, pool, _i32(table), _i32(starts), _i32(kv), *most, out=own.view(len(q), -1))
+    assert got.data_ptr() == own.data_ptr() and torch.equal(got, plain)
+    room = torch.zeros(len(q) + 1, 8 * 128, dtype=torch.bfloat16, device=DEV)
+    fused = room[:-1].view(-1, 8, 128)
+    shifted = torch.zeros(len(q) * 8 * 128 * 2, dtype=torch.bfloat16, device=DEV).view(len(q), 16, 128)
+    for queries, out in [(fused, room[1:]), (shifted[:, 8:], shifted.view(-1)[:len(q) * 1024].view(len(q), -1)),
+                         (q.to(DEV), pool.view(-1)[:len(q) * 1024].view(len(q), -1))]:
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.paged_attention(queries, pool, _i32(table), _i32(starts), _i32(kv), *most, out=out)
