@@ -318,7 +318,7 @@ int subspec_paged_batch_plan(const int32_t* kv_lens, const int32_t* new_lens, in
  * Replaces  flashinfer.append_paged_kv_cache   specdecodes/models/utils/flashinfer/attention_wrapper.py:244-253
  *
  * k, v    device [n_tokens, n_kv_heads, head_dim] with token and head strides in elements (a slice of a fused projection's output);
- *         the elements of a head are consecutive
+ *         the elements of a head are consecutive.  They may be rows of the pool itself (a copy of a page), but none that this call writes
  * slots   device int64 [n_tokens]; a row whose slot lies outside [0, max_pages * page_len) is not written.  Slots are distinct (those of a
  *         plan are): of two rows with one slot either may be left there, or pieces of both
  * dtype   any; the rows are copied as they are

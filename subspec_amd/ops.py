@@ -512,7 +512,8 @@ def _pool_layer_shape(pool_layer: torch.Tensor):
 def kv_append_paged_(pool_layer: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
     """In place: row ``slots[t]`` (page * page_len + token in the page) of one layer [max_pages, 2, page_len, kv_heads, head_dim] of a page pool
     takes ``k[t]`` and ``v[t]`` [tokens, kv_heads, head_dim] (views of a fused projection's output are read where they are); rows whose
-    slot is negative or outside the pool are left out.  The slots are distinct, as a plan's are.  What ``flashinfer.append_paged_kv_cache``
+    slot is negative or outside the pool are left out.  The slots are distinct, as a plan's are, and of no row that ``k`` or ``v`` lies in (a
+    page of the pool may be copied to another).  What ``flashinfer.append_paged_kv_cache``
     does in the reference (specdecodes/models/utils/flashinfer/attention_wrapper.py:244-253)."""
     dev = _require_gpu(pool_layer, k, v, slots)
     max_pages, page_len, heads, D = _pool_layer_shape(pool_layer)

@@ -591,3 +591,14 @@ def test_the_output_may_be_the_queries_themselves_and_nothing_else_that_is_read(
                          (q.to(DEV), pool.view(-1)[:len(q) * 1024].view(len(q), -1))]:
         with pytest.raises(ValueError, match="overlaps"):
             ops.paged_attention(queries, pool, _i32(table), _i32(starts), _i32(kv), *most, out=out)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_page_is_copied_to_another_of_the_same_pool(dtype):
+    g = torch.Generator().manual_seed(74)
+    pool = torch.randn(6, 2, 16, 3, 64, generator=g).to(dtype)
+    want = pool.clone()
+    want[1, :, 5:12] = pool[4, :, 2:9]
+    dev = pool.to(DEV)
+    ops.kv_append_paged_(dev, dev[4, 0, 2:9], dev[4, 1, 2:9], torch.arange(16 + 5, 16 + 12, device=DEV))
+    assert torch.equal(dev.cpu(), want)
