@@ -93,7 +93,6 @@ __device__ __forceinline__ uint64_t whole(double m) { return (uint64_t)__double_
 // Larger logits first, then lower indexes, as ascending keys: the bits of the value that its type has (a bf16's or fp16's float is zero behind
 // them), turned round, and 20 bits of the index.
 template <int DT> constexpr int kDropped = DT == SUBSPEC_F32 ? 0 : DT == SUBSPEC_F16 ? 13 : 16;
-template <int DT> constexpr int kKeyBits = 52 - kDropped<DT>;
 template <int DT>
 __device__ __forceinline__ uint64_t order_key(float l, int i) {
   uint32_t b = __float_as_uint(l == 0.f ? 0.f : l);      // (-0 is 0)
