@@ -12,9 +12,9 @@ namespace subspec {
 // With L cached and n new rows a sequence holds h = ceil(L / P) pages and takes a = ceil((L + n) / P) - h more; tokens and pages are
 // numbered by the exclusive sums of n and a over the sequences, and the free pages are a stack, so new page r of the step is
 // free[n_free - 1 - r].  Nothing a workgroup needs is written by another: a token whose page is new computes it from the rank, and table
-// entries below h are only read.  So every workgroup scans the lengths for itself (4 to 16 KB out of the L2) and ONE launch does all,
+// entries below h are only read.  So every workgroup scans the lengths for itself (8 bytes a sequence, 32 KB at most, out of the L2) and ONE launch does all,
 // where a scan, a table update and a slot map would be three.  There is next to nothing to move (8 sequences 0.3 KB, 500 sequences, sixteen of them with chunks,
-// 400 KB): the kernel is its chain of dependent reads, 4.6 and 6.8 us (the launch that appends 61 tokens takes 2.6).
+// 400 KB): the kernel is its chain of dependent reads, 4.4 and 6.8 us (the launch that appends 61 tokens takes 2.6).
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanItems = SUBSPEC_MAX_BATCH / kPlanThreads;
 

@@ -16,6 +16,8 @@ namespace subspec {
 // travel from memory straight into the wavefront's ring of LDS stages, 32 keys each, which the transposing reads of V need anyway; a stage is
 // asked for again as soon as it has been read.  The rows are read once and copied as streaming data: 64 tokens of up to 4096 rows, 28 : 4
 // heads, 348 MB: 70.8 us against 79.6, 16 of up to 32768 rows, 32 : 8, 1.3 GB: 243 against 262 (5.5 TB/s; a large copy reaches 5.2 here).
+// A probability is rounded once, to the type of the product with V; the row's sum takes it before that, in fp32 (the tiles' kernel takes it after, where
+// one instruction adds a rounded pair).  The two differ by half a step of the type at most (in fp16 and 2^-25 a key), mostly far less: roundings cancel.
 // S^T = K Q^T and O^T = V^T P^T by 16x16x32 products: the two accumulators of a stage (eight keys of one query a lane) are, packed, the
 // operand of the second, with its keys taken in the same order from V.
 // A row's probabilities are relative to a reference that follows its largest score by at most 2^8 (see kSlack), so that a stage without a
@@ -276,9 +278,9 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
 
 // Chunks of `blocks` key blocks each for `units` (tile, KV head) pairs.  In blocks (1.6 us): a compute unit takes one workgroup at a time, whose start and
 // end cost about three; a launch for the merge two and 0.4 for every chunk that it adds up; a chunk's partial results, 128 KB out and back, a
-// thirtieth.  Both launches at 1 / 2 / 3 / 4 / 5 / 8 / 16 chunks, 28 : 4 heads, us: 512 tokens behind 4096 rows (56 pairs, 72 blocks) 121 73 56 50 69 62 88,
-// 33 behind 7967 (4, 125) 199 107 - 60 51 38 29, 2048 behind 6144 (224, 128) 221 243 241 247 249 298 414, four of 200 behind 2800, 32 : 8 heads (72, 47)
-// 86 58 52 60 62 68 -.
+// thirtieth.  Both launches at 1 / 2 / 3 / 4 / 5 / 8 / 16 chunks, 28 : 4 heads, us: 512 tokens behind 4096 rows (56 pairs, 72 blocks) 120 73 56 49 68 61 87,
+// 33 behind 7967 (4, 125) 195 105 75 60 50 37 29, 2048 behind 6144 (224, 128) 218 240 241 243 243 291 407, four of 200 behind 2800, 32 : 8 heads (72, 47)
+// 86 58 52 59 61 67 97, sixteen of up to 33 behind 4000 (64, 63) 109 70 56 60 63 69 84, of which this takes 63.
 static int64_t paged_tile_chunks(int64_t blocks, int64_t units) {
   double best = 1e30;
   int64_t chunks = 1;
@@ -312,10 +314,10 @@ static PagedPlan paged_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64_t
   pl.few_rows = few <= 16 ? 16 : few <= 32 ? 32 : few <= 64 ? 64 : 0;
   if (pl.few_rows) {
     const int64_t keys = std::max<int64_t>(1, span(pl.few_rows / group, kFewKeys)), units = batch * hkv;
-    // A unit's stage takes 0.5 to 0.65 us however deep its ring (16 copies and the products of 32 keys, one after the other), so short calls
-    // want short chunks; a partial result costs the merge as much as 7 keys of 28 : 4 heads, so long ones want long ones.  Both launches,
-    // chunks of 64 / 128 / 256 / 384 / 512 keys, us: one token of 1000 rows, 32 : 8 heads of 64: 8.2 9.4 11.8 14.5 17.2; of 32768, 28 : 4:
-    // 41 27.5 22.5 22.5 21.5; 32 tokens of 1000: 18 15.8 15.6 18 19.8; 64 of 4096: 95 87 87 79 85
+    // A unit's stages follow one another (16 copies and the products of 32 keys each), so short calls want short chunks; a partial result costs
+    // the merge as much as 7 keys of 28 : 4 heads, so long ones want long ones.  Both launches, chunks of 64 / 128 / 256 / 384 / 512 keys, us:
+    // one token of 1000 rows, 32 : 8 heads of 64: 8.2 8.6 10.3 12.1 14.1; of 32768, 28 : 4: 27.0 20.2 18.8 20.9 19.4; 32 tokens of up to 1000:
+    // 19.3 15.9 15.2 17.4 18.0; 64 of up to 4096: 95 85 81 70 74; 16 of up to 32768, 32 : 8: 330 283 253 244 241
     int64_t per = ((int64_t)(0.65 * std::sqrt((double)units * (double)keys)) + kFewKeys - 1) / kFewKeys * kFewKeys;
     per = std::min<int64_t>(std::max<int64_t>(per, 64), 384);
     while (per < keys && units * ((keys + per - 1) / per) * pl.few_rows > (1 << 21)) per *= 2;         // a gigabyte of partial results at 128 a head

@@ -11,8 +11,9 @@
 // block lie in one page (pages of 8 rows and more) that is one number for all lanes.
 // Packing (token, head) rows lets a key block serve the whole group: 28 : 4 heads, 256 rows are 37 tokens of 7 heads, and one copy of a block is
 // read where a workgroup for each head would read seven.
-// 2048 tokens behind 6144 rows, 28 : 4 heads of 128: 219 us, 0.96 PFLOP/s; 8192 tokens, 16 : 8 heads: 259, 1.06; 2048 behind 6144 with heads of 64: 157, 0.77.
-// A block takes 3850 cycles, of which the products' own are 2048: they stand at 47 cycles each instead of 32 even without an LDS read between them.
+// 2048 tokens behind 6144 rows, 28 : 4 heads of 128: 217 to 224 us, 0.97 to 0.94 PFLOP/s; 8192 tokens, 16 : 8 heads: 257, 1.07; 2048 behind 6144, 32 : 8
+// heads of 64: 156, 0.77.  The matrix pipes of a compute unit are busy for 0.54 of its cycles (a block takes 3800, its products' own are 2048); with
+// heads of 64 and a window 0.24.  The products of a phase stand at 47 cycles each instead of 32 even without an LDS read between them.
 // Operands asked for earlier, other priorities and copies in the softmax phase changed nothing.
 #include "paged.h"
 
@@ -113,8 +114,9 @@ __device__ __forceinline__ void matrix_phase(const TileAddress& ad, v16f (&o)[D 
   __builtin_amdgcn_s_setprio(0);
 }
 
-// V phase.  The accumulators hold raw scores relative to the row's reference, which follows the largest score by at most kSlack (in units of
-// exp2's argument) and moves rarely once the first blocks are through.
+// V phase.  A probability is rounded once, to the type of the product with V, and the row's sum is that of the rounded ones in fp32: one instruction
+// adds a pair of them, and what V is multiplied by adds up to what the result is divided by.  The accumulators hold raw scores relative to the row's
+// reference, which follows the largest score by at most kSlack (in units of exp2's argument) and moves rarely once the first blocks are through.
 template <int DT>
 __device__ __forceinline__ float pair_sum(uint32_t packed, float acc) {
   if constexpr (DT == SUBSPEC_BF16) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, packed), __builtin_bit_cast(v2bf, 0x3f803f80u), acc, false);

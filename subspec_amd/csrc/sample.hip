@@ -7,11 +7,14 @@
 // (l_max - l) / T with counts and masses says in which bin each of the three lies; the entries of those bins alone are put in order.
 //
 // Masses are whole numbers, m * 2^42 rounded, of an exponential evaluated in 64 bits (within 0.54 of such a unit, see mass_series.h): their sums are
-// exact and do not depend on the order in which wavefronts add them, 2^20 entries stay below 2^62, and what rounds to zero (less than 2^-43 of the largest) is drawn with a
-// probability below 2^-23 even if a million such entries are there.  In fp32 the sum over a flat row of 150000 entries is off by more
-// than the step between two of them.
-// One row of 152064 fp32: 30 us, four dependent launches of 3 + 9 + 11 + 9; 64 rows bf16 (19.5 MB): 57, the exponentials in 64 bits 19 of them,
-// the sums of the slices' bins and the second pass 20, the search among the candidates 15.
+// exact and do not depend on the order in which wavefronts add them, 2^20 entries stay below 2^62, and what rounds to zero (less than 2^-43 of the
+// largest) is drawn with a probability below 2^-23 even if a million such entries are there.  In fp32 the sum over a flat row of 150000 entries is off
+// by more than the step between two of them.
+// One row of 152064 fp32: 30 us, four dependent launches of 3 + 8 + 11 + 8; 64 rows bf16 (19.5 MB): 58, the largest 6, the exponentials in 64 bits
+// 19, the sums of the slices' bins and the second pass 20, the search among the candidates 15.
+// A row of more candidates than kCandidates (or a slice's share of them) is searched by one workgroup, which reads it again for every ten bits of
+// every search: 152064 logits of deviation 2 at T = 3 and top-p 0.95 320 to 350 us (41 at T = 1), 64 such rows 400 to 455 (66); rows of equal logits
+// 0.65 to 1.3 ms, with a top-k of 70000 and a top-p 3.5.
 #include "common.h"
 #include "mass_series.h"
 #include <algorithm>
@@ -604,7 +607,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_gather_kernel(SampleArgs
   const RowRule r = row_rule(a, row_index);
   const SliceRecord* of = c.slices + (int64_t)row_index * c.count;
   const int lane = threadIdx.x & (kWave - 1);
-  uint64_t kept = lane < c.count ? of[lane].min_p_mass : 0;                                  // (at most 32 slices)
+  uint64_t kept = lane < c.count ? of[lane].min_p_mass : 0;                                  // (at most 16 slices)
   const RowTop top = row_top_of(row_top<kSliceThreads>(c, row_index, scratch), r);
   if (top.value == -INFINITY) return;                                             // (uniform) the last launch says so
   static_assert(kBins == 2 * kSliceThreads, "a thread adds up two bins");
@@ -662,7 +665,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_draw_kernel(SampleArgs a
   const SliceRecord* of = c.slices + (int64_t)row_index * c.count;
   const RowRecord& rec = c.rows[row_index];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
-  const int some = lane < c.count ? of[lane].n_candidates : 0;                               // (at most 32 slices)
+  const int some = lane < c.count ? of[lane].n_candidates : 0;                               // (at most 16 slices)
   const RowTop top = row_top_of(row_top<kSliceThreads>(c, row_index, scratch), r);
   if (top.value == -INFINITY) return nothing_to_draw(a, row_index);               // (uniform)
   for (int i = threadIdx.x; i < kBins; i += kSliceThreads) {
@@ -683,8 +686,9 @@ __global__ __launch_bounds__(kSliceThreads) void sample_draw_kernel(SampleArgs a
 }
 
 // Slices a row is cut into; 1: the row stays whole, which is one launch in the place of four.  More slices shorten the two passes over the row, but
-// each adds up the bins of all for itself.  1 / 4 / 8 / 16 / 32 slices, us: one row of 152064 fp32 93 55 41 34 33, 16 rows bf16 88 54 45 40 46, 64 90 58 58
-// 59 78, 128 94 76 81 89 124, 256 100 109 124 140 213; one row of 32000 31 29 28 26 -, 64 38 36 43 48 -; one of 16384 21 24 24 - -.
+// each adds up the bins of all for itself.  1 / 4 / 8 / 16 / 32 slices, us (top-p 0.95, min-p 0.02): one row of 152064 fp32 92 53 41 34 32, 16 rows bf16
+// 87 53 45 39 45, 64 89 58 57 59 77, 128 93 75 81 88 124, 256 99 110 124 141 215; fp32, one row of 32000 31 28 27 26 27, 64 38 36 42 47 67; one of 16384
+// 21 23 24 23 -.
 static int sample_slices(int64_t rows, int64_t vocab) {
   if (vocab < 24576 || rows >= 192) return 1;
   return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / rows, 16), vocab / (rows <= 8 ? 2048 : 8192)));
