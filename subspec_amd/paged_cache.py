@@ -184,15 +184,18 @@ class KvBatch:
     def __init__(self, pool: KvCachePool, max_batch: int, max_len: int, num_pages: Optional[int] = None):
         if not 1 <= int(max_batch) <= L.MAX_BATCH:
             raise ValueError(f"max_batch={max_batch} outside [1, {L.MAX_BATCH}]")
+        if int(max_len) < 0 or (num_pages is not None and int(num_pages) < 0):
+            raise ValueError(f"max_len={max_len} and num_pages={num_pages} must not be negative")
         self.pool, self.page_len, self.max_len = pool, pool.page_len, int(max_len)
-        self.pages = pool.allocate(int(pool.num_free_pages()) if num_pages is None else int(num_pages))
-        self.num_free = len(self.pages)
         self.lens: List[int] = [0] * int(max_batch)
         dev = pool.device
-        self.free_pages = torch.tensor(self.pages, dtype=torch.int32, device=dev)
-        self.n_free = torch.tensor([self.num_free], dtype=torch.int32, device=dev)
         self.kv_lens = torch.zeros(int(max_batch), dtype=torch.int32, device=dev)
         self.block_table = torch.full((int(max_batch), max(1, self._pages(self.max_len))), -1, dtype=torch.int32, device=dev)
+        # (the pages come last: what fails before them leaves the pool as it was)
+        self.pages = pool.allocate(int(pool.num_free_pages()) if num_pages is None else int(num_pages))
+        self.num_free = len(self.pages)
+        self.free_pages = torch.tensor(self.pages, dtype=torch.int32, device=dev)
+        self.n_free = torch.tensor([self.num_free], dtype=torch.int32, device=dev)
         self.plan: Optional[Dict[str, torch.Tensor]] = None
         self.max_new = self.max_kv = 0
 

@@ -194,3 +194,13 @@ def test_a_sequence_of_more_rows_than_32_bits_number_is_refused():
     assert _attention(n=1 << 30, new=1 << 30, hq=8, hkv=2, kv=64) == -4 and b"tokens of 4 query heads" in L.lib().subspec_last_error()
     assert _attention(n=1 << 30, new=(1 << 29) - 65, hq=8, hkv=2, kv=640) == -2                        # (the workspace is looked at next)
     assert _attention(n=1 << 30, new=1 << 29, hq=8, hkv=2, kv=640) == -4
+
+
+def test_a_batch_that_cannot_be_made_takes_no_pages():
+    """A table that does not fit into memory, a length or a number of pages below zero (which as the end of a slice means all but some)."""
+    from subspec_amd.paged_cache import KvBatch, KvCachePool
+    pool = KvCachePool(max_pages=8, num_layers=1, num_heads=2, head_dim=64, page_len=4, dtype=torch.bfloat16, device="cpu")
+    for bad in (dict(max_len=1 << 58), dict(max_len=-1), dict(max_len=40, num_pages=-1)):
+        with pytest.raises((ValueError, RuntimeError)):
+            KvBatch(pool, 2, **bad)
+        assert int(pool.num_free_pages()) == 8
