@@ -360,6 +360,60 @@ int subspec_paged_attention(const void* q, int64_t q_token_stride, int64_t q_hea
                             int64_t sinks, float scale, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Attention over the blocks of a long sequence that matter to a token: bounds of every full page's keys, the blocks that score highest by them, and
+ * attention over those alone.  A block is a sequence's rows j * page_len .. of one page, block_table[sequence][j]; a token at position p
+ * sees rows 0 .. p, so blocks 0 .. c = p / page_len, all of which but c are full.  No form of it is in the reference, whose paged wrappers read the
+ * whole sequence (specdecodes/models/utils/flashinfer/attention_wrapper.py:71-137); pool, table and plan are those above.
+ *
+ * Bounds: of every page whose last row (slot % page_len == page_len - 1) is among the slots, bounds[page][head][0][d] = the least of
+ * K[row][head][d] over the page's rows and [1][d] the largest (NaN if one of them is NaN).  Rows are appended in order, so the page is full then; call it behind
+ * subspec_kv_append_paged with the same slots.  A page's bounds come from the page alone.
+ * bounds  device [max_pages, n_kv_heads, 2, head_dim], 16-byte aligned, in the pool's type (bf16 / fp16; head_dim 64 or 128); slots outside the
+ *         pool are left out, other pages' bounds stay as they are
+ */
+int subspec_kv_page_bounds(const void* kv_pool_layer, void* bounds, int dtype, int64_t max_pages, int64_t page_len,
+                           int64_t n_kv_heads, int64_t head_dim, const int64_t* slots, int64_t n_tokens, void* stream);
+
+/* Blocks for every (token, KV head): the last `recent` that the token sees (its own among them), and of the others the keep - recent of largest
+ *   s_j = sum over the KV head's query heads g and dimensions d of max(q_gd low_jd, q_gd high_jd)
+ *       = sum_d low_jd sum_g min(q_gd, 0) + high_jd sum_g max(q_gd, 0),
+ * which the heads' summed scores q_g . k of no key of the block exceed; in 64 bits, NaN as +infinity, of equal ones the lower block.  Where a token sees
+ * at most `keep` blocks it gets them all.  Only full blocks before its own are scored: no row behind the token has influence.
+ *
+ * sequences, positions   device int32 [n_tokens], as a plan leaves them: the token's row of block_table and its position.  A token whose sequence lies
+ *         outside [0, batch) or whose position is below 0 sees no block
+ * max_kv  rows from it on are not seen (by a token at position max_kv or behind, its own among them); it sizes the workspace
+ * blocks  device int32 [n_tokens, n_kv_heads, keep], in ascending order, -1 behind the last; it overlaps no input
+ * workspace  subspec_select_blocks_workspace bytes, 16-byte aligned (NULL where that is 256)
+ * Limits: 1 <= recent <= keep <= 2^17, min(max_blocks, ceil(max_kv / page_len)) <= 2^17, n_tokens <= 2^20, n_q_heads <= 1024.  Page numbers are clamped to the
+ * pool.  Made for tokens that decode and for drafts: neighbours of one sequence share a reading of the bounds, up to four.
+ */
+size_t subspec_select_blocks_workspace(int64_t n_tokens, int64_t n_kv_heads, int64_t page_len, int64_t max_blocks, int64_t max_kv);
+
+int subspec_select_blocks(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* bounds, int dtype,
+                          int64_t max_pages, int64_t page_len, const int32_t* block_table, int64_t max_blocks, int64_t table_stride,
+                          const int32_t* sequences, const int32_t* positions, int64_t batch, int64_t n_tokens, int64_t n_q_heads,
+                          int64_t n_kv_heads, int64_t head_dim, int64_t max_kv, int64_t keep, int64_t recent, int32_t* blocks,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* out[t, h] = softmax(scale * q[t, h] . k[j, h / group]) v[j, h / group] over the rows j <= positions[t] of the blocks listed for (t, h / group).
+ * blocks    device int32 [n_tokens, n_kv_heads, keep]: distinct blocks in any order; entries below 0 or behind the token count for nothing (of a block that is
+ *           listed twice the rows count twice).  A token without a row to see gets zeros
+ * out       device [n_tokens, n_q_heads, head_dim]; rows of tokens whose sequence lies outside [0, batch) are left as they were.  It may be q
+ *           itself where that is contiguous; otherwise it overlaps no input
+ * Limits: at most 64 query heads a KV head, keep <= 2^17, keep * page_len <= 2^30, n_tokens <= 2^20; q as for subspec_paged_attention.  Rows of the pool
+ * that the token does not see, or whose block is not listed, have no influence, whatever they hold.
+ */
+size_t subspec_block_attention_workspace(int64_t n_tokens, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim, int64_t page_len,
+                                         int64_t keep);
+
+int subspec_block_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* kv_pool_layer, int dtype,
+                            int64_t max_pages, int64_t page_len, const int32_t* block_table, int64_t max_blocks, int64_t table_stride,
+                            const int32_t* blocks, int64_t keep, const int32_t* sequences, const int32_t* positions, int64_t batch,
+                            int64_t n_tokens, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim, float scale, void* out,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * One token per row of logits, drawn after temperature, top-k, top-p and min-p from one given number per row.
  * Entries are ordered by logit, larger first, equal ones by index, and entry j has the mass exp((l_j - l_max) / T).  Every filter keeps a
  * prefix of that order: top-k the first k; top-p the entries with less than p times the mass of those k before them;
@@ -384,6 +438,34 @@ int subspec_sample_filtered(const void* logits, int dtype, int64_t rows, int64_t
                             const float* temperatures, float temperature, const int32_t* top_ks, int32_t top_k, const float* top_ps,
                             float top_p, const float* min_ps, float min_p, void* workspace, size_t workspace_bytes, int64_t* tokens, float* probs,
                             void* stream);
+
+/* Drafted tokens of a batch of sequences, verified against the target's probabilities with given numbers: what is emitted is distributed like draws of
+ * subspec_sample_filtered from the target alone.  Row i of a sequence's logits gives p_i, the distribution of the token behind its token i (temperature and
+ * filters as there, of the same row); drafts[i + 1] was drawn from q_i = draft_probs[i].  It stays if uniforms[i] * q_i < p_i (both at the draft).  At the first
+ * draft that does not, the sequence's token is drawn from max(p_i - q_i, 0) (from p_i, if that is nothing); after the last row, from p: the first entry, in the
+ * order of the vocabulary, whose mass added to that of all before it exceeds draws[b] times the whole.
+ * Replaces  the stochastic verification that the reference leaves to matching drawn tokens (specdecodes/models/utils/tree_verify.py:8-163 with
+ *           do_sample), whose drafts stay with probability sum_x p(x) q(x) instead of sum_x min(p(x), q(x))
+ *
+ * drafts        device int64 [n_rows]: the tokens that the target's forward took, packed like the rows (a sequence's first one is no draft).  A token outside
+ *               the vocabulary does not stay
+ * query_starts  device int32 [batch + 1], ascending, as a plan leaves them: sequence b has rows query_starts[b] .. query_starts[b + 1] - 1
+ * uniforms      device float [n_rows] in [0, 1), a sequence's last is not used;  draws  device float [batch] in [0, 1)
+ * draft_probs   device [n_rows, vocab] at draft_stride elements, fp32 / fp16 / bf16 whatever the logits are, or NULL: drafts that nothing was drawn for, q_i = 1 at
+ *               the draft.  Entries below 0 and NaN count as 0.  A sequence's last row is not read
+ * tokens        device int64 [n_rows]: a sequence's drafts that stay, its token, then -1; -1 in rows of no sequence, and for the token of
+ *               a row without a logit above -inf
+ * probs         device float [n_rows]: p_i at these tokens (0 beside -1);  accepted  device int32 [batch]: drafts that stay (0 without rows)
+ * filtered      1 where any of the filters is given (a pointer, 0 < top_k < vocab, top_p < 1 or min_p > 0)
+ * The outputs overlap no input.  Limits: n_rows <= 2^20, vocab <= 2^20, 1 <= batch <= SUBSPEC_MAX_BATCH.
+ */
+size_t subspec_verify_drafts_workspace(int64_t n_rows, int64_t batch, int64_t vocab, int filtered);
+
+int subspec_verify_drafts(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride, const int64_t* drafts,
+                          const int32_t* query_starts, int64_t batch, const float* uniforms, const float* draws, const void* draft_probs,
+                          int draft_dtype, int64_t draft_stride, const float* temperatures, float temperature, const int32_t* top_ks,
+                          int32_t top_k, const float* top_ps, float top_p, const float* min_ps, float min_p, void* workspace,
+                          size_t workspace_bytes, int64_t* tokens, float* probs, int32_t* accepted, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Draft probabilities: out = softmax(round(logits / temperature)) over the last axis, in the logits

@@ -80,6 +80,16 @@ _SIGNATURES = {
     "subspec_sample_filtered_workspace": (_sz, [_i64, _i64]),
     "subspec_sample_filtered": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, _p, _p, C.c_float, _p, _i32, _p, C.c_float, _p, C.c_float,
                                           _p, _sz, _p, _p, _p]),
+    "subspec_kv_page_bounds": (C.c_int, [_p, _p, C.c_int, _i64, _i64, _i64, _i64, _p, _i64, _p]),
+    "subspec_select_blocks_workspace": (_sz, [_i64] * 5),
+    "subspec_select_blocks": (C.c_int, [_p, _i64, _i64, _p, C.c_int, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                        _i64, _p, _p, _sz, _p]),
+    "subspec_block_attention_workspace": (_sz, [_i64] * 6),
+    "subspec_block_attention": (C.c_int, [_p, _i64, _i64, _p, C.c_int, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64,
+                                          C.c_float, _p, _p, _sz, _p]),
+    "subspec_verify_drafts_workspace": (_sz, [_i64, _i64, _i64, C.c_int]),
+    "subspec_verify_drafts": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _p, C.c_int, _i64, _p, C.c_float, _p, _i32, _p,
+                                        C.c_float, _p, C.c_float, _p, _sz, _p, _p, _p, _p]),
     "subspec_softmax_temperature_workspace": (_sz, [_i64, _i64]),
     "subspec_softmax_temperature": (C.c_int, [_p, _p, C.c_int, _i64, _i64, C.c_float, _p, _sz, _p]),
     "subspec_temperature_warp": (C.c_int, [_p, _p, C.c_int, _i64, C.c_float, _p]),

@@ -1,0 +1,853 @@
+// Attention of the new tokens of a batch over the blocks of their sequences that matter to them, for gfx950: bounds of every full page's keys, the
+// blocks that a token's queries score highest by these, and attention over those blocks.
+//
+// The pool is that of the paged cache, [max_pages][2 (K, V)][page_len][n_kv_heads][head_dim] a layer.  A block is a sequence's rows j page_len .. of
+// one page, block_table[sequence][j].  A token at position pos sees rows 0 .. pos, so blocks 0 .. c = pos / page_len, of which all but c
+// are full and hold nothing behind it.
+#include "paged.h"
+#include <algorithm>
+#include <cmath>
+
+namespace subspec {
+
+static int block_shift_of(int64_t page_len) {
+  int shift = 0;
+  while ((1ll << shift) < page_len) ++shift;
+  return shift;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- bounds
+// low_d = min over the page's rows of K_d, high_d = max, of every page whose last row is among the slots: the rows of a page are
+// written in order, so it is full then, and its bounds come from the page alone (nothing is read, changed and written back).
+constexpr int kBoundsThreads = 256;
+struct BoundsArgs {
+  const uint16_t* pool;
+  uint16_t* bounds;              // [max_pages][n_kv_heads][2 (low, high)][head_dim]
+  const int64_t* slots;
+  int64_t n_slots, page_elems;
+  int n_tokens, per, page_shift, pieces, head_pieces;         // tokens of a workgroup; 16-byte pieces of a token's K, of a head's
+};
+// a NaN stays: it is neither above nor below, and hides nothing
+__device__ __forceinline__ float lower_of(float a, float b) { return b < a || b != b ? b : a; }
+__device__ __forceinline__ float upper_of(float a, float b) { return b > a || b != b ? b : a; }
+
+template <int DT>
+__global__ __launch_bounds__(kBoundsThreads) void page_bounds_kernel(BoundsArgs a) {
+  __shared__ __attribute__((aligned(16))) float side[kBoundsThreads][16];
+  const int tid = threadIdx.x, page_len = 1 << a.page_shift;
+  const int t0 = blockIdx.x * a.per, t1 = min(t0 + a.per, a.n_tokens);
+  const int lanes = min(a.pieces, kBoundsThreads), groups = kBoundsThreads / lanes, group = tid / lanes, lane = tid % lanes;
+  for (int t = t0; t < t1; ++t) {
+    const int64_t slot = a.slots[t];
+    if (slot < 0 || slot >= a.n_slots || (slot & (page_len - 1)) != page_len - 1) continue;        // (uniform)
+    const int64_t page = slot >> a.page_shift;
+    const dec_u4* rows = (const dec_u4*)(a.pool + page * 2 * a.page_elems);
+    dec_u4* out = (dec_u4*)(a.bounds + page * 2 * (a.page_elems >> a.page_shift));
+    for (int p0 = 0; p0 < a.pieces; p0 += lanes) {
+      const int piece = p0 + lane;
+      const bool mine = group < groups && piece < a.pieces;
+      float low[8], high[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        low[e] = INFINITY;
+        high[e] = -INFINITY;
+      }
+      if (mine) {
+#pragma unroll 4
+        for (int r = group; r < page_len; r += groups) {
+          float x[8];
+          unpack8<DT>(rows[(int64_t)r * a.pieces + piece], x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            low[e] = lower_of(low[e], x[e]);
+            high[e] = upper_of(high[e], x[e]);
+          }
+        }
+      }
+      if (groups > 1) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          side[tid][e] = low[e];
+          side[tid][8 + e] = high[e];
+        }
+        __syncthreads();
+        if (group == 0)
+          for (int g = 1; g < groups; ++g)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              low[e] = lower_of(low[e], side[g * lanes + lane][e]);
+              high[e] = upper_of(high[e], side[g * lanes + lane][8 + e]);
+            }
+        __syncthreads();
+      }
+      if (mine && group == 0) {
+        dec_u4* to = out + (piece / a.head_pieces) * 2 * a.head_pieces + piece % a.head_pieces;
+        to[0] = pack8<DT>(low);
+        to[a.head_pieces] = pack8<DT>(high);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- scores
+// s_j = sum over the KV head's query heads g and dimensions d of max(q_gd low_jd, q_gd high_jd), which no sum of the heads' scores of a key of block j
+// exceeds; with A_d = sum_g max(q_gd, 0) and B_d = sum_g min(q_gd, 0) it is sum_d A_d high_jd + B_d low_jd.  In 64 bits: which block comes out ahead must not
+// hang on an order of addition, and the rows come out of memory no faster than that (4 D operations for 4 D bytes).
+struct SelectArgs {
+  const uint16_t* q;
+  const uint16_t* bounds;
+  const int32_t* table;
+  const int32_t* sequences;
+  const int32_t* positions;
+  int32_t* blocks;               // [tokens][n_kv_heads][keep]
+  double* scores;                // [token - first][n_kv_heads][most]
+  int64_t q_token, q_head, table_stride, most;
+  int batch, n_tokens, first, hkv, group, page_shift, max_pages, keep, recent, last_row, span, spans;
+};
+// Blocks that a token sees (0: none), and of these the first so many that compete.
+struct TokenBlocks { int seen, scored; };
+__device__ __forceinline__ TokenBlocks token_blocks(const SelectArgs& a, int t) {
+  const int b = a.sequences[t], last = min(a.positions[t], a.last_row);
+  if (b < 0 || b >= a.batch || last < 0) return TokenBlocks{0, 0};
+  const int seen = (last >> a.page_shift) + 1;
+  return TokenBlocks{seen, seen > a.keep ? seen - a.recent : 0};
+}
+constexpr int kScoreTokens = 4;
+
+__device__ __forceinline__ double dpp_add(double v, const int which) {
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  const int lo = (int)(uint32_t)u, hi = (int)(uint32_t)(u >> 32);
+  int l, h;
+  if (which == 0) {              // the neighbour of a pair
+    l = __builtin_amdgcn_mov_dpp(lo, 0xB1, 0xf, 0xf, true);
+    h = __builtin_amdgcn_mov_dpp(hi, 0xB1, 0xf, 0xf, true);
+  } else if (which == 1) {       // ... of two pairs
+    l = __builtin_amdgcn_mov_dpp(lo, 0x4E, 0xf, 0xf, true);
+    h = __builtin_amdgcn_mov_dpp(hi, 0x4E, 0xf, 0xf, true);
+  } else if (which == 2) {       // eight lanes mirrored
+    l = __builtin_amdgcn_mov_dpp(lo, 0x141, 0xf, 0xf, true);
+    h = __builtin_amdgcn_mov_dpp(hi, 0x141, 0xf, 0xf, true);
+  } else {                       // sixteen
+    l = __builtin_amdgcn_mov_dpp(lo, 0x140, 0xf, 0xf, true);
+    h = __builtin_amdgcn_mov_dpp(hi, 0x140, 0xf, 0xf, true);
+  }
+  return v + __longlong_as_double((long long)((uint64_t)(uint32_t)h << 32 | (uint32_t)l));
+}
+
+// A wavefront takes `span` blocks of (token, KV head); D / 8 lanes a block.  A token whose neighbour before it is of the same sequence leaves its scores to the
+// wavefront of that one, up to kScoreTokens of them: the bounds are read once for all.
+template <int DT, int D>
+__global__ __launch_bounds__(kWave) void block_score_kernel(SelectArgs a) {
+  constexpr int kLanes = D / 8, kAtOnce = kWave / kLanes;
+  const uint32_t unit = blockIdx.x;
+  const int kvh = (int)(unit % (uint32_t)a.hkv), span = (int)(unit / (uint32_t)a.hkv % (uint32_t)a.spans);
+  const int local = (int)(unit / (uint32_t)a.hkv / (uint32_t)a.spans), t = a.first + local;
+  const int b = a.sequences[t];
+  if (local % kScoreTokens != 0 && a.sequences[t - 1] == b) return;
+  int scored[kScoreTokens], most = 0, tokens = 0;
+#pragma unroll
+  for (int k = 0; k < kScoreTokens; ++k) {
+    scored[k] = 0;
+    if (k > 0 && (tokens < k || (local + k) % kScoreTokens == 0 || t + k >= a.n_tokens || a.sequences[t + k] != b)) continue;
+    tokens = k + 1;
+    scored[k] = token_blocks(a, t + k).scored;
+    most = max(most, scored[k]);
+  }
+  const int j0 = span * a.span, j1 = min(j0 + a.span, most);
+  if (j0 >= j1) return;
+  const int lane = threadIdx.x, part = lane % kLanes, which = lane / kLanes;
+  double up[kScoreTokens][8], down[kScoreTokens][8];
+#pragma unroll
+  for (int k = 0; k < kScoreTokens; ++k) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) up[k][e] = down[k][e] = 0.0;
+    if (k >= tokens) continue;
+    const uint16_t* q = a.q + (t + k) * a.q_token + (int64_t)kvh * a.group * a.q_head + part * 8;
+    for (int g = 0; g < a.group; ++g) {
+      float x[8];
+      unpack8<DT>(*(const dec_u4*)(q + g * a.q_head), x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        // (a NaN goes into both: its blocks all score NaN)
+        up[k][e] += x[e] < 0.f ? 0.0 : (double)x[e];
+        down[k][e] += x[e] > 0.f ? 0.0 : (double)x[e];
+      }
+    }
+  }
+  const int32_t* row = a.table + b * a.table_stride;
+  for (int base = j0; base < j1; base += kWave) {
+    const int page_of = min(max(row[min(base + lane, j1 - 1)], 0), a.max_pages - 1);
+    const int some = min(kWave, j1 - base);
+#pragma unroll 4
+    for (int i = 0; i < some; i += kAtOnce) {
+      const int j = base + i + which;
+      const int page = __shfl(page_of, i + which, kWave);
+      const dec_u4* src = (const dec_u4*)(a.bounds + ((int64_t)page * a.hkv + kvh) * 2 * D) + part;
+      float low[8], high[8];
+      unpack8<DT>(src[0], low);
+      unpack8<DT>(src[kLanes], high);
+#pragma unroll
+      for (int k = 0; k < kScoreTokens; ++k) {
+        if (k >= tokens) break;
+        double s = 0.0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fma(up[k][e], (double)high[e], fma(down[k][e], (double)low[e], s));
+#pragma unroll
+        for (int o = 0; (1 << o) < kLanes; ++o) s = dpp_add(s, o);
+        if (part == 0 && j < scored[k]) a.scores[((int64_t)(local + k) * a.hkv + kvh) * a.most + j] = s != s ? INFINITY : s;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- the best of them
+// The keep - recent blocks of largest score, equal ones from the lowest on, without sorting: the scores as ordered whole numbers, and the digits (eleven bits at
+// a time, from the first that differs) of the smallest that stays; the few entries that share them are ranked one by one.  What stays is a bit each, and the
+// bits in order are the list.
+constexpr int kSelectThreads = 512;
+constexpr int kMostBlocks = 1 << 17;
+constexpr int kDigits = 2048;
+constexpr int kHeld = 8;                 // scores of a thread that stay in registers
+constexpr int kRanked = 256;
+__device__ __forceinline__ uint64_t score_key(double s) {             // ascending
+  const uint64_t u = (uint64_t)__double_as_longlong(s + 0.0);          // (-0 is 0)
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+
+__global__ __launch_bounds__(kSelectThreads) void block_select_kernel(SelectArgs a) {
+  constexpr int kWaves = kSelectThreads / kWave;
+  __shared__ uint64_t stays[kMostBlocks / 64];
+  __shared__ uint64_t even[kMostBlocks / 64];          // equal to the smallest that stays, where too many are
+  __shared__ uint32_t digits[kDigits];
+  __shared__ uint64_t list[kRanked];
+  __shared__ int list_at[kRanked];
+  __shared__ uint64_t lows[kWaves], highs[kWaves];
+  __shared__ uint32_t counts[kWaves];
+  __shared__ int n_list, digit_at;
+  __shared__ uint32_t above_at;
+  const int tid = threadIdx.x, wave = tid / kWave, lane = tid & (kWave - 1);
+  const int local = blockIdx.x / a.hkv, kvh = blockIdx.x % a.hkv, t = a.first + local;
+  int32_t* out = a.blocks + ((int64_t)t * a.hkv + kvh) * a.keep;
+  const TokenBlocks tb = token_blocks(a, t);
+  if (tb.seen <= a.keep) {
+    for (int i = tid; i < a.keep; i += kSelectThreads) out[i] = i < tb.seen ? i : -1;
+    return;
+  }
+  const int n = tb.scored;
+  int need = a.keep - a.recent;
+  for (int i = tid; i < a.recent; i += kSelectThreads) out[need + i] = n + i;
+  if (need == 0) return;
+  const double* scores = a.scores + ((int64_t)local * a.hkv + kvh) * a.most;
+  uint64_t held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int j = tid + i * kSelectThreads;
+    held[i] = j < n ? score_key(scores[j]) : 0;
+  }
+  // f(key, j, whether there is one) for all entries, every wavefront's lanes together
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (i * kSelectThreads < n) f(held[i], tid + i * kSelectThreads, tid + i * kSelectThreads < n);
+    for (int j0 = kHeld * kSelectThreads; j0 < n; j0 += kSelectThreads) {
+      const int j = j0 + tid;
+      f(j < n ? score_key(scores[j]) : 0, j, j < n);
+    }
+  };
+  uint64_t low = ~0ull, high = 0;
+  each([&](uint64_t key, int, bool there) {
+    if (!there) return;
+    low = min(low, key);
+    high = max(high, key);
+  });
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    low = min(low, (uint64_t)__shfl_xor((unsigned long long)low, o, kWave));
+    high = max(high, (uint64_t)__shfl_xor((unsigned long long)high, o, kWave));
+  }
+  if (lane == 0) {
+    lows[wave] = low;
+    highs[wave] = high;
+  }
+  for (int i = tid; i < kDigits; i += kSelectThreads) digits[i] = 0;
+  if (tid == 0) n_list = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    low = min(low, lows[w]);
+    high = max(high, highs[w]);
+  }
+  int top = 64 - __clzll((long long)((low ^ high) | 1));      // bits from here on agree in all entries
+  int shift = max(0, top - 11);
+  uint64_t prefix = top >= 64 ? 0 : low >> top << top;
+  // each turn: of the entries that agree with `prefix` from `top` on, the digit that the last one to stay has
+  int in_digit = 0;
+  for (;;) {
+    auto mine = [&](uint64_t key) { return top >= 64 || (key ^ prefix) >> top == 0; };
+    each([&](uint64_t key, int, bool there) {
+      if (there && mine(key)) atomicAdd(&digits[(int)(key >> shift) & (kDigits - 1)], 1u);
+    });
+    __syncthreads();
+    constexpr int kEach = kDigits / kSelectThreads;             // digits from the largest down: thread 0 has the largest ones
+    uint32_t mine_n = 0, of[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) mine_n += of[i] = digits[kDigits - 1 - (tid * kEach + i)];
+    uint32_t upto = mine_n;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const uint32_t u = __shfl_up(upto, o, kWave);
+      if (lane >= o) upto += u;
+    }
+    if (lane == kWave - 1) counts[wave] = upto;
+    __syncthreads();
+    uint32_t before = upto - mine_n;
+    for (int w = 0; w < wave; ++w) before += counts[w];
+    if (before < (uint32_t)need && (uint32_t)need <= before + mine_n) {
+      uint32_t at = before;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        if (at < (uint32_t)need && (uint32_t)need <= at + of[i]) {
+          digit_at = kDigits - 1 - (tid * kEach + i);
+          above_at = at;
+        }
+        at += of[i];
+      }
+    }
+    __syncthreads();
+    const int digit = digit_at;
+    need -= (int)above_at;
+    in_digit = (int)digits[digit];
+    prefix |= (uint64_t)digit << shift;
+    top = shift;
+    __syncthreads();
+    if (in_digit == need || in_digit <= kRanked || top == 0) break;
+    shift = max(0, top - 11);
+    for (int i = tid; i < kDigits; i += kSelectThreads) digits[i] = 0;
+    __syncthreads();
+  }
+  // larger ones stay; of those that agree with the prefix all, or the `need` first in order
+  const bool all = in_digit == need, ranked = !all && in_digit <= kRanked;
+  each([&](uint64_t key, int j, bool there) {
+    const uint64_t over = key >> top, border = prefix >> top;
+    const bool same = there && over == border;
+    const uint64_t in = __ballot((there && over > border) || (same && all)), equal = __ballot(same && !all && !ranked);
+    if (same && ranked) {
+      const int at = atomicAdd(&n_list, 1);
+      list[at] = key;
+      list_at[at] = j;
+    }
+    if (lane == 0) {
+      stays[j >> 6] = in;
+      even[j >> 6] = equal;
+    }
+  });
+  __syncthreads();
+  if (ranked) {
+    if (tid < in_digit) {
+      int rank = 0;
+      for (int i = 0; i < in_digit; ++i) rank += list[i] > list[tid] || (list[i] == list[tid] && list_at[i] < list_at[tid]);
+      if (rank < need) atomicOr((unsigned long long*)&stays[list_at[tid] >> 6], 1ull << (list_at[tid] & 63));
+    }
+    __syncthreads();
+  }
+  // a thread takes consecutive words
+  const int words = (n + 63) / 64, per = (words + kSelectThreads - 1) / kSelectThreads, w0 = tid * per, w1 = min(w0 + per, words);
+  auto before_of = [&](uint32_t v) {
+    uint32_t upto = v;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const uint32_t u = __shfl_up(upto, o, kWave);
+      if (lane >= o) upto += u;
+    }
+    if (lane == kWave - 1) counts[wave] = upto;
+    __syncthreads();
+    uint32_t before = upto - v;
+    for (int w = 0; w < wave; ++w) before += counts[w];
+    __syncthreads();
+    return before;
+  };
+  if (!all && !ranked) {
+    uint32_t v = 0;
+    for (int w = w0; w < w1; ++w) v += __popcll(even[w]);
+    int left = need - (int)before_of(v);
+    for (int w = w0; w < w1; ++w)
+      for (uint64_t m = even[w]; m && left > 0; m &= m - 1, --left) stays[w] |= m & (~m + 1);
+  }
+  uint32_t v = 0;
+  for (int w = w0; w < w1; ++w) v += __popcll(stays[w]);
+  int at = (int)before_of(v);
+  for (int w = w0; w < w1; ++w)
+    for (uint64_t m = stays[w]; m; m &= m - 1) out[at++] = w * 64 + __ffsll((unsigned long long)m) - 1;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- attention
+// As the attention of few rows over a whole cache (paged_attention.hip): a unit is (token, KV head, chunk of the listed rows) and one wavefront, whose
+// rows travel straight into its own ring of LDS stages, 32 keys each; S^T = K Q^T and O^T = V^T P^T by 16x16x32 products; a row's
+// probabilities are relative to a reference that follows its largest score by at most 2^8.  A probability goes into its product as two numbers
+// of the type, what it rounds to and what that leaves (2^-17 of it in bf16): a few rows carry most of a selected context, so that roundings do not cancel, and the
+// second product costs nothing beside the rows' way out of memory (2-norm against 64 bits with one number 0.0026, with two 0.0016, which is
+// the output's own rounding).  A listed row that the token does not see (behind it, of no block) is a row of zeros and has no probability: what the
+// cache holds there never comes near a product.
+constexpr int kAttendKeys = 32;
+constexpr int kAttendStages = 2;
+constexpr int kAttendSegment = 512;        // keys whose row offsets are in LDS at a time
+__device__ __attribute__((aligned(16))) uint32_t zero_piece[4];
+
+struct AttendArgs {
+  const uint16_t* q;
+  const uint16_t* pool;
+  const int32_t* table;
+  const int32_t* blocks;
+  const int32_t* sequences;
+  const int32_t* positions;
+  uint16_t* out;
+  float* part_o;                 // [token][n_kv_heads][chunks][group][D], fp32
+  float* part_ml;                // (reference, sum)
+  int64_t q_token, q_head, table_stride, page_elems;
+  int batch, first, hq, hkv, group, page_shift, max_pages, keep, last_row, keys, chunk_keys, chunks;
+  float scale_log2;
+};
+template <int D> __device__ __forceinline__ int attend_k_swap(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+template <int D> __device__ __forceinline__ int attend_v_swap(int row) { return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3); }
+
+template <int DT, int D, int ROWT>
+__global__ __launch_bounds__(kWave) void block_attention_kernel(AttendArgs a) {
+  constexpr int kRowBytes = D * 2, kPieces = kRowBytes / 16, kRowsPerCopy = 64 / kPieces, kCopies = kAttendKeys / kRowsPerCopy;
+  constexpr int kHalf = kAttendKeys * kRowBytes, kStage = 2 * kHalf;
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[kAttendStages * kStage];
+  __shared__ int64_t row_at[kAttendSegment];
+  __shared__ uint32_t seen_at[kAttendSegment / kAttendKeys];
+  const uint32_t unit = blockIdx.x;
+  const int kvh = (int)(unit % (uint32_t)a.hkv);
+  const uint32_t tc = unit / (uint32_t)a.hkv;
+  const int chunk = (int)(tc % (uint32_t)a.chunks), local = (int)(tc / (uint32_t)a.chunks), t = a.first + local;
+  const int b = a.sequences[t];
+  if (b < 0 || b >= a.batch) return;
+  const int last = min(a.positions[t], a.last_row), lane = threadIdx.x, lq = lane & 15, lg = lane >> 4;
+
+  dec_u4 q[ROWT][D / 32];
+#pragma unroll
+  for (int nt = 0; nt < ROWT; ++nt) {
+    const int r = nt * 16 + lq;
+    const uint16_t* src = a.q + t * a.q_token + (int64_t)(kvh * a.group + min(r, a.group - 1)) * a.q_head + lg * 8;
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ++ks) q[nt][ks] = r < a.group ? *(const dec_u4*)(src + ks * 32) : dec_u4{0, 0, 0, 0};
+  }
+  v4f o[ROWT][D / 16];
+  float ref[ROWT], l[ROWT];                                  // ref in units of exp2's argument
+#pragma unroll
+  for (int nt = 0; nt < ROWT; ++nt) {
+    ref[nt] = -INFINITY;
+    l[nt] = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < D / 16; ++mt) o[nt][mt] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+  const uint32_t ring0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)ring;
+  const char* kbase = (const char*)(a.pool + kvh * D);
+  const int64_t v_bytes = a.page_elems * 2;
+  const int crow = lane / kPieces, cpiece = lane % kPieces;
+  const uint32_t koff = ring0 + lq * kRowBytes;
+  const uint32_t voff = ring0 + kHalf + (4 * lg + (lq >> 2)) * kRowBytes + (lq & 1) * 8;
+  const int kswap = attend_k_swap<D>(lq), vswap = attend_v_swap<D>(4 * lg + (lq >> 2)), vpiece = (lq >> 1) & 1;
+  const int32_t* list = a.blocks + ((int64_t)t * a.hkv + kvh) * a.keep;
+  const int32_t* row_pages = a.table + b * a.table_stride;
+  const int v_begin = chunk * a.chunk_keys, v_end = min(v_begin + a.chunk_keys, a.keys);
+
+  for (int v0 = v_begin; v0 < v_end; v0 += kAttendSegment) {
+    int stages = 0;                                          // up to the last one of which something is seen
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int u = 0; u < kAttendSegment / 64; ++u) {
+      if (u * 64 >= v_end - v0) continue;
+      const int v = v0 + u * 64 + lane;
+      const int block = v < v_end ? list[v >> a.page_shift] : -1, in = v & ((1 << a.page_shift) - 1);
+      const bool sees = block >= 0 && last >= 0 && block <= last >> a.page_shift && (block << a.page_shift) + in <= last;
+      const int page = sees ? min(max(row_pages[block], 0), a.max_pages - 1) : 0;
+      row_at[u * 64 + lane] = sees ? 2 * ((int64_t)page * 2 * a.page_elems + (int64_t)a.hkv * D * in) : -1;
+      const uint64_t some = __ballot(sees);
+      if (lane < 2) seen_at[u * 2 + lane] = (uint32_t)(some >> (32 * lane));
+      if (some) stages = u * 2 + (some >> 32 ? 2 : 1);
+    }
+    __builtin_amdgcn_s_waitcnt(0);                           // rows' offsets and the queries; from here on only copies are counted
+    int64_t from[kCopies];                                   // of the copies to be asked for next: read together, well before their use
+    auto look_up = [&](int st) {
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c) from[c] = row_at[st * kAttendKeys + c * kRowsPerCopy + crow];
+    };
+    auto request = [&](int st) {
+      const uint32_t at = ring0 + (uint32_t)(st % kAttendStages) * kStage;
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c) {
+        const int row = c * kRowsPerCopy + crow;
+        const char* src = kbase + from[c];
+        const char* k = from[c] < 0 ? (const char*)zero_piece : src + ((cpiece ^ attend_k_swap<D>(row)) << 4);
+        const char* v = from[c] < 0 ? (const char*)zero_piece : src + v_bytes + ((cpiece ^ attend_v_swap<D>(row)) << 4);
+        dma16_nt(at + c * 1024, k);
+        dma16_nt(at + kHalf + c * 1024, v);
+      }
+    };
+    for (int st = 0; st < min(kAttendStages, stages); ++st) {
+      look_up(st);
+      request(st);
+    }
+    for (int st = 0; st < stages; ++st) {
+      if (st + kAttendStages <= stages) wait_vmcnt<(kAttendStages - 1) * 2 * kCopies>();
+      else wait_vmcnt<0>();
+      look_up(min(st + kAttendStages, stages - 1));
+      const uint32_t at = (uint32_t)(st % kAttendStages) * kStage;
+      const uint32_t seen = __builtin_amdgcn_readfirstlane(seen_at[st]);
+      v4f s[ROWT][2];
+#pragma unroll
+      for (int nt = 0; nt < ROWT; ++nt) s[nt][0] = s[nt][1] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < D / 32; ++ks)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const dec_u4 k = lds_16(koff + at + h * 16 * kRowBytes + (((ks * 4 + lg) ^ kswap) << 4));
+#pragma unroll
+          for (int nt = 0; nt < ROWT; ++nt) s[nt][h] = mfma16x16x32<DT>(k, q[nt][ks], s[nt][h]);
+        }
+      dec_u4 vt[D / 16];
+#pragma unroll
+      for (int mt = 0; mt < D / 16; ++mt) {
+        const uint32_t va = voff + at + (((mt * 2 + vpiece) ^ vswap) << 4);
+        const uint2 lo = lds_tr16(va), hi = lds_tr16(va + 16 * kRowBytes);
+        vt[mt] = dec_u4{lo.x, lo.y, hi.x, hi.y};
+      }
+      dec_u4 pb[ROWT], rest[ROWT];
+#pragma unroll
+      for (int nt = 0; nt < ROWT; ++nt) {
+        float x[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) x[r] = s[nt][r >> 2][r & 3] * a.scale_log2;
+        if (seen != ~0u) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (!(seen >> ((r >> 2) * 16 + 4 * lg + (r & 3)) & 1)) x[r] = -INFINITY;
+        }
+        const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        if (__any(top > ref[nt] + kSlack)) {                 // (also where the reference is still -inf)
+          float m = fmaxf(top, __shfl_xor(top, 16, kWave));
+          m = fmaxf(m, __shfl_xor(m, 32, kWave));
+          const float next = m > ref[nt] + kSlack ? m : ref[nt];
+          const float alpha = next == ref[nt] ? 1.f : __builtin_amdgcn_exp2f(ref[nt] - next);
+          ref[nt] = next;
+          l[nt] *= alpha;
+#pragma unroll
+          for (int mt = 0; mt < D / 16; ++mt) o[nt][mt] *= alpha;
+        }
+        const float base = ref[nt] == -INFINITY ? 0.f : ref[nt];
+        float e[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) e[r] = __builtin_amdgcn_exp2f(x[r] - base);
+        l[nt] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+        pb[nt] = pack8<DT>(e);
+        float near[8];
+        unpack8<DT>(pb[nt], near);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) e[r] -= near[r];
+        rest[nt] = pack8<DT>(e);
+      }
+#pragma unroll
+      for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < ROWT; ++nt) {
+          o[nt][mt] = mfma16x16x32<DT>(vt[mt], pb[nt], o[nt][mt]);
+          o[nt][mt] = mfma16x16x32<DT>(vt[mt], rest[nt], o[nt][mt]);
+        }
+      if (st + kAttendStages < stages) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the stage has been read
+        request(st + kAttendStages);
+      }
+    }
+  }
+
+#pragma unroll
+  for (int nt = 0; nt < ROWT; ++nt) {
+    float sum = l[nt] + __shfl_xor(l[nt], 16, kWave);
+    sum += __shfl_xor(sum, 32, kWave);
+    const int r = nt * 16 + lq;
+    if (r >= a.group) continue;
+    if (a.chunks == 1) {
+      const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+      uint16_t* dst = a.out + ((int64_t)t * a.hq + kvh * a.group + r) * D + lg * 4;
+#pragma unroll
+      for (int mt = 0; mt < D / 16; ++mt)
+        *(uint2*)(dst + mt * 16) = make_uint2(pack2<DT>(o[nt][mt][0] * inv, o[nt][mt][1] * inv), pack2<DT>(o[nt][mt][2] * inv, o[nt][mt][3] * inv));
+    } else {
+      const int64_t slot = (((int64_t)local * a.hkv + kvh) * a.chunks + chunk) * a.group + r;
+      float* dst = a.part_o + slot * D + lg * 4;
+#pragma unroll
+      for (int mt = 0; mt < D / 16; ++mt) *(v4f*)(dst + mt * 16) = o[nt][mt];
+      if (lg == 0) *(v2f*)(a.part_ml + slot * 2) = v2f{ref[nt], sum};
+    }
+  }
+}
+
+// out = sum_c 2^(ref_c - max ref) O_c / sum_c 2^(ref_c - max ref) l_c, a wavefront a row
+template <int DT, int D>
+__global__ __launch_bounds__(256) void block_merge_kernel(AttendArgs a, int64_t rows) {
+  constexpr int kLanes = D / 4, kSide = kWave / kLanes;
+  const int64_t id = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;              // (token, KV head, row)
+  if (id >= rows) return;
+  const int lane = threadIdx.x & (kWave - 1), r = (int)(id % a.group);
+  const int64_t tk = id / a.group;
+  const int t = a.first + (int)(tk / a.hkv), kvh = (int)(tk % a.hkv);
+  const int b = a.sequences[t];
+  if (b < 0 || b >= a.batch) return;
+  const int64_t slot = tk * a.chunks * a.group + r;
+  const float* ml = a.part_ml + slot * 2;
+  const float* po = a.part_o + slot * D + (lane % kLanes) * 4;
+  float top = -INFINITY;
+  for (int c = lane; c < a.chunks; c += kWave) top = fmaxf(top, ml[(int64_t)c * a.group * 2]);
+  top = wave_max(top);
+  const float base = top == -INFINITY ? 0.f : top;
+  v4f num = {0.f, 0.f, 0.f, 0.f};
+  float den = 0.f;
+#pragma unroll 8
+  for (int c = lane / kLanes; c < a.chunks; c += kSide) {
+    const v4f part = *(const v4f*)(po + (int64_t)c * a.group * D);
+    const v2f m = *(const v2f*)(ml + (int64_t)c * a.group * 2);
+    const float w = __builtin_amdgcn_exp2f(m[0] - base);
+    den = fmaf(w, m[1], den);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) num[e] = fmaf(w, part[e], num[e]);
+  }
+#pragma unroll
+  for (int s = kLanes; s < kWave; s <<= 1) {
+    den += __shfl_xor(den, s, kWave);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) num[e] += __shfl_xor(num[e], s, kWave);
+  }
+  if (lane >= kLanes) return;
+  const float inv = den > 0.f ? 1.f / den : 0.f;
+  *(uint2*)(a.out + ((int64_t)t * a.hq + kvh * a.group + r) * D + lane * 4) =
+      make_uint2(pack2<DT>(num[0] * inv, num[1] * inv), pack2<DT>(num[2] * inv, num[3] * inv));
+}
+
+// Chunks of a unit's listed rows, as those of few rows over a whole cache; tokens whose partial results are held at a time.
+struct AttendPlan { int chunk_keys, chunks; int64_t tokens; size_t part_o, part_ml, bytes; };
+static AttendPlan attend_plan(int64_t n_tokens, int64_t hq, int64_t hkv, int64_t head_dim, int64_t keys) {
+  AttendPlan p{};
+  const int64_t units = n_tokens * hkv;
+  int64_t per = ((int64_t)(0.65 * std::sqrt((double)units * (double)keys)) + kAttendKeys - 1) / kAttendKeys * kAttendKeys;
+  per = std::min<int64_t>(std::max<int64_t>(per, 64), 384);
+  while (keys > per * 256) per *= 2;
+  p.chunk_keys = (int)per;
+  p.chunks = (int)((keys + per - 1) / per);
+  p.tokens = n_tokens;
+  if (p.chunks > 1) {
+    p.tokens = std::min<int64_t>(n_tokens, std::max<int64_t>(1, (1 << 20) / (hq * p.chunks)));      // half a gigabyte of partial results at 128 a head
+    const size_t slots = (size_t)p.tokens * hq * p.chunks;
+    p.part_o = align_up(slots * head_dim * sizeof(float), 256);
+    p.part_ml = align_up(slots * 2 * sizeof(float), 256);
+  }
+  p.bytes = 256 + p.part_o + p.part_ml;
+  return p;
+}
+
+// Scores of so many tokens are held at a time (a quarter of a gigabyte)
+static int64_t select_tokens(int64_t n_tokens, int64_t hkv, int64_t most) {
+  const int64_t fit = std::max<int64_t>(kScoreTokens, (1 << 25) / (hkv * std::max<int64_t>(most, 1)) / kScoreTokens * kScoreTokens);
+  return std::min(n_tokens, fit);
+}
+
+template <int DT, int D>
+static void launch_attend_of(const AttendArgs& a, int64_t tokens, hipStream_t st) {
+  const dim3 grid((unsigned)(tokens * a.chunks * a.hkv)), block(kWave);
+  if (a.group <= 16) hipLaunchKernelGGL((block_attention_kernel<DT, D, 1>), grid, block, 0, st, a);
+  else if (a.group <= 32) hipLaunchKernelGGL((block_attention_kernel<DT, D, 2>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((block_attention_kernel<DT, D, 4>), grid, block, 0, st, a);
+}
+template <int DT, int D>
+static void launch_block_merge_of(const AttendArgs& a, int64_t tokens, hipStream_t st) {
+  const int64_t rows = tokens * a.hq;
+  hipLaunchKernelGGL((block_merge_kernel<DT, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, rows);
+}
+
+}  // namespace subspec
+
+using namespace subspec;
+
+static int check_pool_shape(const char* what, int dtype, int64_t head_dim, int64_t max_pages, int64_t page_len) {
+  if (dtype != SUBSPEC_BF16 && dtype != SUBSPEC_F16)
+    SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: dtype %d not supported (bf16 / fp16 only)", what, dtype);
+  if (head_dim != 64 && head_dim != 128)
+    SUBSPEC_FAIL(SUBSPEC_ERR_LIMIT, "%s: head_dim=%lld (built for 64 and 128)", what, (long long)head_dim);
+  if (page_len < 1 || page_len > (1 << 20) || (page_len & (page_len - 1)))
+    SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: page_len=%lld is no power of two up to 2^20", what, (long long)page_len);
+  if (max_pages < 1 || max_pages > INT32_MAX) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: %lld pages", what, (long long)max_pages);
+  return SUBSPEC_OK;
+}
+static int check_batch(const char* what, int64_t batch, int64_t n_tokens, int64_t hq, int64_t hkv, int64_t max_blocks, int64_t table_stride) {
+  if (batch < 1 || batch > SUBSPEC_MAX_BATCH)
+    SUBSPEC_FAIL(SUBSPEC_ERR_LIMIT, "%s: batch=%lld outside [1, %d]", what, (long long)batch, SUBSPEC_MAX_BATCH);
+  if (n_tokens < 0 || n_tokens > (1 << 20)) SUBSPEC_FAIL(SUBSPEC_ERR_LIMIT, "%s: n_tokens=%lld outside [0, 2^20]", what, (long long)n_tokens);
+  if (hq < 1 || hkv < 1 || hq % hkv || hq > 1024) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: heads=%lld/%lld", what, (long long)hq, (long long)hkv);
+  if (max_blocks < 1 || max_blocks > INT32_MAX || table_stride < max_blocks)
+    SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: a table of %lld columns with a row stride of %lld", what, (long long)max_blocks, (long long)table_stride);
+  return SUBSPEC_OK;
+}
+
+extern "C" int subspec_kv_page_bounds(const void* kv_pool_layer, void* bounds, int dtype, int64_t max_pages, int64_t page_len,
+                                      int64_t n_kv_heads, int64_t head_dim, const int64_t* slots, int64_t n_tokens, void* stream) {
+  const char* what = "kv_page_bounds";
+  if (const int code = check_pool_shape(what, dtype, head_dim, max_pages, page_len)) return code;
+  if (n_kv_heads < 1 || n_kv_heads > 1024) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: %lld heads", what, (long long)n_kv_heads);
+  if (n_tokens < 0 || n_tokens > (1ll << 30)) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: n_tokens=%lld", what, (long long)n_tokens);
+  if (n_tokens == 0) return SUBSPEC_OK;
+  if (!kv_pool_layer || !bounds || !slots) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: null pointer argument", what);
+  if ((uintptr_t)kv_pool_layer % 16 || (uintptr_t)bounds % 16) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: the pool and bounds must be 16-byte aligned", what);
+  BoundsArgs a;
+  a.pool = (const uint16_t*)kv_pool_layer; a.bounds = (uint16_t*)bounds; a.slots = slots;
+  a.n_slots = max_pages * page_len; a.page_elems = page_len * n_kv_heads * head_dim;
+  a.n_tokens = (int)n_tokens; a.page_shift = block_shift_of(page_len);
+  a.pieces = (int)(n_kv_heads * head_dim / 8); a.head_pieces = (int)(head_dim / 8);
+  a.per = n_tokens > 4096 ? 16 : 1;
+  hipStream_t st = (hipStream_t)stream;
+  const dim3 grid((unsigned)((n_tokens + a.per - 1) / a.per)), block(kBoundsThreads);
+  DominantKernelTimer timer(st);
+  if (dtype == SUBSPEC_BF16) hipLaunchKernelGGL(page_bounds_kernel<SUBSPEC_BF16>, grid, block, 0, st, a);
+  else hipLaunchKernelGGL(page_bounds_kernel<SUBSPEC_F16>, grid, block, 0, st, a);
+  SUBSPEC_CHECK_HIP(hipGetLastError());
+  return SUBSPEC_OK;
+}
+
+// blocks that any token of a call can see
+static int64_t most_blocks(int64_t page_len, int64_t max_blocks, int64_t max_kv) {
+  return std::min(max_blocks, (max_kv + page_len - 1) / page_len);
+}
+
+extern "C" size_t subspec_select_blocks_workspace(int64_t n_tokens, int64_t n_kv_heads, int64_t page_len, int64_t max_blocks, int64_t max_kv) {
+  if (n_tokens < 1 || n_tokens > (1 << 20) || n_kv_heads < 1 || n_kv_heads > 1024 || page_len < 1 || max_blocks < 1 || max_kv < 0 ||
+      max_kv > (1ll << 30) || max_blocks > INT32_MAX)
+    return 256;
+  const int64_t most = most_blocks(page_len, max_blocks, max_kv);
+  if (most > kMostBlocks) return 256;
+  return 256 + (size_t)select_tokens(n_tokens, n_kv_heads, most) * n_kv_heads * most * sizeof(double);
+}
+
+extern "C" int subspec_select_blocks(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* bounds, int dtype,
+                                     int64_t max_pages, int64_t page_len, const int32_t* block_table, int64_t max_blocks,
+                                     int64_t table_stride, const int32_t* sequences, const int32_t* positions, int64_t batch,
+                                     int64_t n_tokens, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim, int64_t max_kv,
+                                     int64_t keep, int64_t recent, int32_t* blocks, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "select_blocks";
+  if (const int code = check_pool_shape(what, dtype, head_dim, max_pages, page_len)) return code;
+  if (const int code = check_batch(what, batch, n_tokens, n_q_heads, n_kv_heads, max_blocks, table_stride)) return code;
+  if (max_kv < 0 || max_kv > (1ll << 30)) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: max_kv=%lld outside [0, 2^30]", what, (long long)max_kv);
+  if (recent < 1 || keep < recent || keep > kMostBlocks)
+    SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: keep=%lld (at most 2^17), recent=%lld (1 to keep)", what, (long long)keep, (long long)recent);
+  const int64_t most = most_blocks(page_len, max_blocks, max_kv);
+  if (most > kMostBlocks)
+    SUBSPEC_FAIL(SUBSPEC_ERR_LIMIT, "%s: %lld blocks a sequence (at most 2^17): larger pages, or a smaller max_kv", what, (long long)most);
+  if (n_tokens == 0) return SUBSPEC_OK;
+  if (!q || !bounds || !block_table || !sequences || !positions || !blocks) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: null pointer argument", what);
+  if ((uintptr_t)q % 16 || (uintptr_t)bounds % 16 || q_token_stride % 8 || q_head_stride % 8 || q_token_stride < 0 || q_head_stride < 0)
+    SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: q and bounds must be 16-byte aligned, q's strides multiples of 8 elements", what);
+  const size_t need = subspec_select_blocks_workspace(n_tokens, n_kv_heads, page_len, max_blocks, max_kv);
+  if (need > 256 && (!workspace || workspace_bytes < need))
+    SUBSPEC_FAIL(SUBSPEC_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the %zu required", what, workspace_bytes, need);
+  if ((uintptr_t)workspace % 16) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
+  SelectArgs a;
+  a.q = (const uint16_t*)q; a.bounds = (const uint16_t*)bounds; a.table = block_table; a.sequences = sequences; a.positions = positions;
+  a.blocks = blocks; a.scores = (double*)workspace;
+  a.q_token = q_token_stride; a.q_head = q_head_stride; a.table_stride = table_stride; a.most = most;
+  a.batch = (int)batch; a.n_tokens = (int)n_tokens; a.hkv = (int)n_kv_heads; a.group = (int)(n_q_heads / n_kv_heads);
+  a.page_shift = block_shift_of(page_len); a.max_pages = (int)max_pages; a.keep = (int)keep; a.recent = (int)recent;
+  a.last_row = (int)(std::min(max_kv, max_blocks * page_len) - 1);
+  const int64_t at_once = select_tokens(n_tokens, n_kv_heads, most);
+  hipStream_t st = (hipStream_t)stream;
+  for (int64_t first = 0; first < n_tokens; first += at_once) {
+    const int64_t some = std::min(at_once, n_tokens - first);
+    a.first = (int)first;
+    a.span = some * n_kv_heads * most < (1 << 17) ? 16 : 64;
+    a.spans = (int)((most + a.span - 1) / a.span);
+    const dim3 grid((unsigned)(some * n_kv_heads * a.spans)), block(kWave);
+    if (most > keep) {
+      DominantKernelTimer timer(st);
+      if (dtype == SUBSPEC_BF16) {
+        if (head_dim == 128) hipLaunchKernelGGL((block_score_kernel<SUBSPEC_BF16, 128>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((block_score_kernel<SUBSPEC_BF16, 64>), grid, block, 0, st, a);
+      } else {
+        if (head_dim == 128) hipLaunchKernelGGL((block_score_kernel<SUBSPEC_F16, 128>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((block_score_kernel<SUBSPEC_F16, 64>), grid, block, 0, st, a);
+      }
+    }
+    hipLaunchKernelGGL(block_select_kernel, dim3((unsigned)(some * n_kv_heads)), dim3(kSelectThreads), 0, st, a);
+  }
+  SUBSPEC_CHECK_HIP(hipGetLastError());
+  return SUBSPEC_OK;
+}
+
+extern "C" size_t subspec_block_attention_workspace(int64_t n_tokens, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
+                                                    int64_t page_len, int64_t keep) {
+  if (n_tokens < 1 || n_tokens > (1 << 20) || n_kv_heads < 1 || n_q_heads < n_kv_heads || n_q_heads > 1024 || head_dim < 1 || head_dim > 1024 ||
+      page_len < 1 || page_len > (1 << 20) || keep < 1 || keep > kMostBlocks || keep * page_len > (1 << 30))
+    return 256;
+  return attend_plan(n_tokens, n_q_heads, n_kv_heads, head_dim, keep * page_len).bytes;
+}
+
+extern "C" int subspec_block_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* kv_pool_layer, int dtype,
+                                       int64_t max_pages, int64_t page_len, const int32_t* block_table, int64_t max_blocks,
+                                       int64_t table_stride, const int32_t* blocks, int64_t keep, const int32_t* sequences,
+                                       const int32_t* positions, int64_t batch, int64_t n_tokens, int64_t n_q_heads, int64_t n_kv_heads,
+                                       int64_t head_dim, float scale, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "block_attention";
+  if (const int code = check_pool_shape(what, dtype, head_dim, max_pages, page_len)) return code;
+  if (const int code = check_batch(what, batch, n_tokens, n_q_heads, n_kv_heads, max_blocks, table_stride)) return code;
+  if (n_q_heads / n_kv_heads > 64)
+    SUBSPEC_FAIL(SUBSPEC_ERR_LIMIT, "%s: %lld query heads a KV head (at most 64)", what, (long long)(n_q_heads / n_kv_heads));
+  if (keep < 1 || keep > kMostBlocks || keep * page_len > (1 << 30))
+    SUBSPEC_FAIL(SUBSPEC_ERR_LIMIT, "%s: %lld blocks of %lld rows a token (2^17 blocks, 2^30 rows at most)", what, (long long)keep,
+                 (long long)page_len);
+  if (!(scale > 0.f) || scale > 1e30f) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: scale=%g must be positive", what, (double)scale);
+  if (n_tokens == 0) return SUBSPEC_OK;
+  if (!q || !kv_pool_layer || !block_table || !blocks || !sequences || !positions || !out)
+    SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: null pointer argument", what);
+  if ((uintptr_t)q % 16 || (uintptr_t)kv_pool_layer % 16 || (uintptr_t)out % 16 || q_token_stride % 8 || q_head_stride % 8 ||
+      q_token_stride < 0 || q_head_stride < 0)
+    SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: q, the pool and out must be 16-byte aligned, q's strides multiples of 8 elements", what);
+  const AttendPlan p = attend_plan(n_tokens, n_q_heads, n_kv_heads, head_dim, keep * page_len);
+  if (p.bytes > 256 && (!workspace || workspace_bytes < p.bytes))
+    SUBSPEC_FAIL(SUBSPEC_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the %zu required", what, workspace_bytes, p.bytes);
+  if ((uintptr_t)workspace % 16) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
+  AttendArgs a;
+  a.q = (const uint16_t*)q; a.pool = (const uint16_t*)kv_pool_layer; a.table = block_table; a.blocks = blocks; a.sequences = sequences;
+  a.positions = positions; a.out = (uint16_t*)out;
+  a.part_o = (float*)workspace; a.part_ml = (float*)((char*)workspace + p.part_o);
+  a.q_token = q_token_stride; a.q_head = q_head_stride; a.table_stride = table_stride; a.page_elems = page_len * n_kv_heads * head_dim;
+  a.batch = (int)batch; a.hq = (int)n_q_heads; a.hkv = (int)n_kv_heads; a.group = (int)(n_q_heads / n_kv_heads);
+  a.page_shift = block_shift_of(page_len); a.max_pages = (int)max_pages; a.keep = (int)keep;
+  a.last_row = (int)(std::min<int64_t>(max_blocks * page_len, 1ll << 30) - 1);
+  a.keys = (int)(keep * page_len); a.chunk_keys = p.chunk_keys; a.chunks = p.chunks;
+  a.scale_log2 = scale * kLog2e;
+  if (p.tokens * p.chunks * n_kv_heads > INT32_MAX)
+    SUBSPEC_FAIL(SUBSPEC_ERR_LIMIT, "%s: too large (%lld tokens of %lld heads)", what, (long long)n_tokens, (long long)n_kv_heads);
+  hipStream_t st = (hipStream_t)stream;
+  for (int64_t first = 0; first < n_tokens; first += p.tokens) {
+    const int64_t some = std::min(p.tokens, n_tokens - first);
+    a.first = (int)first;
+    {
+      DominantKernelTimer timer(st);
+      if (dtype == SUBSPEC_BF16) {
+        if (head_dim == 128) launch_attend_of<SUBSPEC_BF16, 128>(a, some, st);
+        else launch_attend_of<SUBSPEC_BF16, 64>(a, some, st);
+      } else {
+        if (head_dim == 128) launch_attend_of<SUBSPEC_F16, 128>(a, some, st);
+        else launch_attend_of<SUBSPEC_F16, 64>(a, some, st);
+      }
+    }
+    if (p.chunks > 1) {
+      if (dtype == SUBSPEC_BF16) {
+        if (head_dim == 128) launch_block_merge_of<SUBSPEC_BF16, 128>(a, some, st);
+        else launch_block_merge_of<SUBSPEC_BF16, 64>(a, some, st);
+      } else {
+        if (head_dim == 128) launch_block_merge_of<SUBSPEC_F16, 128>(a, some, st);
+        else launch_block_merge_of<SUBSPEC_F16, 64>(a, some, st);
+      }
+    }
+  }
+  SUBSPEC_CHECK_HIP(hipGetLastError());
+  return SUBSPEC_OK;
+}

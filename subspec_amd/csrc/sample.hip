@@ -15,8 +15,7 @@
 // A row of more candidates than kCandidates (or a slice's share of them) is searched by one workgroup, which reads it again for every ten bits of
 // every search: 152064 logits of deviation 2 at T = 3 and top-p 0.95 320 to 350 us (41 at T = 1), 64 such rows 400 to 455 (66); rows of equal logits
 // 0.65 to 1.3 ms, with a top-k of 70000 and a top-p 3.5.
-#include "common.h"
-#include "mass_series.h"
+#include "sample.h"
 #include <algorithm>
 
 namespace subspec {
@@ -24,89 +23,10 @@ namespace subspec {
 constexpr int kSampleThreads = 1024;      // of a workgroup that has a whole row
 constexpr int kSliceThreads = 512;        // ... a slice of one
 constexpr int kBins = 1024;
-constexpr float kReach = 29.9f;           // 43 ln 2 = 29.81: masses beyond round to zero
 constexpr int kCandidates = 4096;
 constexpr int kSliceCandidates = 1024;
 
-struct SampleArgs {
-  const void* logits;
-  const float* uniforms;
-  const float* temperatures;     // null: the scalar below, for these four
-  const int32_t* top_ks;
-  const float* top_ps;
-  const float* min_ps;
-  int64_t* tokens;
-  float* probs;
-  int64_t row_stride;
-  int vocab, top_k;
-  float temperature, top_p, min_p;
-};
-
-// What a row is drawn with.
-struct RowRule { double inv_t_log2e; float inv_t; bool greedy; int k; double p, min_p, u; };
-__device__ __forceinline__ RowRule row_rule(const SampleArgs& a, int row) {
-  RowRule r;
-  const float t = a.temperatures ? a.temperatures[row] : a.temperature;
-  const int k = a.top_ks ? a.top_ks[row] : a.top_k;
-  const float p = a.top_ps ? a.top_ps[row] : a.top_p, q = a.min_ps ? a.min_ps[row] : a.min_p, u = a.uniforms[row];
-  r.greedy = !(t >= 1.17549435e-38f);                    // (below the smallest normal number 1 / T is infinite)
-  const double inv_t = r.greedy ? 1.0 : 1.0 / (double)t;
-  r.inv_t_log2e = inv_t * 1.44269504088896340736;
-  r.inv_t = (float)inv_t;
-  r.k = r.greedy ? 1 : k <= 0 ? INT32_MAX : k;
-  r.p = p < 1.f ? (double)p : 1.0;                       // (a NaN filters nothing)
-  r.min_p = q > 0.f ? fmin((double)q, 1.0) : 0.0;
-  r.u = u > 0.f ? (double)u : 0.0;
-  return r;
-}
-// The largest logit, and whether only entries that equal it have mass (T = 0, or it is infinite).
-struct RowTop { float value; double wide; bool only; };
-__device__ __forceinline__ RowTop row_top_of(float top, const RowRule& r) { return RowTop{top, (double)top, r.greedy || top == INFINITY}; }
-
-// 2^f * 2^42 for |f| <= 1/2.  (The coefficients are held in registers of the wavefront: left to itself the compiler copies each into the result before
-// it adds.)
-struct Series {
-  double c[kSeriesTerms];
-  __device__ __forceinline__ Series() {
-    constexpr SeriesTable of = series_table();
-#pragma unroll
-    for (int i = 0; i < kSeriesTerms; ++i) {
-      c[i] = of.c[i];
-      asm("" : "+v"(c[i]));
-    }
-  }
-  __device__ __forceinline__ double operator()(double f) const { return series_value(c, f); }
-};
-// How far entry l is below the largest in units of T, in 32 bits: what the bins go by (falls as l rises, so bins keep the order).  Entries at kReach
-// and beyond, and NaN, have no mass and no bin.
-__device__ __forceinline__ float entry_distance(float l, const RowTop& top, const RowRule& r) {
-  if (top.only) return l == top.value ? 0.f : INFINITY;
-  return (top.value - l) * r.inv_t;
-}
 __device__ __forceinline__ int bin_of(float d) { return (int)(d * (0.999999f * kBins / kReach)); }      // (below kBins, rounding or not)
-// The mass of an entry less than kReach below the largest, in units of 2^-42 and before rounding.
-__device__ __forceinline__ double entry_mass(float l, const RowTop& top, const RowRule& r, const Series& exp2_part) {
-  if (top.only) return (double)(1ull << kMassBits);
-  const double x = ((double)l - top.wide) * r.inv_t_log2e, n = rint(x);
-  return ldexp(exp2_part(x - n), (int)n);
-}
-// ... rounded (to even): below 2^52 a sum with 2^52 has no bits behind the point
-__device__ __forceinline__ uint64_t whole(double m) { return (uint64_t)__double_as_longlong(m + 4503599627370496.0) & 0xfffffffffffffull; }
-
-// Larger logits first, then lower indexes, as ascending keys: the bits of the value that its type has (a bf16's or fp16's float is zero behind
-// them), turned round, and 20 bits of the index.
-template <int DT> constexpr int kDropped = DT == SUBSPEC_F32 ? 0 : DT == SUBSPEC_F16 ? 13 : 16;
-template <int DT>
-__device__ __forceinline__ uint64_t order_key(float l, int i) {
-  uint32_t b = __float_as_uint(l == 0.f ? 0.f : l);      // (-0 is 0)
-  b = b >> 31 ? b : ~b & 0x7fffffffu;                     // positive values below, negative ones with the sign bit above
-  return (uint64_t)(b >> kDropped<DT>) << 20 | (uint32_t)i;
-}
-template <int DT>
-__device__ __forceinline__ float key_logit(uint64_t key) {
-  const uint32_t b = (uint32_t)(key >> 20) << kDropped<DT>;
-  return __uint_as_float(b >> 31 ? b : ~(b | ((1u << kDropped<DT>) - 1)) & 0x7fffffffu);
-}
 
 struct Hist {
   uint64_t mass[kBins];            // a bin's own, or inclusive sums after scan_bins
@@ -122,15 +42,6 @@ struct Search {
   int n;
 };
 
-__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {      // inclusive
-  const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const uint64_t u = __shfl_up((unsigned long long)v, o, kWave);
-    if (lane >= o) v += u;
-  }
-  return v;
-}
 __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
   const int lane = threadIdx.x & (kWave - 1);
 #pragma unroll
@@ -310,10 +221,7 @@ __device__ __forceinline__ uint64_t fill_bins(Hist& h, const void* row, int i0, 
 struct BinRanges { int lo[3], hi[3]; bool by_k, by_p; };
 __device__ __forceinline__ uint64_t below(const Hist& h, int b) { return b > 0 ? h.mass[b - 1] : 0; }
 __device__ __forceinline__ uint64_t top_p_goal(double p, uint64_t z) { return (uint64_t)fmax(ceil(p * (double)z), 1.0) - 1; }
-__device__ __forceinline__ uint64_t draw_goal(double u, uint64_t z) {
-  const uint64_t t = (uint64_t)(u * (double)z);
-  return z > 0 ? min(t, z - 1) : 0;
-}
+template <bool DRAW>
 __device__ __forceinline__ BinRanges bin_ranges(const Hist& h, uint64_t min_p_mass, const RowRule& r) {      // (min_p_mass counts with a min-p only)
   BinRanges g;
   uint64_t z_lo = h.mass[kBins - 1], z_hi = z_lo;
@@ -331,6 +239,11 @@ __device__ __forceinline__ BinRanges bin_ranges(const Hist& h, uint64_t min_p_ma
     g.hi[1] = bin_at(h, false, top_p_goal(r.p, z_hi));
     z_lo = below(h, g.lo[1]) + 1;
     z_hi = h.mass[g.hi[1]];
+  }
+  if constexpr (!DRAW) {
+    g.lo[2] = 1;
+    g.hi[2] = 0;
+    return g;
   }
   if (r.min_p > 0.0) {
     z_lo = min(z_lo, min_p_mass);
@@ -470,14 +383,15 @@ __device__ Found find_entry(Search& s, const Hist& bins, bool by_count, uint64_t
   return Found{s.key, s.upto};
 }
 
-// The row's token from the scanned bins and the candidates (`n` of them, or more than `most`: then from the row itself).
-template <int DT, int THREADS>
-__device__ void draw_row(Search& s, const Hist& bins, const uint64_t* keys, int n, int most, const SampleArgs& a, int row_index, const void* row,
-                         const RowTop& top, const RowRule& r, bool by_k, bool by_p, uint64_t min_p_mass) {
+// The row's token from the scanned bins and the candidates (`n` of them, or more than `most`: then from the row itself).  Without DRAW: what the filters
+// leave, into the row's RowCut.
+template <int DT, int THREADS, bool DRAW>
+__device__ void draw_row(Search& s, const Hist& bins, const uint64_t* keys, int n, int most, const SampleArgs& a, RowCut* cuts, int row_index,
+                         const void* row, const RowTop& top, const RowRule& r, bool by_k, bool by_p, uint64_t min_p_mass) {
   uint64_t z = bins.mass[kBins - 1];
-  Found found{};
+  Found found{~0ull, 0};
 #pragma unroll 1
-  for (int which = by_k ? 0 : by_p ? 1 : 2; which < 3; which += which == 0 && !by_p ? 2 : 1) {       // (one copy of the search in the code)
+  for (int which = by_k ? 0 : by_p ? 1 : 2; which < (DRAW ? 3 : 2); which += which == 0 && !by_p ? 2 : 1) {       // (one copy of the search in the code)
     if (which == 2 && r.min_p > 0.0) z = min(z, min_p_mass);
     const uint64_t t = which == 0 ? (uint32_t)r.k - 1 : which == 1 ? top_p_goal(r.p, z) : draw_goal(r.u, z);
     found = find_entry<DT, THREADS>(s, bins, which == 0, t, top, r, n <= most ? n : a.vocab, [&](auto f) {
@@ -491,15 +405,22 @@ __device__ void draw_row(Search& s, const Hist& bins, const uint64_t* keys, int 
     });
     if (which < 2) z = found.upto;
   }
-  if (threadIdx.x == 0) {
+  if (threadIdx.x != 0) return;
+  if constexpr (DRAW) {
     a.tokens[row_index] = (int64_t)(found.key & 0xfffff);
     a.probs[row_index] = (float)(entry_mass(key_logit<DT>(found.key), top, r, Series()) / (double)z);
+  } else {
+    cuts[row_index] = RowCut{(double)(r.min_p > 0.0 ? min(z, min_p_mass) : z), found.key, top.value};
   }
 }
-__device__ __forceinline__ void nothing_to_draw(const SampleArgs& a, int row_index) {
-  if (threadIdx.x == 0) {
+template <bool DRAW>
+__device__ __forceinline__ void nothing_to_draw(const SampleArgs& a, RowCut* cuts, int row_index) {
+  if (threadIdx.x != 0) return;
+  if constexpr (DRAW) {
     a.tokens[row_index] = -1;
     a.probs[row_index] = 0.f;
+  } else {
+    cuts[row_index] = RowCut{0.0, 0, -INFINITY};
   }
 }
 
@@ -509,8 +430,8 @@ __device__ __forceinline__ const void* row_of(const SampleArgs& a, int row_index
 }
 
 // One workgroup a row, the row read three times: the largest, the bins, the entries of the bins that matter.
-template <int DT>
-__global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a) {
+template <int DT, bool DRAW>
+__global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a, RowCut* cuts) {
   __shared__ Hist bins;
   __shared__ Search s;
   __shared__ uint64_t keys[kCandidates];
@@ -521,7 +442,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
   const void* row = row_of<DT>(a, row_index);
   const RowRule r = row_rule(a, row_index);
   const RowTop top = row_top_of(block_max<kSampleThreads>(part_top<DT, kSampleThreads>(row, 0, a.vocab), scratch), r);
-  if (top.value == -INFINITY) return nothing_to_draw(a, row_index);              // (uniform)
+  if (top.value == -INFINITY) return nothing_to_draw<DRAW>(a, cuts, row_index);              // (uniform)
   clear_hist<kSampleThreads>(bins);
   if (threadIdx.x == 0) {
     min_p_mass = 0;
@@ -532,10 +453,10 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
   if ((threadIdx.x & (kWave - 1)) == kWave - 1) atomicAdd(&min_p_mass, (unsigned long long)kept);
   __syncthreads();
   scan_bins<kSampleThreads>(bins, s.wave_mass, s.wave_count);
-  const BinRanges g = bin_ranges(bins, min_p_mass, r);
+  const BinRanges g = bin_ranges<DRAW>(bins, min_p_mass, r);
   gather<DT, kSampleThreads>(keys, kCandidates, &n, row, 0, a.vocab, top, r, g);
   __syncthreads();
-  draw_row<DT, kSampleThreads>(s, bins, keys, n, kCandidates, a, row_index, row, top, r, g.by_k, g.by_p, min_p_mass);
+  draw_row<DT, kSampleThreads, DRAW>(s, bins, keys, n, kCandidates, a, cuts, row_index, row, top, r, g.by_k, g.by_p, min_p_mass);
 }
 
 // Few long rows: a row is cut into slices so that all compute units have a part of one, and the steps are launches: the slices' largest; their
@@ -595,7 +516,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_bins_kernel(SampleArgs a
   if (threadIdx.x == 0) out.min_p_mass = min_p_mass;
 }
 
-template <int DT>
+template <int DT, bool DRAW>
 __global__ __launch_bounds__(kSliceThreads) void sample_gather_kernel(SampleArgs a, SliceArgs c) {
   __shared__ Hist h;
   __shared__ float scratch[kSliceThreads / kWave];
@@ -635,7 +556,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_gather_kernel(SampleArgs
   kept = __shfl((unsigned long long)wave_scan_u64(kept), kWave - 1, kWave);
   __syncthreads();
   scan_bins<kSliceThreads>(h, wave_mass, wave_count);
-  const BinRanges g = bin_ranges(h, kept, r);
+  const BinRanges g = bin_ranges<DRAW>(h, kept, r);
   SliceRecord& out = c.slices[blockIdx.x];
   gather<DT, kSliceThreads>(out.key, kSliceCandidates, &n, row_of<DT>(a, row_index), slice * c.length, min((slice + 1) * c.length, a.vocab), top, r, g);
   if (slice == 0) {
@@ -654,8 +575,8 @@ __global__ __launch_bounds__(kSliceThreads) void sample_gather_kernel(SampleArgs
   if (threadIdx.x == 0) out.n_candidates = n;
 }
 
-template <int DT>
-__global__ __launch_bounds__(kSliceThreads) void sample_draw_kernel(SampleArgs a, SliceArgs c) {
+template <int DT, bool DRAW>
+__global__ __launch_bounds__(kSliceThreads) void sample_draw_kernel(SampleArgs a, SliceArgs c, RowCut* cuts) {
   __shared__ Hist bins;
   __shared__ Search s;
   __shared__ uint64_t keys[kCandidates];
@@ -667,7 +588,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_draw_kernel(SampleArgs a
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
   const int some = lane < c.count ? of[lane].n_candidates : 0;                               // (at most 16 slices)
   const RowTop top = row_top_of(row_top<kSliceThreads>(c, row_index, scratch), r);
-  if (top.value == -INFINITY) return nothing_to_draw(a, row_index);               // (uniform)
+  if (top.value == -INFINITY) return nothing_to_draw<DRAW>(a, cuts, row_index);               // (uniform)
   for (int i = threadIdx.x; i < kBins; i += kSliceThreads) {
     bins.mass[i] = rec.bins.mass[i];
     bins.count[i] = rec.bins.count[i];
@@ -681,8 +602,8 @@ __global__ __launch_bounds__(kSliceThreads) void sample_draw_kernel(SampleArgs a
     }
   }
   __syncthreads();
-  draw_row<DT, kSliceThreads>(s, bins, keys, all ? n : 1, all ? kCandidates : 0, a, row_index, row_of<DT>(a, row_index), top, r, rec.by_k, rec.by_p,
-                              rec.min_p_mass);
+  draw_row<DT, kSliceThreads, DRAW>(s, bins, keys, all ? n : 1, all ? kCandidates : 0, a, cuts, row_index, row_of<DT>(a, row_index), top, r, rec.by_k,
+                                    rec.by_p, rec.min_p_mass);
 }
 
 // Slices a row is cut into; 1: the row stays whole, which is one launch in the place of four.  More slices shorten the two passes over the row, but
@@ -694,15 +615,49 @@ static int sample_slices(int64_t rows, int64_t vocab) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / rows, 16), vocab / (rows <= 8 ? 2048 : 8192)));
 }
 
+size_t row_search_workspace(int64_t rows, int64_t vocab) {
+  const int count = sample_slices(rows, vocab);
+  if (count == 1) return 256;
+  return 256 + align_up((size_t)rows * count * sizeof(SliceRecord), 256) + (size_t)rows * sizeof(RowRecord);
+}
+template <int DT, bool DRAW>
+static void launch_row_search_of(const SampleArgs& a, int64_t rows, RowCut* cuts, void* workspace, hipStream_t st) {
+  SliceArgs c;
+  c.count = sample_slices(rows, a.vocab);
+  c.length = (a.vocab + c.count - 1) / c.count;
+  c.slices = (SliceRecord*)workspace;
+  c.rows = (RowRecord*)((char*)workspace + align_up((size_t)rows * c.count * sizeof(SliceRecord), 256));
+  const dim3 grid((unsigned)rows), slices((unsigned)(rows * c.count));
+  if (c.count == 1) {
+    DominantKernelTimer timer(st);
+    hipLaunchKernelGGL((sample_row_kernel<DT, DRAW>), grid, dim3(kSampleThreads), 0, st, a, cuts);
+    return;
+  }
+  hipLaunchKernelGGL(sample_top_kernel<DT>, slices, dim3(kSliceThreads), 0, st, a, c);
+  {
+    DominantKernelTimer timer(st);
+    hipLaunchKernelGGL(sample_bins_kernel<DT>, slices, dim3(kSliceThreads), 0, st, a, c);
+  }
+  hipLaunchKernelGGL((sample_gather_kernel<DT, DRAW>), slices, dim3(kSliceThreads), 0, st, a, c);
+  hipLaunchKernelGGL((sample_draw_kernel<DT, DRAW>), grid, dim3(kSliceThreads), 0, st, a, c, cuts);
+}
+template <bool DRAW>
+static void launch_row_search(const SampleArgs& a, int dtype, int64_t rows, RowCut* cuts, void* workspace, hipStream_t st) {
+  if (dtype == SUBSPEC_F32) launch_row_search_of<SUBSPEC_F32, DRAW>(a, rows, cuts, workspace, st);
+  else if (dtype == SUBSPEC_F16) launch_row_search_of<SUBSPEC_F16, DRAW>(a, rows, cuts, workspace, st);
+  else launch_row_search_of<SUBSPEC_BF16, DRAW>(a, rows, cuts, workspace, st);
+}
+void launch_row_cuts(const SampleArgs& a, int dtype, int64_t rows, RowCut* cuts, void* workspace, hipStream_t st) {
+  launch_row_search<false>(a, dtype, rows, cuts, workspace, st);
+}
+
 }  // namespace subspec
 
 using namespace subspec;
 
 extern "C" size_t subspec_sample_filtered_workspace(int64_t rows, int64_t vocab) {
   if (rows < 1 || vocab < 1 || vocab > (1 << 20)) return 256;
-  const int count = sample_slices(rows, vocab);
-  if (count == 1) return 256;
-  return 256 + align_up((size_t)rows * count * sizeof(SliceRecord), 256) + (size_t)rows * sizeof(RowRecord);
+  return row_search_workspace(rows, vocab);
 }
 
 extern "C" int subspec_sample_filtered(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride, const float* uniforms,
@@ -722,32 +677,7 @@ extern "C" int subspec_sample_filtered(const void* logits, int dtype, int64_t ro
     SUBSPEC_FAIL(SUBSPEC_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the %zu required", what, workspace_bytes, need);
   if ((uintptr_t)workspace % 16) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
   const SampleArgs a{logits, uniforms, temperatures, top_ks, top_ps, min_ps, tokens, probs, row_stride, (int)vocab, top_k, temperature, top_p, min_p};
-  SliceArgs c;
-  c.count = sample_slices(rows, vocab);
-  c.length = (int)((vocab + c.count - 1) / c.count);
-  c.slices = (SliceRecord*)workspace;
-  c.rows = (RowRecord*)((char*)workspace + align_up((size_t)rows * c.count * sizeof(SliceRecord), 256));
-  hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)rows), slices((unsigned)(rows * c.count));
-#define SUBSPEC_SAMPLE(DT)                                                                                                 \
-  do {                                                                                                                     \
-    if (c.count == 1) {                                                                                                    \
-      DominantKernelTimer timer(st);                                                                                       \
-      hipLaunchKernelGGL(sample_row_kernel<DT>, grid, dim3(kSampleThreads), 0, st, a);                                     \
-    } else {                                                                                                               \
-      hipLaunchKernelGGL(sample_top_kernel<DT>, slices, dim3(kSliceThreads), 0, st, a, c);                                 \
-      {                                                                                                                    \
-        DominantKernelTimer timer(st);                                                                                     \
-        hipLaunchKernelGGL(sample_bins_kernel<DT>, slices, dim3(kSliceThreads), 0, st, a, c);                              \
-      }                                                                                                                    \
-      hipLaunchKernelGGL(sample_gather_kernel<DT>, slices, dim3(kSliceThreads), 0, st, a, c);                              \
-      hipLaunchKernelGGL(sample_draw_kernel<DT>, grid, dim3(kSliceThreads), 0, st, a, c);                                  \
-    }                                                                                                                      \
-  } while (0)
-  if (dtype == SUBSPEC_F32) SUBSPEC_SAMPLE(SUBSPEC_F32);
-  else if (dtype == SUBSPEC_F16) SUBSPEC_SAMPLE(SUBSPEC_F16);
-  else SUBSPEC_SAMPLE(SUBSPEC_BF16);
-#undef SUBSPEC_SAMPLE
+  launch_row_search<true>(a, dtype, rows, nullptr, workspace, (hipStream_t)stream);
   SUBSPEC_CHECK_HIP(hipGetLastError());
   return SUBSPEC_OK;
 }

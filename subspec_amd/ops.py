@@ -586,11 +586,142 @@ def paged_attention(q: torch.Tensor, pool_layer: torch.Tensor, block_table: torc
     return out
 
 
-def _per_row(value, rows: int, dtype: torch.dtype, dev: torch.device, what: str):
+# ---------------------------------------------------------------------------------------------- the blocks of long sequences that matter
+def _bounds_shape(bounds: torch.Tensor):
+    if bounds.dim() != 4 or bounds.shape[2] != 2 or not bounds.is_contiguous():
+        raise ValueError("expected contiguous bounds [max_pages, kv_heads, 2, head_dim]")
+    return bounds.shape[0], bounds.shape[1], bounds.shape[3]
+
+
+def kv_page_bounds_(bounds: torch.Tensor, pool_layer: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
+    """In place: of every page of one layer [max_pages, 2, page_len, kv_heads, head_dim] (bf16 / fp16, head_dim 64 or 128) whose last row is among
+    ``slots`` (int64; those that ``kv_append_paged_`` has just filled), ``bounds`` [max_pages, kv_heads, 2, head_dim] takes the least and the
+    largest of every element of its keys, NaN if one of them is; other pages' bounds stay.  ``select_blocks`` scores blocks by them."""
+    dev = _require_gpu(bounds, pool_layer, slots)
+    max_pages, page_len, heads, D = _pool_layer_shape(pool_layer)
+    if _bounds_shape(bounds) != (max_pages, heads, D) or bounds.dtype != pool_layer.dtype:
+        raise ValueError(f"kv_page_bounds_: bounds must be {pool_layer.dtype} [{max_pages}, {heads}, 2, {D}]")
+    if slots.dtype is not torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
+        raise ValueError("kv_page_bounds_: slots must be a contiguous int64 vector")
+    begin, end = _extent(bounds)
+    for given in (pool_layer, slots):
+        first, last = _extent(given)
+        if begin < last and first < end:
+            raise ValueError("kv_page_bounds_: bounds overlap what is read")
+    _call(dev, "subspec_kv_page_bounds", pool_layer.data_ptr(), bounds.data_ptr(), _dtype_code(bounds), max_pages, page_len, heads, D,
+          slots.data_ptr(), slots.numel(), _stream(dev))
+    return bounds
+
+
+def _token_maps(q: torch.Tensor, sequences: torch.Tensor, positions: torch.Tensor, Hkv: int, D: int, what: str):
+    """Heads of ``q`` [tokens, Hq, D], which is copied where its rows are not 16-byte pieces."""
+    if q.dim() != 3 or q.shape[2] != D:
+        raise ValueError(f"{what}: expected q [tokens, Hq, {D}]")
+    T, Hq, _ = q.shape
+    _int32_vector(sequences, T, "sequences")
+    _int32_vector(positions, T, "positions")
+    if Hq < 1 or Hkv < 1 or Hq % Hkv:
+        raise ValueError(f"{what}: {Hq} query heads over {Hkv} KV heads")
+    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+    return q, T, Hq
+
+
+def _scratch(workspace: Optional[torch.Tensor], need: int, dev: torch.device, what: str):
+    """(tensor to keep, pointer, bytes) of a workspace that the caller gives or the call allocates."""
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need > 256 else None
+        return workspace, None if workspace is None else workspace.data_ptr(), need
+    if workspace.device != dev or not workspace.is_contiguous():
+        raise ValueError(f"{what}: the workspace must be contiguous and on {dev}")
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def _apart(what: str, outs, ins) -> None:
+    """Refuses an output that shares bytes with an input, or with another output."""
+    spans = [(*_extent(t), name) for name, t in outs]
+    others = [(*_extent(t), name) for name, t in ins]
+    for i, (begin, end, name) in enumerate(spans):
+        for first, last, other in others + spans[:i]:
+            if begin < last and first < end:
+                raise ValueError(f"{what}: {name} overlaps {other}")
+
+
+def select_blocks(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, sequences: torch.Tensor, positions: torch.Tensor,
+                  page_len: int, keep: int, *, recent: int = 1, max_kv: Optional[int] = None, out: Optional[torch.Tensor] = None,
+                  workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Blocks (page_len rows of a sequence each) that every token's queries ``q`` [tokens, Hq, D] attend to: int32 [tokens, Hkv, keep], ascending, -1
+    behind the last.  A token at position p sees blocks 0 to p // page_len: the last ``recent`` of them are taken, and of the others
+    the ``keep - recent`` of largest score, equal ones from the lowest on; all, where there are no more than ``keep``.  The score is an upper bound of a KV head's
+    summed scores over a block, sum over its query heads and dimensions of ``max(q * low, q * high)`` with the page's ``bounds`` [max_pages, Hkv, 2,
+    D] (``kv_page_bounds_``), in 64 bits.
+
+    ``block_table`` [batch, max_blocks], ``sequences`` and ``positions`` (int32 [tokens]) as ``paged_batch_plan`` leaves them; tokens of no sequence (-1) get no
+    blocks.  ``max_kv`` bounds the rows of any sequence (rows from it on are not seen); without it the table's width does.  For
+    tokens that decode and drafts under verification; a prompt's own tokens are better served by ``paged_attention``."""
+    dev = _require_gpu(q, bounds, block_table, sequences, positions)
+    max_pages, Hkv, D = _bounds_shape(bounds)
+    q, T, Hq = _token_maps(q, sequences, positions, Hkv, D, "select_blocks")
+    if q.dtype != bounds.dtype:
+        raise ValueError("select_blocks: q and bounds must share a dtype")
+    max_blocks, stride = _table_shape(block_table, block_table.shape[0])
+    page_len, keep, recent = int(page_len), int(keep), int(recent)
+    if page_len < 1 or recent < 1 or keep < recent:
+        raise ValueError(f"select_blocks: page_len={page_len}, keep={keep}, recent={recent}: recent is 1 to keep")
+    max_kv = min(max_blocks * page_len, 1 << 30) if max_kv is None else int(max_kv)
+    if out is None:
+        out = torch.empty((T, Hkv, keep), dtype=torch.int32, device=dev)
+    else:
+        if out.dtype is not torch.int32 or out.shape != (T, Hkv, keep) or not out.is_contiguous() or out.device != dev:
+            raise ValueError(f"select_blocks: out must be a contiguous int32 tensor [{T}, {Hkv}, {keep}]")
+        _apart("select_blocks", [("out", out)], [("q", q), ("bounds", bounds), ("block_table", block_table), ("sequences", sequences),
+                                                 ("positions", positions)])
+    need = L.lib().subspec_select_blocks_workspace(T, Hkv, page_len, max_blocks, max_kv)
+    workspace, ws_ptr, ws_bytes = _scratch(workspace, need, dev, "select_blocks")
+    _call(dev, "subspec_select_blocks", q.data_ptr(), q.stride(0), q.stride(1), bounds.data_ptr(), _dtype_code(q), max_pages, page_len,
+          block_table.data_ptr(), max_blocks, stride, sequences.data_ptr(), positions.data_ptr(), block_table.shape[0], T, Hq, Hkv, D, max_kv,
+          keep, recent, out.data_ptr(), ws_ptr, ws_bytes, _stream(dev))
+    return out
+
+
+def block_attention(q: torch.Tensor, pool_layer: torch.Tensor, block_table: torch.Tensor, blocks: torch.Tensor, sequences: torch.Tensor,
+                    positions: torch.Tensor, *, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                    workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of ``q`` [tokens, Hq, D] (D 64 or 128, bf16 / fp16; a view of a fused projection's output is read where it is; at most 64 query heads a KV
+    head) over the rows up to each token's position of the blocks listed for it, ``blocks`` int32 [tokens, Hkv, keep] (``select_blocks``; distinct,
+    in any order, entries below 0 or behind the token count for nothing), in ``pool_layer`` [max_pages, 2, page_len, Hkv, D].  ``block_table``, ``sequences``
+    and ``positions`` as ``paged_batch_plan`` leaves them.  Returns [tokens, Hq * D]: zeros for a token that sees no row; rows of tokens of no sequence (-1) are left as
+    they were in ``out``, which may be a contiguous ``q`` itself and otherwise overlaps no input."""
+    dev = _require_gpu(q, pool_layer, block_table, blocks, sequences, positions)
+    max_pages, page_len, Hkv, D = _pool_layer_shape(pool_layer)
+    q, T, Hq = _token_maps(q, sequences, positions, Hkv, D, "block_attention")
+    if q.dtype != pool_layer.dtype:
+        raise ValueError("block_attention: q and the pool must share a dtype")
+    if blocks.dtype is not torch.int32 or blocks.dim() != 3 or blocks.shape[:2] != (T, Hkv) or blocks.shape[2] < 1 or not blocks.is_contiguous():
+        raise ValueError(f"block_attention: blocks must be a contiguous int32 tensor [{T}, {Hkv}, keep]")
+    max_blocks, stride = _table_shape(block_table, block_table.shape[0])
+    keep = blocks.shape[2]
+    if out is None:
+        out = torch.empty((T, Hq * D), dtype=q.dtype, device=dev)
+    elif out.dtype != q.dtype or out.shape != (T, Hq * D) or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f"block_attention: out must be a contiguous {q.dtype} tensor [{T}, {Hq * D}]")
+    else:
+        same = q.is_contiguous() and out.data_ptr() == q.data_ptr()
+        _apart("block_attention", [("out", out)], [("the pool", pool_layer), ("block_table", block_table), ("blocks", blocks),
+                                                   ("sequences", sequences), ("positions", positions)] + ([] if same else [("q", q)]))
+    need = L.lib().subspec_block_attention_workspace(T, Hq, Hkv, D, page_len, keep)
+    workspace, ws_ptr, ws_bytes = _scratch(workspace, need, dev, "block_attention")
+    _call(dev, "subspec_block_attention", q.data_ptr(), q.stride(0), q.stride(1), pool_layer.data_ptr(), _dtype_code(q), max_pages, page_len,
+          block_table.data_ptr(), max_blocks, stride, blocks.data_ptr(), keep, sequences.data_ptr(), positions.data_ptr(), block_table.shape[0], T,
+          Hq, Hkv, D, float(D ** -0.5 if scale is None else scale), out.data_ptr(), ws_ptr, ws_bytes, _stream(dev))
+    return out
+
+
+def _per_row(value, rows: int, dtype: torch.dtype, dev: torch.device, what: str, op: str = "sample_filtered"):
     """(pointer, scalar) of a setting given for all rows or for each."""
     if isinstance(value, torch.Tensor):
         if value.dtype is not dtype or value.shape != (rows,) or not value.is_contiguous() or value.device != dev:
-            raise ValueError(f"sample_filtered: {what} must be a number or a contiguous {dtype} tensor of {rows} elements on {dev}")
+            raise ValueError(f"{op}: {what} must be a number or a contiguous {dtype} tensor of {rows} elements on {dev}")
         return value.data_ptr(), 0
     return None, value
 
@@ -624,6 +755,75 @@ def sample_filtered(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.
           t_ptr, float(t), k_ptr, min(int(k), (1 << 31) - 1), p_ptr, float(p), m_ptr, float(m), None if ws is None else ws.data_ptr(), need,
           tokens.data_ptr(), probs.data_ptr(), _stream(dev))
     return tokens, probs
+
+
+_DRAFTS_OUT = (("tokens", torch.int64), ("probs", torch.float32), ("accepted", torch.int32))
+
+
+def _rows_of(t: torch.Tensor) -> torch.Tensor:
+    """A matrix whose rows' elements are consecutive and do not overlap, copied where they are not."""
+    return t if (t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, query_starts: torch.Tensor, uniforms: torch.Tensor, draws: torch.Tensor,
+                  draft_probs: Optional[torch.Tensor] = None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, *,
+                  out: Optional[Dict[str, torch.Tensor]] = None, workspace: Optional[torch.Tensor] = None) -> Dict[str, torch.Tensor]:
+    """Drafted tokens of a batch of sequences against the target's ``logits`` [rows, vocab], so that what is emitted is distributed like the target's own draws
+    (``sample_filtered``).  ``tokens`` int64 [rows] are what the forward took, packed by ``query_starts`` int32 [batch + 1] (a plan's): a sequence's last emitted token,
+    then its drafts.  Row i gives p, the distribution of the token behind token i (settings as ``sample_filtered`` takes them, numbers or a
+    value a row); the draft there was drawn from q, row i of ``draft_probs`` [rows, vocab] (any type; a sequence's last row is not read), and stays if
+    ``uniforms[i] * q < p``.  At the first that does not, the next token is drawn from ``max(p - q, 0)``, after the last row from p: the first entry in the order of
+    the vocabulary whose mass added to that of all before it exceeds ``draws[b]`` times the whole.  Without ``draft_probs`` the drafts were not drawn (a best
+    guess, a lookup): q is 1 at the draft.  ``uniforms`` [rows] and ``draws`` [batch]: float32 in [0, 1).
+
+    Returns device tensors: ``tokens`` int64 [rows], packed like the input: the drafts that stay, the next token, -1 behind (and in rows of no sequence, and where
+    no logit is above -inf), ``probs`` float32 [rows]: p at these tokens, ``accepted`` int32 [batch]: drafts that stay.  ``out``: the
+    dictionary an earlier call of the same sizes returned, written again.  Beside the reference's matching of drawn
+    tokens (specdecodes/models/utils/tree_verify.py:8-163 with do_sample; ``tree_verify``)."""
+    if logits.dim() != 2:
+        raise ValueError("verify_drafts: expected logits [rows, vocab]")
+    dev = _require_gpu(logits, tokens, query_starts, uniforms, draws, *(() if draft_probs is None else (draft_probs,)))
+    rows, V = logits.shape
+    _int32_vector(query_starts, None, "query_starts")
+    batch = query_starts.numel() - 1
+    if batch < 1:
+        raise ValueError("verify_drafts: query_starts must have a place for each sequence and one more")
+    for name, t, dtype, n in (("tokens", tokens, torch.int64, rows), ("uniforms", uniforms, torch.float32, rows), ("draws", draws, torch.float32, batch)):
+        if t.dtype is not dtype or t.shape != (n,) or not t.is_contiguous():
+            raise ValueError(f"verify_drafts: {name} must be a contiguous {dtype} tensor of {n} elements")
+    if draft_probs is not None and draft_probs.shape != (rows, V):
+        raise ValueError(f"verify_drafts: draft_probs must be [{rows}, {V}]")
+    logits = _rows_of(logits)
+    q = None if draft_probs is None else _rows_of(draft_probs)
+    t_ptr, t = _per_row(temperature, rows, torch.float32, dev, "temperature", "verify_drafts")
+    k_ptr, k = _per_row(top_k, rows, torch.int32, dev, "top_k", "verify_drafts")
+    p_ptr, p = _per_row(top_p, rows, torch.float32, dev, "top_p", "verify_drafts")
+    m_ptr, m = _per_row(min_p, rows, torch.float32, dev, "min_p", "verify_drafts")
+    if t < 0 or p < 0 or m < 0 or k < 0:
+        raise ValueError("verify_drafts: temperature, top_k, top_p and min_p must not be negative")
+    k = min(int(k), (1 << 31) - 1)
+    sizes = (rows, rows, batch)
+    if out is None:
+        out = {name: torch.empty(n, dtype=dtype, device=dev) for (name, dtype), n in zip(_DRAFTS_OUT, sizes)}
+    else:
+        for (name, dtype), n in zip(_DRAFTS_OUT, sizes):
+            o = out[name]
+            if o.dtype is not dtype or o.shape != (n,) or o.device != dev or not o.is_contiguous():
+                raise ValueError(f"out[{name!r}] must be a contiguous {dtype} tensor of shape ({n},) on {dev}")
+        given = [("logits", logits), ("tokens", tokens), ("query_starts", query_starts), ("uniforms", uniforms), ("draws", draws)]
+        given += [(name, v) for name, v in (("draft_probs", q), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p))
+                  if isinstance(v, torch.Tensor)]
+        _apart("verify_drafts", [(f"out[{name!r}]", out[name]) for name, _ in _DRAFTS_OUT], given)
+    filtered = bool(k_ptr or p_ptr or m_ptr or 0 < k < V or p < 1 or m > 0)
+    need = L.lib().subspec_verify_drafts_workspace(rows, batch, V, int(filtered))
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    workspace, ws_ptr, ws_bytes = _scratch(workspace, need, dev, "verify_drafts")
+    _call(dev, "subspec_verify_drafts", logits.data_ptr(), _dtype_code(logits), rows, V, max(logits.stride(0), V), tokens.data_ptr(),
+          query_starts.data_ptr(), batch, uniforms.data_ptr(), draws.data_ptr(), None if q is None else q.data_ptr(),
+          L.F32 if q is None else _dtype_code(q), V if q is None else max(q.stride(0), V), t_ptr, float(t), k_ptr, k, p_ptr, float(p), m_ptr, float(m),
+          ws_ptr, ws_bytes, out["tokens"].data_ptr(), out["probs"].data_ptr(), out["accepted"].data_ptr(), _stream(dev))
+    return {name: out[name] for name, _ in _DRAFTS_OUT}
 
 
 def int4_linear(x: torch.Tensor, wq: torch.Tensor, sz: torch.Tensor, out_features: int,

@@ -176,19 +176,33 @@ class KvBatch:
         batch.append(layer, k, v)                  # k, v [tokens, kv_heads, head_dim], the sequences' new tokens one after the other
         out = batch.attention(layer, q)            # q [tokens, heads, head_dim] -> [tokens, heads * head_dim]
 
-    The host keeps the lengths too, so running out of pages or of table columns is an error before anything is launched, and nothing waits
-    for the device.  That is also why ``step`` and ``release`` cannot be part of a captured graph, whose replays would move no host length (and
-    would copy new lengths out of host memory long given back): a captured step calls the operators with ``out=`` itself.  Sequences grow
-    and end; none is shortened."""
+    With ``bounds=True`` the keys' bounds of every full page are kept beside the pool (``append`` does it), and ``attention(..., blocks=64)`` reads the 64
+    blocks of a long sequence that matter to a token instead of all.  Drafts go into a step behind their sequence's last token; ``verify`` says which stay,
+    and ``keep`` takes the others' rows back:
 
-    def __init__(self, pool: KvCachePool, max_batch: int, max_len: int, num_pages: Optional[int] = None):
+        plan = batch.step([1 + 4] * n)             # the last token and four drafts of every sequence
+        ...                                        # layers: append, attention; logits of all rows
+        got = batch.verify(logits, tokens, uniforms, draws, draft_probs)
+        batch.keep([1 + a for a in got["accepted"].tolist()])
+
+    The host keeps the lengths too, so running out of pages or of table columns is an error before anything is launched, and nothing waits
+    for the device.  That is also why ``step``, ``keep`` and ``release`` cannot be part of a captured graph, whose replays would move no host length (and
+    would copy new lengths out of host memory long given back): a captured step calls the operators with ``out=`` itself."""
+
+    def __init__(self, pool: KvCachePool, max_batch: int, max_len: int, num_pages: Optional[int] = None, bounds: bool = False):
         if not 1 <= int(max_batch) <= L.MAX_BATCH:
             raise ValueError(f"max_batch={max_batch} outside [1, {L.MAX_BATCH}]")
         if int(max_len) < 0 or (num_pages is not None and int(num_pages) < 0):
             raise ValueError(f"max_len={max_len} and num_pages={num_pages} must not be negative")
         self.pool, self.page_len, self.max_len = pool, pool.page_len, int(max_len)
         self.lens: List[int] = [0] * int(max_batch)
+        self.new: List[int] = [0] * int(max_batch)            # of the last step, what of it is still there
         dev = pool.device
+        self.bounds: Optional[torch.Tensor] = None
+        if bounds:
+            if pool.dtype not in (torch.bfloat16, torch.float16) or pool.head_dims not in (64, 128):
+                raise ValueError("bounds are kept of bf16 / fp16 pools with heads of 64 or 128")
+            self.bounds = torch.zeros(pool.num_layers, pool.max_pages, pool.num_heads, 2, pool.head_dims, dtype=pool.dtype, device=dev)
         self.kv_lens = torch.zeros(int(max_batch), dtype=torch.int32, device=dev)
         self.block_table = torch.full((int(max_batch), max(1, self._pages(self.max_len))), -1, dtype=torch.int32, device=dev)
         # (the pages come last: what fails before them leaves the pool as it was)
@@ -206,6 +220,10 @@ class KvBatch:
         if self.pool.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
             raise ValueError(f"KvBatch.{what} keeps lengths on the host and cannot be captured into a graph")
 
+    def _to_device(self, numbers: Sequence[int]) -> torch.Tensor:
+        # (from pinned memory: a copy from pageable memory would wait for everything the stream has to do)
+        return torch.tensor(numbers, dtype=torch.int32, pin_memory=self.pool.device.type == "cuda").to(self.pool.device, non_blocking=True)
+
     def step(self, new_lens: Sequence[int], n_tokens: Optional[int] = None) -> Dict[str, torch.Tensor]:
         """Pages and slots for ``new_lens[b]`` new tokens of every sequence; returns the plan (``ops.paged_batch_plan``).  ``n_tokens``: rows of
         its token outputs, default the new tokens of all sequences."""
@@ -222,11 +240,10 @@ class KvBatch:
         rows = sum(new) if n_tokens is None else int(n_tokens)
         if rows < sum(new):
             raise ValueError(f"n_tokens={rows} is less than the {sum(new)} new tokens")
-        # (from pinned memory: a copy from pageable memory would wait for everything the stream has to do)
-        fresh = torch.tensor(new, dtype=torch.int32, pin_memory=self.pool.device.type == "cuda").to(self.pool.device, non_blocking=True)
+        fresh = self._to_device(new)
         self.plan = ops.paged_batch_plan(self.kv_lens, fresh, self.free_pages, self.n_free, self.block_table, self.page_len, rows)
         self.kv_lens, self.n_free = self.plan["kv_lens"], self.plan["counts"][2:3]
-        self.lens, self.num_free = total, self.num_free - taken
+        self.lens, self.new, self.num_free = total, new, self.num_free - taken
         self.max_new, self.max_kv = max(new), max(total)
         return self.plan
 
@@ -236,13 +253,52 @@ class KvBatch:
         return self.plan
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
-        ops.kv_append_paged_(self.pool.cache_data[layer], k, v, self._current()["slots"])
+        slots = self._current()["slots"]
+        ops.kv_append_paged_(self.pool.cache_data[layer], k, v, slots)
+        if self.bounds is not None:
+            ops.kv_page_bounds_(self.bounds[layer], self.pool.cache_data[layer], slots)
 
     def attention(self, layer: int, q: torch.Tensor, window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None,
-                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                  out: Optional[torch.Tensor] = None, *, blocks: Optional[int] = None, recent: int = 1) -> torch.Tensor:
+        """``ops.paged_attention`` of the step's new tokens; with ``blocks`` (which takes ``bounds=True``, and no window) ``ops.block_attention`` over so many blocks a
+        token and KV head, the last ``recent`` and the others by score (``ops.select_blocks``)."""
         plan = self._current()                                 # (its lengths, not self.kv_lens: those may already lack a released sequence)
-        return ops.paged_attention(q, self.pool.cache_data[layer], self.block_table, plan["query_starts"], plan["kv_lens"], self.max_new,
-                                   self.max_kv, window=window, sinks=sinks, scale=scale, out=out)
+        if blocks is None:
+            return ops.paged_attention(q, self.pool.cache_data[layer], self.block_table, plan["query_starts"], plan["kv_lens"], self.max_new,
+                                       self.max_kv, window=window, sinks=sinks, scale=scale, out=out)
+        if self.bounds is None or window or sinks:
+            raise ValueError("attention over selected blocks takes a batch made with bounds=True, and no window")
+        chosen = ops.select_blocks(q, self.bounds[layer], self.block_table, plan["sequences"], plan["positions"], self.page_len, blocks,
+                                   recent=recent, max_kv=self.max_kv)
+        return ops.block_attention(q, self.pool.cache_data[layer], self.block_table, chosen, plan["sequences"], plan["positions"], scale=scale,
+                                   out=out)
+
+    def verify(self, logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor, draws: torch.Tensor,
+               draft_probs: Optional[torch.Tensor] = None, **settings) -> Dict[str, torch.Tensor]:
+        """``ops.verify_drafts`` of the step's new tokens: every sequence's last emitted token and the drafts behind it."""
+        return ops.verify_drafts(logits, tokens, self._current()["query_starts"], uniforms, draws, draft_probs, **settings)
+
+    def keep(self, kept: Sequence[int]) -> None:
+        """Of the last step's new tokens the first ``kept[b]`` of sequence b stay, the others' rows are given up from the next ``step`` on (drafts that
+        were not accepted): a token and ``accepted[b]`` drafts of a sequence that had any, 0 of one that rested or has been released.  Until then nobody gets their
+        pages.  A second call counts from what the first has left."""
+        self._not_captured("keep")
+        self._current()
+        kept = [int(n) for n in kept]
+        if len(kept) != len(self.lens) or any(not 0 <= k <= n for k, n in zip(kept, self.new)):
+            raise ValueError(f"expected {len(self.lens)} numbers of tokens to keep, each at most the new ones of its sequence: {self.new}")
+        lens = [t - n + k for t, n, k in zip(self.lens, self.new, kept)]
+        given_up = [(b, j) for b, (t, l) in enumerate(zip(self.lens, lens)) for j in range(self._pages(l), self._pages(t))]
+        if lens != self.lens:
+            moved = self._to_device([l - t for t, l in zip(self.lens, lens)] + [b for b, _ in given_up] + [j for _, j in given_up])
+            rows, columns = moved[len(lens):].long().view(2, -1).unbind(0)
+            self.kv_lens = self.kv_lens + moved[:len(lens)]
+            if given_up:
+                self.free_pages = self.free_pages.clone()     # (a step on another stream may still read the old ones)
+                self.free_pages[self.num_free:self.num_free + len(given_up)] = self.block_table[rows, columns]
+                self.num_free += len(given_up)
+                self.n_free = torch.full_like(self.n_free, self.num_free)
+        self.lens, self.new = lens, kept
 
     def release(self, index: int) -> None:
         """Sequence ``index`` is done: its pages are free again and its place is empty, from the next ``step`` on.  Until then nobody gets the pages,
@@ -252,7 +308,7 @@ class KvBatch:
         self.free_pages = self.free_pages.clone()             # (a step on another stream may still read the old ones)
         self.free_pages[self.num_free:self.num_free + n] = self.block_table[index, :n]
         self.num_free += n
-        self.lens[index] = 0
+        self.lens[index] = self.new[index] = 0
         self.n_free = torch.full_like(self.n_free, self.num_free)
         self.kv_lens = self.kv_lens.clone()
         self.kv_lens[index].zero_()                            # (an assignment of a number would wait for the device)
@@ -261,7 +317,7 @@ class KvBatch:
         """All pages go back to the pool, which may hand them to anyone: the last step's plan, whose slots lie in them, goes with them."""
         self.pool.deallocate(self.pages)
         self.plan = None
-        self.pages, self.num_free, self.lens = [], 0, [0] * len(self.lens)
+        self.pages, self.num_free, self.lens, self.new = [], 0, [0] * len(self.lens), [0] * len(self.lens)
         self.n_free, self.kv_lens = torch.zeros_like(self.n_free), torch.zeros_like(self.kv_lens)
 
 
