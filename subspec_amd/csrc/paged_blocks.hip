@@ -35,12 +35,13 @@ template <int DT>
 __global__ __launch_bounds__(kBoundsThreads) void page_bounds_kernel(BoundsArgs a) {
   __shared__ __attribute__((aligned(16))) float side[kBoundsThreads][16];
   const int tid = threadIdx.x, page_len = 1 << a.page_shift;
-  const int t0 = blockIdx.x * a.per, t1 = min(t0 + a.per, a.n_tokens);
   const int lanes = min(a.pieces, kBoundsThreads), groups = kBoundsThreads / lanes, group = tid / lanes, lane = tid % lanes;
-  for (int t = t0; t < t1; ++t) {
-    const int64_t slot = a.slots[t];
-    if (slot < 0 || slot >= a.n_slots || (slot & (page_len - 1)) != page_len - 1) continue;        // (uniform)
-    const int64_t page = slot >> a.page_shift;
+  // every wavefront looks the workgroup's slots over, together: one after the other they would be sixteen trips to memory
+  const int t = blockIdx.x * a.per + (tid & (kWave - 1));
+  const int64_t slot = (tid & (kWave - 1)) < a.per && t < a.n_tokens ? a.slots[t] : -1;
+  uint64_t last_rows = __ballot(slot >= 0 && slot < a.n_slots && (slot & (page_len - 1)) == page_len - 1);
+  for (; last_rows; last_rows &= last_rows - 1) {                                                // (the same in all wavefronts)
+    const int64_t page = __shfl((long long)slot, __ffsll((unsigned long long)last_rows) - 1, kWave) >> a.page_shift;
     const dec_u4* rows = (const dec_u4*)(a.pool + page * 2 * a.page_elems);
     dec_u4* out = (dec_u4*)(a.bounds + page * 2 * (a.page_elems >> a.page_shift));
     for (int p0 = 0; p0 < a.pieces; p0 += lanes) {
@@ -53,7 +54,7 @@ __global__ __launch_bounds__(kBoundsThreads) void page_bounds_kernel(BoundsArgs 
         high[e] = -INFINITY;
       }
       if (mine) {
-#pragma unroll 4
+#pragma unroll 8
         for (int r = group; r < page_len; r += groups) {
           float x[8];
           unpack8<DT>(rows[(int64_t)r * a.pieces + piece], x);
@@ -106,95 +107,148 @@ struct SelectArgs {
 };
 // Blocks that a token sees (0: none), and of these the first so many that compete.
 struct TokenBlocks { int seen, scored; };
-__device__ __forceinline__ TokenBlocks token_blocks(const SelectArgs& a, int t) {
-  const int b = a.sequences[t], last = min(a.positions[t], a.last_row);
+__device__ __forceinline__ TokenBlocks token_blocks(const SelectArgs& a, int b, int position) {
+  const int last = min(position, a.last_row);
   if (b < 0 || b >= a.batch || last < 0) return TokenBlocks{0, 0};
   const int seen = (last >> a.page_shift) + 1;
   return TokenBlocks{seen, seen > a.keep ? seen - a.recent : 0};
 }
-constexpr int kScoreTokens = 4;
+constexpr int kScoreTokens = 4;           // tokens of a sequence that share a reading of the bounds
+constexpr int kScoreThreads = 256;
+constexpr int kScoreDepth = 8;            // readings of a wavefront
 
-__device__ __forceinline__ double dpp_add(double v, const int which) {
+// a double from another lane of sixteen (a DPP control)
+template <int CTRL>
+__device__ __forceinline__ double from_lane(double v) {
   const uint64_t u = (uint64_t)__double_as_longlong(v);
-  const int lo = (int)(uint32_t)u, hi = (int)(uint32_t)(u >> 32);
-  int l, h;
-  if (which == 0) {              // the neighbour of a pair
-    l = __builtin_amdgcn_mov_dpp(lo, 0xB1, 0xf, 0xf, true);
-    h = __builtin_amdgcn_mov_dpp(hi, 0xB1, 0xf, 0xf, true);
-  } else if (which == 1) {       // ... of two pairs
-    l = __builtin_amdgcn_mov_dpp(lo, 0x4E, 0xf, 0xf, true);
-    h = __builtin_amdgcn_mov_dpp(hi, 0x4E, 0xf, 0xf, true);
-  } else if (which == 2) {       // eight lanes mirrored
-    l = __builtin_amdgcn_mov_dpp(lo, 0x141, 0xf, 0xf, true);
-    h = __builtin_amdgcn_mov_dpp(hi, 0x141, 0xf, 0xf, true);
-  } else {                       // sixteen
-    l = __builtin_amdgcn_mov_dpp(lo, 0x140, 0xf, 0xf, true);
-    h = __builtin_amdgcn_mov_dpp(hi, 0x140, 0xf, 0xf, true);
+  const int lo = __builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xf, 0xf, true), hi = __builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
+  return __longlong_as_double((long long)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo));
+}
+constexpr int kPair = 0xB1, kTwoPairs = 0x4E, kTurnFour = 0x124, kTurnEight = 0x128, kMirrorEight = 0x141;
+// Sums of eight values over LANES neighbouring lanes: lane p, p % 4 = r, ends up with those of values r and 4 + r.  Where lanes swap values, each keeps half
+// of them, so the later steps have fewer to add: 54 instructions in the place of 96.
+template <int LANES>
+__device__ __forceinline__ void sum_eight(double (&v)[8], int lane, double* out) {
+  if constexpr (LANES == 8) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += from_lane<kMirrorEight>(v[i]);
   }
-  return v + __longlong_as_double((long long)((uint64_t)(uint32_t)h << 32 | (uint32_t)l));
+  double w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const double keep = lane & 1 ? v[2 * i + 1] : v[2 * i], give = lane & 1 ? v[2 * i] : v[2 * i + 1];
+    w[i] = keep + from_lane<kPair>(give);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const double keep = lane & 2 ? w[2 * i + 1] : w[2 * i], give = lane & 2 ? w[2 * i] : w[2 * i + 1];
+    out[i] = keep + from_lane<kTwoPairs>(give);
+    if constexpr (LANES == 16) {
+      out[i] += from_lane<kTurnFour>(out[i]);
+      out[i] += from_lane<kTurnEight>(out[i]);
+    }
+  }
 }
 
-// A wavefront takes `span` blocks of (token, KV head); D / 8 lanes a block.  A token whose neighbour before it is of the same sequence leaves its scores to the
-// wavefront of that one, up to kScoreTokens of them: the bounds are read once for all.
-template <int DT, int D>
-__global__ __launch_bounds__(kWave) void block_score_kernel(SelectArgs a) {
-  constexpr int kLanes = D / 8, kAtOnce = kWave / kLanes;
+// A workgroup takes `span` blocks of (token, KV head), a wavefront a quarter of them: D / 8 lanes a block, all requests of a wavefront under way
+// before the first score.  Meanwhile the four of them add the query heads up.  A token whose neighbour before it is of the same sequence leaves its scores to the
+// workgroup of that one, up to TOKENS of them: the bounds are read once for all.
+template <int DT, int D, int TOKENS>
+__global__ __launch_bounds__(kScoreThreads) void block_score_kernel(SelectArgs a) {
+  constexpr int kLanes = D / 8, kAtOnce = kWave / kLanes, kTurn = kAtOnce * kScoreDepth, kTeams = kScoreThreads / (TOKENS * kLanes);
+  static_assert(kTurn <= kWave, "a lane holds a page number of a turn");
+  __shared__ __attribute__((aligned(16))) double weight[kTeams][TOKENS][2][D];        // (of high, of low), a part of the heads each
   const uint32_t unit = blockIdx.x;
   const int kvh = (int)(unit % (uint32_t)a.hkv), span = (int)(unit / (uint32_t)a.hkv % (uint32_t)a.spans);
   const int local = (int)(unit / (uint32_t)a.hkv / (uint32_t)a.spans), t = a.first + local;
-  const int b = a.sequences[t];
-  if (local % kScoreTokens != 0 && a.sequences[t - 1] == b) return;
-  int scored[kScoreTokens], most = 0, tokens = 0;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1), part = lane % kLanes, which = lane / kLanes;
+  // the token before this one and those behind it, in one trip to memory
+  const int near = min(max(t - 1 + lane, 0), a.n_tokens - 1);
+  const int sequence_of = a.sequences[near], position_of = a.positions[near];
+  const int b = __builtin_amdgcn_readlane(sequence_of, 1);
+  if (TOKENS > 1 && local % TOKENS != 0 && __builtin_amdgcn_readlane(sequence_of, 0) == b) return;
+  int scored[TOKENS], most = 0, tokens = 0;
 #pragma unroll
-  for (int k = 0; k < kScoreTokens; ++k) {
+  for (int k = 0; k < TOKENS; ++k) {
     scored[k] = 0;
-    if (k > 0 && (tokens < k || (local + k) % kScoreTokens == 0 || t + k >= a.n_tokens || a.sequences[t + k] != b)) continue;
+    if (k > 0 && (tokens < k || (local + k) % TOKENS == 0 || t + k >= a.n_tokens || __builtin_amdgcn_readlane(sequence_of, 1 + k) != b)) continue;
     tokens = k + 1;
-    scored[k] = token_blocks(a, t + k).scored;
+    scored[k] = token_blocks(a, b, __builtin_amdgcn_readlane(position_of, 1 + k)).scored;
     most = max(most, scored[k]);
   }
-  const int j0 = span * a.span, j1 = min(j0 + a.span, most);
-  if (j0 >= j1) return;
-  const int lane = threadIdx.x, part = lane % kLanes, which = lane / kLanes;
-  double up[kScoreTokens][8], down[kScoreTokens][8];
+  if (span * a.span >= most) return;                         // (the whole workgroup)
+  const int j0 = span * a.span + wave * kTurn, j1 = min(j0 + kTurn, most);
+  dec_u4 low[kScoreDepth], high[kScoreDepth];
+  if (j0 < j1) {
+    const int page_of = min(max(a.table[b * a.table_stride + min(j0 + lane, j1 - 1)], 0), a.max_pages - 1);
+    const dec_u4* bounds = (const dec_u4*)(a.bounds + (int64_t)kvh * 2 * D) + part;
 #pragma unroll
-  for (int k = 0; k < kScoreTokens; ++k) {
+    for (int i = 0; i < kScoreDepth; ++i) {
+      const dec_u4* src = bounds + (int64_t)__shfl(page_of, i * kAtOnce + which, kWave) * a.hkv * 2 * kLanes;
+      low[i] = src[0];
+      high[i] = src[kLanes];
+    }
+  }
+  {
+    const int team = threadIdx.x / (TOKENS * kLanes), k = threadIdx.x / kLanes % TOKENS, piece = threadIdx.x % kLanes;
+    double up[8], down[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) up[k][e] = down[k][e] = 0.0;
-    if (k >= tokens) continue;
-    const uint16_t* q = a.q + (t + k) * a.q_token + (int64_t)kvh * a.group * a.q_head + part * 8;
-    for (int g = 0; g < a.group; ++g) {
+    for (int e = 0; e < 8; ++e) up[e] = down[e] = 0.0;
+    const uint16_t* q = a.q + (t + min(k, tokens - 1)) * a.q_token + (int64_t)kvh * a.group * a.q_head + piece * 8;
+#pragma unroll 2
+    for (int g = team; g < a.group; g += kTeams) {
       float x[8];
       unpack8<DT>(*(const dec_u4*)(q + g * a.q_head), x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         // (a NaN goes into both: its blocks all score NaN)
-        up[k][e] += x[e] < 0.f ? 0.0 : (double)x[e];
-        down[k][e] += x[e] > 0.f ? 0.0 : (double)x[e];
+        up[e] += x[e] < 0.f ? 0.0 : (double)x[e];
+        down[e] += x[e] > 0.f ? 0.0 : (double)x[e];
       }
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      weight[team][k][0][piece * 8 + e] = up[e];
+      weight[team][k][1][piece * 8 + e] = down[e];
+    }
   }
-  const int32_t* row = a.table + b * a.table_stride;
-  for (int base = j0; base < j1; base += kWave) {
-    const int page_of = min(max(row[min(base + lane, j1 - 1)], 0), a.max_pages - 1);
-    const int some = min(kWave, j1 - base);
-#pragma unroll 4
-    for (int i = 0; i < some; i += kAtOnce) {
-      const int j = base + i + which;
-      const int page = __shfl(page_of, i + which, kWave);
-      const dec_u4* src = (const dec_u4*)(a.bounds + ((int64_t)page * a.hkv + kvh) * 2 * D) + part;
-      float low[8], high[8];
-      unpack8<DT>(src[0], low);
-      unpack8<DT>(src[kLanes], high);
+  __syncthreads();
+  const int teams = min(kTeams, a.group);
+  double* flat = &weight[0][0][0][0];
+  for (int i = threadIdx.x; i < TOKENS * 2 * D; i += kScoreThreads) {
+    double sum = flat[i];
+    for (int m = 1; m < teams; ++m) sum += flat[m * TOKENS * 2 * D + i];
+    flat[i] = sum;
+  }
+  __syncthreads();
+  if (j0 >= j1) return;
+#pragma unroll 1
+  for (int k = 0; k < tokens; ++k) {
+    double up[8], down[8], s[kScoreDepth], out[2];
 #pragma unroll
-      for (int k = 0; k < kScoreTokens; ++k) {
-        if (k >= tokens) break;
-        double s = 0.0;
+    for (int e = 0; e < 8; ++e) {
+      up[e] = weight[0][k][0][part * 8 + e];
+      down[e] = weight[0][k][1][part * 8 + e];
+    }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s = fma(up[k][e], (double)high[e], fma(down[k][e], (double)low[e], s));
+    for (int i = 0; i < kScoreDepth; ++i) {
+      if constexpr (TOKENS > 1) asm("" : "+v"(low[i]), "+v"(high[i]));      // (128 converted numbers kept for the next token are more registers than there are)
+      float l[8], h[8];
+      unpack8<DT>(low[i], l);
+      unpack8<DT>(high[i], h);
+      s[i] = 0.0;
 #pragma unroll
-        for (int o = 0; (1 << o) < kLanes; ++o) s = dpp_add(s, o);
-        if (part == 0 && j < scored[k]) a.scores[((int64_t)(local + k) * a.hkv + kvh) * a.most + j] = s != s ? INFINITY : s;
+      for (int e = 0; e < 8; ++e) s[i] = fma(up[e], (double)h[e], fma(down[e], (double)l[e], s[i]));
+    }
+    sum_eight<kLanes>(s, lane, out);
+    if (part < 4) {
+      int n = scored[0];
+#pragma unroll
+      for (int m = 1; m < TOKENS; ++m) n = k == m ? scored[m] : n;
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const int j = j0 + (4 * m + part) * kAtOnce + which;
+        if (j < min(j1, n)) a.scores[((int64_t)(local + k) * a.hkv + kvh) * a.most + j] = out[m] != out[m] ? INFINITY : out[m];
       }
     }
   }
@@ -228,7 +282,7 @@ __global__ __launch_bounds__(kSelectThreads) void block_select_kernel(SelectArgs
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid & (kWave - 1);
   const int local = blockIdx.x / a.hkv, kvh = blockIdx.x % a.hkv, t = a.first + local;
   int32_t* out = a.blocks + ((int64_t)t * a.hkv + kvh) * a.keep;
-  const TokenBlocks tb = token_blocks(a, t);
+  const TokenBlocks tb = token_blocks(a, a.sequences[t], a.positions[t]);
   if (tb.seen <= a.keep) {
     for (int i = tid; i < a.keep; i += kSelectThreads) out[i] = i < tb.seen ? i : -1;
     return;
@@ -652,6 +706,16 @@ static int64_t select_tokens(int64_t n_tokens, int64_t hkv, int64_t most) {
   return std::min(n_tokens, fit);
 }
 
+// More tokens than sequences: some have several, which share readings.
+template <int DT, int D>
+static void launch_scores(SelectArgs a, int64_t tokens, hipStream_t st) {
+  a.span = kScoreThreads / (D / 8) * kScoreDepth;
+  a.spans = (int)((a.most + a.span - 1) / a.span);
+  const dim3 grid((unsigned)(tokens * a.hkv * a.spans)), block(kScoreThreads);
+  if (tokens > a.batch) hipLaunchKernelGGL((block_score_kernel<DT, D, kScoreTokens>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((block_score_kernel<DT, D, 1>), grid, block, 0, st, a);
+}
+
 template <int DT, int D>
 static void launch_attend_of(const AttendArgs& a, int64_t tokens, hipStream_t st) {
   const dim3 grid((unsigned)(tokens * a.chunks * a.hkv)), block(kWave);
@@ -761,17 +825,14 @@ extern "C" int subspec_select_blocks(const void* q, int64_t q_token_stride, int6
   for (int64_t first = 0; first < n_tokens; first += at_once) {
     const int64_t some = std::min(at_once, n_tokens - first);
     a.first = (int)first;
-    a.span = some * n_kv_heads * most < (1 << 17) ? 16 : 64;
-    a.spans = (int)((most + a.span - 1) / a.span);
-    const dim3 grid((unsigned)(some * n_kv_heads * a.spans)), block(kWave);
     if (most > keep) {
       DominantKernelTimer timer(st);
       if (dtype == SUBSPEC_BF16) {
-        if (head_dim == 128) hipLaunchKernelGGL((block_score_kernel<SUBSPEC_BF16, 128>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((block_score_kernel<SUBSPEC_BF16, 64>), grid, block, 0, st, a);
+        if (head_dim == 128) launch_scores<SUBSPEC_BF16, 128>(a, some, st);
+        else launch_scores<SUBSPEC_BF16, 64>(a, some, st);
       } else {
-        if (head_dim == 128) hipLaunchKernelGGL((block_score_kernel<SUBSPEC_F16, 128>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((block_score_kernel<SUBSPEC_F16, 64>), grid, block, 0, st, a);
+        if (head_dim == 128) launch_scores<SUBSPEC_F16, 128>(a, some, st);
+        else launch_scores<SUBSPEC_F16, 64>(a, some, st);
       }
     }
     hipLaunchKernelGGL(block_select_kernel, dim3((unsigned)(some * n_kv_heads)), dim3(kSelectThreads), 0, st, a);
