@@ -15,22 +15,22 @@
 namespace subspec {
 
 constexpr int kVerifyThreads = 256;
+constexpr int kVerifyWaves = kVerifyThreads / kWave;
 constexpr int kVerifyRound = 8 * kVerifyThreads;       // entries that a workgroup takes at a time, eight a thread
+constexpr int kChunk = 8 * kWave;                      // ... a wavefront: sums are kept of these
 
-// A slice's mass, relative to its own largest logit: rows without filters need no more than the sums of these.
-struct SliceMass {
-  double mass;
-  float top;
-  int first;                       // index of the first entry that equals it
+// A slice of a row without filters, in 32 bits: its largest logit, the masses relative to it, the first entry that equals it.
+struct SliceStats {
+  float top, sum;
+  int first, unused;
 };
 // The row that a sequence ends with.
 struct EndRecord {
-  RowCut cut;
-  int row, sequence_row;           // row of the call (-1: the sequence has none), row of the sequence
+  RowCut cut;                      // (its mass is that of the chunks: it counts for rows with filters)
+  int row;                         // of the call (-1: the sequence has none)
   int last;                        // no draft stands behind it
   int draft;                       // ... or the one that did not stay (-1: none of the vocabulary)
 };
-struct RestSum { uint64_t rest, all; };
 struct VerifyArgs {
   SampleArgs s;
   const int64_t* drafts;
@@ -39,11 +39,12 @@ struct VerifyArgs {
   const void* q;
   int64_t q_stride;
   int32_t* accepted;
-  RowCut* cuts;                    // of every row, where `slices` is 0
-  SliceMass* masses;               // [row][slices]
+  RowCut* cuts;                    // of every row, with filters
+  SliceStats* stats;               // [row][slices], without
   EndRecord* ends;
-  RestSum* sums;                   // [sequence][end_slices]
-  int q_dtype, slices, length, end_slices, end_length, batch, n_rows, wide, q_wide;
+  uint64_t* all;                   // [sequence][chunks] masses of the row that it ends with
+  uint64_t* rest;                  // ... what the draft leaves of them
+  int q_dtype, slices, end_slices, end_length, chunks, batch, n_rows, wide, q_wide, filtered;
 };
 
 struct VerifySpan { int first, n; };
@@ -55,31 +56,55 @@ template <int DT>
 __device__ __forceinline__ const char* verify_row(const VerifyArgs& a, int row) {
   return (const char*)a.s.logits + (int64_t)row * a.s.row_stride * Elem<DT>::kBytes;
 }
-// Entries i .. i + 7 of a row of n; `fill` behind its end.  wide: rows start at multiples of 16 bytes.
-template <int DT>
-__device__ __forceinline__ void load_eight(const void* row, int i, int n, int wide, float fill, float* x) {
-  if (wide && i + 8 <= n) {
-    const dec_u4* p = (const dec_u4*)((const char*)row + (size_t)i * Elem<DT>::kBytes);
-    if constexpr (DT == SUBSPEC_F32) {
-      const dec_u4 a = p[0], b = p[1];
+// ROUNDS chunks of a row of n entries from c0 on, `apart` entries from one to the next: lane l has entries 8 l .. 8 l + 7 of each, `fill` behind the row's end.  wide:
+// rows start at multiples of 16 bytes.  All are asked for before the first is looked at, which takes that nothing branches between the requests: a lane's
+// own end of the row is the business of the last chunk alone.
+template <int DT, int ROUNDS>
+__device__ __forceinline__ void load_chunks(const void* row, int c0, int apart, int n, int wide, float fill, float (&x)[ROUNDS][8]) {
+  const int at = c0 + 8 * (int)(threadIdx.x & (kWave - 1));
+  constexpr int kPieces = Elem<DT>::kBytes / 2;
+  if (wide && c0 + (ROUNDS - 1) * apart + kChunk <= n) {                 // (uniform)
+    dec_u4 raw[ROUNDS][kPieces];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[e] = __uint_as_float(a[e]);
-        x[4 + e] = __uint_as_float(b[e]);
+    for (int k = 0; k < ROUNDS; ++k)
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) raw[k][p] = ((const dec_u4*)((const char*)row + (size_t)(at + k * apart) * Elem<DT>::kBytes))[p];
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k) {
+      if constexpr (DT == SUBSPEC_F32) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[k][e] = __uint_as_float(raw[k][e / 4][e % 4]);
+      } else {
+        unpack8<DT>(raw[k][0], x[k]);
       }
-    } else {
-      unpack8<DT>(p[0], x);
     }
     return;
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = i + e < n ? Elem<DT>::load(row, i + e) : fill;
+  for (int k = 0; k < ROUNDS; ++k)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int i = at + k * apart + e;
+      const float v = Elem<DT>::load(row, min(i, n - 1));
+      x[k][e] = i < n ? v : fill;
+    }
 }
-__device__ __forceinline__ void load_eight_q(const VerifyArgs& a, int row, int i, float* x) {
+// the draft's probabilities of the same entries
+template <int ROUNDS>
+__device__ __forceinline__ void load_drafts(const VerifyArgs& a, int row, int draft, int c0, int apart, float (&x)[ROUNDS][8]) {
   const int n = a.s.vocab;
-  if (a.q_dtype == SUBSPEC_F32) load_eight<SUBSPEC_F32>((const char*)a.q + row * a.q_stride * 4, i, n, a.q_wide, 0.f, x);
-  else if (a.q_dtype == SUBSPEC_F16) load_eight<SUBSPEC_F16>((const char*)a.q + row * a.q_stride * 2, i, n, a.q_wide, 0.f, x);
-  else load_eight<SUBSPEC_BF16>((const char*)a.q + row * a.q_stride * 2, i, n, a.q_wide, 0.f, x);
+  if (!a.q) {
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[k][e] = c0 + k * apart + 8 * (int)(threadIdx.x & (kWave - 1)) + e == draft ? 1.f : 0.f;
+  } else if (a.q_dtype == SUBSPEC_F32) {
+    load_chunks<SUBSPEC_F32, ROUNDS>((const char*)a.q + row * a.q_stride * 4, c0, apart, n, a.q_wide, 0.f, x);
+  } else if (a.q_dtype == SUBSPEC_F16) {
+    load_chunks<SUBSPEC_F16, ROUNDS>((const char*)a.q + row * a.q_stride * 2, c0, apart, n, a.q_wide, 0.f, x);
+  } else {
+    load_chunks<SUBSPEC_BF16, ROUNDS>((const char*)a.q + row * a.q_stride * 2, c0, apart, n, a.q_wide, 0.f, x);
+  }
 }
 __device__ __forceinline__ double draft_prob(float q) { return q > 0.f ? (double)q : 0.0; }       // (a NaN is none)
 __device__ __forceinline__ float load_q(const VerifyArgs& a, int row, int i) {
@@ -94,83 +119,157 @@ __device__ __forceinline__ double kept_mass(float l, int i, const RowCut& cut, c
   if (r.min_p > 0.0 && m < r.min_p * (double)(1ull << kMassBits)) return 0.0;
   return cut.last != ~0ull && order_key<DT>(l, i) > cut.last ? 0.0 : m;
 }
+// ... of eight entries from i on, without a branch an entry: what is 60 or more below the largest (in bits), and a NaN, is taken to be at 60, which rounds
+// to nothing
+template <int DT>
+__device__ __forceinline__ void eight_masses(const float* l, int i, const RowCut& cut, const RowTop& top, const RowRule& r, const Series& series, double* m) {
+  if (top.only) {                                                        // (uniform)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m[k] = l[k] == top.value ? (double)(1ull << kMassBits) : 0.0;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const double x = fmax(((double)l[k] - top.wide) * r.inv_t_log2e, -60.0), n = rint(x);
+      m[k] = ldexp(series(x - n), (int)n);
+    }
+  }
+  if (r.min_p > 0.0) {
+    const double least = r.min_p * (double)(1ull << kMassBits);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m[k] = m[k] < least ? 0.0 : m[k];
+  }
+  if (cut.last != ~0ull) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m[k] = order_key<DT>(l[k], i + k) > cut.last ? 0.0 : m[k];
+  }
+}
+__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor((unsigned long long)v, o, kWave);
+  return v;
+}
 __device__ __forceinline__ uint64_t block_sum_u64(uint64_t v, uint64_t* scratch) {
-  v = wave_scan_u64(v);
-  if ((threadIdx.x & (kWave - 1)) == kWave - 1) scratch[threadIdx.x / kWave] = v;
+  v = wave_sum_u64(v);
+  if ((threadIdx.x & (kWave - 1)) == 0) scratch[threadIdx.x / kWave] = v;
   __syncthreads();
   uint64_t sum = 0;
 #pragma unroll
-  for (int w = 0; w < kVerifyThreads / kWave; ++w) sum += scratch[w];
+  for (int w = 0; w < kVerifyWaves; ++w) sum += scratch[w];
   __syncthreads();
   return sum;
 }
 
 // ---------------------------------------------------------------------------------------------------------------- rows without filters
-template <int DT, int ROUNDS>
-__global__ __launch_bounds__(kVerifyThreads) void verify_mass_kernel(VerifyArgs a) {
-  __shared__ float tops[kVerifyThreads / kWave];
-  __shared__ int firsts[kVerifyThreads / kWave];
-  __shared__ uint64_t sums[kVerifyThreads / kWave];
-  const int row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
-  if (row < a.starts[0] || row >= a.starts[a.batch]) return;           // a row of no sequence
-  const RowRule r = row_rule(a.s, row);
+// A row's mass in 32 bits says of nearly every draft whether it stays, so all rows are read once, as fast as they come; masses in 64 bits are worked out
+// for the one row that a sequence ends with (and for a row whose draft the 32 bits leave undecided, see kUnsure).
+// A slice is a wavefront's, so nobody waits for anybody.
+constexpr int kSliceChunks = 4;
+template <int DT>
+__global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs a) {
+  constexpr int ROUNDS = kSliceChunks, kLength = kSliceChunks * kChunk;
+  const uint32_t unit = blockIdx.x * kVerifyWaves + threadIdx.x / kWave;
+  const int row = __builtin_amdgcn_readfirstlane(unit / (uint32_t)a.slices), slice = (int)(unit - (uint32_t)row * a.slices), lane = threadIdx.x & (kWave - 1);
+  if (row < a.starts[0] || row >= min(a.starts[a.batch], a.n_rows)) return;      // a row of no sequence, or none
   const char* src = verify_row<DT>(a, row);
-  const int i0 = slice * a.length + 8 * (int)threadIdx.x;
-  float x[8 * ROUNDS], top = -INFINITY;
+  float of[ROUNDS][8], top = -INFINITY, sum = 0.f;
+  load_chunks<DT, ROUNDS>(src, slice * kLength, kChunk, a.s.vocab, a.wide, -INFINITY, of);
+  const RowRule r = row_rule(a.s, row);
+  float* x = of[0];
 #pragma unroll
-  for (int k = 0; k < ROUNDS; ++k) load_eight<DT>(src, i0 + k * kVerifyRound, a.s.vocab, a.wide, -INFINITY, x + 8 * k);
-#pragma unroll
-  for (int e = 0; e < 8 * ROUNDS; ++e) top = x[e] > top ? x[e] : top;   // (a NaN never is)
-  top = block_max<kVerifyThreads>(top, tops);
-  const RowTop t = row_top_of(top, r);
-  const Series series;
-  uint64_t sum = 0;
-  int first = INT32_MAX;
-  if (top > -INFINITY) {
-#pragma unroll
-    for (int e = 0; e < 8 * ROUNDS; ++e) {
-      if (entry_distance(x[e], t, r) < kReach) sum += whole(entry_mass(x[e], t, r, series));
-      if (r.greedy && x[e] == top) first = min(first, i0 + (e / 8) * kVerifyRound + e % 8);
-    }
-  }
-  if (r.greedy) first = block_min_i<kVerifyThreads>(first, firsts);     // (uniform)
-  sum = block_sum_u64(sum, sums);
-  if (threadIdx.x == 0) a.masses[blockIdx.x] = SliceMass{(double)sum, top, first};
-}
-
-// A row's cut from its slices (a wavefront; the same in all its lanes)
-template <int DT>
-__device__ RowCut row_cut(const VerifyArgs& a, int row, const RowRule& r, const Series& series) {
-  if (a.slices == 0) return a.cuts[row];
-  const int lane = threadIdx.x & (kWave - 1);
-  const SliceMass* of = a.masses + (int64_t)row * a.slices;
-  float top = -INFINITY;
-  for (int s = lane; s < a.slices; s += kWave) top = fmaxf(top, of[s].top);
+  for (int e = 0; e < 8 * ROUNDS; ++e) top = fmaxf(top, x[e]);           // (a NaN never is)
   top = wave_max(top);
-  if (top == -INFINITY) return RowCut{0.0, 0, top};
-  const RowTop t = row_top_of(top, r);
-  if (r.greedy) {                                                       // the first of the largest alone
-    int first = INT32_MAX;
-    for (int s = lane; s < a.slices; s += kWave)
-      if (of[s].top == top) first = min(first, of[s].first);
-    return RowCut{(double)(1ull << kMassBits), order_key<DT>(top, wave_min_i(first)), top};
-  }
-  double z = 0.0;
-  for (int s = lane; s < a.slices; s += kWave) {
-    const SliceMass m = of[s];
-    if (entry_distance(m.top, t, r) < kReach) z = fma(m.mass, entry_mass(m.top, t, r, series) * 0x1p-42, z);
-  }
+  int first = INT32_MAX;
+  if (r.greedy || top == INFINITY) {                                   // only entries that equal the largest have mass
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) z += __shfl_xor(z, o, kWave);
-  return RowCut{z, ~0ull, top};
+    for (int e = 8 * ROUNDS - 1; e >= 0; --e) {
+      if (x[e] != top) continue;
+      sum += 1.f;
+      first = slice * kLength + 8 * lane + (e / 8) * kChunk + e % 8;
+    }
+    first = wave_min_i(first);
+    sum = wave_sum(sum);
+  } else if (top > -INFINITY) {
+    // 2^((l - top) scale) = 2^(l scale - (top scale rounded)) 2^(what the rounding left out)
+    const float scale = (float)r.inv_t_log2e, base = top * scale, left = fmaf(top, scale, -base);
+#pragma unroll
+    for (int e = 0; e < 8 * ROUNDS; ++e) sum += __builtin_amdgcn_exp2f(fmaf(x[e], scale, -base));
+    sum = wave_sum(sum);
+    if (sum != sum) {                                                  // there is a NaN, which has no mass
+      sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8 * ROUNDS; ++e) sum += x[e] != x[e] ? 0.f : __builtin_amdgcn_exp2f(fmaf(x[e], scale, -base));
+      sum = wave_sum(sum);
+    }
+    sum *= __builtin_amdgcn_exp2f(-left);
+  }
+  if (lane == 0) a.stats[unit] = SliceStats{top, sum, first, 0};
 }
 
-// ---------------------------------------------------------------------------------------------------------------- which drafts stay
-// A workgroup a sequence, a wavefront a row at a time; one more for the rows of nobody.
+// A row from its slices (kRowLanes lanes; the same in all of them): the cut, with the mass relative to the largest and in 32 bits.
+constexpr int kRowLanes = 16, kRowsAtOnce = kVerifyThreads / kRowLanes;
 template <int DT>
-__global__ __launch_bounds__(kVerifyThreads) void verify_accept_kernel(VerifyArgs a) {
-  __shared__ int end;
-  if ((int)blockIdx.x == a.batch) {
+__device__ RowCut row_from_slices(const VerifyArgs& a, int row, const RowRule& r) {
+  const int lane = threadIdx.x % kRowLanes;
+  const SliceStats* of = a.stats + (int64_t)row * a.slices;
+  float top = -INFINITY;
+#pragma unroll 4
+  for (int s = lane; s < a.slices; s += kRowLanes) top = fmaxf(top, of[s].top);
+#pragma unroll
+  for (int o = kRowLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
+  const float scale = (float)r.inv_t_log2e;
+  float z = 0.f;
+  int first = INT32_MAX;
+#pragma unroll 4
+  for (int s = lane; s < a.slices; s += kRowLanes) {
+    const SliceStats m = of[s];
+    z = fmaf(m.sum, m.top == top ? 1.f : __builtin_amdgcn_exp2f(fmaxf((m.top - top) * scale, -200.f)), z);
+    first = m.top == top ? min(first, m.first) : first;
+  }
+#pragma unroll
+  for (int o = kRowLanes / 2; o > 0; o >>= 1) {
+    z += __shfl_xor(z, o, kWave);
+    first = min(first, __shfl_xor(first, o, kWave));
+  }
+  if (top == -INFINITY) return RowCut{0.0, 0, top};
+  if (r.greedy) return RowCut{1.0, order_key<DT>(top, first), top};      // the first of the largest alone
+  return RowCut{(double)z, ~0ull, top};
+}
+// The row's mass in 64 bits (a workgroup)
+template <int DT>
+__device__ uint64_t exact_mass(const VerifyArgs& a, int row, const RowCut& cut, const RowTop& top, const RowRule& r, const Series& series,
+                               uint64_t* scratch) {
+  uint64_t sum = 0;
+#pragma unroll 1
+  for (int c = (int)threadIdx.x / kWave * kChunk; c < a.s.vocab; c += kVerifyRound) {
+    float x[1][8];
+    load_chunks<DT, 1>(verify_row<DT>(a, row), c, 0, a.s.vocab, a.wide, -INFINITY, x);
+    double m[8];
+    eight_masses<DT>(x[0], c + 8 * (int)(threadIdx.x & (kWave - 1)), cut, top, r, series, m);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += whole(m[k]);
+  }
+  return block_sum_u64(sum, scratch);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- the row a sequence ends with
+// What a draft leaves of an entry's mass
+__device__ __forceinline__ uint64_t rest_of(double m, float q, double z) { return whole(fmax(fma(-draft_prob(q), z, m), 0.0)); }
+// How far u q Z and m may be apart, relative to m, for 32 bits to say which is larger.  With d = (l - top) / (T ln 2) a term 2^d is off by 3 |d| 2^-24 ln 2
+// (the exponent's rounding, the factor's; a slice's largest logit against the row's) and 2^-23; 2^20 terms of a size below 2^-20 make no more than one, so by
+// 20 * 3 * 2^-24 * 0.7 on average; a lane adds 32 terms, a wavefront 64 sums in a tree, a row 512 of these, 32 a
+// lane: 2.5e-6 + 2^-23 + 74 * 2^-24 < 2^-17.
+constexpr double kUnsure = 0x1p-16;
+
+// A workgroup a slice of that row.  Each looks for itself which drafts of the sequence stay (kRowsAtOnce rows at a time: few words, out of the caches), which
+// is cheaper than a launch of its own for that; the first of a sequence's writes it down.  Then the masses of the slice's chunks, and where the
+// row's mass is known (with filters) what the draft leaves of them.  One more workgroup is for the rows of nobody.
+template <int DT, bool FILTERED, int ROUNDS>
+__global__ __launch_bounds__(kVerifyThreads) void verify_end_kernel(VerifyArgs a) {
+  __shared__ uint64_t scratch[kVerifyWaves];
+  __shared__ RowCut cuts[kRowsAtOnce];
+  __shared__ int stop;                                                  // 2 i: the sequence ends with row i; 2 i + 1: 32 bits do not say
+  const int b = blockIdx.x / a.end_slices, slice = blockIdx.x % a.end_slices;
+  if (b == a.batch) {
     const int begin = min(max(a.starts[0], 0), a.n_rows), behind = min(max(a.starts[a.batch], 0), a.n_rows);
     for (int t = threadIdx.x; t < a.n_rows; t += kVerifyThreads)
       if (t < begin || t >= behind) {
@@ -179,235 +278,280 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_accept_kernel(VerifyArg
       }
     return;
   }
-  const VerifySpan sp = verify_span(a, blockIdx.x);
+  const VerifySpan sp = verify_span(a, b);
   if (sp.n == 0) {
-    if (threadIdx.x == 0) {
-      a.accepted[blockIdx.x] = 0;
-      a.ends[blockIdx.x].row = -1;
+    if (slice == 0 && threadIdx.x == 0) {
+      a.accepted[b] = 0;
+      a.ends[b].row = -1;
     }
     return;
   }
-  if (threadIdx.x == 0) end = sp.n - 1;
-  __syncthreads();
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1), end = slice == 0;
   const Series series;
-  for (int i = wave; i < sp.n - 1; i += kVerifyThreads / kWave) {
-    const int row = sp.first + i;
-    const RowRule r = row_rule(a.s, row);
-    const int64_t x = a.drafts[row + 1];
-    const bool known = x >= 0 && x < a.s.vocab;
-    const float l = known ? Elem<DT>::load(verify_row<DT>(a, row), x) : -INFINITY;
-    const double q = !a.q ? 1.0 : known ? draft_prob(load_q(a, row, (int)x)) : 0.0;
-    const RowCut cut = row_cut<DT>(a, row, r, series);
-    const double m = cut.mass > 0.0 ? kept_mass<DT>(l, (int)x, cut, row_top_of(cut.top, r), r, series) : 0.0;
-    if (lane == 0) {
-      a.s.probs[row] = cut.mass > 0.0 ? (float)(m / cut.mass) : 0.f;
-      if (!(r.u * q * cut.mass < m)) atomicMin(&end, i);
-    }
-  }
+  int base = 0, here;
+  if (threadIdx.x == 0) stop = INT32_MAX;
   __syncthreads();
-  const int stop = end;
-  for (int i = threadIdx.x; i < sp.n; i += kVerifyThreads) {            // (the row it ends with is the draw's)
-    if (i < stop) {
-      a.s.tokens[sp.first + i] = a.drafts[sp.first + i + 1];
-    } else if (i > stop) {
-      a.s.tokens[sp.first + i] = -1;
-      a.s.probs[sp.first + i] = 0.f;
-    }
-  }
-  if (wave != 0) return;
-  const int row = sp.first + stop;
-  const RowCut cut = row_cut<DT>(a, row, row_rule(a.s, row), series);
-  if (lane == 0) {
-    const int64_t x = stop == sp.n - 1 ? -1 : a.drafts[row + 1];
-    a.accepted[blockIdx.x] = stop;
-    a.ends[blockIdx.x] = EndRecord{cut, row, stop, stop == sp.n - 1, x >= 0 && x < a.s.vocab ? (int)x : -1};
-  }
-}
-
-// ---------------------------------------------------------------------------------------------------------------- the token behind them
-// What the draw gives an entry: its rest, or (all) its mass.
-template <int DT>
-struct RestOf {
-  const EndRecord& e;
-  RowRule r;
-  RowTop top;
-  Series series;
-  __device__ __forceinline__ RestOf(const VerifyArgs& a, const EndRecord& end) : e(end), r(row_rule(a.s, end.row)), top(row_top_of(end.cut.top, r)) {}
-  __device__ __forceinline__ double mass(float l, int i) const { return kept_mass<DT>(l, i, e.cut, top, r, series); }
-  __device__ __forceinline__ uint64_t rest(double m, float q) const {
-    const double left = fma(-draft_prob(q), e.cut.mass, m);
-    return left > 0.0 ? whole(left) : 0;
-  }
-};
-// the draft's probabilities of eight entries
-__device__ __forceinline__ void eight_drafts(const VerifyArgs& a, const EndRecord& e, int i, float* q) {
-  if (e.last) return;
-  if (a.q) {
-    load_eight_q(a, e.row, i, q);
-    return;
-  }
-#pragma unroll
-  for (int k = 0; k < 8; ++k) q[k] = i + k == e.draft ? 1.f : 0.f;
-}
-
-template <int DT>
-__global__ __launch_bounds__(kVerifyThreads) void verify_rest_kernel(VerifyArgs a) {
-  __shared__ uint64_t scratch[kVerifyThreads / kWave];
-  const int b = blockIdx.x / a.end_slices, slice = blockIdx.x % a.end_slices;
-  const EndRecord e = a.ends[b];
-  if (e.row < 0 || !(e.cut.mass > 0.0)) return;
-  const RestOf<DT> of(a, e);
-  const char* src = verify_row<DT>(a, e.row);
-  const int end = min((slice + 1) * a.end_length, a.s.vocab);
-  uint64_t rest = 0, all = 0;
-  for (int i = slice * a.end_length + 8 * (int)threadIdx.x; i < end; i += kVerifyRound) {
-    float x[8], q[8];
-    load_eight<DT>(src, i, a.s.vocab, a.wide, -INFINITY, x);
-    eight_drafts(a, e, i, q);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const double m = of.mass(x[k], i + k);
-      all += whole(m);
-      if (!e.last) rest += of.rest(m, q[k]);
-    }
-  }
-  rest = block_sum_u64(rest, scratch);
-  all = block_sum_u64(all, scratch);
-  if (threadIdx.x == 0) a.sums[blockIdx.x] = RestSum{rest, all};
-}
-
-// sum over the threads before this one, and over all of them
-__device__ __forceinline__ uint64_t block_before_u64(uint64_t v, uint64_t* scratch, uint64_t* total) {
-  const uint64_t upto = wave_scan_u64(v);
-  if ((threadIdx.x & (kWave - 1)) == kWave - 1) scratch[threadIdx.x / kWave] = upto;
-  __syncthreads();
-  uint64_t before = upto - v, sum = 0;
-#pragma unroll
-  for (int w = 0; w < kVerifyThreads / kWave; ++w) {
-    if (w < (int)threadIdx.x / kWave) before += scratch[w];
-    sum += scratch[w];
-  }
-  __syncthreads();
-  *total = sum;
-  return before;
-}
-
-template <int DT>
-__global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs a) {
-  __shared__ uint64_t scratch[kVerifyThreads / kWave], goal_left;
-  __shared__ int found;
-  const EndRecord e = a.ends[blockIdx.x];
-  if (e.row < 0) return;                                                // (uniform, as the other return below)
-  if (threadIdx.x == 0) {                                               // (what stays where nothing can be drawn)
-    a.s.tokens[e.row] = -1;
-    a.s.probs[e.row] = 0.f;
-    found = 0;
-    goal_left = 0;
-  }
-  if (!(e.cut.mass > 0.0)) return;
-  // the slice that the number falls into: a thread has consecutive ones
-  const RestSum* sums = a.sums + (int64_t)blockIdx.x * a.end_slices;
-  const int each = (a.end_slices + kVerifyThreads - 1) / kVerifyThreads, s0 = threadIdx.x * each;
-  uint64_t rest = 0, all = 0, total;
-  for (int s = s0; s < min(s0 + each, a.end_slices); ++s) {
-    rest += sums[s].rest;
-    all += sums[s].all;
-  }
-  const uint64_t rest_before = block_before_u64(rest, scratch, &total);
-  const bool by_rest = total > 0;
-  uint64_t all_total;
-  const uint64_t all_before = block_before_u64(all, scratch, &all_total);
-  if (!by_rest) total = all_total;
-  const float v = a.draws[blockIdx.x];
-  const uint64_t goal = draw_goal(v > 0.f ? (double)v : 0.0, total);
-  uint64_t before = by_rest ? rest_before : all_before;
-  if (before <= goal && goal < before + (by_rest ? rest : all)) {        // (one thread: the goal is below the total)
-    int s = s0;
-    for (;; ++s) {
-      const uint64_t here = by_rest ? sums[s].rest : sums[s].all;
-      if (s + 1 >= min(s0 + each, a.end_slices) || goal < before + here) break;
-      before += here;
-    }
-    found = s;
-    goal_left = goal - before;
-  }
-  __syncthreads();
-  // ... and the entry in it: a thread has consecutive ones again
-  const RestOf<DT> of(a, e);
-  const char* src = verify_row<DT>(a, e.row);
-  const int per = a.end_length / kVerifyThreads, i0 = found * a.end_length + (int)threadIdx.x * per;
-  const uint64_t left = goal_left;
-  auto weight = [&](const float* x, const float* q, int k, int i) {
-    const double m = of.mass(x[k], i + k);
-    return by_rest ? of.rest(m, q[k]) : whole(m);
-  };
-  uint64_t sum = 0;
-  float x[8], q[8];
-  for (int i = i0; i < i0 + per; i += 8) {
-    load_eight<DT>(src, i, a.s.vocab, a.wide, -INFINITY, x);
-    eight_drafts(a, e, i, q);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) sum += weight(x, q, k, i);
-  }
-  uint64_t at = block_before_u64(sum, scratch, &total);
-  if (!(at <= left && left < at + sum)) return;                          // (one thread is left)
-  for (int i = i0; i < i0 + per; i += 8) {
-    load_eight<DT>(src, i, a.s.vocab, a.wide, -INFINITY, x);
-    eight_drafts(a, e, i, q);
-    for (int k = 0; k < 8; ++k) {
-      at += weight(x, q, k, i);
-      if (at > left) {
-        a.s.tokens[e.row] = i + k;
-        a.s.probs[e.row] = (float)(of.mass(x[k], i + k) / e.cut.mass);
-        return;
+  for (;;) {
+    const int i = base + (int)threadIdx.x / kRowLanes;
+    if (i < sp.n) {
+      const int row = sp.first + i, last = i == sp.n - 1;
+      const RowRule r = row_rule(a.s, row);
+      const int64_t x = last ? -1 : a.drafts[row + 1];
+      const bool known = x >= 0 && x < a.s.vocab;
+      const float l = known ? Elem<DT>::load(verify_row<DT>(a, row), x) : -INFINITY;
+      const double q = !a.q ? 1.0 : known ? draft_prob(load_q(a, row, (int)x)) : 0.0;
+      const RowCut cut = FILTERED ? a.cuts[row] : row_from_slices<DT>(a, row, r);
+      if (threadIdx.x % kRowLanes == 0) {
+        const double unit = FILTERED ? 1.0 : 0x1p-42;                    // (masses in 32 bits are relative to the largest)
+        const double m = cut.mass > 0.0 ? kept_mass<DT>(l, (int)x, cut, row_top_of(cut.top, r), r, series) * unit : 0.0;
+        const double goal = r.u * q * cut.mass;
+        const bool unsure = !FILTERED && !r.greedy && m > 0.0 && fabs(goal - m) <= kUnsure * m;
+        if (unsure) atomicMin(&stop, 2 * i + 1);
+        else if (!(goal < m)) atomicMin(&stop, 2 * i);                   // (the last row has no draft, of no mass)
+        if (end && !last) a.s.probs[row] = cut.mass > 0.0 ? (float)(m / cut.mass) : 0.f;
+        cuts[threadIdx.x / kRowLanes] = cut;
       }
     }
+    __syncthreads();
+    here = stop;
+    if (here == INT32_MAX) {                                             // (uniform) the next rows
+      __syncthreads();
+      base += kRowsAtOnce;
+      continue;
+    }
+    if (FILTERED || !(here & 1)) break;
+    const int row = sp.first + here / 2;
+    const RowRule r = row_rule(a.s, row);
+    const RowCut cut = cuts[here / 2 - base];
+    const RowTop top = row_top_of(cut.top, r);
+    const double z = (double)exact_mass<DT>(a, row, cut, top, r, series, scratch);
+    const int64_t x = a.drafts[row + 1];                                 // (one of the vocabulary: it has mass)
+    const double m = kept_mass<DT>(Elem<DT>::load(verify_row<DT>(a, row), x), (int)x, cut, top, r, series);
+    if (!(r.u * (!a.q ? 1.0 : draft_prob(load_q(a, row, (int)x))) * z < m)) break;
+    base = here / 2 + 1;
+    if (threadIdx.x == 0) stop = INT32_MAX;                              // (all have read it: exact_mass has barriers)
+    __syncthreads();
+  }
+  const int stays = here / 2, row = sp.first + stays, last = stays == sp.n - 1;
+  const RowRule r = row_rule(a.s, row);
+  const RowCut cut = cuts[stays - base];
+  const int64_t x = last ? -1 : a.drafts[row + 1];
+  const int draft = x >= 0 && x < a.s.vocab ? (int)x : -1;
+  if (end) {
+    for (int i = threadIdx.x; i < sp.n; i += kVerifyThreads) {          // (the row it ends with is the draw's)
+      if (i < stays) {
+        a.s.tokens[sp.first + i] = a.drafts[sp.first + i + 1];
+      } else if (i > stays) {
+        a.s.tokens[sp.first + i] = -1;
+        a.s.probs[sp.first + i] = 0.f;
+      }
+    }
+    if (threadIdx.x == 0) {
+      a.accepted[b] = stays;
+      a.ends[b] = EndRecord{cut, row, last, draft};
+    }
+  }
+  const RowTop top = row_top_of(cut.top, r);
+  const char* src = verify_row<DT>(a, row);
+  // (all of the wavefront's entries asked for before the first is looked at)
+  const int c0 = slice * a.end_length + wave * kChunk;
+  float l[ROUNDS][8], q[ROUNDS][8];
+  load_chunks<DT, ROUNDS>(src, c0, kVerifyRound, a.s.vocab, a.wide, -INFINITY, l);
+  if (FILTERED && !last) load_drafts<ROUNDS>(a, row, draft, c0, kVerifyRound, q);
+#pragma unroll
+  for (int k = 0; k < ROUNDS; ++k) {
+    const int c = c0 + k * kVerifyRound;
+    if (c >= a.s.vocab) break;
+    uint64_t all = 0, rest = 0;
+    double m[8];
+    eight_masses<DT>(l[k], c + 8 * lane, cut, top, r, series, m);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      all += whole(m[e]);
+      if (FILTERED && !last) rest += rest_of(m[e], q[k][e], cut.mass);
+    }
+    all = wave_sum_u64(all);
+    if (FILTERED) rest = wave_sum_u64(rest);
+    if (lane == 0) {
+      const int64_t at = (int64_t)b * a.chunks + c / kChunk;
+      a.all[at] = all;
+      if (FILTERED || last) a.rest[at] = rest;
+    }
   }
 }
 
-// Entries of a slice: a round or more of a workgroup's threads, so that `rows` rows make some thousands of workgroups.
-static int verify_slice_length(int64_t rows, int64_t vocab) {
+// the mass of a sequence's last row, from its chunks (a workgroup)
+__device__ __forceinline__ double end_mass(const VerifyArgs& a, int b, uint64_t* scratch) {
+  uint64_t sum = 0;
+  for (int c = threadIdx.x; c < a.chunks; c += kVerifyThreads) sum += a.all[(int64_t)b * a.chunks + c];
+  return (double)block_sum_u64(sum, scratch);
+}
+
+// What the draft leaves, without filters: the row's mass is known now.
+template <int DT, int ROUNDS>
+__global__ __launch_bounds__(kVerifyThreads) void verify_rest_kernel(VerifyArgs a) {
+  __shared__ uint64_t scratch[kVerifyWaves];
+  const int b = blockIdx.x / a.end_slices, slice = blockIdx.x % a.end_slices;
+  const EndRecord e = a.ends[b];
+  if (e.row < 0 || e.last) return;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+  const char* src = verify_row<DT>(a, e.row);
+  const int c0 = slice * a.end_length + wave * kChunk;
+  float l[ROUNDS][8], q[ROUNDS][8];
+  load_chunks<DT, ROUNDS>(src, c0, kVerifyRound, a.s.vocab, a.wide, -INFINITY, l);
+  load_drafts<ROUNDS>(a, e.row, e.draft, c0, kVerifyRound, q);
+  const RowRule r = row_rule(a.s, e.row);
+  const RowTop top = row_top_of(e.cut.top, r);
+  const Series series;
+  const double z = end_mass(a, b, scratch);
+#pragma unroll
+  for (int k = 0; k < ROUNDS; ++k) {
+    const int c = c0 + k * kVerifyRound;
+    if (c >= a.s.vocab) break;
+    uint64_t rest = 0;
+    double m[8];
+    eight_masses<DT>(l[k], c + 8 * lane, e.cut, top, r, series, m);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rest += rest_of(m[i], q[k][i], z);
+    rest = wave_sum_u64(rest);
+    if (lane == 0) a.rest[(int64_t)b * a.chunks + c / kChunk] = rest;
+  }
+}
+
+// The token: the chunk that the number falls into, then the entry.  A wavefront a sequence.
+template <int DT>
+__global__ __launch_bounds__(kWave) void verify_draw_kernel(VerifyArgs a) {
+  const int b = blockIdx.x, lane = threadIdx.x;
+  const EndRecord e = a.ends[b];
+  if (e.row < 0) return;
+  const uint64_t* alls = a.all + (int64_t)b * a.chunks;
+  const uint64_t* rests = a.rest + (int64_t)b * a.chunks;
+  // a lane has consecutive chunks; of the usual vocabularies at most eight, which stay in registers
+  constexpr int kHeld = 8;
+  const int per = (a.chunks + kWave - 1) / kWave, c0 = min(lane * per, a.chunks), c1 = min(c0 + per, a.chunks);
+  uint64_t all = 0, rest = 0, alls_at[kHeld], rests_at[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    alls_at[i] = c0 + i < c1 ? alls[c0 + i] : 0;
+    rests_at[i] = c0 + i < c1 ? rests[c0 + i] : 0;
+    all += alls_at[i];
+    rest += rests_at[i];
+  }
+  for (int c = c0 + kHeld; c < c1; ++c) {
+    all += alls[c];
+    rest += rests[c];
+  }
+  const uint64_t z = wave_sum_u64(all);
+  const bool by_rest = wave_sum_u64(rest) > 0;
+  const uint64_t* sums = by_rest ? rests : alls;
+  const uint64_t mine = by_rest ? rest : all, upto = wave_scan_u64(mine), total = __shfl((unsigned long long)upto, kWave - 1, kWave);
+  int64_t token = -1;
+  float prob = 0.f;
+  if (total > 0) {
+    const float v = a.draws[b];
+    const uint64_t goal = draw_goal(v > 0.f ? (double)v : 0.0, total);
+    const int owner = __ffsll((unsigned long long)__ballot(goal < upto)) - 1;       // (the last lane's is the total)
+    int chunk = c0;
+    uint64_t before = upto - mine;
+    bool here = false;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const uint64_t next = before + (by_rest ? rests_at[i] : alls_at[i]);
+      here = here || goal < next;
+      before = here ? before : next;
+      chunk += here ? 0 : 1;
+    }
+    for (; !here && chunk + 1 < c1; ++chunk) {
+      const uint64_t next = before + sums[chunk];
+      if (goal < next) break;
+      before = next;
+    }
+    chunk = __shfl(chunk, owner, kWave);
+    const uint64_t left = goal - __shfl((unsigned long long)before, owner, kWave);
+    const RowRule r = row_rule(a.s, e.row);
+    const RowTop top = row_top_of(e.cut.top, r);
+    const Series series;
+    const double zd = a.filtered ? e.cut.mass : (double)z;
+    const int i = chunk * kChunk + 8 * lane;
+    float l[1][8], q[1][8];
+    load_chunks<DT, 1>(verify_row<DT>(a, e.row), chunk * kChunk, 0, a.s.vocab, a.wide, -INFINITY, l);
+    if (by_rest) load_drafts<1>(a, e.row, e.draft, chunk * kChunk, 0, q);
+    uint64_t w[8], sum = 0;
+    double m[8];
+    eight_masses<DT>(l[0], i, e.cut, top, r, series, m);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += w[k] = by_rest ? rest_of(m[k], q[0][k], zd) : whole(m[k]);
+    uint64_t at = wave_scan_u64(sum) - sum;
+    const uint64_t hit = __ballot(at <= left && left < at + sum);
+    double mass = 0.0;
+    int k_hit = 0;
+#pragma unroll
+    for (int k = 7; k >= 0; --k) {
+      const uint64_t ahead = at + (sum -= w[k]);                                    // mass before entry k
+      if (ahead <= left && left < ahead + w[k]) {
+        mass = m[k];
+        k_hit = k;
+      }
+    }
+    const int finder = hit ? __ffsll((unsigned long long)hit) - 1 : 0;
+    if (hit) {
+      token = __shfl(i + k_hit, finder, kWave);
+      prob = __shfl((float)(mass / zd), finder, kWave);
+    }
+  }
+  if (lane == 0) {
+    a.s.tokens[e.row] = token;
+    a.s.probs[e.row] = prob;
+  }
+}
+
+// Entries of a slice of the rows that sequences end with: one round of a workgroup's threads, two or four, while there are more workgroups than fit at once
+static int verify_end_length(int64_t batch, int64_t vocab) {
   int64_t length = kVerifyRound;
-  while (length < 4 * kVerifyRound && rows * ((vocab + 2 * length - 1) / (2 * length)) >= 2048) length *= 2;
+  while (length < 4 * kVerifyRound && batch * ((vocab + 2 * length - 1) / (2 * length)) >= 768) length *= 2;
   return (int)length;
 }
 
 struct VerifyPlan {
-  int length, slices, end_length, end_slices;
-  size_t search, masses, cuts, ends, sums, bytes;
+  int slices, end_length, end_slices, chunks;
+  size_t search, stats, cuts, ends, sums, bytes;
 };
 static VerifyPlan verify_plan(int64_t n_rows, int64_t batch, int64_t vocab, bool filtered) {
   VerifyPlan p{};
-  p.length = verify_slice_length(n_rows, vocab);
-  p.slices = (int)((vocab + p.length - 1) / p.length);
-  p.end_length = verify_slice_length(batch, vocab);
+  p.slices = (int)((vocab + kSliceChunks * kChunk - 1) / (kSliceChunks * kChunk));
+  p.end_length = verify_end_length(batch, vocab);
   p.end_slices = (int)((vocab + p.end_length - 1) / p.end_length);
+  p.chunks = (int)((vocab + kChunk - 1) / kChunk);
   if (filtered && n_rows > 0) p.search = align_up(row_search_workspace(n_rows, vocab), 256);
-  else p.masses = align_up((size_t)n_rows * p.slices * sizeof(SliceMass), 256);
-  p.cuts = filtered ? align_up((size_t)n_rows * sizeof(RowCut), 256) : 0;
+  if (filtered) p.cuts = align_up((size_t)n_rows * sizeof(RowCut), 256);
+  else p.stats = align_up((size_t)n_rows * p.slices * sizeof(SliceStats), 256);
   p.ends = align_up((size_t)batch * sizeof(EndRecord), 256);
-  p.sums = align_up((size_t)batch * p.end_slices * sizeof(RestSum), 256);
-  p.bytes = p.search + p.masses + p.cuts + p.ends + p.sums;
+  p.sums = align_up((size_t)batch * p.chunks * sizeof(uint64_t), 256);
+  p.bytes = p.search + p.stats + p.cuts + p.ends + 2 * p.sums;
   return p;
 }
 
+template <int DT, int ROUNDS>
+static void launch_ends(const VerifyArgs& a, hipStream_t st) {
+  const dim3 block(kVerifyThreads), ends((unsigned)(a.batch * a.end_slices)), ends_and_nobody((unsigned)(a.batch * a.end_slices + 1));
+  if (a.filtered) {
+    hipLaunchKernelGGL((verify_end_kernel<DT, true, ROUNDS>), ends_and_nobody, block, 0, st, a);
+  } else {
+    hipLaunchKernelGGL((verify_end_kernel<DT, false, ROUNDS>), ends_and_nobody, block, 0, st, a);
+    if (a.n_rows > 0) hipLaunchKernelGGL((verify_rest_kernel<DT, ROUNDS>), ends, block, 0, st, a);
+  }
+}
 template <int DT>
 static void launch_verify(const VerifyArgs& a, hipStream_t st) {
-  if (a.n_rows > 0) {
-    if (a.slices) {
-      DominantKernelTimer timer(st);
-      const dim3 grid((unsigned)((int64_t)a.n_rows * a.slices)), block(kVerifyThreads);
-      if (a.length == kVerifyRound) hipLaunchKernelGGL((verify_mass_kernel<DT, 1>), grid, block, 0, st, a);
-      else if (a.length == 2 * kVerifyRound) hipLaunchKernelGGL((verify_mass_kernel<DT, 2>), grid, block, 0, st, a);
-      else hipLaunchKernelGGL((verify_mass_kernel<DT, 4>), grid, block, 0, st, a);
-    }
+  if (!a.filtered && a.n_rows > 0) {
+    DominantKernelTimer timer(st);
+    const dim3 grid((unsigned)(((int64_t)a.n_rows * a.slices + kVerifyWaves - 1) / kVerifyWaves)), block(kVerifyThreads);
+    hipLaunchKernelGGL(verify_stats_kernel<DT>, grid, block, 0, st, a);
   }
-  hipLaunchKernelGGL(verify_accept_kernel<DT>, dim3((unsigned)a.batch + 1), dim3(kVerifyThreads), 0, st, a);
-  if (a.n_rows > 0) {
-    hipLaunchKernelGGL(verify_rest_kernel<DT>, dim3((unsigned)(a.batch * a.end_slices)), dim3(kVerifyThreads), 0, st, a);
-    hipLaunchKernelGGL(verify_draw_kernel<DT>, dim3((unsigned)a.batch), dim3(kVerifyThreads), 0, st, a);
-  }
+  if (a.end_length == kVerifyRound) launch_ends<DT, 1>(a, st);
+  else if (a.end_length == 2 * kVerifyRound) launch_ends<DT, 2>(a, st);
+  else launch_ends<DT, 4>(a, st);
+  if (a.n_rows > 0) hipLaunchKernelGGL(verify_draw_kernel<DT>, dim3((unsigned)a.batch), dim3(kWave), 0, st, a);
 }
 
 }  // namespace subspec
@@ -444,7 +588,7 @@ extern "C" int subspec_verify_drafts(const void* logits, int dtype, int64_t n_ro
   if (!workspace || workspace_bytes < p.bytes)
     SUBSPEC_FAIL(SUBSPEC_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the %zu required", what, workspace_bytes, p.bytes);
   if ((uintptr_t)workspace % 16) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
-  if (n_rows * p.slices > INT32_MAX || batch * p.end_slices > INT32_MAX)
+  if (n_rows * p.slices > INT32_MAX || batch * p.end_slices >= INT32_MAX)
     SUBSPEC_FAIL(SUBSPEC_ERR_LIMIT, "%s: too large (%lld rows of %lld)", what, (long long)n_rows, (long long)vocab);
   VerifyArgs a{};
   a.s = SampleArgs{logits, uniforms, temperatures, top_ks, top_ps, min_ps, tokens, probs, row_stride, (int)vocab, top_k, temperature, top_p, min_p};
@@ -452,12 +596,13 @@ extern "C" int subspec_verify_drafts(const void* logits, int dtype, int64_t n_ro
   char* ws = (char*)workspace;
   void* search = ws;
   ws += p.search;
-  a.masses = (SliceMass*)ws; ws += p.masses;
+  a.stats = (SliceStats*)ws; ws += p.stats;
   a.cuts = (RowCut*)ws; ws += p.cuts;
   a.ends = (EndRecord*)ws; ws += p.ends;
-  a.sums = (RestSum*)ws;
-  a.q_dtype = draft_dtype; a.slices = filtered ? 0 : p.slices; a.length = p.length; a.end_slices = p.end_slices; a.end_length = p.end_length;
-  a.batch = (int)batch; a.n_rows = (int)n_rows;
+  a.all = (uint64_t*)ws; ws += p.sums;
+  a.rest = (uint64_t*)ws;
+  a.q_dtype = draft_dtype; a.slices = p.slices; a.end_slices = p.end_slices; a.end_length = p.end_length; a.chunks = p.chunks;
+  a.batch = (int)batch; a.n_rows = (int)n_rows; a.filtered = filtered;
   const int64_t es = (int64_t)dtype_size(dtype), qs = (int64_t)dtype_size(draft_dtype);
   a.wide = (uintptr_t)logits % 16 == 0 && row_stride * es % 16 == 0;
   a.q_wide = (uintptr_t)draft_probs % 16 == 0 && draft_stride * qs % 16 == 0;

@@ -95,6 +95,7 @@ __device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {      // inclusiv
   }
   return v;
 }
+__device__ __forceinline__ float larger(float m, float l) { return l > m ? l : m; }      // a NaN never is
 __device__ __forceinline__ uint64_t draw_goal(double u, uint64_t z) {
   const uint64_t t = (uint64_t)(u * (double)z);
   return z > 0 ? min(t, z - 1) : 0;

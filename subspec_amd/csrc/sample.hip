@@ -169,7 +169,6 @@ __device__ __forceinline__ void each_entry(const void* row, int i0, int i1, F f)
   part.template ends<THREADS>(f);
 }
 // The largest of a part of a row (a thread's own)
-__device__ __forceinline__ float larger(float m, float l) { return l > m ? l : m; }      // a NaN never is
 template <int DT, int THREADS>
 __device__ __forceinline__ float part_top(const void* row, int i0, int i1) {
   constexpr int kFlight = 4;

@@ -11,16 +11,19 @@ from subspec_amd import ops
 
 DEV = "cuda:0"
 # Tokens have to be equal: masses are exact to 2^-42 of a row's largest, so a draw falls on the other side of an entry's border than in float64 once
-# in a million rows.  Probabilities are rounded once to fp32 (2^-24 relative) from masses within 0.54 * 2^-42 of the largest each.
+# in a million rows.  Probabilities are rounded once to fp32 (2^-24 relative) from masses within 0.54 * 2^-42 of the largest each; without filters those
+# of drafts that stay are over a row's mass in 32 bits.  Of that a term 2^d, d = (l - top) / (T ln 2), is off by 3 |d| 2^-24 ln 2 (the exponent's rounding, the
+# factor's, a slice's largest against the row's) and 2^-23; 2^20 terms of a size below 2^-20 make no more than one, so by 20 * 3 * 2^-24 * 0.7 on average at
+# most; a lane adds 32 terms, a wavefront 64 sums in a tree, a row 512 of these, 32 a lane: 2.5e-6 + 2^-23 + 74 * 2^-24 < 2^-17.
 
 
 def _i32(x):
     return torch.tensor(x, dtype=torch.int32, device=DEV)
 
 
-def _near(got, want):
+def _near(got, want, filtered=False):
     want = torch.tensor(want, dtype=torch.float64)
-    return ((got.cpu().double() - want).abs() <= 2.0 ** -23 * want + 2.0 ** -40).all()
+    return ((got.cpu().double() - want).abs() <= 2.0 ** (-23 if filtered else -17) * want + 2.0 ** -40).all()
 
 
 def _case(g, rows, V, dtype, q_dtype, t=1.0, noise=0.5, first=0, behind=0):
@@ -43,10 +46,10 @@ def _run(case, **settings):
     return ops.verify_drafts(logits.to(DEV), tokens.to(DEV), _i32(starts), uniforms.to(DEV), draws.to(DEV), None if q is None else q.to(DEV), **settings)
 
 
-def _check(case, got, settings=None):
+def _check(case, got, settings=None, filtered=False):
     tokens, probs, accepted = ok.verify_drafts(*case, settings=settings)
     assert got["accepted"].tolist() == accepted and got["tokens"].tolist() == tokens
-    assert _near(got["probs"], probs)
+    assert _near(got["probs"], probs, filtered)
 
 
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
@@ -74,7 +77,7 @@ def test_filters(rows, V, dtype, q_dtype, top_k, top_p, min_p, t):
     g = torch.Generator().manual_seed(V + top_k % 97)
     case = _case(g, rows, V, dtype, q_dtype, t)
     settings = dict(temperature=t, top_k=top_k, top_p=top_p, min_p=min_p)
-    _check(case, _run(case, **settings), lambda row: settings)
+    _check(case, _run(case, **settings), lambda row: settings, filtered=not (top_k in (0, 1 << 31) and top_p == 1.0 and min_p == 0.0))
 
 
 def test_settings_of_every_row():
@@ -268,3 +271,23 @@ def test_refusals():
         call(logits=logits.cpu())
     again = call(out=good)
     assert again["tokens"] is good["tokens"]
+
+
+@pytest.mark.parametrize("V", [3000, 152064])
+def test_numbers_at_the_border_in_32_bits(V):
+    """u q within 2^-30 of p on either side, nearer than a row's mass in 32 bits can tell: the row's mass in 64 bits decides, draft after draft."""
+    g = torch.Generator().manual_seed(V)
+    logits, tokens, starts, u, v, _ = _case(g, [9, 5], V, F32, None)
+    q = torch.zeros(14, V)
+    side = torch.rand(14, generator=g) < 0.8
+    for i in range(13):
+        x = int(tokens[i + 1])
+        p = float(ok.target_probs(logits[i])[x])
+        u[i] = 0.75
+        q[i, x] = p / 0.75                                    # rounded to fp32: 0.75 q is within 2^-24 of p, on the side that the rounding is
+        while (0.75 * float(q[i, x]) < p) != bool(side[i]):
+            q[i, x] = torch.nextafter(q[i, x], torch.tensor(0.0 if side[i] else 9.0))
+    case = (logits, tokens, starts, u, v, q)
+    got = _run(case)
+    _check(case, got)
+    assert got["accepted"].tolist() == [int(side[:8].int().cumprod(0).sum()), int(side[9:13].int().cumprod(0).sum())]
