@@ -397,15 +397,16 @@ int subspec_select_blocks(const void* q, int64_t q_token_stride, int64_t q_head_
                           void* workspace, size_t workspace_bytes, void* stream);
 
 /* out[t, h] = softmax(scale * q[t, h] . k[j, h / group]) v[j, h / group] over the rows j <= positions[t] of the blocks listed for (t, h / group).
- * blocks    device int32 [n_tokens, n_kv_heads, keep]: distinct blocks in any order; entries below 0 or behind the token count for nothing (of a block that is
- *           listed twice the rows count twice).  A token without a row to see gets zeros
+ * blocks    device int32 [n_tokens, n_kv_heads, keep]: distinct blocks in any order; entries below 0 or behind the token count for nothing (the rows of a block
+ *           that is listed twice may count twice).  A token without a row to see gets zeros
  * out       device [n_tokens, n_q_heads, head_dim]; rows of tokens whose sequence lies outside [0, batch) are left as they were.  It may be q
  *           itself where that is contiguous; otherwise it overlaps no input
- * Limits: at most 64 query heads a KV head, keep <= 2^17, keep * page_len <= 2^30, n_tokens <= 2^20; q as for subspec_paged_attention.  Rows of the pool
- * that the token does not see, or whose block is not listed, have no influence, whatever they hold.
+ * Limits: at most 64 query heads a KV head, keep <= 2^17, keep * page_len <= 2^30, n_tokens <= 2^20; q as for subspec_paged_attention.  Page numbers are
+ * clamped to the pool.  Rows of the pool that no token of the call sees, or whose block none lists, have no influence, whatever they hold; where a call has more
+ * tokens than sequences, neighbours of one sequence read their blocks together, and an infinite or NaN VALUE row that one of them sees may reach the others.
  */
-size_t subspec_block_attention_workspace(int64_t n_tokens, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim, int64_t page_len,
-                                         int64_t keep);
+size_t subspec_block_attention_workspace(int64_t batch, int64_t n_tokens, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
+                                         int64_t page_len, int64_t max_blocks, int64_t keep);
 
 int subspec_block_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* kv_pool_layer, int dtype,
                             int64_t max_pages, int64_t page_len, const int32_t* block_table, int64_t max_blocks, int64_t table_stride,

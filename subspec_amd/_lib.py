@@ -84,7 +84,7 @@ _SIGNATURES = {
     "subspec_select_blocks_workspace": (_sz, [_i64] * 5),
     "subspec_select_blocks": (C.c_int, [_p, _i64, _i64, _p, C.c_int, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                         _i64, _p, _p, _sz, _p]),
-    "subspec_block_attention_workspace": (_sz, [_i64] * 6),
+    "subspec_block_attention_workspace": (_sz, [_i64] * 8),
     "subspec_block_attention": (C.c_int, [_p, _i64, _i64, _p, C.c_int, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64,
                                           C.c_float, _p, _p, _sz, _p]),
     "subspec_verify_drafts_workspace": (_sz, [_i64, _i64, _i64, C.c_int]),

@@ -442,9 +442,14 @@ __global__ __launch_bounds__(kSelectThreads) void block_select_kernel(SelectArgs
 // second product costs nothing beside the rows' way out of memory (2-norm against 64 bits with one number 0.0026, with two 0.0016, which is
 // the output's own rounding).  A listed row that the token does not see (behind it, of no block) is a row of zeros and has no probability: what the
 // cache holds there never comes near a product.
+// Tokens of one sequence list much the same blocks, so where a call has more tokens than sequences up to eight of them share a unit (32 rows of a KV head): its
+// blocks are those that any of them lists, ascending, each with a bit a token (block_union_kernel), and a row sees a key by its token's bit and position.
+// 72 drafts of 16 sequences, 32 blocks of 64 rows each, 32 : 8 heads: a unit a token reads 600 MB, out of the caches, in 92 us.
 constexpr int kAttendKeys = 32;
 constexpr int kAttendStages = 2;
 constexpr int kAttendSegment = 512;        // keys whose row offsets are in LDS at a time
+constexpr int kShareRows = 32;             // rows of a unit that several tokens share
+typedef int dec_i4 __attribute__((ext_vector_type(4)));
 __device__ __attribute__((aligned(16))) uint32_t zero_piece[4];
 
 struct AttendArgs {
@@ -457,35 +462,130 @@ struct AttendArgs {
   uint16_t* out;
   float* part_o;                 // [token][n_kv_heads][chunks][group][D], fp32
   float* part_ml;                // (reference, sum)
+  int2* merged;                  // [n_kv_heads][token][keep], from a tile's first token on: the blocks of the tile, a bit for each token that lists them
+  int32_t* counts;               // [n_kv_heads][token]: blocks of the token's tile
+  int32_t* leads;                // ... tokens of the tile that it is the first of, or 0
   int64_t q_token, q_head, table_stride, page_elems;
-  int batch, first, hq, hkv, group, page_shift, max_pages, keep, last_row, keys, chunk_keys, chunks;
+  int batch, first, tokens, hq, hkv, group, page_shift, max_pages, keep, last_row, keys, chunk_keys, chunks, share;
   float scale_log2;
 };
+// Keys of a chunk of a tile, whose lists may agree in all blocks or in none: the plan's number, or as many as its number of chunks takes.
+__device__ __forceinline__ int shared_chunk_keys(const AttendArgs& a, int keys) {
+  return max(a.chunk_keys, ((keys + a.chunks - 1) / a.chunks + 31) & -32);
+}
+__device__ __forceinline__ int attend_last(const AttendArgs& a, int t) { return min(a.positions[t], a.last_row); }
+
+// ---- tiles of up to `share` neighbouring tokens of a sequence, and their blocks: a byte a block in LDS, a bit of it a token, then the bytes in order
+constexpr int kUnionThreads = 256;
+constexpr int kUnionBlocks = 1 << 15;
+__global__ __launch_bounds__(kUnionThreads) void block_union_kernel(AttendArgs a) {
+  __shared__ uint32_t marks[kUnionBlocks / 4];
+  __shared__ int sums[kUnionThreads / kWave];
+  const int local = blockIdx.x / a.hkv, kvh = blockIdx.x % a.hkv, t = a.first + local, tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int b = a.sequences[t], at = kvh * a.tokens + local;
+  const int end = a.first + a.tokens;
+  int behind = 0;                                            // neighbours of the sequence before this token
+  for (;;) {
+    const int other = t - 1 - behind - lane;
+    const uint64_t others = __ballot(other < a.first || a.sequences[max(other, 0)] != b);
+    behind += others ? __ffsll((unsigned long long)others) - 1 : kWave;
+    if (others) break;
+  }
+  if (b < 0 || b >= a.batch || behind % a.share) {           // (the whole workgroup)
+    if (tid == 0) a.leads[at] = 0;
+    return;
+  }
+  const int other = t + 1 + lane;
+  const uint64_t others = __ballot(other >= end || a.sequences[min(other, end - 1)] != b);
+  const int tokens = min(a.share, others ? __ffsll((unsigned long long)others) : kWave);
+  int most = 0;
+  for (int i = 0; i < tokens; ++i) most = max(most, (attend_last(a, t + i) >> a.page_shift) + 1);
+  const int words = (most + 3) / 4;
+  for (int w = tid; w < words; w += kUnionThreads) marks[w] = 0;
+  __syncthreads();
+  for (int n = tid; n < tokens * a.keep; n += kUnionThreads) {
+    const int i = n / a.keep, last = attend_last(a, t + i);
+    const int block = a.blocks[((int64_t)(t + i) * a.hkv + kvh) * a.keep + (n - i * a.keep)];
+    if (block >= 0 && last >= 0 && block <= last >> a.page_shift) atomicOr(&marks[block >> 2], 1u << (8 * (block & 3) + i));
+  }
+  __syncthreads();
+  const int per = (words + kUnionThreads - 1) / kUnionThreads, w0 = min(tid * per, words), w1 = min(w0 + per, words);
+  int mine = 0;
+  for (int w = w0; w < w1; ++w)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) mine += (marks[w] >> 8 * k & 0xff) != 0;
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int u = __shfl_up(upto, o, kWave);
+    if (lane >= o) upto += u;
+  }
+  if (lane == kWave - 1) sums[tid / kWave] = upto;
+  __syncthreads();
+  int before = upto - mine, count = 0;
+#pragma unroll
+  for (int w = 0; w < kUnionThreads / kWave; ++w) {
+    if (w < tid / kWave) before += sums[w];
+    count += sums[w];
+  }
+  int2* out = a.merged + (int64_t)at * a.keep;
+  for (int w = w0; w < w1; ++w)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (const int mark = marks[w] >> 8 * k & 0xff) out[before++] = make_int2(4 * w + k, mark);
+  if (tid < tokens) a.counts[at + tid] = count;
+  if (tid == 0) a.leads[at] = tokens;
+}
+
 template <int D> __device__ __forceinline__ int attend_k_swap(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
 template <int D> __device__ __forceinline__ int attend_v_swap(int row) { return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3); }
 
-template <int DT, int D, int ROWT>
+template <int DT, int D, int ROWT, bool SHARED>
 __global__ __launch_bounds__(kWave) void block_attention_kernel(AttendArgs a) {
   constexpr int kRowBytes = D * 2, kPieces = kRowBytes / 16, kRowsPerCopy = 64 / kPieces, kCopies = kAttendKeys / kRowsPerCopy;
   constexpr int kHalf = kAttendKeys * kRowBytes, kStage = 2 * kHalf;
   __shared__ __attribute__((aligned(1024))) uint8_t ring[kAttendStages * kStage];
   __shared__ int64_t row_at[kAttendSegment];
   __shared__ uint32_t seen_at[kAttendSegment / kAttendKeys];
+  __shared__ __attribute__((aligned(16))) int place_at[SHARED ? kAttendSegment : 4];        // a key's row of the sequence, and its block's bits
+  __shared__ uint32_t bits_at[SHARED ? kAttendSegment / 4 : 1];
   const uint32_t unit = blockIdx.x;
   const int kvh = (int)(unit % (uint32_t)a.hkv);
   const uint32_t tc = unit / (uint32_t)a.hkv;
   const int chunk = (int)(tc % (uint32_t)a.chunks), local = (int)(tc / (uint32_t)a.chunks), t = a.first + local;
+  int tokens = 1, keys = a.keys, chunk_keys = a.chunk_keys;
+  if constexpr (SHARED) {
+    tokens = a.leads[kvh * a.tokens + local];                // (0: of no sequence, or in another's tile)
+    if (tokens == 0) return;
+    keys = a.counts[kvh * a.tokens + local] << a.page_shift;
+    chunk_keys = shared_chunk_keys(a, keys);
+  }
   const int b = a.sequences[t];
   if (b < 0 || b >= a.batch) return;
-  const int last = min(a.positions[t], a.last_row), lane = threadIdx.x, lq = lane & 15, lg = lane >> 4;
+  const int v_begin = chunk * chunk_keys, v_end = min(v_begin + chunk_keys, keys);
+  if (SHARED && chunk > 0 && v_begin >= keys) return;        // (the merge knows how many there are)
+  const int lane = threadIdx.x, lq = lane & 15, lg = lane >> 4, rows = tokens * a.group;
 
   dec_u4 q[ROWT][D / 32];
+  int token[ROWT], place[ROWT];                              // of a row: its token in the tile, the last row it sees
+  int last = -1, least = INT32_MAX;
 #pragma unroll
   for (int nt = 0; nt < ROWT; ++nt) {
-    const int r = nt * 16 + lq;
-    const uint16_t* src = a.q + t * a.q_token + (int64_t)(kvh * a.group + min(r, a.group - 1)) * a.q_head + lg * 8;
+    const int r = min(nt * 16 + lq, rows - 1), i = SHARED ? r / a.group : 0;
+    token[nt] = i;
+    place[nt] = attend_last(a, t + i);
+    const uint16_t* src = a.q + (t + i) * a.q_token + (int64_t)(kvh * a.group + r - i * a.group) * a.q_head + lg * 8;
 #pragma unroll
-    for (int ks = 0; ks < D / 32; ++ks) q[nt][ks] = r < a.group ? *(const dec_u4*)(src + ks * 32) : dec_u4{0, 0, 0, 0};
+    for (int ks = 0; ks < D / 32; ++ks) q[nt][ks] = nt * 16 + lq < rows ? *(const dec_u4*)(src + ks * 32) : dec_u4{0, 0, 0, 0};
+    last = max(last, place[nt]);
+    least = min(least, place[nt]);
+  }
+  if constexpr (SHARED) {
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+      last = max(last, __shfl_xor(last, o, kWave));
+      least = min(least, __shfl_xor(least, o, kWave));
+    }
   }
   v4f o[ROWT][D / 16];
   float ref[ROWT], l[ROWT];                                  // ref in units of exp2's argument
@@ -504,8 +604,8 @@ __global__ __launch_bounds__(kWave) void block_attention_kernel(AttendArgs a) {
   const uint32_t voff = ring0 + kHalf + (4 * lg + (lq >> 2)) * kRowBytes + (lq & 1) * 8;
   const int kswap = attend_k_swap<D>(lq), vswap = attend_v_swap<D>(4 * lg + (lq >> 2)), vpiece = (lq >> 1) & 1;
   const int32_t* list = a.blocks + ((int64_t)t * a.hkv + kvh) * a.keep;
+  const int2* merged = a.merged + ((int64_t)kvh * a.tokens + local) * a.keep;
   const int32_t* row_pages = a.table + b * a.table_stride;
-  const int v_begin = chunk * a.chunk_keys, v_end = min(v_begin + a.chunk_keys, a.keys);
 
   for (int v0 = v_begin; v0 < v_end; v0 += kAttendSegment) {
     int stages = 0;                                          // up to the last one of which something is seen
@@ -514,12 +614,29 @@ __global__ __launch_bounds__(kWave) void block_attention_kernel(AttendArgs a) {
     for (int u = 0; u < kAttendSegment / 64; ++u) {
       if (u * 64 >= v_end - v0) continue;
       const int v = v0 + u * 64 + lane;
-      const int block = v < v_end ? list[v >> a.page_shift] : -1, in = v & ((1 << a.page_shift) - 1);
+      const int in = v & ((1 << a.page_shift) - 1);
+      int block = -1, bits = 1;
+      if constexpr (SHARED) {
+        if (v < v_end) {
+          const int2 entry = merged[v >> a.page_shift];
+          block = entry.x;
+          bits = entry.y;
+        }
+      } else if (v < v_end) {
+        block = list[v >> a.page_shift];
+      }
       const bool sees = block >= 0 && last >= 0 && block <= last >> a.page_shift && (block << a.page_shift) + in <= last;
       const int page = sees ? min(max(row_pages[block], 0), a.max_pages - 1) : 0;
       row_at[u * 64 + lane] = sees ? 2 * ((int64_t)page * 2 * a.page_elems + (int64_t)a.hkv * D * in) : -1;
       const uint64_t some = __ballot(sees);
-      if (lane < 2) seen_at[u * 2 + lane] = (uint32_t)(some >> (32 * lane));
+      uint64_t all = some;                                   // (shared: seen by all rows)
+      if constexpr (SHARED) {
+        const int row = sees ? (block << a.page_shift) + in : INT32_MAX;
+        place_at[u * 64 + lane] = row;
+        ((uint8_t*)bits_at)[u * 64 + lane] = (uint8_t)bits;
+        all = __ballot(row <= least && bits == (1 << tokens) - 1);
+      }
+      if (lane < 2) seen_at[u * 2 + lane] = (uint32_t)(all >> (32 * lane));
       if (some) stages = u * 2 + (some >> 32 ? 2 : 1);
     }
     __builtin_amdgcn_s_waitcnt(0);                           // rows' offsets and the queries; from here on only copies are counted
@@ -568,6 +685,15 @@ __global__ __launch_bounds__(kWave) void block_attention_kernel(AttendArgs a) {
         const uint2 lo = lds_tr16(va), hi = lds_tr16(va + 16 * kRowBytes);
         vt[mt] = dec_u4{lo.x, lo.y, hi.x, hi.y};
       }
+      dec_i4 places[2] = {};
+      uint32_t bits[2] = {};
+      if (SHARED && seen != ~0u) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          places[h] = *(const dec_i4*)&place_at[st * kAttendKeys + h * 16 + 4 * lg];
+          bits[h] = bits_at[(st * kAttendKeys + h * 16) / 4 + lg];
+        }
+      }
       dec_u4 pb[ROWT], rest[ROWT];
 #pragma unroll
       for (int nt = 0; nt < ROWT; ++nt) {
@@ -576,8 +702,12 @@ __global__ __launch_bounds__(kWave) void block_attention_kernel(AttendArgs a) {
         for (int r = 0; r < 8; ++r) x[r] = s[nt][r >> 2][r & 3] * a.scale_log2;
         if (seen != ~0u) {
 #pragma unroll
-          for (int r = 0; r < 8; ++r)
-            if (!(seen >> ((r >> 2) * 16 + 4 * lg + (r & 3)) & 1)) x[r] = -INFINITY;
+          for (int r = 0; r < 8; ++r) {
+            const int key = (r >> 2) * 16 + 4 * lg + (r & 3);
+            bool there = seen >> key & 1;
+            if constexpr (SHARED) there = places[r >> 2][r & 3] <= place[nt] && (bits[r >> 2] >> (8 * (r & 3) + token[nt]) & 1);
+            if (!there) x[r] = -INFINITY;
+          }
         }
         const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
         if (__any(top > ref[nt] + kSlack)) {                 // (also where the reference is still -inf)
@@ -621,15 +751,16 @@ __global__ __launch_bounds__(kWave) void block_attention_kernel(AttendArgs a) {
     float sum = l[nt] + __shfl_xor(l[nt], 16, kWave);
     sum += __shfl_xor(sum, 32, kWave);
     const int r = nt * 16 + lq;
-    if (r >= a.group) continue;
+    if (r >= rows) continue;
+    const int head = r - token[nt] * a.group;
     if (a.chunks == 1) {
       const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-      uint16_t* dst = a.out + ((int64_t)t * a.hq + kvh * a.group + r) * D + lg * 4;
+      uint16_t* dst = a.out + ((int64_t)(t + token[nt]) * a.hq + kvh * a.group + head) * D + lg * 4;
 #pragma unroll
       for (int mt = 0; mt < D / 16; ++mt)
         *(uint2*)(dst + mt * 16) = make_uint2(pack2<DT>(o[nt][mt][0] * inv, o[nt][mt][1] * inv), pack2<DT>(o[nt][mt][2] * inv, o[nt][mt][3] * inv));
     } else {
-      const int64_t slot = (((int64_t)local * a.hkv + kvh) * a.chunks + chunk) * a.group + r;
+      const int64_t slot = (((int64_t)(local + token[nt]) * a.hkv + kvh) * a.chunks + chunk) * a.group + head;
       float* dst = a.part_o + slot * D + lg * 4;
 #pragma unroll
       for (int mt = 0; mt < D / 16; ++mt) *(v4f*)(dst + mt * 16) = o[nt][mt];
@@ -648,55 +779,92 @@ __global__ __launch_bounds__(256) void block_merge_kernel(AttendArgs a, int64_t 
   const int64_t tk = id / a.group;
   const int t = a.first + (int)(tk / a.hkv), kvh = (int)(tk % a.hkv);
   const int b = a.sequences[t];
-  if (b < 0 || b >= a.batch) return;
   const int64_t slot = tk * a.chunks * a.group + r;
   const float* ml = a.part_ml + slot * 2;
   const float* po = a.part_o + slot * D + (lane % kLanes) * 4;
-  float top = -INFINITY;
-  for (int c = lane; c < a.chunks; c += kWave) top = fmaxf(top, ml[(int64_t)c * a.group * 2]);
+  const int side = lane / kLanes;
+  // the first chunks' parts, and every lane's chunk's reference and sum, on their way before anything is known of them
+  constexpr int kHeld = 16 / kSide;
+  v4f early[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) early[i] = *(const v4f*)(po + (int64_t)min(i * kSide + side, a.chunks - 1) * a.group * D);
+  v2f mine = *(const v2f*)(ml + (int64_t)min(lane, a.chunks - 1) * a.group * 2);
+  if (b < 0 || b >= a.batch) return;
+  int chunks = a.chunks;
+  if (a.share) {
+    const int keys = a.counts[kvh * a.tokens + (t - a.first)] << a.page_shift, chunk_keys = shared_chunk_keys(a, keys);
+    chunks = max(1, (keys + chunk_keys - 1) / chunk_keys);
+  }
+  float top = lane < chunks ? mine[0] : -INFINITY;
+  for (int c = lane + kWave; c < chunks; c += kWave) top = fmaxf(top, ml[(int64_t)c * a.group * 2]);
   top = wave_max(top);
   const float base = top == -INFINITY ? 0.f : top;
   v4f num = {0.f, 0.f, 0.f, 0.f};
   float den = 0.f;
-#pragma unroll 8
-  for (int c = lane / kLanes; c < a.chunks; c += kSide) {
-    const v4f part = *(const v4f*)(po + (int64_t)c * a.group * D);
-    const v2f m = *(const v2f*)(ml + (int64_t)c * a.group * 2);
-    const float w = __builtin_amdgcn_exp2f(m[0] - base);
-    den = fmaf(w, m[1], den);
+  for (int c0 = 0; c0 < chunks; c0 += kWave) {
+    if (c0 > 0) mine = *(const v2f*)(ml + (int64_t)min(c0 + lane, chunks - 1) * a.group * 2);
+    const float weight = c0 + lane < chunks ? __builtin_amdgcn_exp2f(mine[0] - base) : 0.f;
+    den = fmaf(weight, c0 + lane < chunks ? mine[1] : 0.f, den);
+    const int some = min(kWave, chunks - c0);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) num[e] = fmaf(w, part[e], num[e]);
+    for (int i = 0; i < kHeld; ++i) {
+      if (c0 > 0 || i * kSide >= some) break;                // (uniform)
+      const float w = __shfl(weight, i * kSide + side, kWave);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) num[e] = i * kSide + side < some ? fmaf(w, early[i][e], num[e]) : num[e];
+    }
+    for (int c = c0 > 0 ? 0 : kHeld * kSide; c < some; c += 4 * kSide) {
+      v4f part[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) part[i] = *(const v4f*)(po + (int64_t)(c0 + min(c + i * kSide + side, some - 1)) * a.group * D);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int from = c + i * kSide + side;
+        const float w = __shfl(weight, min(from, kWave - 1), kWave);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) num[e] = from < some ? fmaf(w, part[i][e], num[e]) : num[e];
+      }
+    }
   }
+  den = wave_sum(den);
 #pragma unroll
-  for (int s = kLanes; s < kWave; s <<= 1) {
-    den += __shfl_xor(den, s, kWave);
+  for (int s = kLanes; s < kWave; s <<= 1)
 #pragma unroll
     for (int e = 0; e < 4; ++e) num[e] += __shfl_xor(num[e], s, kWave);
-  }
   if (lane >= kLanes) return;
   const float inv = den > 0.f ? 1.f / den : 0.f;
   *(uint2*)(a.out + ((int64_t)t * a.hq + kvh * a.group + r) * D + lane * 4) =
       make_uint2(pack2<DT>(num[0] * inv, num[1] * inv), pack2<DT>(num[2] * inv, num[3] * inv));
 }
 
-// Chunks of a unit's listed rows, as those of few rows over a whole cache; tokens whose partial results are held at a time.
-struct AttendPlan { int chunk_keys, chunks; int64_t tokens; size_t part_o, part_ml, bytes; };
-static AttendPlan attend_plan(int64_t n_tokens, int64_t hq, int64_t hkv, int64_t head_dim, int64_t keys) {
+// Tokens of a sequence that share a unit (1: none do), chunks of a unit's rows, tokens whose partial results are held at a time.
+struct AttendPlan { int share, chunk_keys, chunks; int64_t tokens; size_t part_o, part_ml, merged, counts, bytes; };
+static AttendPlan attend_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64_t hkv, int64_t head_dim, int64_t page_len, int64_t max_blocks, int64_t keep) {
   AttendPlan p{};
-  const int64_t units = n_tokens * hkv;
+  const int64_t group = hq / hkv;
+  p.share = 1;
+  if (n_tokens > batch && max_blocks <= kUnionBlocks)
+    while (p.share < 8 && 2 * p.share * group <= kShareRows) p.share *= 2;
+  // rows of a unit: those of a token, or, of several, as many as lists that agree in most blocks have together
+  const int64_t most = std::min(p.share * keep, std::max(max_blocks, keep)) * page_len, keys = p.share > 1 ? std::min(most, 2 * keep * page_len) : keep * page_len;
+  const int64_t units = std::max<int64_t>(1, n_tokens / p.share) * hkv;
   int64_t per = ((int64_t)(0.65 * std::sqrt((double)units * (double)keys)) + kAttendKeys - 1) / kAttendKeys * kAttendKeys;
-  per = std::min<int64_t>(std::max<int64_t>(per, 64), 384);
+  per = std::min<int64_t>(std::max<int64_t>(per, 64), p.share > 1 ? 256 : 384);
   while (keys > per * 256) per *= 2;
   p.chunk_keys = (int)per;
   p.chunks = (int)((keys + per - 1) / per);
   p.tokens = n_tokens;
+  if (p.chunks > 1) p.tokens = std::min<int64_t>(n_tokens, std::max<int64_t>(64, (1 << 20) / (hq * p.chunks)));      // half a gigabyte at 128 a head
+  const size_t slots = (size_t)p.tokens * hq * p.chunks;
   if (p.chunks > 1) {
-    p.tokens = std::min<int64_t>(n_tokens, std::max<int64_t>(1, (1 << 20) / (hq * p.chunks)));      // half a gigabyte of partial results at 128 a head
-    const size_t slots = (size_t)p.tokens * hq * p.chunks;
     p.part_o = align_up(slots * head_dim * sizeof(float), 256);
     p.part_ml = align_up(slots * 2 * sizeof(float), 256);
   }
-  p.bytes = 256 + p.part_o + p.part_ml;
+  if (p.share > 1) {
+    p.merged = align_up((size_t)p.tokens * hkv * keep * sizeof(int2), 256);
+    p.counts = align_up((size_t)p.tokens * hkv * sizeof(int32_t), 256);
+  }
+  p.bytes = 256 + p.part_o + p.part_ml + p.merged + 2 * p.counts;
   return p;
 }
 
@@ -719,9 +887,14 @@ static void launch_scores(SelectArgs a, int64_t tokens, hipStream_t st) {
 template <int DT, int D>
 static void launch_attend_of(const AttendArgs& a, int64_t tokens, hipStream_t st) {
   const dim3 grid((unsigned)(tokens * a.chunks * a.hkv)), block(kWave);
-  if (a.group <= 16) hipLaunchKernelGGL((block_attention_kernel<DT, D, 1>), grid, block, 0, st, a);
-  else if (a.group <= 32) hipLaunchKernelGGL((block_attention_kernel<DT, D, 2>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((block_attention_kernel<DT, D, 4>), grid, block, 0, st, a);
+  if (a.share) {
+    if (a.share * a.group <= 16) hipLaunchKernelGGL((block_attention_kernel<DT, D, 1, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((block_attention_kernel<DT, D, 2, true>), grid, block, 0, st, a);
+  } else {
+    if (a.group <= 16) hipLaunchKernelGGL((block_attention_kernel<DT, D, 1, false>), grid, block, 0, st, a);
+    else if (a.group <= 32) hipLaunchKernelGGL((block_attention_kernel<DT, D, 2, false>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((block_attention_kernel<DT, D, 4, false>), grid, block, 0, st, a);
+  }
 }
 template <int DT, int D>
 static void launch_block_merge_of(const AttendArgs& a, int64_t tokens, hipStream_t st) {
@@ -841,12 +1014,12 @@ extern "C" int subspec_select_blocks(const void* q, int64_t q_token_stride, int6
   return SUBSPEC_OK;
 }
 
-extern "C" size_t subspec_block_attention_workspace(int64_t n_tokens, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
-                                                    int64_t page_len, int64_t keep) {
-  if (n_tokens < 1 || n_tokens > (1 << 20) || n_kv_heads < 1 || n_q_heads < n_kv_heads || n_q_heads > 1024 || head_dim < 1 || head_dim > 1024 ||
+extern "C" size_t subspec_block_attention_workspace(int64_t batch, int64_t n_tokens, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
+                                                    int64_t page_len, int64_t max_blocks, int64_t keep) {
+  if (batch < 1 || max_blocks < 1 || max_blocks > INT32_MAX || n_tokens < 1 || n_tokens > (1 << 20) || n_kv_heads < 1 || n_q_heads < n_kv_heads || n_q_heads > 1024 || head_dim < 1 || head_dim > 1024 ||
       page_len < 1 || page_len > (1 << 20) || keep < 1 || keep > kMostBlocks || keep * page_len > (1 << 30))
     return 256;
-  return attend_plan(n_tokens, n_q_heads, n_kv_heads, head_dim, keep * page_len).bytes;
+  return attend_plan(batch, n_tokens, n_q_heads, n_kv_heads, head_dim, page_len, most_blocks(page_len, max_blocks, 1ll << 30), keep).bytes;
 }
 
 extern "C" int subspec_block_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* kv_pool_layer, int dtype,
@@ -869,14 +1042,20 @@ extern "C" int subspec_block_attention(const void* q, int64_t q_token_stride, in
   if ((uintptr_t)q % 16 || (uintptr_t)kv_pool_layer % 16 || (uintptr_t)out % 16 || q_token_stride % 8 || q_head_stride % 8 ||
       q_token_stride < 0 || q_head_stride < 0)
     SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: q, the pool and out must be 16-byte aligned, q's strides multiples of 8 elements", what);
-  const AttendPlan p = attend_plan(n_tokens, n_q_heads, n_kv_heads, head_dim, keep * page_len);
+  const AttendPlan p = attend_plan(batch, n_tokens, n_q_heads, n_kv_heads, head_dim, page_len, most_blocks(page_len, max_blocks, 1ll << 30), keep);
   if (p.bytes > 256 && (!workspace || workspace_bytes < p.bytes))
     SUBSPEC_FAIL(SUBSPEC_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the %zu required", what, workspace_bytes, p.bytes);
   if ((uintptr_t)workspace % 16) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
   AttendArgs a;
   a.q = (const uint16_t*)q; a.pool = (const uint16_t*)kv_pool_layer; a.table = block_table; a.blocks = blocks; a.sequences = sequences;
   a.positions = positions; a.out = (uint16_t*)out;
-  a.part_o = (float*)workspace; a.part_ml = (float*)((char*)workspace + p.part_o);
+  char* ws = (char*)workspace;
+  a.part_o = (float*)ws; ws += p.part_o;
+  a.part_ml = (float*)ws; ws += p.part_ml;
+  a.merged = (int2*)ws; ws += p.merged;
+  a.counts = (int32_t*)ws; ws += p.counts;
+  a.leads = (int32_t*)ws;
+  a.share = p.share > 1 ? p.share : 0;
   a.q_token = q_token_stride; a.q_head = q_head_stride; a.table_stride = table_stride; a.page_elems = page_len * n_kv_heads * head_dim;
   a.batch = (int)batch; a.hq = (int)n_q_heads; a.hkv = (int)n_kv_heads; a.group = (int)(n_q_heads / n_kv_heads);
   a.page_shift = block_shift_of(page_len); a.max_pages = (int)max_pages; a.keep = (int)keep;
@@ -889,6 +1068,8 @@ extern "C" int subspec_block_attention(const void* q, int64_t q_token_stride, in
   for (int64_t first = 0; first < n_tokens; first += p.tokens) {
     const int64_t some = std::min(p.tokens, n_tokens - first);
     a.first = (int)first;
+    a.tokens = (int)some;
+    if (a.share) hipLaunchKernelGGL(block_union_kernel, dim3((unsigned)(some * n_kv_heads)), dim3(kUnionThreads), 0, st, a);
     {
       DominantKernelTimer timer(st);
       if (dtype == SUBSPEC_BF16) {

@@ -709,7 +709,7 @@ def block_attention(q: torch.Tensor, pool_layer: torch.Tensor, block_table: torc
         same = q.is_contiguous() and out.data_ptr() == q.data_ptr()
         _apart("block_attention", [("out", out)], [("the pool", pool_layer), ("block_table", block_table), ("blocks", blocks),
                                                    ("sequences", sequences), ("positions", positions)] + ([] if same else [("q", q)]))
-    need = L.lib().subspec_block_attention_workspace(T, Hq, Hkv, D, page_len, keep)
+    need = L.lib().subspec_block_attention_workspace(block_table.shape[0], T, Hq, Hkv, D, page_len, max_blocks, keep)
     workspace, ws_ptr, ws_bytes = _scratch(workspace, need, dev, "block_attention")
     _call(dev, "subspec_block_attention", q.data_ptr(), q.stride(0), q.stride(1), pool_layer.data_ptr(), _dtype_code(q), max_pages, page_len,
           block_table.data_ptr(), max_blocks, stride, blocks.data_ptr(), keep, sequences.data_ptr(), positions.data_ptr(), block_table.shape[0], T,

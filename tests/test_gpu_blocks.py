@@ -500,3 +500,38 @@ def test_refusals():
     shifted = torch.zeros(3, 4, 64, dtype=torch.bfloat16, device=DEV)
     with pytest.raises(ValueError):
         attend(q=shifted[:2], out=shifted.view(-1)[256:768].view(2, 256))         # the outputs over part of q
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,P,keep", [(8, 8, 64, 4, 9), (28, 4, 128, 16, 4), (16, 2, 64, 1, 70), (32, 2, 128, 8, 5), (20, 1, 64, 8, 5)])
+def test_neighbours_of_a_sequence_read_their_blocks_together(Hq, Hkv, D, P, keep):
+    """Runs of every length beside each other, sequences in turn, tokens of nobody between; lists that agree, in part, or not at all."""
+    print("together", Hq, Hkv, D, P, keep, flush=True)
+    g = torch.Generator().manual_seed(keep)
+    lens = [(260, 0), (150, 0), (77, 0)]
+    _, pool, table, _, _ = _cache(g, lens, P, Hq, Hkv, D, torch.float16)
+    seq = [0] * 5 + [1] * 9 + [0, 1, 0, 1, -1, -1, 2, 2, 7, 2] + [2] * 70 + [0] * 3
+    pos = [int(torch.randint(-1, lens[b][0], (1,), generator=g)) if 0 <= b < 3 else 5 for b in seq]
+    q = (torch.randn(len(seq), Hq, D, generator=g) * 2).half()
+    base = torch.randn(3, Hkv, 260, generator=g)
+    blocks = []
+    for t, b in enumerate(seq):
+        own = max(pos[t], 0) // P
+        noise = torch.randn(Hkv, own + 1, generator=g) * (0.0, 0.3, 5.0)[t % 3]
+        want = base[max(b, 0) % 3, :, :own + 1] + noise
+        some = want.topk(min(keep, own + 1), 1).indices
+        blocks.append(torch.nn.functional.pad(some, (0, keep - some.shape[1]), value=-1).tolist())
+    clean = [[[j if j >= 0 and pos[t] >= 0 else -1 for j in row] for row in heads] for t, heads in enumerate(blocks)]
+    want, weight, worst = ok.attention(q, pool, table, clean, seq, pos)
+    mine = torch.tensor([0 <= b < 3 for b in seq])
+    out = torch.full((len(seq), Hq * D), 7.0, dtype=torch.float16, device=DEV)
+    got = ops.block_attention(q.to(DEV), pool.to(DEV), _i32(table), _i32(blocks), _i32(seq), _i32(pos), out=out).cpu()
+    assert got[~mine].eq(7.0).all()
+    off = (got.double().view_as(want) - want)[mine].abs() / _tolerance(want, weight, worst, torch.float16, D, keep * P, 6.0)[mine]
+    assert off.max() <= 1, float(off.max())
+    again = ops.block_attention(q.to(DEV), pool.to(DEV), _i32(table), _i32(blocks), _i32(seq), _i32(pos))
+    assert torch.equal(again.cpu()[mine], got[mine])
+    for t in (0, 4, 13, 20, 24, 93, 96):                           # a token by itself: the same but for the order of its sums
+        one = ops.block_attention(q[t:t + 1].to(DEV), pool.to(DEV), _i32(table), _i32(blocks[t:t + 1]), _i32(seq[t:t + 1]), _i32(pos[t:t + 1]))
+        if mine[t]:
+            off = (one.cpu().double().view(Hq, D) - want[t]).abs() / _tolerance(want, weight, worst, torch.float16, D, keep * P, 6.0)[t]
+            assert off.max() <= 1, (t, float(off.max()))
