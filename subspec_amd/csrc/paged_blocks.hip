@@ -90,6 +90,46 @@ __global__ __launch_bounds__(kBoundsThreads) void page_bounds_kernel(BoundsArgs 
   }
 }
 
+// Sums up to each lane, and a wavefront's largest, by lanes that neighbour in a row of sixteen and the rows' last ones: a dozen instructions, where six exchanges
+// through LDS one after the other take 0.3 us.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t shifted_in(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ uint32_t lanes_upto(uint32_t v) {
+  v += shifted_in<0x111, 0xf>(v);
+  v += shifted_in<0x112, 0xf>(v);
+  v += shifted_in<0x114, 0xf>(v);
+  v += shifted_in<0x118, 0xf>(v);
+  v += shifted_in<0x142, 0xa>(v);
+  v += shifted_in<0x143, 0xc>(v);
+  return v;
+}
+__device__ __forceinline__ uint32_t lanes_largest(uint32_t v) {
+  v = max(v, shifted_in<0x111, 0xf>(v));
+  v = max(v, shifted_in<0x112, 0xf>(v));
+  v = max(v, shifted_in<0x114, 0xf>(v));
+  v = max(v, shifted_in<0x118, 0xf>(v));
+  v = max(v, shifted_in<0x142, 0xa>(v));
+  v = max(v, shifted_in<0x143, 0xc>(v));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, kWave - 1);
+}
+
+// Tiles of up to `share` neighbouring tokens of one sequence, from the first of a run of them on: how many token t is the first of (0: it lies in another's
+// tile, or its sequence is below 0).  Every wavefront looks for itself; tokens outside [first, end) are nobody's neighbours.
+struct TokenTile { int sequence, tokens; };
+__device__ __forceinline__ TokenTile token_tile(const int32_t* sequences, int t, int first, int end, int share) {
+  const int lane = threadIdx.x & (kWave - 1), b = sequences[t], next = t + 1 + lane;
+  const uint64_t ends = __ballot(next >= end || sequences[min(next, end - 1)] != b);
+  int behind = 0;                                            // neighbours of the sequence before this token
+  for (;;) {
+    const int other = t - 1 - behind - lane;
+    const uint64_t others = __ballot(other < first || sequences[max(other, 0)] != b);
+    behind += others ? __ffsll((unsigned long long)others) - 1 : kWave;
+    if (others) break;
+  }
+  if (b < 0 || behind % share) return TokenTile{b, 0};
+  return TokenTile{b, min(share, ends ? __ffsll((unsigned long long)ends) : kWave)};
+}
+
 // ---------------------------------------------------------------------------------------------------------------- scores
 // s_j = sum over the KV head's query heads g and dimensions d of max(q_gd low_jd, q_gd high_jd), which no sum of the heads' scores of a key of block j
 // exceeds; with A_d = sum_g max(q_gd, 0) and B_d = sum_g min(q_gd, 0) it is sum_d A_d high_jd + B_d low_jd.  In 64 bits: which block comes out ahead must not
@@ -103,7 +143,7 @@ struct SelectArgs {
   int32_t* blocks;               // [tokens][n_kv_heads][keep]
   double* scores;                // [token - first][n_kv_heads][most]
   int64_t q_token, q_head, table_stride, most;
-  int batch, n_tokens, first, hkv, group, page_shift, max_pages, keep, recent, last_row, span, spans;
+  int batch, first, tokens, hkv, group, page_shift, max_pages, keep, recent, last_row, span, spans;
 };
 // Blocks that a token sees (0: none), and of these the first so many that compete.
 struct TokenBlocks { int seen, scored; };
@@ -113,9 +153,9 @@ __device__ __forceinline__ TokenBlocks token_blocks(const SelectArgs& a, int b, 
   const int seen = (last >> a.page_shift) + 1;
   return TokenBlocks{seen, seen > a.keep ? seen - a.recent : 0};
 }
-constexpr int kScoreTokens = 4;           // tokens of a sequence that share a reading of the bounds
+constexpr int kScoreTokens = 8;           // tokens of a sequence that share a reading of the bounds
 constexpr int kScoreThreads = 256;
-constexpr int kScoreDepth = 8;            // readings of a wavefront
+constexpr int kSharedDepth = 2;           // readings of a wavefront then
 
 // a double from another lane of sixteen (a DPP control)
 template <int CTRL>
@@ -150,106 +190,166 @@ __device__ __forceinline__ void sum_eight(double (&v)[8], int lane, double* out)
   }
 }
 
-// A workgroup takes `span` blocks of (token, KV head), a wavefront a quarter of them: D / 8 lanes a block, all requests of a wavefront under way
-// before the first score.  Meanwhile the four of them add the query heads up.  A token whose neighbour before it is of the same sequence leaves its scores to the
-// workgroup of that one, up to TOKENS of them: the bounds are read once for all.
-template <int DT, int D, int TOKENS>
+// The query heads of `tokens` tokens added up by a workgroup, into LDS: (of high, of low) of each.  A thread has DIMS neighbouring dimensions; where there are more
+// threads than these, every team of them has a part of the heads, and the teams' sums are added in their order.  Ends with a barrier.
+template <int DT, int D, int TOKENS, int THREADS, int DIMS>
+__device__ __forceinline__ void score_weights(const SelectArgs& a, int t, int tokens, int kvh, double* weight) {
+  constexpr int kTeam = TOKENS * D / DIMS, kTeams = THREADS / kTeam;
+  const int team = threadIdx.x / kTeam, k = threadIdx.x / (D / DIMS) % TOKENS, d = threadIdx.x % (D / DIMS) * DIMS;
+  double up[DIMS], down[DIMS];
+#pragma unroll
+  for (int e = 0; e < DIMS; ++e) up[e] = down[e] = 0.0;
+  const uint16_t* q = a.q + (t + min(k, tokens - 1)) * a.q_token + (int64_t)kvh * a.group * a.q_head + d;
+#pragma unroll 4
+  for (int g = team; g < a.group; g += kTeams) {
+    const uint32_t* src = (const uint32_t*)(q + g * a.q_head);
+#pragma unroll
+    for (int p = 0; p < DIMS / 2; ++p) {
+      float x[2];
+      unpack2<DT>(src[p], x);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        // (a NaN goes into both: its blocks all score NaN)
+        up[2 * p + e] += x[e] < 0.f ? 0.0 : (double)x[e];
+        down[2 * p + e] += x[e] > 0.f ? 0.0 : (double)x[e];
+      }
+    }
+  }
+  double* mine = weight + ((team * TOKENS + k) * 2) * D + d;
+#pragma unroll
+  for (int e = 0; e < DIMS; ++e) {
+    mine[e] = up[e];
+    mine[D + e] = down[e];
+  }
+  __syncthreads();
+  if constexpr (kTeams > 1) {
+    const int teams = min(kTeams, a.group);
+    for (int i = threadIdx.x; i < TOKENS * 2 * D; i += THREADS) {
+      double sum = weight[i];
+      for (int m = 1; m < teams; ++m) sum += weight[m * TOKENS * 2 * D + i];
+      weight[i] = sum;
+    }
+    __syncthreads();
+  }
+}
+// Bounds of DEPTH * kAtOnce blocks from j0 on (below j1; past it the last one again), all asked for at once: 16-byte pieces of `low` and `high` a lane
+template <int D, int DEPTH>
+__device__ __forceinline__ void load_bounds(const SelectArgs& a, int b, int kvh, int j0, int j1, dec_u4* low, dec_u4* high) {
+  constexpr int kLanes = D / 8, kAtOnce = kWave / kLanes;
+  static_assert(DEPTH * kAtOnce <= kWave, "a lane holds a page number");
+  const int lane = threadIdx.x & (kWave - 1);
+  const int page_of = min(max(a.table[b * a.table_stride + min(j0 + lane, j1 - 1)], 0), a.max_pages - 1);
+  const dec_u4* bounds = (const dec_u4*)(a.bounds + (int64_t)kvh * 2 * D) + lane % kLanes;
+#pragma unroll
+  for (int i = 0; i < DEPTH; ++i) {
+    const dec_u4* src = bounds + (int64_t)__shfl(page_of, i * kAtOnce + lane / kLanes, kWave) * a.hkv * 2 * kLanes;
+    low[i] = src[0];
+    high[i] = src[kLanes];
+  }
+}
+__device__ __forceinline__ double score_of(double s) { return s != s ? INFINITY : s; }
+
+// A workgroup takes `span` blocks of (token, KV head), a wavefront a quarter of them: D / 8 lanes a block, all requests of a wavefront under way before
+// the first score; meanwhile the four of them add the query heads up.
+template <int DT, int D>
 __global__ __launch_bounds__(kScoreThreads) void block_score_kernel(SelectArgs a) {
-  constexpr int kLanes = D / 8, kAtOnce = kWave / kLanes, kTurn = kAtOnce * kScoreDepth, kTeams = kScoreThreads / (TOKENS * kLanes);
-  static_assert(kTurn <= kWave, "a lane holds a page number of a turn");
-  __shared__ __attribute__((aligned(16))) double weight[kTeams][TOKENS][2][D];        // (of high, of low), a part of the heads each
+  constexpr int kLanes = D / 8, kAtOnce = kWave / kLanes, kDepth = 8;
+  __shared__ __attribute__((aligned(16))) double weight[kScoreThreads / (D / 2) * 2 * D];
+  const uint32_t unit = blockIdx.x;
+  const int kvh = (int)(unit % (uint32_t)a.hkv), span = (int)(unit / (uint32_t)a.hkv % (uint32_t)a.spans);
+  const int local = (int)(unit / (uint32_t)a.hkv / (uint32_t)a.spans), t = a.first + local, b = a.sequences[t];
+  const int most = token_blocks(a, b, a.positions[t]).scored;
+  if (span * a.span >= most) return;                         // (the whole workgroup)
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1), part = lane % kLanes, which = lane / kLanes;
+  const int j0 = span * a.span + wave * kAtOnce * kDepth, j1 = min(j0 + kAtOnce * kDepth, most);
+  dec_u4 low[kDepth], high[kDepth];
+  if (j0 < j1) load_bounds<D, kDepth>(a, b, kvh, j0, j1, low, high);
+  score_weights<DT, D, 1, kScoreThreads, 2>(a, t, 1, kvh, weight);
+  if (j0 >= j1) return;
+  double up[8], down[8], s[kDepth], out[2];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    up[e] = weight[part * 8 + e];
+    down[e] = weight[D + part * 8 + e];
+  }
+#pragma unroll
+  for (int i = 0; i < kDepth; ++i) {
+    float l[8], h[8];
+    unpack8<DT>(low[i], l);
+    unpack8<DT>(high[i], h);
+    s[i] = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[i] = fma(up[e], (double)h[e], fma(down[e], (double)l[e], s[i]));
+  }
+  sum_eight<kLanes>(s, lane, out);
+  if (part >= 4) return;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const int j = j0 + (4 * m + part) * kAtOnce + which;
+    if (j < j1) a.scores[((int64_t)local * a.hkv + kvh) * a.most + j] = score_of(out[m]);
+  }
+}
+
+// The same for up to kScoreTokens neighbouring tokens of one sequence: the bounds are read and converted once for all, the weights come out of LDS again
+// for every block.  A token that has a neighbour of its sequence before it is left to the workgroup of the tile's first one.
+// (72 drafts of 16 sequences, 32 : 8 heads, up to 255 blocks: a conversion a token 17.4 us.)
+template <int DT, int D>
+__global__ __launch_bounds__(kScoreThreads) void block_score_shared_kernel(SelectArgs a) {
+  constexpr int kLanes = D / 8, kAtOnce = kWave / kLanes;
+  __shared__ __attribute__((aligned(16))) double weight[kScoreThreads / (D / 4) * 2 * D];
   const uint32_t unit = blockIdx.x;
   const int kvh = (int)(unit % (uint32_t)a.hkv), span = (int)(unit / (uint32_t)a.hkv % (uint32_t)a.spans);
   const int local = (int)(unit / (uint32_t)a.hkv / (uint32_t)a.spans), t = a.first + local;
+  const TokenTile tile = token_tile(a.sequences, t, a.first, a.first + a.tokens, kScoreTokens);
+  if (!tile.tokens) return;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1), part = lane % kLanes, which = lane / kLanes;
-  // the token before this one and those behind it, in one trip to memory
-  const int near = min(max(t - 1 + lane, 0), a.n_tokens - 1);
-  const int sequence_of = a.sequences[near], position_of = a.positions[near];
-  const int b = __builtin_amdgcn_readlane(sequence_of, 1);
-  if (TOKENS > 1 && local % TOKENS != 0 && __builtin_amdgcn_readlane(sequence_of, 0) == b) return;
-  int scored[TOKENS], most = 0, tokens = 0;
-#pragma unroll
-  for (int k = 0; k < TOKENS; ++k) {
-    scored[k] = 0;
-    if (k > 0 && (tokens < k || (local + k) % TOKENS == 0 || t + k >= a.n_tokens || __builtin_amdgcn_readlane(sequence_of, 1 + k) != b)) continue;
-    tokens = k + 1;
-    scored[k] = token_blocks(a, b, __builtin_amdgcn_readlane(position_of, 1 + k)).scored;
-    most = max(most, scored[k]);
-  }
+  // a lane has a token's number of blocks
+  const int mine = lane < tile.tokens ? token_blocks(a, tile.sequence, a.positions[t + lane]).scored : 0;
+  const int most = (int)lanes_largest((uint32_t)mine);
   if (span * a.span >= most) return;                         // (the whole workgroup)
-  const int j0 = span * a.span + wave * kTurn, j1 = min(j0 + kTurn, most);
-  dec_u4 low[kScoreDepth], high[kScoreDepth];
-  if (j0 < j1) {
-    const int page_of = min(max(a.table[b * a.table_stride + min(j0 + lane, j1 - 1)], 0), a.max_pages - 1);
-    const dec_u4* bounds = (const dec_u4*)(a.bounds + (int64_t)kvh * 2 * D) + part;
-#pragma unroll
-    for (int i = 0; i < kScoreDepth; ++i) {
-      const dec_u4* src = bounds + (int64_t)__shfl(page_of, i * kAtOnce + which, kWave) * a.hkv * 2 * kLanes;
-      low[i] = src[0];
-      high[i] = src[kLanes];
-    }
-  }
-  {
-    const int team = threadIdx.x / (TOKENS * kLanes), k = threadIdx.x / kLanes % TOKENS, piece = threadIdx.x % kLanes;
-    double up[8], down[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) up[e] = down[e] = 0.0;
-    const uint16_t* q = a.q + (t + min(k, tokens - 1)) * a.q_token + (int64_t)kvh * a.group * a.q_head + piece * 8;
-#pragma unroll 2
-    for (int g = team; g < a.group; g += kTeams) {
-      float x[8];
-      unpack8<DT>(*(const dec_u4*)(q + g * a.q_head), x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        // (a NaN goes into both: its blocks all score NaN)
-        up[e] += x[e] < 0.f ? 0.0 : (double)x[e];
-        down[e] += x[e] > 0.f ? 0.0 : (double)x[e];
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      weight[team][k][0][piece * 8 + e] = up[e];
-      weight[team][k][1][piece * 8 + e] = down[e];
-    }
-  }
-  __syncthreads();
-  const int teams = min(kTeams, a.group);
-  double* flat = &weight[0][0][0][0];
-  for (int i = threadIdx.x; i < TOKENS * 2 * D; i += kScoreThreads) {
-    double sum = flat[i];
-    for (int m = 1; m < teams; ++m) sum += flat[m * TOKENS * 2 * D + i];
-    flat[i] = sum;
-  }
-  __syncthreads();
+  const int j0 = span * a.span + wave * kAtOnce * kSharedDepth, j1 = min(j0 + kAtOnce * kSharedDepth, most);
+  dec_u4 low[kSharedDepth], high[kSharedDepth];
+  if (j0 < j1) load_bounds<D, kSharedDepth>(a, tile.sequence, kvh, j0, j1, low, high);
+  score_weights<DT, D, kScoreTokens, kScoreThreads, 4>(a, t, tile.tokens, kvh, weight);
   if (j0 >= j1) return;
-#pragma unroll 1
-  for (int k = 0; k < tokens; ++k) {
-    double up[8], down[8], s[kScoreDepth], out[2];
+  double low_of[kSharedDepth][8], high_of[kSharedDepth][8];
+#pragma unroll
+  for (int i = 0; i < kSharedDepth; ++i) {
+    float l[8], h[8];
+    unpack8<DT>(low[i], l);
+    unpack8<DT>(high[i], h);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      up[e] = weight[0][k][0][part * 8 + e];
-      down[e] = weight[0][k][1][part * 8 + e];
+      low_of[i][e] = (double)l[e];
+      high_of[i][e] = (double)h[e];
     }
+  }
+  constexpr int kAtOnceTokens = 8 / kSharedDepth;             // that make eight sums
 #pragma unroll
-    for (int i = 0; i < kScoreDepth; ++i) {
-      if constexpr (TOKENS > 1) asm("" : "+v"(low[i]), "+v"(high[i]));      // (128 converted numbers kept for the next token are more registers than there are)
-      float l[8], h[8];
-      unpack8<DT>(low[i], l);
-      unpack8<DT>(high[i], h);
-      s[i] = 0.0;
+  for (int k0 = 0; k0 < kScoreTokens; k0 += kAtOnceTokens) {
+    if (k0 >= tile.tokens) break;
+    double s[8], out[2];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[i] = fma(up[e], (double)h[e], fma(down[e], (double)l[e], s[i]));
+    for (int k = 0; k < kAtOnceTokens; ++k) {
+      // (of a token that is not there: what the last one's queries gave once more, and nobody takes it)
+      const double* of = weight + (k0 + k) * 2 * D + part * 8;
+#pragma unroll
+      for (int i = 0; i < kSharedDepth; ++i) {
+        double above = 0.0, below = 0.0;                      // (two chains of sums: a wavefront has few others to wait beside)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          above = fma(of[e], high_of[i][e], above);
+          below = fma(of[D + e], low_of[i][e], below);
+        }
+        s[k * kSharedDepth + i] = above + below;
+      }
     }
     sum_eight<kLanes>(s, lane, out);
-    if (part < 4) {
-      int n = scored[0];
 #pragma unroll
-      for (int m = 1; m < TOKENS; ++m) n = k == m ? scored[m] : n;
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const int j = j0 + (4 * m + part) * kAtOnce + which;
-        if (j < min(j1, n)) a.scores[((int64_t)(local + k) * a.hkv + kvh) * a.most + j] = out[m] != out[m] ? INFINITY : out[m];
-      }
+    for (int m = 0; m < 2; ++m) {
+      const int v = 4 * m + part, k = k0 + v / kSharedDepth, j = j0 + v % kSharedDepth * kAtOnce + which;
+      const int n = __shfl(mine, k & 7, kWave);
+      if (part < 4 && j < min(j1, n)) a.scores[((int64_t)(local + k) * a.hkv + kvh) * a.most + j] = score_of(out[m]);
     }
   }
 }
@@ -258,7 +358,6 @@ __global__ __launch_bounds__(kScoreThreads) void block_score_kernel(SelectArgs a
 // The keep - recent blocks of largest score, equal ones from the lowest on, without sorting: the scores as ordered whole numbers, and the digits (eleven bits at
 // a time, from the first that differs) of the smallest that stays; the few entries that share them are ranked one by one.  What stays is a bit each, and the
 // bits in order are the list.
-constexpr int kSelectThreads = 512;
 constexpr int kMostBlocks = 1 << 17;
 constexpr int kDigits = 2048;
 constexpr int kHeld = 8;                 // scores of a thread that stay in registers
@@ -268,72 +367,72 @@ __device__ __forceinline__ uint64_t score_key(double s) {             // ascendi
   return u >> 63 ? ~u : u | 1ull << 63;
 }
 
-__global__ __launch_bounds__(kSelectThreads) void block_select_kernel(SelectArgs a) {
-  constexpr int kWaves = kSelectThreads / kWave;
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void block_select_kernel(SelectArgs a) {
+  constexpr int kWaves = THREADS / kWave;
   __shared__ uint64_t stays[kMostBlocks / 64];
   __shared__ uint64_t even[kMostBlocks / 64];          // equal to the smallest that stays, where too many are
   __shared__ uint32_t digits[kDigits];
   __shared__ uint64_t list[kRanked];
   __shared__ int list_at[kRanked];
-  __shared__ uint64_t lows[kWaves], highs[kWaves];
+  __shared__ uint32_t lows[kWaves], highs[kWaves];
   __shared__ uint32_t counts[kWaves];
   __shared__ int n_list, digit_at;
   __shared__ uint32_t above_at;
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid & (kWave - 1);
   const int local = blockIdx.x / a.hkv, kvh = blockIdx.x % a.hkv, t = a.first + local;
   int32_t* out = a.blocks + ((int64_t)t * a.hkv + kvh) * a.keep;
+  const double* scores = a.scores + ((int64_t)local * a.hkv + kvh) * a.most;
+  double early[kHeld];                                  // asked for before it is known how many there are
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) early[i] = i * THREADS < a.most ? scores[min((int64_t)tid + i * THREADS, a.most - 1)] : 0.0;
   const TokenBlocks tb = token_blocks(a, a.sequences[t], a.positions[t]);
   if (tb.seen <= a.keep) {
-    for (int i = tid; i < a.keep; i += kSelectThreads) out[i] = i < tb.seen ? i : -1;
+    for (int i = tid; i < a.keep; i += THREADS) out[i] = i < tb.seen ? i : -1;
     return;
   }
   const int n = tb.scored;
   int need = a.keep - a.recent;
-  for (int i = tid; i < a.recent; i += kSelectThreads) out[need + i] = n + i;
+  for (int i = tid; i < a.recent; i += THREADS) out[need + i] = n + i;
   if (need == 0) return;
-  const double* scores = a.scores + ((int64_t)local * a.hkv + kvh) * a.most;
   uint64_t held[kHeld];
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-    const int j = tid + i * kSelectThreads;
-    held[i] = j < n ? score_key(scores[j]) : 0;
-  }
+  for (int i = 0; i < kHeld; ++i) held[i] = score_key(early[i]);
   // f(key, j, whether there is one) for all entries, every wavefront's lanes together
   auto each = [&](auto f) {
 #pragma unroll
     for (int i = 0; i < kHeld; ++i)
-      if (i * kSelectThreads < n) f(held[i], tid + i * kSelectThreads, tid + i * kSelectThreads < n);
-    for (int j0 = kHeld * kSelectThreads; j0 < n; j0 += kSelectThreads) {
+      if (i * THREADS < n) f(held[i], tid + i * THREADS, tid + i * THREADS < n);
+    for (int j0 = kHeld * THREADS; j0 < n; j0 += THREADS) {
       const int j = j0 + tid;
       f(j < n ? score_key(scores[j]) : 0, j, j < n);
     }
   };
-  uint64_t low = ~0ull, high = 0;
+  // (the keys' upper halves say well enough from which bit on they agree)
+  uint32_t low = 0, high = 0;                            // (of the complements, so that both are largest ones)
   each([&](uint64_t key, int, bool there) {
     if (!there) return;
-    low = min(low, key);
-    high = max(high, key);
+    low = max(low, ~(uint32_t)(key >> 32));
+    high = max(high, (uint32_t)(key >> 32));
   });
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    low = min(low, (uint64_t)__shfl_xor((unsigned long long)low, o, kWave));
-    high = max(high, (uint64_t)__shfl_xor((unsigned long long)high, o, kWave));
-  }
+  low = lanes_largest(low);
+  high = lanes_largest(high);
   if (lane == 0) {
     lows[wave] = low;
     highs[wave] = high;
   }
-  for (int i = tid; i < kDigits; i += kSelectThreads) digits[i] = 0;
+  for (int i = tid; i < kDigits; i += THREADS) digits[i] = 0;
   if (tid == 0) n_list = 0;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    low = min(low, lows[w]);
+    low = max(low, lows[w]);
     high = max(high, highs[w]);
   }
-  int top = 64 - __clzll((long long)((low ^ high) | 1));      // bits from here on agree in all entries
+  low = ~low;
+  int top = 32 + (low == high ? 0 : 32 - __clz((int)(low ^ high)));      // bits from here on agree in all entries
   int shift = max(0, top - 11);
-  uint64_t prefix = top >= 64 ? 0 : low >> top << top;
+  uint64_t prefix = top >= 64 ? 0 : (uint64_t)low << 32 >> top << top;
   // each turn: of the entries that agree with `prefix` from `top` on, the digit that the last one to stay has
   int in_digit = 0;
   for (;;) {
@@ -342,16 +441,11 @@ __global__ __launch_bounds__(kSelectThreads) void block_select_kernel(SelectArgs
       if (there && mine(key)) atomicAdd(&digits[(int)(key >> shift) & (kDigits - 1)], 1u);
     });
     __syncthreads();
-    constexpr int kEach = kDigits / kSelectThreads;             // digits from the largest down: thread 0 has the largest ones
+    constexpr int kEach = kDigits / THREADS;             // digits from the largest down: thread 0 has the largest ones
     uint32_t mine_n = 0, of[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) mine_n += of[i] = digits[kDigits - 1 - (tid * kEach + i)];
-    uint32_t upto = mine_n;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      const uint32_t u = __shfl_up(upto, o, kWave);
-      if (lane >= o) upto += u;
-    }
+    const uint32_t upto = lanes_upto(mine_n);
     if (lane == kWave - 1) counts[wave] = upto;
     __syncthreads();
     uint32_t before = upto - mine_n;
@@ -376,7 +470,7 @@ __global__ __launch_bounds__(kSelectThreads) void block_select_kernel(SelectArgs
     __syncthreads();
     if (in_digit == need || in_digit <= kRanked || top == 0) break;
     shift = max(0, top - 11);
-    for (int i = tid; i < kDigits; i += kSelectThreads) digits[i] = 0;
+    for (int i = tid; i < kDigits; i += THREADS) digits[i] = 0;
     __syncthreads();
   }
   // larger ones stay; of those that agree with the prefix all, or the `need` first in order
@@ -405,14 +499,9 @@ __global__ __launch_bounds__(kSelectThreads) void block_select_kernel(SelectArgs
     __syncthreads();
   }
   // a thread takes consecutive words
-  const int words = (n + 63) / 64, per = (words + kSelectThreads - 1) / kSelectThreads, w0 = tid * per, w1 = min(w0 + per, words);
+  const int words = (n + 63) / 64, per = (words + THREADS - 1) / THREADS, w0 = tid * per, w1 = min(w0 + per, words);
   auto before_of = [&](uint32_t v) {
-    uint32_t upto = v;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      const uint32_t u = __shfl_up(upto, o, kWave);
-      if (lane >= o) upto += u;
-    }
+    const uint32_t upto = lanes_upto(v);
     if (lane == kWave - 1) counts[wave] = upto;
     __syncthreads();
     uint32_t before = upto - v;
@@ -482,22 +571,13 @@ __global__ __launch_bounds__(kUnionThreads) void block_union_kernel(AttendArgs a
   __shared__ uint32_t marks[kUnionBlocks / 4];
   __shared__ int sums[kUnionThreads / kWave];
   const int local = blockIdx.x / a.hkv, kvh = blockIdx.x % a.hkv, t = a.first + local, tid = threadIdx.x, lane = tid & (kWave - 1);
-  const int b = a.sequences[t], at = kvh * a.tokens + local;
-  const int end = a.first + a.tokens;
-  int behind = 0;                                            // neighbours of the sequence before this token
-  for (;;) {
-    const int other = t - 1 - behind - lane;
-    const uint64_t others = __ballot(other < a.first || a.sequences[max(other, 0)] != b);
-    behind += others ? __ffsll((unsigned long long)others) - 1 : kWave;
-    if (others) break;
-  }
-  if (b < 0 || b >= a.batch || behind % a.share) {           // (the whole workgroup)
+  const int at = kvh * a.tokens + local;
+  const TokenTile tile = token_tile(a.sequences, t, a.first, a.first + a.tokens, a.share);
+  if (tile.sequence >= a.batch || tile.tokens == 0) {        // (the whole workgroup)
     if (tid == 0) a.leads[at] = 0;
     return;
   }
-  const int other = t + 1 + lane;
-  const uint64_t others = __ballot(other >= end || a.sequences[min(other, end - 1)] != b);
-  const int tokens = min(a.share, others ? __ffsll((unsigned long long)others) : kWave);
+  const int tokens = tile.tokens;
   int most = 0;
   for (int i = 0; i < tokens; ++i) most = max(most, (attend_last(a, t + i) >> a.page_shift) + 1);
   const int words = (most + 3) / 4;
@@ -514,12 +594,7 @@ __global__ __launch_bounds__(kUnionThreads) void block_union_kernel(AttendArgs a
   for (int w = w0; w < w1; ++w)
 #pragma unroll
     for (int k = 0; k < 4; ++k) mine += (marks[w] >> 8 * k & 0xff) != 0;
-  int upto = mine;
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int u = __shfl_up(upto, o, kWave);
-    if (lane >= o) upto += u;
-  }
+  const int upto = (int)lanes_upto((uint32_t)mine);
   if (lane == kWave - 1) sums[tid / kWave] = upto;
   __syncthreads();
   int before = upto - mine, count = 0;
@@ -876,12 +951,13 @@ static int64_t select_tokens(int64_t n_tokens, int64_t hkv, int64_t most) {
 
 // More tokens than sequences: some have several, which share readings.
 template <int DT, int D>
-static void launch_scores(SelectArgs a, int64_t tokens, hipStream_t st) {
-  a.span = kScoreThreads / (D / 8) * kScoreDepth;
+static void launch_scores(SelectArgs a, hipStream_t st) {
+  const bool shared = a.tokens > a.batch;
+  a.span = kScoreThreads / (D / 8) * (shared ? kSharedDepth : 8);
   a.spans = (int)((a.most + a.span - 1) / a.span);
-  const dim3 grid((unsigned)(tokens * a.hkv * a.spans)), block(kScoreThreads);
-  if (tokens > a.batch) hipLaunchKernelGGL((block_score_kernel<DT, D, kScoreTokens>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((block_score_kernel<DT, D, 1>), grid, block, 0, st, a);
+  const dim3 grid((unsigned)((int64_t)a.tokens * a.hkv * a.spans)), block(kScoreThreads);
+  if (shared) hipLaunchKernelGGL((block_score_shared_kernel<DT, D>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((block_score_kernel<DT, D>), grid, block, 0, st, a);
 }
 
 template <int DT, int D>
@@ -990,7 +1066,7 @@ extern "C" int subspec_select_blocks(const void* q, int64_t q_token_stride, int6
   a.q = (const uint16_t*)q; a.bounds = (const uint16_t*)bounds; a.table = block_table; a.sequences = sequences; a.positions = positions;
   a.blocks = blocks; a.scores = (double*)workspace;
   a.q_token = q_token_stride; a.q_head = q_head_stride; a.table_stride = table_stride; a.most = most;
-  a.batch = (int)batch; a.n_tokens = (int)n_tokens; a.hkv = (int)n_kv_heads; a.group = (int)(n_q_heads / n_kv_heads);
+  a.batch = (int)batch; a.hkv = (int)n_kv_heads; a.group = (int)(n_q_heads / n_kv_heads);
   a.page_shift = block_shift_of(page_len); a.max_pages = (int)max_pages; a.keep = (int)keep; a.recent = (int)recent;
   a.last_row = (int)(std::min(max_kv, max_blocks * page_len) - 1);
   const int64_t at_once = select_tokens(n_tokens, n_kv_heads, most);
@@ -998,17 +1074,21 @@ extern "C" int subspec_select_blocks(const void* q, int64_t q_token_stride, int6
   for (int64_t first = 0; first < n_tokens; first += at_once) {
     const int64_t some = std::min(at_once, n_tokens - first);
     a.first = (int)first;
+    a.tokens = (int)some;
     if (most > keep) {
       DominantKernelTimer timer(st);
       if (dtype == SUBSPEC_BF16) {
-        if (head_dim == 128) launch_scores<SUBSPEC_BF16, 128>(a, some, st);
-        else launch_scores<SUBSPEC_BF16, 64>(a, some, st);
+        if (head_dim == 128) launch_scores<SUBSPEC_BF16, 128>(a, st);
+        else launch_scores<SUBSPEC_BF16, 64>(a, st);
       } else {
-        if (head_dim == 128) launch_scores<SUBSPEC_F16, 128>(a, some, st);
-        else launch_scores<SUBSPEC_F16, 64>(a, some, st);
+        if (head_dim == 128) launch_scores<SUBSPEC_F16, 128>(a, st);
+        else launch_scores<SUBSPEC_F16, 64>(a, st);
       }
     }
-    hipLaunchKernelGGL(block_select_kernel, dim3((unsigned)(some * n_kv_heads)), dim3(kSelectThreads), 0, st, a);
+    // (up to 256 blocks 6.8 us with 256 threads and 9.0 with 512, 2048 blocks 8.6 and 7.6)
+    const dim3 lists((unsigned)(some * n_kv_heads));
+    if (most <= 512) hipLaunchKernelGGL(block_select_kernel<256>, lists, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(block_select_kernel<512>, lists, dim3(512), 0, st, a);
   }
   SUBSPEC_CHECK_HIP(hipGetLastError());
   return SUBSPEC_OK;
