@@ -18,6 +18,7 @@ constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWaves = kVerifyThreads / kWave;
 constexpr int kVerifyRound = 8 * kVerifyThreads;       // entries that a workgroup takes at a time, eight a thread
 constexpr int kChunk = 8 * kWave;                      // ... a wavefront: sums are kept of these
+constexpr int kMostChunks = (1 << 20) / kChunk;
 
 // A slice of a row without filters, in 32 bits: its largest logit, the masses relative to it, the first entry that equals it.
 struct SliceStats {
@@ -43,7 +44,8 @@ struct VerifyArgs {
   SliceStats* stats;               // [row][slices], without
   EndRecord* ends;
   uint64_t* all;                   // [sequence][chunks] masses of the row that it ends with
-  uint64_t* rest;                  // ... what the draft leaves of them
+  uint64_t* part;                  // ... of the entries of which the draft leaves something (kOpen beside it: of some it is not clear whether)
+  double* taken;                   // ... what the draft has of these, in probabilities: part - taken * the row's mass is left
   int q_dtype, slices, end_slices, end_length, chunks, batch, n_rows, wide, q_wide, filtered;
 };
 
@@ -142,11 +144,6 @@ __device__ __forceinline__ void eight_masses(const float* l, int i, const RowCut
 #pragma unroll
     for (int k = 0; k < 8; ++k) m[k] = order_key<DT>(l[k], i + k) > cut.last ? 0.0 : m[k];
   }
-}
-__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor((unsigned long long)v, o, kWave);
-  return v;
 }
 __device__ __forceinline__ uint64_t block_sum_u64(uint64_t v, uint64_t* scratch) {
   v = wave_sum_u64(v);
@@ -258,8 +255,13 @@ __device__ __forceinline__ uint64_t rest_of(double m, float q, double z) { retur
 // (the exponent's rounding, the factor's; a slice's largest logit against the row's) and 2^-23; 2^20 terms of a size below 2^-20 make no more than one, so by
 // 20 * 3 * 2^-24 * 0.7 on average; a lane adds 32 terms, a wavefront 64 sums in a tree, a row 512 of these, 32 a
 // lane: 2.5e-6 + 2^-23 + 74 * 2^-24 < 2^-17.
-constexpr double kUnsure = 0x1p-16;
+constexpr double kUnsure = 0x1p-17;
+constexpr uint64_t kOpen = 1ull << 63;               // (a chunk's masses stay below 2^51)
 
+// What the draft leaves of a row, sum over j of max(m_j - q_j Z, 0), takes Z, which is complete only when all slices have been seen; but which terms are above zero
+// the mass in 32 bits says already, up to those within kUnsure of it, and the sum of these terms is sum m_j - Z sum q_j.  So a chunk keeps both
+// sums, the row is read once, and a chunk that has a term too near to call is looked at again when Z is there (one or two of 300 where p and q
+// are those of two models; a pass of its own for Z took 13 us of 56 for 48 rows of 152064).
 // A workgroup a slice of that row.  Each looks for itself which drafts of the sequence stay (kRowsAtOnce rows at a time: few words, out of the caches), which
 // is cheaper than a launch of its own for that; the first of a sequence's writes it down.  Then the masses of the slice's chunks, and where the
 // row's mass is known (with filters) what the draft leaves of them.  One more workgroup is for the rows of nobody.
@@ -357,94 +359,97 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_end_kernel(VerifyArgs a
   const int c0 = slice * a.end_length + wave * kChunk;
   float l[ROUNDS][8], q[ROUNDS][8];
   load_chunks<DT, ROUNDS>(src, c0, kVerifyRound, a.s.vocab, a.wide, -INFINITY, l);
-  if (FILTERED && !last) load_drafts<ROUNDS>(a, row, draft, c0, kVerifyRound, q);
+  if (!last) load_drafts<ROUNDS>(a, row, draft, c0, kVerifyRound, q);
+  const double z = FILTERED ? cut.mass : cut.mass * (double)(1ull << kMassBits);
 #pragma unroll
   for (int k = 0; k < ROUNDS; ++k) {
     const int c = c0 + k * kVerifyRound;
     if (c >= a.s.vocab) break;
-    uint64_t all = 0, rest = 0;
-    double m[8];
+    uint64_t all = 0, part = 0;
+    double m[8], taken = 0.0;
+    bool open = false;
     eight_masses<DT>(l[k], c + 8 * lane, cut, top, r, series, m);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      all += whole(m[e]);
-      if (FILTERED && !last) rest += rest_of(m[e], q[k][e], cut.mass);
+      const uint64_t w = whole(m[e]);
+      all += w;
+      if (last) continue;
+      if (FILTERED) {                                        // (the row's mass is known)
+        part += rest_of(m[e], q[k][e], z);
+      } else {
+        const double p = draft_prob(q[k][e]), left = fma(-p, z, m[e]);
+        const bool some = left > 0.0;
+        part += some ? w : 0;
+        taken += some ? p : 0.0;
+        open |= fabs(left) <= kUnsure * m[e];
+      }
     }
     all = wave_sum_u64(all);
-    if (FILTERED) rest = wave_sum_u64(rest);
+    part = wave_sum_u64(part);
+    if (!FILTERED) {
+      taken = wave_sum_f64(taken);
+      if (__any(open) && !last) part |= kOpen;
+    }
     if (lane == 0) {
       const int64_t at = (int64_t)b * a.chunks + c / kChunk;
       a.all[at] = all;
-      if (FILTERED || last) a.rest[at] = rest;
+      a.part[at] = part;
+      a.taken[at] = taken;
     }
   }
 }
 
-// the mass of a sequence's last row, from its chunks (a workgroup)
-__device__ __forceinline__ double end_mass(const VerifyArgs& a, int b, uint64_t* scratch) {
-  uint64_t sum = 0;
-  for (int c = threadIdx.x; c < a.chunks; c += kVerifyThreads) sum += a.all[(int64_t)b * a.chunks + c];
-  return (double)block_sum_u64(sum, scratch);
-}
-
-// What the draft leaves, without filters: the row's mass is known now.
-template <int DT, int ROUNDS>
-__global__ __launch_bounds__(kVerifyThreads) void verify_rest_kernel(VerifyArgs a) {
-  __shared__ uint64_t scratch[kVerifyWaves];
-  const int b = blockIdx.x / a.end_slices, slice = blockIdx.x % a.end_slices;
+// The token: the chunk that the number falls into, then the entry.  A workgroup a sequence, whose wavefronts share the chunks that have to be looked at again;
+// one of them finds the entry.
+template <int DT>
+__global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs a) {
+  __shared__ uint64_t alls[kMostChunks], rests[kMostChunks], scratch[kVerifyWaves];
+  const int b = blockIdx.x, lane = threadIdx.x & (kWave - 1);
   const EndRecord e = a.ends[b];
-  if (e.row < 0 || e.last) return;
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
-  const char* src = verify_row<DT>(a, e.row);
-  const int c0 = slice * a.end_length + wave * kChunk;
-  float l[ROUNDS][8], q[ROUNDS][8];
-  load_chunks<DT, ROUNDS>(src, c0, kVerifyRound, a.s.vocab, a.wide, -INFINITY, l);
-  load_drafts<ROUNDS>(a, e.row, e.draft, c0, kVerifyRound, q);
+  if (e.row < 0) return;
   const RowRule r = row_rule(a.s, e.row);
   const RowTop top = row_top_of(e.cut.top, r);
   const Series series;
-  const double z = end_mass(a, b, scratch);
+  const char* src = verify_row<DT>(a, e.row);
+  const int64_t first = (int64_t)b * a.chunks;
+  uint64_t z_units = 0;
+  for (int c = threadIdx.x; c < a.chunks; c += kVerifyThreads) z_units += alls[c] = a.all[first + c];
+  z_units = block_sum_u64(z_units, scratch);
+  const double z = a.filtered ? e.cut.mass : (double)z_units;
+  uint64_t rest = 0;
+  if (!e.last) {
+    for (int c = (int)threadIdx.x / kWave * kWave; c < a.chunks; c += kVerifyThreads) {
+      const int at = c + lane;
+      const uint64_t part = at < a.chunks ? a.part[first + at] : 0;
+      const double left = (double)(part & ~kOpen) - z * (at < a.chunks ? a.taken[first + at] : 0.0);
+      uint64_t mine = whole(fmax(left, 0.0));
+      for (uint64_t open = __ballot(part >= kOpen); open; open &= open - 1) {                  // once more, with Z
+        const int which = __ffsll((unsigned long long)open) - 1;
+        float l[1][8], q[1][8];
+        double m[8];
+        load_chunks<DT, 1>(src, (c + which) * kChunk, 0, a.s.vocab, a.wide, -INFINITY, l);
+        load_drafts<1>(a, e.row, e.draft, (c + which) * kChunk, 0, q);
+        eight_masses<DT>(l[0], (c + which) * kChunk + 8 * lane, e.cut, top, r, series, m);
+        uint64_t exact = 0;
 #pragma unroll
-  for (int k = 0; k < ROUNDS; ++k) {
-    const int c = c0 + k * kVerifyRound;
-    if (c >= a.s.vocab) break;
-    uint64_t rest = 0;
-    double m[8];
-    eight_masses<DT>(l[k], c + 8 * lane, e.cut, top, r, series, m);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) rest += rest_of(m[i], q[k][i], z);
-    rest = wave_sum_u64(rest);
-    if (lane == 0) a.rest[(int64_t)b * a.chunks + c / kChunk] = rest;
+        for (int k = 0; k < 8; ++k) exact += rest_of(m[k], q[0][k], z);
+        exact = wave_sum_u64(exact);
+        if (lane == which) mine = exact;
+      }
+      if (at < a.chunks) rests[at] = mine;
+      rest += mine;
+    }
+    rest = block_sum_u64(rest, scratch);
   }
-}
-
-// The token: the chunk that the number falls into, then the entry.  A wavefront a sequence.
-template <int DT>
-__global__ __launch_bounds__(kWave) void verify_draw_kernel(VerifyArgs a) {
-  const int b = blockIdx.x, lane = threadIdx.x;
-  const EndRecord e = a.ends[b];
-  if (e.row < 0) return;
-  const uint64_t* alls = a.all + (int64_t)b * a.chunks;
-  const uint64_t* rests = a.rest + (int64_t)b * a.chunks;
-  // a lane has consecutive chunks; of the usual vocabularies at most eight, which stay in registers
-  constexpr int kHeld = 8;
-  const int per = (a.chunks + kWave - 1) / kWave, c0 = min(lane * per, a.chunks), c1 = min(c0 + per, a.chunks);
-  uint64_t all = 0, rest = 0, alls_at[kHeld], rests_at[kHeld];
-#pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-    alls_at[i] = c0 + i < c1 ? alls[c0 + i] : 0;
-    rests_at[i] = c0 + i < c1 ? rests[c0 + i] : 0;
-    all += alls_at[i];
-    rest += rests_at[i];
-  }
-  for (int c = c0 + kHeld; c < c1; ++c) {
-    all += alls[c];
-    rest += rests[c];
-  }
-  const uint64_t z = wave_sum_u64(all);
-  const bool by_rest = wave_sum_u64(rest) > 0;
+  __syncthreads();
+  if (threadIdx.x >= kWave) return;
+  const bool by_rest = rest > 0;
   const uint64_t* sums = by_rest ? rests : alls;
-  const uint64_t mine = by_rest ? rest : all, upto = wave_scan_u64(mine), total = __shfl((unsigned long long)upto, kWave - 1, kWave);
+  // a lane has consecutive chunks
+  const int per = (a.chunks + kWave - 1) / kWave, c0 = min(lane * per, a.chunks), c1 = min(c0 + per, a.chunks);
+  uint64_t mine = 0;
+  for (int c = c0; c < c1; ++c) mine += sums[c];
+  const uint64_t upto = wave_scan_u64(mine), total = lane_u64(upto, kWave - 1);
   int64_t token = -1;
   float prob = 0.f;
   if (total > 0) {
@@ -453,34 +458,31 @@ __global__ __launch_bounds__(kWave) void verify_draw_kernel(VerifyArgs a) {
     const int owner = __ffsll((unsigned long long)__ballot(goal < upto)) - 1;       // (the last lane's is the total)
     int chunk = c0;
     uint64_t before = upto - mine;
-    bool here = false;
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      const uint64_t next = before + (by_rest ? rests_at[i] : alls_at[i]);
-      here = here || goal < next;
-      before = here ? before : next;
-      chunk += here ? 0 : 1;
-    }
-    for (; !here && chunk + 1 < c1; ++chunk) {
+    for (; chunk + 1 < c1; ++chunk) {
       const uint64_t next = before + sums[chunk];
       if (goal < next) break;
       before = next;
     }
     chunk = __shfl(chunk, owner, kWave);
-    const uint64_t left = goal - __shfl((unsigned long long)before, owner, kWave);
-    const RowRule r = row_rule(a.s, e.row);
-    const RowTop top = row_top_of(e.cut.top, r);
-    const Series series;
-    const double zd = a.filtered ? e.cut.mass : (double)z;
+    uint64_t left = goal - __shfl((unsigned long long)before, owner, kWave);
     const int i = chunk * kChunk + 8 * lane;
     float l[1][8], q[1][8];
-    load_chunks<DT, 1>(verify_row<DT>(a, e.row), chunk * kChunk, 0, a.s.vocab, a.wide, -INFINITY, l);
+    load_chunks<DT, 1>(src, chunk * kChunk, 0, a.s.vocab, a.wide, -INFINITY, l);
     if (by_rest) load_drafts<1>(a, e.row, e.draft, chunk * kChunk, 0, q);
     uint64_t w[8], sum = 0;
     double m[8];
     eight_masses<DT>(l[0], i, e.cut, top, r, series, m);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sum += w[k] = by_rest ? rest_of(m[k], q[0][k], zd) : whole(m[k]);
+    for (int k = 0; k < 8; ++k) sum += w[k] = by_rest ? rest_of(m[k], q[0][k], z) : whole(m[k]);
+    const uint64_t here = wave_sum_u64(sum);
+    if (here == 0) {                                           // (a chunk whose terms round to nothing, one by one: its masses)
+      sum = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += w[k] = whole(m[k]);
+      left = 0;
+    } else {
+      left = min(left, here - 1);                              // (the chunk's sum was of its terms before rounding)
+    }
     uint64_t at = wave_scan_u64(sum) - sum;
     const uint64_t hit = __ballot(at <= left && left < at + sum);
     double mass = 0.0;
@@ -496,7 +498,7 @@ __global__ __launch_bounds__(kWave) void verify_draw_kernel(VerifyArgs a) {
     const int finder = hit ? __ffsll((unsigned long long)hit) - 1 : 0;
     if (hit) {
       token = __shfl(i + k_hit, finder, kWave);
-      prob = __shfl((float)(mass / zd), finder, kWave);
+      prob = __shfl((float)(mass / z), finder, kWave);
     }
   }
   if (lane == 0) {
@@ -527,19 +529,15 @@ static VerifyPlan verify_plan(int64_t n_rows, int64_t batch, int64_t vocab, bool
   else p.stats = align_up((size_t)n_rows * p.slices * sizeof(SliceStats), 256);
   p.ends = align_up((size_t)batch * sizeof(EndRecord), 256);
   p.sums = align_up((size_t)batch * p.chunks * sizeof(uint64_t), 256);
-  p.bytes = p.search + p.stats + p.cuts + p.ends + 2 * p.sums;
+  p.bytes = p.search + p.stats + p.cuts + p.ends + 3 * p.sums;
   return p;
 }
 
 template <int DT, int ROUNDS>
 static void launch_ends(const VerifyArgs& a, hipStream_t st) {
-  const dim3 block(kVerifyThreads), ends((unsigned)(a.batch * a.end_slices)), ends_and_nobody((unsigned)(a.batch * a.end_slices + 1));
-  if (a.filtered) {
-    hipLaunchKernelGGL((verify_end_kernel<DT, true, ROUNDS>), ends_and_nobody, block, 0, st, a);
-  } else {
-    hipLaunchKernelGGL((verify_end_kernel<DT, false, ROUNDS>), ends_and_nobody, block, 0, st, a);
-    if (a.n_rows > 0) hipLaunchKernelGGL((verify_rest_kernel<DT, ROUNDS>), ends, block, 0, st, a);
-  }
+  const dim3 block(kVerifyThreads), ends_and_nobody((unsigned)(a.batch * a.end_slices + 1));
+  if (a.filtered) hipLaunchKernelGGL((verify_end_kernel<DT, true, ROUNDS>), ends_and_nobody, block, 0, st, a);
+  else hipLaunchKernelGGL((verify_end_kernel<DT, false, ROUNDS>), ends_and_nobody, block, 0, st, a);
 }
 template <int DT>
 static void launch_verify(const VerifyArgs& a, hipStream_t st) {
@@ -551,7 +549,7 @@ static void launch_verify(const VerifyArgs& a, hipStream_t st) {
   if (a.end_length == kVerifyRound) launch_ends<DT, 1>(a, st);
   else if (a.end_length == 2 * kVerifyRound) launch_ends<DT, 2>(a, st);
   else launch_ends<DT, 4>(a, st);
-  if (a.n_rows > 0) hipLaunchKernelGGL(verify_draw_kernel<DT>, dim3((unsigned)a.batch), dim3(kWave), 0, st, a);
+  if (a.n_rows > 0) hipLaunchKernelGGL(verify_draw_kernel<DT>, dim3((unsigned)a.batch), dim3(kVerifyThreads), 0, st, a);
 }
 
 }  // namespace subspec
@@ -600,7 +598,8 @@ extern "C" int subspec_verify_drafts(const void* logits, int dtype, int64_t n_ro
   a.cuts = (RowCut*)ws; ws += p.cuts;
   a.ends = (EndRecord*)ws; ws += p.ends;
   a.all = (uint64_t*)ws; ws += p.sums;
-  a.rest = (uint64_t*)ws;
+  a.part = (uint64_t*)ws; ws += p.sums;
+  a.taken = (double*)ws;
   a.q_dtype = draft_dtype; a.slices = p.slices; a.end_slices = p.end_slices; a.end_length = p.end_length; a.chunks = p.chunks;
   a.batch = (int)batch; a.n_rows = (int)n_rows; a.filtered = filtered;
   const int64_t es = (int64_t)dtype_size(dtype), qs = (int64_t)dtype_size(draft_dtype);

@@ -86,14 +86,36 @@ __device__ __forceinline__ float key_logit(uint64_t key) {
   return __uint_as_float(b >> 31 ? b : ~(b | ((1u << kDropped<DT>) - 1)) & 0x7fffffffu);
 }
 
-__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {      // inclusive
-  const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const uint64_t u = __shfl_up((unsigned long long)v, o, kWave);
-    if (lane >= o) v += u;
-  }
+// Sums up to each lane (all lanes active), by lanes that neighbour in a row of sixteen and the rows' last ones: registers alone, where exchanges through LDS wait
+// for one another.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t lanes_shifted_u64(uint64_t v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+  return (uint64_t)(uint32_t)hi << 32 | (uint32_t)lo;
+}
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
+  v += lanes_shifted_u64<0x111, 0xf>(v);
+  v += lanes_shifted_u64<0x112, 0xf>(v);
+  v += lanes_shifted_u64<0x114, 0xf>(v);
+  v += lanes_shifted_u64<0x118, 0xf>(v);
+  v += lanes_shifted_u64<0x142, 0xa>(v);
+  v += lanes_shifted_u64<0x143, 0xc>(v);
   return v;
+}
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int lane) {        // (the lane is the same in all)
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) { return lane_u64(wave_scan_u64(v), kWave - 1); }
+__device__ __forceinline__ double wave_sum_f64(double v) {
+  auto add = [&](uint64_t u) { v += __longlong_as_double((long long)u); };
+  add(lanes_shifted_u64<0x111, 0xf>((uint64_t)__double_as_longlong(v)));
+  add(lanes_shifted_u64<0x112, 0xf>((uint64_t)__double_as_longlong(v)));
+  add(lanes_shifted_u64<0x114, 0xf>((uint64_t)__double_as_longlong(v)));
+  add(lanes_shifted_u64<0x118, 0xf>((uint64_t)__double_as_longlong(v)));
+  add(lanes_shifted_u64<0x142, 0xa>((uint64_t)__double_as_longlong(v)));
+  add(lanes_shifted_u64<0x143, 0xc>((uint64_t)__double_as_longlong(v)));
+  return __longlong_as_double((long long)lane_u64((uint64_t)__double_as_longlong(v), kWave - 1));
 }
 __device__ __forceinline__ float larger(float m, float l) { return l > m ? l : m; }      // a NaN never is
 __device__ __forceinline__ uint64_t draw_goal(double u, uint64_t z) {
