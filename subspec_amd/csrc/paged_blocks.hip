@@ -232,7 +232,8 @@ __device__ __forceinline__ void score_weights(const SelectArgs& a, int t, int to
     __syncthreads();
   }
 }
-// Bounds of DEPTH * kAtOnce blocks from j0 on (below j1; past it the last one again), all asked for at once: 16-byte pieces of `low` and `high` a lane
+// Bounds of DEPTH * kAtOnce blocks from j0 on (below j1; past it the last one again), all asked for at once: 16-byte pieces of `low` and `high` a lane.  A step reads
+// them once, as streaming data: 64 tokens of up to 32768 rows, 193 MB, 43.6 -> 38.9 us (5.0 TB/s; a large copy reaches 5.1).
 template <int D, int DEPTH>
 __device__ __forceinline__ void load_bounds(const SelectArgs& a, int b, int kvh, int j0, int j1, dec_u4* low, dec_u4* high) {
   constexpr int kLanes = D / 8, kAtOnce = kWave / kLanes;
@@ -243,8 +244,8 @@ __device__ __forceinline__ void load_bounds(const SelectArgs& a, int b, int kvh,
 #pragma unroll
   for (int i = 0; i < DEPTH; ++i) {
     const dec_u4* src = bounds + (int64_t)__shfl(page_of, i * kAtOnce + lane / kLanes, kWave) * a.hkv * 2 * kLanes;
-    low[i] = src[0];
-    high[i] = src[kLanes];
+    low[i] = __builtin_nontemporal_load(src);
+    high[i] = __builtin_nontemporal_load(src + kLanes);
   }
 }
 __device__ __forceinline__ double score_of(double s) { return s != s ? INFINITY : s; }

@@ -23,13 +23,13 @@ def _dtype_code(t: torch.Tensor) -> int:
 
 
 def _require_gpu(*tensors: torch.Tensor) -> torch.device:
-    dev = tensors[0].device
+    index = tensors[0].get_device()                          # (a number: comparing device objects takes three times as long)
     for t in tensors:
         if not t.is_cuda:
             raise L.SubspecHipError("the HIP kernels need device tensors (no CPU fallback)")
-        if t.device != dev:
+        if t.get_device() != index:
             raise ValueError("all tensors must live on the same device")
-    return dev
+    return tensors[0].device
 
 
 # The smallest calls are bound by what happens before their first launch (a draft expansion's four launches last 22 us, its
@@ -443,10 +443,11 @@ def _extent(t: torch.Tensor):
 
 
 def _table_shape(block_table: torch.Tensor, batch: int):
-    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch or block_table.shape[1] < 1 \
-            or block_table.stride(1) != 1 or (batch > 1 and block_table.stride(0) < block_table.shape[1]):
+    shape, stride = block_table.shape, block_table.stride()
+    if block_table.dtype is not torch.int32 or len(shape) != 2 or shape[0] != batch or shape[1] < 1 or stride[1] != 1 \
+            or (batch > 1 and stride[0] < shape[1]):
         raise ValueError(f"block_table must be int32 [{batch}, max_blocks] with consecutive columns")
-    return block_table.shape[1], max(block_table.stride(0), block_table.shape[1])
+    return shape[1], max(stride[0], shape[1])
 
 
 def paged_batch_plan(kv_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor, n_free: torch.Tensor,
@@ -504,9 +505,10 @@ def paged_batch_plan(kv_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: 
 
 
 def _pool_layer_shape(pool_layer: torch.Tensor):
-    if pool_layer.dim() != 5 or pool_layer.shape[1] != 2 or not pool_layer.is_contiguous():
+    shape = pool_layer.shape
+    if len(shape) != 5 or shape[1] != 2 or not pool_layer.is_contiguous():
         raise ValueError("expected a contiguous pool layer [max_pages, 2, page_len, kv_heads, head_dim]")
-    return pool_layer.shape[0], pool_layer.shape[2], pool_layer.shape[3], pool_layer.shape[4]
+    return shape[0], shape[2], shape[3], shape[4]
 
 
 def kv_append_paged_(pool_layer: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
@@ -588,9 +590,10 @@ def paged_attention(q: torch.Tensor, pool_layer: torch.Tensor, block_table: torc
 
 # ---------------------------------------------------------------------------------------------- the blocks of long sequences that matter
 def _bounds_shape(bounds: torch.Tensor):
-    if bounds.dim() != 4 or bounds.shape[2] != 2 or not bounds.is_contiguous():
+    shape = bounds.shape
+    if len(shape) != 4 or shape[2] != 2 or not bounds.is_contiguous():
         raise ValueError("expected contiguous bounds [max_pages, kv_heads, 2, head_dim]")
-    return bounds.shape[0], bounds.shape[1], bounds.shape[3]
+    return shape[0], shape[1], shape[3]
 
 
 def kv_page_bounds_(bounds: torch.Tensor, pool_layer: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
@@ -603,28 +606,31 @@ def kv_page_bounds_(bounds: torch.Tensor, pool_layer: torch.Tensor, slots: torch
         raise ValueError(f"kv_page_bounds_: bounds must be {pool_layer.dtype} [{max_pages}, {heads}, 2, {D}]")
     if slots.dtype is not torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
         raise ValueError("kv_page_bounds_: slots must be a contiguous int64 vector")
-    begin, end = _extent(bounds)
-    for given in (pool_layer, slots):
-        first, last = _extent(given)
-        if begin < last and first < end:
-            raise ValueError("kv_page_bounds_: bounds overlap what is read")
+    begin, pool, last = bounds.data_ptr(), pool_layer.data_ptr(), slots.data_ptr()      # (all three are contiguous)
+    end = begin + bounds.numel() * bounds.element_size()
+    if (begin < pool + pool_layer.numel() * pool_layer.element_size() and pool < end) or (begin < last + 8 * slots.numel() and last < end):
+        raise ValueError("kv_page_bounds_: bounds overlap what is read")
     _call(dev, "subspec_kv_page_bounds", pool_layer.data_ptr(), bounds.data_ptr(), _dtype_code(bounds), max_pages, page_len, heads, D,
           slots.data_ptr(), slots.numel(), _stream(dev))
     return bounds
 
 
 def _token_maps(q: torch.Tensor, sequences: torch.Tensor, positions: torch.Tensor, Hkv: int, D: int, what: str):
-    """Heads of ``q`` [tokens, Hq, D], which is copied where its rows are not 16-byte pieces."""
-    if q.dim() != 3 or q.shape[2] != D:
+    """(q, tokens, Hq, token stride, head stride) of ``q`` [tokens, Hq, D], which is copied where its rows are not 16-byte pieces."""
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != D:
         raise ValueError(f"{what}: expected q [tokens, Hq, {D}]")
-    T, Hq, _ = q.shape
-    _int32_vector(sequences, T, "sequences")
-    _int32_vector(positions, T, "positions")
+    T, Hq = shape[0], shape[1]
+    if sequences.dtype is not torch.int32 or positions.dtype is not torch.int32 or sequences.shape != (T,) or positions.shape != (T,) \
+            or not sequences.is_contiguous() or not positions.is_contiguous():
+        raise ValueError(f"{what}: sequences and positions must be contiguous int32 vectors of {T} elements")
     if Hq < 1 or Hkv < 1 or Hq % Hkv:
         raise ValueError(f"{what}: {Hq} query heads over {Hkv} KV heads")
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+    token, head, element = q.stride()
+    if element != 1 or token % 8 or head % 8 or q.data_ptr() % 16:
         q = q.contiguous()
-    return q, T, Hq
+        token, head, element = q.stride()
+    return q, T, Hq, token, head
 
 
 def _scratch(workspace: Optional[torch.Tensor], need: int, dev: torch.device, what: str):
@@ -661,10 +667,11 @@ def select_blocks(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tens
     tokens that decode and drafts under verification; a prompt's own tokens are better served by ``paged_attention``."""
     dev = _require_gpu(q, bounds, block_table, sequences, positions)
     max_pages, Hkv, D = _bounds_shape(bounds)
-    q, T, Hq = _token_maps(q, sequences, positions, Hkv, D, "select_blocks")
+    q, T, Hq, token, head = _token_maps(q, sequences, positions, Hkv, D, "select_blocks")
     if q.dtype != bounds.dtype:
         raise ValueError("select_blocks: q and bounds must share a dtype")
-    max_blocks, stride = _table_shape(block_table, block_table.shape[0])
+    batch = block_table.shape[0]
+    max_blocks, stride = _table_shape(block_table, batch)
     page_len, keep, recent = int(page_len), int(keep), int(recent)
     if page_len < 1 or recent < 1 or keep < recent:
         raise ValueError(f"select_blocks: page_len={page_len}, keep={keep}, recent={recent}: recent is 1 to keep")
@@ -678,8 +685,8 @@ def select_blocks(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tens
                                                  ("positions", positions)])
     need = L.lib().subspec_select_blocks_workspace(T, Hkv, page_len, max_blocks, max_kv)
     workspace, ws_ptr, ws_bytes = _scratch(workspace, need, dev, "select_blocks")
-    _call(dev, "subspec_select_blocks", q.data_ptr(), q.stride(0), q.stride(1), bounds.data_ptr(), _dtype_code(q), max_pages, page_len,
-          block_table.data_ptr(), max_blocks, stride, sequences.data_ptr(), positions.data_ptr(), block_table.shape[0], T, Hq, Hkv, D, max_kv,
+    _call(dev, "subspec_select_blocks", q.data_ptr(), token, head, bounds.data_ptr(), _dtype_code(q), max_pages, page_len,
+          block_table.data_ptr(), max_blocks, stride, sequences.data_ptr(), positions.data_ptr(), batch, T, Hq, Hkv, D, max_kv,
           keep, recent, out.data_ptr(), ws_ptr, ws_bytes, _stream(dev))
     return out
 
@@ -694,13 +701,14 @@ def block_attention(q: torch.Tensor, pool_layer: torch.Tensor, block_table: torc
     they were in ``out``, which may be a contiguous ``q`` itself and otherwise overlaps no input."""
     dev = _require_gpu(q, pool_layer, block_table, blocks, sequences, positions)
     max_pages, page_len, Hkv, D = _pool_layer_shape(pool_layer)
-    q, T, Hq = _token_maps(q, sequences, positions, Hkv, D, "block_attention")
+    q, T, Hq, token, head = _token_maps(q, sequences, positions, Hkv, D, "block_attention")
     if q.dtype != pool_layer.dtype:
         raise ValueError("block_attention: q and the pool must share a dtype")
-    if blocks.dtype is not torch.int32 or blocks.dim() != 3 or blocks.shape[:2] != (T, Hkv) or blocks.shape[2] < 1 or not blocks.is_contiguous():
+    shape = blocks.shape
+    if blocks.dtype is not torch.int32 or len(shape) != 3 or shape[0] != T or shape[1] != Hkv or shape[2] < 1 or not blocks.is_contiguous():
         raise ValueError(f"block_attention: blocks must be a contiguous int32 tensor [{T}, {Hkv}, keep]")
-    max_blocks, stride = _table_shape(block_table, block_table.shape[0])
-    keep = blocks.shape[2]
+    batch, keep = block_table.shape[0], shape[2]
+    max_blocks, stride = _table_shape(block_table, batch)
     if out is None:
         out = torch.empty((T, Hq * D), dtype=q.dtype, device=dev)
     elif out.dtype != q.dtype or out.shape != (T, Hq * D) or not out.is_contiguous() or out.device != dev:
@@ -709,10 +717,10 @@ def block_attention(q: torch.Tensor, pool_layer: torch.Tensor, block_table: torc
         same = q.is_contiguous() and out.data_ptr() == q.data_ptr()
         _apart("block_attention", [("out", out)], [("the pool", pool_layer), ("block_table", block_table), ("blocks", blocks),
                                                    ("sequences", sequences), ("positions", positions)] + ([] if same else [("q", q)]))
-    need = L.lib().subspec_block_attention_workspace(block_table.shape[0], T, Hq, Hkv, D, page_len, max_blocks, keep)
+    need = L.lib().subspec_block_attention_workspace(batch, T, Hq, Hkv, D, page_len, max_blocks, keep)
     workspace, ws_ptr, ws_bytes = _scratch(workspace, need, dev, "block_attention")
-    _call(dev, "subspec_block_attention", q.data_ptr(), q.stride(0), q.stride(1), pool_layer.data_ptr(), _dtype_code(q), max_pages, page_len,
-          block_table.data_ptr(), max_blocks, stride, blocks.data_ptr(), keep, sequences.data_ptr(), positions.data_ptr(), block_table.shape[0], T,
+    _call(dev, "subspec_block_attention", q.data_ptr(), token, head, pool_layer.data_ptr(), _dtype_code(q), max_pages, page_len,
+          block_table.data_ptr(), max_blocks, stride, blocks.data_ptr(), keep, sequences.data_ptr(), positions.data_ptr(), batch, T,
           Hq, Hkv, D, float(D ** -0.5 if scale is None else scale), out.data_ptr(), ws_ptr, ws_bytes, _stream(dev))
     return out
 
@@ -788,9 +796,11 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, query_starts: torc
     batch = query_starts.numel() - 1
     if batch < 1:
         raise ValueError("verify_drafts: query_starts must have a place for each sequence and one more")
-    for name, t, dtype, n in (("tokens", tokens, torch.int64, rows), ("uniforms", uniforms, torch.float32, rows), ("draws", draws, torch.float32, batch)):
-        if t.dtype is not dtype or t.shape != (n,) or not t.is_contiguous():
-            raise ValueError(f"verify_drafts: {name} must be a contiguous {dtype} tensor of {n} elements")
+    if tokens.dtype is not torch.int64 or tokens.shape != (rows,) or not tokens.is_contiguous():
+        raise ValueError(f"verify_drafts: tokens must be a contiguous int64 tensor of {rows} elements")
+    if uniforms.dtype is not torch.float32 or draws.dtype is not torch.float32 or uniforms.shape != (rows,) or draws.shape != (batch,) \
+            or not uniforms.is_contiguous() or not draws.is_contiguous():
+        raise ValueError(f"verify_drafts: uniforms and draws must be contiguous float32 tensors of {rows} and {batch} elements")
     if draft_probs is not None and draft_probs.shape != (rows, V):
         raise ValueError(f"verify_drafts: draft_probs must be [{rows}, {V}]")
     logits = _rows_of(logits)
@@ -804,7 +814,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, query_starts: torc
     k = min(int(k), (1 << 31) - 1)
     sizes = (rows, rows, batch)
     if out is None:
-        out = {name: torch.empty(n, dtype=dtype, device=dev) for (name, dtype), n in zip(_DRAFTS_OUT, sizes)}
+        o_tokens, o_probs, o_accepted = torch.empty(3 * rows + batch, dtype=torch.int32, device=dev).split_with_sizes((2 * rows, rows, batch))
+        out = {"tokens": o_tokens.view(torch.int64), "probs": o_probs.view(torch.float32), "accepted": o_accepted}
     else:
         for (name, dtype), n in zip(_DRAFTS_OUT, sizes):
             o = out[name]
@@ -816,14 +827,12 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, query_starts: torc
         _apart("verify_drafts", [(f"out[{name!r}]", out[name]) for name, _ in _DRAFTS_OUT], given)
     filtered = bool(k_ptr or p_ptr or m_ptr or 0 < k < V or p < 1 or m > 0)
     need = L.lib().subspec_verify_drafts_workspace(rows, batch, V, int(filtered))
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     workspace, ws_ptr, ws_bytes = _scratch(workspace, need, dev, "verify_drafts")
     _call(dev, "subspec_verify_drafts", logits.data_ptr(), _dtype_code(logits), rows, V, max(logits.stride(0), V), tokens.data_ptr(),
           query_starts.data_ptr(), batch, uniforms.data_ptr(), draws.data_ptr(), None if q is None else q.data_ptr(),
           L.F32 if q is None else _dtype_code(q), V if q is None else max(q.stride(0), V), t_ptr, float(t), k_ptr, k, p_ptr, float(p), m_ptr, float(m),
           ws_ptr, ws_bytes, out["tokens"].data_ptr(), out["probs"].data_ptr(), out["accepted"].data_ptr(), _stream(dev))
-    return {name: out[name] for name, _ in _DRAFTS_OUT}
+    return out
 
 
 def int4_linear(x: torch.Tensor, wq: torch.Tensor, sz: torch.Tensor, out_features: int,
