@@ -307,9 +307,9 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_end_kernel(VerifyArgs a
         const double unit = FILTERED ? 1.0 : 0x1p-42;                    // (masses in 32 bits are relative to the largest)
         const double m = cut.mass > 0.0 ? kept_mass<DT>(l, (int)x, cut, row_top_of(cut.top, r), r, series) * unit : 0.0;
         const double goal = r.u * q * cut.mass;
-        const bool unsure = !FILTERED && !r.greedy && m > 0.0 && fabs(goal - m) <= kUnsure * m;
+        const bool unsure = !FILTERED && !r.greedy && !last && m > 0.0 && fabs(goal - m) <= kUnsure * m;
         if (unsure) atomicMin(&stop, 2 * i + 1);
-        else if (!(goal < m)) atomicMin(&stop, 2 * i);                   // (the last row has no draft, of no mass)
+        else if (last || !(goal < m)) atomicMin(&stop, 2 * i);
         if (end && !last) a.s.probs[row] = cut.mass > 0.0 ? (float)(m / cut.mass) : 0.f;
         cuts[threadIdx.x / kRowLanes] = cut;
       }

@@ -195,6 +195,19 @@ def test_starts_out_of_order_stay_inside_the_call(starts):
         assert got["tokens"].min() >= -1 and got["tokens"].max() < 5000 and got["accepted"].min() >= 0 and got["accepted"].max() < 6
 
 
+@pytest.mark.parametrize("left", [-1.0, -3e38, float("nan")])
+def test_starts_out_of_order_after_other_work(left):
+    """A sequence whose rows begin before the first start has no sums of them: whatever the workspace held, it ends with its last row."""
+    case = _case(torch.Generator().manual_seed(8), [3, 3], 5000, F32, F32)
+    for _ in range(3):
+        held = [torch.full((1 << 16,), left, device=DEV) for _ in range(16)]
+        torch.cuda.synchronize()
+        del held
+        got = _run((case[0], case[1], [5, 0, 6], *case[3:]))
+        assert 0 <= int(got["accepted"].min()) and int(got["accepted"].max()) < 6
+        assert got["tokens"].min() >= -1 and got["tokens"].max() < 5000
+
+
 def test_what_comes_out_is_distributed_like_the_target():
     """4096 sequences over one pair of distributions, three drafts each: the tokens at every place follow p (each count within five standard deviations of
     its mean: one entry in 3.5 million is further off), and as many drafts stay as sum min(p, q) says."""
