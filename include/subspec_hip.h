@@ -386,7 +386,7 @@ int subspec_kv_page_bounds(const void* kv_pool_layer, void* bounds, int dtype, i
  * blocks  device int32 [n_tokens, n_kv_heads, keep], in ascending order, -1 behind the last; it overlaps no input
  * workspace  subspec_select_blocks_workspace bytes, 16-byte aligned (NULL where that is 256)
  * Limits: 1 <= recent <= keep <= 2^17, min(max_blocks, ceil(max_kv / page_len)) <= 2^17, n_tokens <= 2^20, n_q_heads <= 1024.  Page numbers are clamped to the
- * pool.  Made for tokens that decode and for drafts: neighbours of one sequence share a reading of the bounds, up to four.
+ * pool.  Made for tokens that decode and for drafts: neighbours of one sequence share a reading of the bounds, up to eight.
  */
 size_t subspec_select_blocks_workspace(int64_t n_tokens, int64_t n_kv_heads, int64_t page_len, int64_t max_blocks, int64_t max_kv);
 
@@ -402,8 +402,8 @@ int subspec_select_blocks(const void* q, int64_t q_token_stride, int64_t q_head_
  * out       device [n_tokens, n_q_heads, head_dim]; rows of tokens whose sequence lies outside [0, batch) are left as they were.  It may be q
  *           itself where that is contiguous; otherwise it overlaps no input
  * Limits: at most 64 query heads a KV head, keep <= 2^17, keep * page_len <= 2^30, n_tokens <= 2^20; q as for subspec_paged_attention.  Page numbers are
- * clamped to the pool.  Rows of the pool that no token of the call sees, or whose block none lists, have no influence, whatever they hold; where a call has more
- * tokens than sequences, neighbours of one sequence read their blocks together, and an infinite or NaN VALUE row that one of them sees may reach the others.
+ * clamped to the pool.  A row of the pool that a token does not see, or whose block it does not list, has no influence on it, whatever it holds.  Where a call has more
+ * tokens than sequences, neighbours of one sequence read their blocks together (a chunk with an infinite or NaN value is read again for each of them).
  */
 size_t subspec_block_attention_workspace(int64_t batch, int64_t n_tokens, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
                                          int64_t page_len, int64_t max_blocks, int64_t keep);

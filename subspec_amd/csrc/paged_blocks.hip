@@ -616,8 +616,10 @@ __global__ __launch_bounds__(kUnionThreads) void block_union_kernel(AttendArgs a
 template <int D> __device__ __forceinline__ int attend_k_swap(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
 template <int D> __device__ __forceinline__ int attend_v_swap(int row) { return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3); }
 
+// Chunk `chunk` of the rows listed for `tokens` tokens from t on.  Where several share it, a row of the pool that one of them does not see has the probability 0 for it, and 0
+// times an infinity or a NaN is no 0: true then (and nothing written), for the tokens' results to be found one after the other, `alone`, with zeros in such rows.
 template <int DT, int D, int ROWT, bool SHARED>
-__global__ __launch_bounds__(kWave) void block_attention_kernel(AttendArgs a) {
+__device__ __forceinline__ bool attend_unit(const AttendArgs& a, int kvh, int chunk, int t, int tokens, int keys, int chunk_keys, int alone) {
   constexpr int kRowBytes = D * 2, kPieces = kRowBytes / 16, kRowsPerCopy = 64 / kPieces, kCopies = kAttendKeys / kRowsPerCopy;
   constexpr int kHalf = kAttendKeys * kRowBytes, kStage = 2 * kHalf;
   __shared__ __attribute__((aligned(1024))) uint8_t ring[kAttendStages * kStage];
@@ -625,21 +627,10 @@ __global__ __launch_bounds__(kWave) void block_attention_kernel(AttendArgs a) {
   __shared__ uint32_t seen_at[kAttendSegment / kAttendKeys];
   __shared__ __attribute__((aligned(16))) int place_at[SHARED ? kAttendSegment : 4];        // a key's row of the sequence, and its block's bits
   __shared__ uint32_t bits_at[SHARED ? kAttendSegment / 4 : 1];
-  const uint32_t unit = blockIdx.x;
-  const int kvh = (int)(unit % (uint32_t)a.hkv);
-  const uint32_t tc = unit / (uint32_t)a.hkv;
-  const int chunk = (int)(tc % (uint32_t)a.chunks), local = (int)(tc / (uint32_t)a.chunks), t = a.first + local;
-  int tokens = 1, keys = a.keys, chunk_keys = a.chunk_keys;
-  if constexpr (SHARED) {
-    tokens = a.leads[kvh * a.tokens + local];                // (0: of no sequence, or in another's tile)
-    if (tokens == 0) return;
-    keys = a.counts[kvh * a.tokens + local] << a.page_shift;
-    chunk_keys = shared_chunk_keys(a, keys);
-  }
-  const int b = a.sequences[t];
-  if (b < 0 || b >= a.batch) return;
+  const int b = a.sequences[t], local = t - a.first;
+  if (b < 0 || b >= a.batch) return false;
   const int v_begin = chunk * chunk_keys, v_end = min(v_begin + chunk_keys, keys);
-  if (SHARED && chunk > 0 && v_begin >= keys) return;        // (the merge knows how many there are)
+  if (SHARED && chunk > 0 && v_begin >= keys) return false;  // (the merge knows how many there are)
   const int lane = threadIdx.x, lq = lane & 15, lg = lane >> 4, rows = tokens * a.group;
 
   dec_u4 q[ROWT][D / 32];
@@ -662,6 +653,7 @@ __global__ __launch_bounds__(kWave) void block_attention_kernel(AttendArgs a) {
       last = max(last, __shfl_xor(last, o, kWave));
       least = min(least, __shfl_xor(least, o, kWave));
     }
+    if (alone >= 0) last = attend_last(a, t + alone);
   }
   v4f o[ROWT][D / 16];
   float ref[ROWT], l[ROWT];                                  // ref in units of exp2's argument
@@ -701,7 +693,8 @@ __global__ __launch_bounds__(kWave) void block_attention_kernel(AttendArgs a) {
       } else if (v < v_end) {
         block = list[v >> a.page_shift];
       }
-      const bool sees = block >= 0 && last >= 0 && block <= last >> a.page_shift && (block << a.page_shift) + in <= last;
+      bool sees = block >= 0 && last >= 0 && block <= last >> a.page_shift && (block << a.page_shift) + in <= last;
+      if (SHARED && alone >= 0) sees = sees && (bits >> alone & 1);
       const int page = sees ? min(max(row_pages[block], 0), a.max_pages - 1) : 0;
       row_at[u * 64 + lane] = sees ? 2 * ((int64_t)page * 2 * a.page_elems + (int64_t)a.hkv * D * in) : -1;
       const uint64_t some = __ballot(sees);
@@ -822,12 +815,22 @@ __global__ __launch_bounds__(kWave) void block_attention_kernel(AttendArgs a) {
     }
   }
 
+  if (SHARED && alone < 0 && tokens > 1) {
+    float none = 0.f;                                        // (NaN where a sum is infinite or NaN)
+#pragma unroll
+    for (int nt = 0; nt < ROWT; ++nt)
+#pragma unroll
+      for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) none = fmaf(o[nt][mt][e], 0.f, none);
+    if (__any(none != none)) return true;
+  }
 #pragma unroll
   for (int nt = 0; nt < ROWT; ++nt) {
     float sum = l[nt] + __shfl_xor(l[nt], 16, kWave);
     sum += __shfl_xor(sum, 32, kWave);
     const int r = nt * 16 + lq;
-    if (r >= rows) continue;
+    if (r >= rows || (SHARED && alone >= 0 && token[nt] != alone)) continue;
     const int head = r - token[nt] * a.group;
     if (a.chunks == 1) {
       const float inv = sum > 0.f ? 1.0f / sum : 0.f;
@@ -841,6 +844,24 @@ __global__ __launch_bounds__(kWave) void block_attention_kernel(AttendArgs a) {
 #pragma unroll
       for (int mt = 0; mt < D / 16; ++mt) *(v4f*)(dst + mt * 16) = o[nt][mt];
       if (lg == 0) *(v2f*)(a.part_ml + slot * 2) = v2f{ref[nt], sum};
+    }
+  }
+  return false;
+}
+
+template <int DT, int D, int ROWT, bool SHARED>
+__global__ __launch_bounds__(kWave) void block_attention_kernel(AttendArgs a) {
+  const uint32_t unit = blockIdx.x, tc = unit / (uint32_t)a.hkv;
+  const int kvh = (int)(unit % (uint32_t)a.hkv), chunk = (int)(tc % (uint32_t)a.chunks), local = (int)(tc / (uint32_t)a.chunks);
+  if constexpr (!SHARED) {
+    attend_unit<DT, D, ROWT, false>(a, kvh, chunk, a.first + local, 1, a.keys, a.chunk_keys, -1);
+  } else {
+    const int tokens = a.leads[kvh * a.tokens + local];      // (0: of no sequence, or in another's tile)
+    if (tokens == 0) return;
+    const int keys = a.counts[kvh * a.tokens + local] << a.page_shift;
+    for (int alone = -1; alone < tokens;) {
+      const bool apart = attend_unit<DT, D, ROWT, true>(a, kvh, chunk, a.first + local, tokens, keys, shared_chunk_keys(a, keys), alone);
+      alone = alone < 0 && !apart ? tokens : alone + 1;
     }
   }
 }

@@ -535,3 +535,34 @@ def test_neighbours_of_a_sequence_read_their_blocks_together(Hq, Hkv, D, P, keep
         if mine[t]:
             off = (one.cpu().double().view(Hq, D) - want[t]).abs() / _tolerance(want, weight, worst, torch.float16, D, keep * P, 6.0)[t]
             assert off.max() <= 1, (t, float(off.max()))
+
+
+@pytest.mark.parametrize("D,keep,P", [(128, 6, 16), (64, 40, 16), (64, 3, 4)])
+@pytest.mark.parametrize("what", [float("inf"), float("nan")])
+def test_a_value_that_one_token_does_not_see_stays_out_of_its_sums(D, keep, P, what):
+    """Drafts that share a reading: a row behind one of them, and a block that only others list, hold an infinity.  Those that see it get it, the others what they get alone."""
+    print("apart", D, keep, P, what, flush=True)
+    Hq, Hkv, n = 8, 2, 700
+    g = torch.Generator().manual_seed(D + keep)
+    _, pool, table, _, _ = _cache(g, [(n, 0), (n, 0)], P, Hq, Hkv, D, torch.bfloat16)
+    seq, pos = [0] * 5 + [1] * 3, [n - 5 + i for i in range(5)] + [n - 3 + i for i in range(3)]
+    q = torch.randn(8, Hq, D, generator=g).bfloat16()
+    last = (n - 1) // P
+    blocks = [[[j % last for j in range(t + h, t + h + keep - 1)] + [pos[t] // P] for h in range(Hkv)] for t in range(8)]
+    clean = ops.block_attention(q.to(DEV), pool.to(DEV), _i32(table), _i32(blocks), _i32(seq), _i32(pos))
+    hit = torch.zeros(8, Hq, dtype=torch.bool)
+    bad = pool.clone()
+    # the last draft's own row, head 1; a row of the first block that token 4's head 0 lists alone
+    row = pos[4]
+    bad[table[0][row // P], 1, row % P, 1, 3] = what
+    hit[4, Hq // 2:] = True
+    alone = [j for j in blocks[4][0] if all(j not in blocks[t][0] for t in range(4))]
+    bad[table[0][alone[0]], 1, 1, 0, 5] = what
+    hit[4, :Hq // 2] = True
+    got = ops.block_attention(q.to(DEV), bad.to(DEV), _i32(table), _i32(blocks), _i32(seq), _i32(pos)).cpu().view(8, Hq, D)
+    clean = clean.cpu().view(8, Hq, D)
+    assert not torch.isfinite(got[hit]).all(-1).any()
+    assert torch.equal(got[~hit], clean[~hit])
+    fine = torch.ones(D, dtype=torch.bool)
+    fine[[3, 5]] = False
+    assert torch.equal(got[hit][:, fine], clean[hit][:, fine])
