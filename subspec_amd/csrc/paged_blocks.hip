@@ -113,22 +113,40 @@ __device__ __forceinline__ uint32_t lanes_largest(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_readlane((int)v, kWave - 1);
 }
 
-// Tiles of up to `share` neighbouring tokens of one sequence, from the first of a run of them on: how many token t is the first of (0: it lies in another's
-// tile, or its sequence is below 0).  Every wavefront looks for itself; tokens outside [first, end) are nobody's neighbours.
-struct TokenTile { int sequence, tokens; };
-__device__ __forceinline__ TokenTile token_tile(const int32_t* sequences, int t, int first, int end, int share) {
-  const int lane = threadIdx.x & (kWave - 1), b = sequences[t], next = t + 1 + lane;
-  const uint64_t ends = __ballot(next >= end || sequences[min(next, end - 1)] != b);
-  int behind = 0;                                            // neighbours of the sequence before this token
-  for (;;) {
-    const int other = t - 1 - behind - lane;
-    const uint64_t others = __ballot(other < first || sequences[max(other, 0)] != b);
-    behind += others ? __ffsll((unsigned long long)others) - 1 : kWave;
-    if (others) break;
+// Tiles of up to `share` (a power of two) neighbouring tokens of one sequence, from the first of a run of them on: the m-th of those of tokens [first, end), and how
+// many there are.  Tokens outside are nobody's neighbours, those of no sequence are in no tile.  Every wavefront looks for itself, 64 tokens at a time: for the few
+// hundred tokens of a step less than a launch for it, or a workgroup for every token that is not the first of a tile, to leave at once.
+struct TokenTile { int first, tokens, sequence, all; };
+__device__ __forceinline__ TokenTile token_tile(const int32_t* sequences, int first, int end, int batch, int share, int m) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const uint64_t upto = ~0ull >> (kWave - 1 - lane);
+  TokenTile tile{0, 0, -1, 0};
+  int run = first, before = -1;                              // where the last run began, the sequence of the token before
+  int ahead = sequences[min(first + lane, end - 1)];
+  for (int x0 = first; x0 < end; x0 += kWave) {
+    const int x = x0 + lane, b = ahead;
+    ahead = sequences[min(x + kWave, end - 1)];
+    const int left = __shfl_up(b, 1, kWave);
+    const uint64_t begins = __ballot(x == first || b != (lane ? left : before)) & upto;
+    const int pos = begins ? lane - (kWave - 1 - __clzll((long long)begins)) : x - run;
+    const bool counts = x < end && b >= 0 && b < batch;
+    const uint64_t leads = __ballot(counts && (pos & (share - 1)) == 0);
+    const uint64_t here = __ballot(counts && tile.all + __popcll(leads & upto) - 1 == m);
+    if (here && tile.tokens == 0) {
+      const int at = __ffsll((unsigned long long)here) - 1;
+      tile.first = x0 + at;
+      tile.sequence = __builtin_amdgcn_readlane(b, at);
+    }
+    tile.tokens += __popcll(here);
+    tile.all += __popcll(leads);
+    run = __builtin_amdgcn_readlane(x - pos, kWave - 1);
+    before = __builtin_amdgcn_readlane(b, kWave - 1);
   }
-  if (b < 0 || behind % share) return TokenTile{b, 0};
-  return TokenTile{b, min(share, ends ? __ffsll((unsigned long long)ends) : kWave)};
+  return tile;
 }
+constexpr int kTileTokens = 1024;          // tokens of a launch whose tiles are looked for
+// Tiles of so many tokens where every sequence's are neighbours: as many are looked for at once, and then the next.
+static int tiles_at_once(int64_t tokens, int64_t batch, int64_t share) { return (int)std::min(tokens, std::min(tokens, batch) + tokens / share); }
 
 // ---------------------------------------------------------------------------------------------------------------- scores
 // s_j = sum over the KV head's query heads g and dimensions d of max(q_gd low_jd, q_gd high_jd), which no sum of the heads' scores of a key of block j
@@ -143,7 +161,7 @@ struct SelectArgs {
   int32_t* blocks;               // [tokens][n_kv_heads][keep]
   double* scores;                // [token - first][n_kv_heads][most]
   int64_t q_token, q_head, table_stride, most;
-  int batch, first, tokens, hkv, group, page_shift, max_pages, keep, recent, last_row, span, spans;
+  int batch, first, tokens, hkv, group, page_shift, max_pages, keep, recent, last_row, span, spans, tiles_at_once;
 };
 // Blocks that a token sees (0: none), and of these the first so many that compete.
 struct TokenBlocks { int seen, scored; };
@@ -155,7 +173,7 @@ __device__ __forceinline__ TokenBlocks token_blocks(const SelectArgs& a, int b, 
 }
 constexpr int kScoreTokens = 8;           // tokens of a sequence that share a reading of the bounds
 constexpr int kScoreThreads = 256;
-constexpr int kSharedDepth = 2;           // readings of a wavefront then
+constexpr int kSharedDepth = 4;           // readings of a wavefront then (1 / 2 / 4: 20.4 / 15.2 / 10.5 us for 72 drafts)
 
 // a double from another lane of sixteen (a DPP control)
 template <int CTRL>
@@ -192,8 +210,9 @@ __device__ __forceinline__ void sum_eight(double (&v)[8], int lane, double* out)
 
 // The query heads of `tokens` tokens added up by a workgroup, into LDS: (of high, of low) of each.  A thread has DIMS neighbouring dimensions; where there are more
 // threads than these, every team of them has a part of the heads, and the teams' sums are added in their order.  Ends with a barrier.
-template <int DT, int D, int TOKENS, int THREADS, int DIMS>
-__device__ __forceinline__ void score_weights(const SelectArgs& a, int t, int tokens, int kvh, double* weight) {
+// (`meanwhile` runs before the first barrier)
+template <int DT, int D, int TOKENS, int THREADS, int DIMS, typename F>
+__device__ __forceinline__ void score_weights(const SelectArgs& a, int t, int tokens, int kvh, double* weight, F meanwhile) {
   constexpr int kTeam = TOKENS * D / DIMS, kTeams = THREADS / kTeam;
   const int team = threadIdx.x / kTeam, k = threadIdx.x / (D / DIMS) % TOKENS, d = threadIdx.x % (D / DIMS) * DIMS;
   double up[DIMS], down[DIMS];
@@ -221,6 +240,7 @@ __device__ __forceinline__ void score_weights(const SelectArgs& a, int t, int to
     mine[e] = up[e];
     mine[D + e] = down[e];
   }
+  meanwhile();
   __syncthreads();
   if constexpr (kTeams > 1) {
     const int teams = min(kTeams, a.group);
@@ -235,11 +255,10 @@ __device__ __forceinline__ void score_weights(const SelectArgs& a, int t, int to
 // Bounds of DEPTH * kAtOnce blocks from j0 on (below j1; past it the last one again), all asked for at once: 16-byte pieces of `low` and `high` a lane.  A step reads
 // them once, as streaming data: 64 tokens of up to 32768 rows, 193 MB, 43.6 -> 38.9 us (5.0 TB/s; a large copy reaches 5.1).
 template <int D, int DEPTH>
-__device__ __forceinline__ void load_bounds(const SelectArgs& a, int b, int kvh, int j0, int j1, dec_u4* low, dec_u4* high) {
+__device__ __forceinline__ void load_bounds(const SelectArgs& a, int page, int kvh, dec_u4* low, dec_u4* high) {
   constexpr int kLanes = D / 8, kAtOnce = kWave / kLanes;
   static_assert(DEPTH * kAtOnce <= kWave, "a lane holds a page number");
-  const int lane = threadIdx.x & (kWave - 1);
-  const int page_of = min(max(a.table[b * a.table_stride + min(j0 + lane, j1 - 1)], 0), a.max_pages - 1);
+  const int lane = threadIdx.x & (kWave - 1), page_of = min(max(page, 0), a.max_pages - 1);
   const dec_u4* bounds = (const dec_u4*)(a.bounds + (int64_t)kvh * 2 * D) + lane % kLanes;
 #pragma unroll
   for (int i = 0; i < DEPTH; ++i) {
@@ -264,8 +283,9 @@ __global__ __launch_bounds__(kScoreThreads) void block_score_kernel(SelectArgs a
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1), part = lane % kLanes, which = lane / kLanes;
   const int j0 = span * a.span + wave * kAtOnce * kDepth, j1 = min(j0 + kAtOnce * kDepth, most);
   dec_u4 low[kDepth], high[kDepth];
-  if (j0 < j1) load_bounds<D, kDepth>(a, b, kvh, j0, j1, low, high);
-  score_weights<DT, D, 1, kScoreThreads, 2>(a, t, 1, kvh, weight);
+  const int page = a.table[b * a.table_stride + max(min(j0 + lane, j1 - 1), 0)];
+  if (j0 < j1) load_bounds<D, kDepth>(a, page, kvh, low, high);
+  score_weights<DT, D, 1, kScoreThreads, 2>(a, t, 1, kvh, weight, [] {});
   if (j0 >= j1) return;
   double up[8], down[8], s[kDepth], out[2];
 #pragma unroll
@@ -296,62 +316,69 @@ __global__ __launch_bounds__(kScoreThreads) void block_score_kernel(SelectArgs a
 // (72 drafts of 16 sequences, 32 : 8 heads, up to 255 blocks: a conversion a token 17.4 us.)
 template <int DT, int D>
 __global__ __launch_bounds__(kScoreThreads) void block_score_shared_kernel(SelectArgs a) {
-  constexpr int kLanes = D / 8, kAtOnce = kWave / kLanes;
+  constexpr int kLanes = D / 8, kAtOnce = kWave / kLanes, kAtOnceTokens = 8 / kSharedDepth;            // (tokens that make eight sums)
   __shared__ __attribute__((aligned(16))) double weight[kScoreThreads / (D / 4) * 2 * D];
   const uint32_t unit = blockIdx.x;
   const int kvh = (int)(unit % (uint32_t)a.hkv), span = (int)(unit / (uint32_t)a.hkv % (uint32_t)a.spans);
-  const int local = (int)(unit / (uint32_t)a.hkv / (uint32_t)a.spans), t = a.first + local;
-  const TokenTile tile = token_tile(a.sequences, t, a.first, a.first + a.tokens, kScoreTokens);
-  if (!tile.tokens) return;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1), part = lane % kLanes, which = lane / kLanes;
-  // a lane has a token's number of blocks
-  const int mine = lane < tile.tokens ? token_blocks(a, tile.sequence, a.positions[t + lane]).scored : 0;
-  const int most = (int)lanes_largest((uint32_t)mine);
-  if (span * a.span >= most) return;                         // (the whole workgroup)
-  const int j0 = span * a.span + wave * kAtOnce * kSharedDepth, j1 = min(j0 + kAtOnce * kSharedDepth, most);
-  dec_u4 low[kSharedDepth], high[kSharedDepth];
-  if (j0 < j1) load_bounds<D, kSharedDepth>(a, tile.sequence, kvh, j0, j1, low, high);
-  score_weights<DT, D, kScoreTokens, kScoreThreads, 4>(a, t, tile.tokens, kvh, weight);
-  if (j0 >= j1) return;
-  double low_of[kSharedDepth][8], high_of[kSharedDepth][8];
+  for (int m = (int)(unit / (uint32_t)a.hkv / (uint32_t)a.spans);; m += a.tiles_at_once) {
+    const TokenTile tile = token_tile(a.sequences, a.first, a.first + a.tokens, a.batch, kScoreTokens, m);
+    if (!tile.tokens) return;
+    const int t = tile.first, local = t - a.first;
+    // a lane has a token's number of blocks
+    const int mine = lane < tile.tokens ? token_blocks(a, tile.sequence, a.positions[t + lane]).scored : 0;
+    const int most = (int)lanes_largest((uint32_t)mine);
+    const int j0 = span * a.span + wave * kAtOnce * kSharedDepth, j1 = min(j0 + kAtOnce * kSharedDepth, most);
+    if (span * a.span < most) {                               // (the whole workgroup)
+      dec_u4 low[kSharedDepth], high[kSharedDepth];
+      const int page = a.table[tile.sequence * a.table_stride + max(min(j0 + lane, j1 - 1), 0)];
+      score_weights<DT, D, kScoreTokens, kScoreThreads, 4>(a, t, tile.tokens, kvh, weight, [&]() {
+        if (j0 < j1) load_bounds<D, kSharedDepth>(a, page, kvh, low, high);
+      });
+      double low_of[kSharedDepth][8], high_of[kSharedDepth][8];
+      if (j0 < j1) {
 #pragma unroll
-  for (int i = 0; i < kSharedDepth; ++i) {
-    float l[8], h[8];
-    unpack8<DT>(low[i], l);
-    unpack8<DT>(high[i], h);
+        for (int i = 0; i < kSharedDepth; ++i) {
+          float l[8], h[8];
+          unpack8<DT>(low[i], l);
+          unpack8<DT>(high[i], h);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      low_of[i][e] = (double)l[e];
-      high_of[i][e] = (double)h[e];
-    }
-  }
-  constexpr int kAtOnceTokens = 8 / kSharedDepth;             // that make eight sums
-#pragma unroll
-  for (int k0 = 0; k0 < kScoreTokens; k0 += kAtOnceTokens) {
-    if (k0 >= tile.tokens) break;
-    double s[8], out[2];
-#pragma unroll
-    for (int k = 0; k < kAtOnceTokens; ++k) {
-      // (of a token that is not there: what the last one's queries gave once more, and nobody takes it)
-      const double* of = weight + (k0 + k) * 2 * D + part * 8;
-#pragma unroll
-      for (int i = 0; i < kSharedDepth; ++i) {
-        double above = 0.0, below = 0.0;                      // (two chains of sums: a wavefront has few others to wait beside)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          above = fma(of[e], high_of[i][e], above);
-          below = fma(of[D + e], low_of[i][e], below);
+          for (int e = 0; e < 8; ++e) {
+            low_of[i][e] = (double)l[e];
+            high_of[i][e] = (double)h[e];
+          }
         }
-        s[k * kSharedDepth + i] = above + below;
+      }
+#pragma unroll
+      for (int k0 = 0; k0 < kScoreTokens; k0 += kAtOnceTokens) {
+        if (k0 >= tile.tokens || j0 >= j1) break;
+        double s[8], out[2];
+#pragma unroll
+        for (int k = 0; k < kAtOnceTokens; ++k) {
+          // (of a token that is not there: what the last one's queries gave once more, and nobody takes it)
+          const double* of = weight + (k0 + k) * 2 * D + part * 8;
+#pragma unroll
+          for (int i = 0; i < kSharedDepth; ++i) {
+            double above = 0.0, below = 0.0;                  // (two chains of sums: a wavefront has few others to wait beside)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              above = fma(of[e], high_of[i][e], above);
+              below = fma(of[D + e], low_of[i][e], below);
+            }
+            s[k * kSharedDepth + i] = above + below;
+          }
+        }
+        sum_eight<kLanes>(s, lane, out);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int v = 4 * i + part, k = k0 + v / kSharedDepth, j = j0 + v % kSharedDepth * kAtOnce + which;
+          const int n = __shfl(mine, k & 7, kWave);
+          if (part < 4 && j < min(j1, n)) a.scores[((int64_t)(local + k) * a.hkv + kvh) * a.most + j] = score_of(out[i]);
+        }
       }
     }
-    sum_eight<kLanes>(s, lane, out);
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      const int v = 4 * m + part, k = k0 + v / kSharedDepth, j = j0 + v % kSharedDepth * kAtOnce + which;
-      const int n = __shfl(mine, k & 7, kWave);
-      if (part < 4 && j < min(j1, n)) a.scores[((int64_t)(local + k) * a.hkv + kvh) * a.most + j] = score_of(out[m]);
-    }
+    if (m + a.tiles_at_once >= tile.all) return;
+    __syncthreads();                                          // (the weights have been read)
   }
 }
 
@@ -553,15 +580,21 @@ struct AttendArgs {
   float* part_o;                 // [token][n_kv_heads][chunks][group][D], fp32
   float* part_ml;                // (reference, sum)
   int2* merged;                  // [n_kv_heads][token][keep], from a tile's first token on: the blocks of the tile, a bit for each token that lists them
-  int32_t* counts;               // [n_kv_heads][token]: blocks of the token's tile
-  int32_t* leads;                // ... tokens of the tile that it is the first of, or 0
+  int32_t* parts;                // [n_kv_heads][token]: chunks of the token's tile
+  int4* tiles;                   // [tile][n_kv_heads]: first token, tokens (0: there is no such tile), blocks, how many tiles there are
   int64_t q_token, q_head, table_stride, page_elems;
-  int batch, first, tokens, hq, hkv, group, page_shift, max_pages, keep, last_row, keys, chunk_keys, chunks, share;
+  int batch, first, tokens, hq, hkv, group, page_shift, max_pages, keep, last_row, keys, chunk_keys, chunks, share, tiles_at_once;
   float scale_log2;
 };
-// Keys of a chunk of a tile, whose lists may agree in all blocks or in none: the plan's number, or as many as its number of chunks takes.
-__device__ __forceinline__ int shared_chunk_keys(const AttendArgs& a, int keys) {
-  return max(a.chunk_keys, ((keys + a.chunks - 1) / a.chunks + 31) & -32);
+// Chunks of a tile of `keys` keys where there are so many tiles: as many units as the GPU holds at once (four of 39 KB a CU) end together, and some more wait for a round of
+// their own (128 tiles of 2933 keys, 8 heads' tiles of 16 sequences: 5 / 6 / 7 / 8 chunks 47.0 / 45.4 / 45.0 / 42.6 us, 9 / 10 54.5 / 52.2), so units are as many as that or a
+// multiple of it.  Short ones are a few trips to memory for little: a chunk has 64 keys at least, and 0.5 sqrt of all the tiles' keys.
+constexpr int kSharedKeys = 1024;
+constexpr int kUnitsAtOnce = 4 * 256;
+__host__ __device__ __forceinline__ int tile_chunks(int keys, int tiles) {
+  const int rounds = (int)(((int64_t)tiles * ((keys + kSharedKeys - 1) / kSharedKeys) + kUnitsAtOnce - 1) / kUnitsAtOnce);
+  const float least = fmaxf(64.f, 0.5f * sqrtf((float)tiles * (float)keys));
+  return max(1, min(max(rounds, 1) * kUnitsAtOnce / max(tiles, 1), (int)((float)keys / least)));
 }
 __device__ __forceinline__ int attend_last(const AttendArgs& a, int t) { return min(a.positions[t], a.last_row); }
 
@@ -570,47 +603,55 @@ constexpr int kUnionThreads = 256;
 constexpr int kUnionBlocks = 1 << 15;
 __global__ __launch_bounds__(kUnionThreads) void block_union_kernel(AttendArgs a) {
   __shared__ uint32_t marks[kUnionBlocks / 4];
-  __shared__ int sums[kUnionThreads / kWave];
-  const int local = blockIdx.x / a.hkv, kvh = blockIdx.x % a.hkv, t = a.first + local, tid = threadIdx.x, lane = tid & (kWave - 1);
-  const int at = kvh * a.tokens + local;
-  const TokenTile tile = token_tile(a.sequences, t, a.first, a.first + a.tokens, a.share);
-  if (tile.sequence >= a.batch || tile.tokens == 0) {        // (the whole workgroup)
-    if (tid == 0) a.leads[at] = 0;
-    return;
-  }
-  const int tokens = tile.tokens;
-  int most = 0;
-  for (int i = 0; i < tokens; ++i) most = max(most, (attend_last(a, t + i) >> a.page_shift) + 1);
-  const int words = (most + 3) / 4;
-  for (int w = tid; w < words; w += kUnionThreads) marks[w] = 0;
-  __syncthreads();
-  for (int n = tid; n < tokens * a.keep; n += kUnionThreads) {
-    const int i = n / a.keep, last = attend_last(a, t + i);
-    const int block = a.blocks[((int64_t)(t + i) * a.hkv + kvh) * a.keep + (n - i * a.keep)];
-    if (block >= 0 && last >= 0 && block <= last >> a.page_shift) atomicOr(&marks[block >> 2], 1u << (8 * (block & 3) + i));
-  }
-  __syncthreads();
-  const int per = (words + kUnionThreads - 1) / kUnionThreads, w0 = min(tid * per, words), w1 = min(w0 + per, words);
-  int mine = 0;
-  for (int w = w0; w < w1; ++w)
+  __shared__ int sums[kUnionThreads / kWave], places[8];
+  const int kvh = blockIdx.x % a.hkv, tid = threadIdx.x, lane = tid & (kWave - 1);
+  for (int m = blockIdx.x / a.hkv;; m += a.tiles_at_once) {
+    const TokenTile tile = token_tile(a.sequences, a.first, a.first + a.tokens, a.batch, a.share, m);
+    const int t = tile.first, tokens = tile.tokens, at = kvh * a.tokens + t - a.first;
+    if (tokens == 0) {                                       // (the whole workgroup; the tiles of a later m are looked for only if there are any)
+      if (tid == 0) a.tiles[m * a.hkv + kvh] = make_int4(0, 0, 0, 0);
+      return;
+    }
+    // the tokens' places and the first entries of their lists, asked for together
+    const int entries = tokens * a.keep, place = attend_last(a, t + min(lane, tokens - 1));
+    auto entry = [&](int n) {
+      const int i = n / a.keep;
+      return a.blocks[((int64_t)(t + i) * a.hkv + kvh) * a.keep + (n - i * a.keep)];
+    };
+    int block = entry(min(tid, entries - 1));
+    const int most = (int)lanes_largest((uint32_t)max((place >> a.page_shift) + 1, 0)), words = (most + 3) / 4;
+    if (tid < 8) places[tid] = place;
+    for (int w = tid; w < words; w += kUnionThreads) marks[w] = 0;
+    __syncthreads();
+    for (int n = tid; n < entries; n += kUnionThreads) {
+      const int i = n / a.keep, last = places[i];
+      if (n != tid) block = entry(n);
+      if (block >= 0 && last >= 0 && block <= last >> a.page_shift) atomicOr(&marks[block >> 2], 1u << (8 * (block & 3) + i));
+    }
+    __syncthreads();
+    const int per = (words + kUnionThreads - 1) / kUnionThreads, w0 = min(tid * per, words), w1 = min(w0 + per, words);
+    int mine = 0;
+    for (int w = w0; w < w1; ++w)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) mine += (marks[w] >> 8 * k & 0xff) != 0;
-  const int upto = (int)lanes_upto((uint32_t)mine);
-  if (lane == kWave - 1) sums[tid / kWave] = upto;
-  __syncthreads();
-  int before = upto - mine, count = 0;
+      for (int k = 0; k < 4; ++k) mine += (marks[w] >> 8 * k & 0xff) != 0;
+    const int upto = (int)lanes_upto((uint32_t)mine);
+    if (lane == kWave - 1) sums[tid / kWave] = upto;
+    __syncthreads();
+    int before = upto - mine, count = 0;
 #pragma unroll
-  for (int w = 0; w < kUnionThreads / kWave; ++w) {
-    if (w < tid / kWave) before += sums[w];
-    count += sums[w];
+    for (int w = 0; w < kUnionThreads / kWave; ++w) {
+      if (w < tid / kWave) before += sums[w];
+      count += sums[w];
+    }
+    int2* out = a.merged + (int64_t)at * a.keep;
+    for (int w = w0; w < w1; ++w)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (const int mark = marks[w] >> 8 * k & 0xff) out[before++] = make_int2(4 * w + k, mark);
+    if (tid == 0) a.tiles[m * a.hkv + kvh] = make_int4(t - a.first, tokens, count, tile.all);
+    if (m + a.tiles_at_once >= tile.all) return;
+    __syncthreads();                                         // (marks and sums have been read)
   }
-  int2* out = a.merged + (int64_t)at * a.keep;
-  for (int w = w0; w < w1; ++w)
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (const int mark = marks[w] >> 8 * k & 0xff) out[before++] = make_int2(4 * w + k, mark);
-  if (tid < tokens) a.counts[at + tid] = count;
-  if (tid == 0) a.leads[at] = tokens;
 }
 
 template <int D> __device__ __forceinline__ int attend_k_swap(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
@@ -619,7 +660,7 @@ template <int D> __device__ __forceinline__ int attend_v_swap(int row) { return 
 // Chunk `chunk` of the rows listed for `tokens` tokens from t on.  Where several share it, a row of the pool that one of them does not see has the probability 0 for it, and 0
 // times an infinity or a NaN is no 0: true then (and nothing written), for the tokens' results to be found one after the other, `alone`, with zeros in such rows.
 template <int DT, int D, int ROWT, bool SHARED>
-__device__ __forceinline__ bool attend_unit(const AttendArgs& a, int kvh, int chunk, int t, int tokens, int keys, int chunk_keys, int alone) {
+__device__ __forceinline__ bool attend_unit(const AttendArgs& a, int kvh, int chunk, int t, int b, int tokens, int keys, int chunk_keys, int alone) {
   constexpr int kRowBytes = D * 2, kPieces = kRowBytes / 16, kRowsPerCopy = 64 / kPieces, kCopies = kAttendKeys / kRowsPerCopy;
   constexpr int kHalf = kAttendKeys * kRowBytes, kStage = 2 * kHalf;
   __shared__ __attribute__((aligned(1024))) uint8_t ring[kAttendStages * kStage];
@@ -627,11 +668,31 @@ __device__ __forceinline__ bool attend_unit(const AttendArgs& a, int kvh, int ch
   __shared__ uint32_t seen_at[kAttendSegment / kAttendKeys];
   __shared__ __attribute__((aligned(16))) int place_at[SHARED ? kAttendSegment : 4];        // a key's row of the sequence, and its block's bits
   __shared__ uint32_t bits_at[SHARED ? kAttendSegment / 4 : 1];
-  const int b = a.sequences[t], local = t - a.first;
-  if (b < 0 || b >= a.batch) return false;
-  const int v_begin = chunk * chunk_keys, v_end = min(v_begin + chunk_keys, keys);
-  if (SHARED && chunk > 0 && v_begin >= keys) return false;  // (the merge knows how many there are)
+  const int v_begin = chunk * chunk_keys, v_end = min(v_begin + chunk_keys, keys), local = t - a.first;
   const int lane = threadIdx.x, lq = lane & 15, lg = lane >> 4, rows = tokens * a.group;
+  const int32_t* list = a.blocks + ((int64_t)t * a.hkv + kvh) * a.keep;
+  const int2* merged = a.merged + ((int64_t)kvh * a.tokens + local) * a.keep;
+  const int32_t* row_pages = a.table + b * a.table_stride;
+  // The blocks of a segment's rows, and then their pages: each asked for all at once.  One after the other they are a trip to memory for every 64 rows and more
+  // than the rows' own way takes.
+  int block[kAttendSegment / 64], bits[kAttendSegment / 64];
+  auto look_at = [&](int v0) {
+#pragma unroll
+    for (int u = 0; u < kAttendSegment / 64; ++u) {
+      block[u] = -1;
+      bits[u] = 1;
+      if (u * 64 >= v_end - v0) continue;
+      const int at = min(v0 + u * 64 + lane, v_end - 1) >> a.page_shift;
+      if constexpr (SHARED) {
+        const int2 entry = merged[at];
+        block[u] = entry.x;
+        bits[u] = entry.y;
+      } else {
+        block[u] = list[at];
+      }
+    }
+  };
+  look_at(v_begin);
 
   dec_u4 q[ROWT][D / 32];
   int token[ROWT], place[ROWT];                              // of a row: its token in the tile, the last row it sees
@@ -671,39 +732,36 @@ __device__ __forceinline__ bool attend_unit(const AttendArgs& a, int kvh, int ch
   const uint32_t koff = ring0 + lq * kRowBytes;
   const uint32_t voff = ring0 + kHalf + (4 * lg + (lq >> 2)) * kRowBytes + (lq & 1) * 8;
   const int kswap = attend_k_swap<D>(lq), vswap = attend_v_swap<D>(4 * lg + (lq >> 2)), vpiece = (lq >> 1) & 1;
-  const int32_t* list = a.blocks + ((int64_t)t * a.hkv + kvh) * a.keep;
-  const int2* merged = a.merged + ((int64_t)kvh * a.tokens + local) * a.keep;
-  const int32_t* row_pages = a.table + b * a.table_stride;
 
   for (int v0 = v_begin; v0 < v_end; v0 += kAttendSegment) {
     int stages = 0;                                          // up to the last one of which something is seen
+    if (v0 > v_begin) look_at(v0);
+    uint32_t sees = 0;                                       // a bit for each of the lane's rows
+    int page[kAttendSegment / 64];
+#pragma unroll
+    for (int u = 0; u < kAttendSegment / 64; ++u) {
+      page[u] = 0;
+      if (u * 64 >= v_end - v0) continue;
+      const int v = v0 + u * 64 + lane, in = v & ((1 << a.page_shift) - 1);
+      bool there = v < v_end && block[u] >= 0 && last >= 0 && block[u] <= last >> a.page_shift && (block[u] << a.page_shift) + in <= last;
+      if (SHARED && alone >= 0) there = there && (bits[u] >> alone & 1);
+      sees |= (uint32_t)there << u;
+      page[u] = row_pages[there ? block[u] : 0];
+    }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
     for (int u = 0; u < kAttendSegment / 64; ++u) {
       if (u * 64 >= v_end - v0) continue;
-      const int v = v0 + u * 64 + lane;
-      const int in = v & ((1 << a.page_shift) - 1);
-      int block = -1, bits = 1;
-      if constexpr (SHARED) {
-        if (v < v_end) {
-          const int2 entry = merged[v >> a.page_shift];
-          block = entry.x;
-          bits = entry.y;
-        }
-      } else if (v < v_end) {
-        block = list[v >> a.page_shift];
-      }
-      bool sees = block >= 0 && last >= 0 && block <= last >> a.page_shift && (block << a.page_shift) + in <= last;
-      if (SHARED && alone >= 0) sees = sees && (bits >> alone & 1);
-      const int page = sees ? min(max(row_pages[block], 0), a.max_pages - 1) : 0;
-      row_at[u * 64 + lane] = sees ? 2 * ((int64_t)page * 2 * a.page_elems + (int64_t)a.hkv * D * in) : -1;
-      const uint64_t some = __ballot(sees);
+      const bool there = sees >> u & 1;
+      const int in = (v0 + u * 64 + lane) & ((1 << a.page_shift) - 1);
+      row_at[u * 64 + lane] = there ? 2 * ((int64_t)min(max(page[u], 0), a.max_pages - 1) * 2 * a.page_elems + (int64_t)a.hkv * D * in) : -1;
+      const uint64_t some = __ballot(there);
       uint64_t all = some;                                   // (shared: seen by all rows)
       if constexpr (SHARED) {
-        const int row = sees ? (block << a.page_shift) + in : INT32_MAX;
+        const int row = there ? (block[u] << a.page_shift) + in : INT32_MAX;
         place_at[u * 64 + lane] = row;
-        ((uint8_t*)bits_at)[u * 64 + lane] = (uint8_t)bits;
-        all = __ballot(row <= least && bits == (1 << tokens) - 1);
+        ((uint8_t*)bits_at)[u * 64 + lane] = (uint8_t)bits[u];
+        all = __ballot(row <= least && bits[u] == (1 << tokens) - 1);
       }
       if (lane < 2) seen_at[u * 2 + lane] = (uint32_t)(all >> (32 * lane));
       if (some) stages = u * 2 + (some >> 32 ? 2 : 1);
@@ -739,21 +797,25 @@ __device__ __forceinline__ bool attend_unit(const AttendArgs& a, int kvh, int ch
       v4f s[ROWT][2];
 #pragma unroll
       for (int nt = 0; nt < ROWT; ++nt) s[nt][0] = s[nt][1] = v4f{0.f, 0.f, 0.f, 0.f};
+      // a stage's pieces asked for together: left to itself the compiler waits for each before it asks for the next
+      dec_u4 kt[D / 32][2], vt[D / 16];
 #pragma unroll
       for (int ks = 0; ks < D / 32; ++ks)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const dec_u4 k = lds_16(koff + at + h * 16 * kRowBytes + (((ks * 4 + lg) ^ kswap) << 4));
-#pragma unroll
-          for (int nt = 0; nt < ROWT; ++nt) s[nt][h] = mfma16x16x32<DT>(k, q[nt][ks], s[nt][h]);
-        }
-      dec_u4 vt[D / 16];
+        for (int h = 0; h < 2; ++h) kt[ks][h] = lds_16(koff + at + h * 16 * kRowBytes + (((ks * 4 + lg) ^ kswap) << 4));
 #pragma unroll
       for (int mt = 0; mt < D / 16; ++mt) {
         const uint32_t va = voff + at + (((mt * 2 + vpiece) ^ vswap) << 4);
         const uint2 lo = lds_tr16(va), hi = lds_tr16(va + 16 * kRowBytes);
         vt[mt] = dec_u4{lo.x, lo.y, hi.x, hi.y};
       }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int ks = 0; ks < D / 32; ++ks)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int nt = 0; nt < ROWT; ++nt) s[nt][h] = mfma16x16x32<DT>(kt[ks][h], q[nt][ks], s[nt][h]);
       dec_i4 places[2] = {};
       uint32_t bits[2] = {};
       if (SHARED && seen != ~0u) {
@@ -768,7 +830,7 @@ __device__ __forceinline__ bool attend_unit(const AttendArgs& a, int kvh, int ch
       for (int nt = 0; nt < ROWT; ++nt) {
         float x[8];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) x[r] = s[nt][r >> 2][r & 3] * a.scale_log2;
+        for (int r = 0; r < 8; ++r) x[r] = s[nt][r >> 2][r & 3];
         if (seen != ~0u) {
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
@@ -778,7 +840,7 @@ __device__ __forceinline__ bool attend_unit(const AttendArgs& a, int kvh, int ch
             if (!there) x[r] = -INFINITY;
           }
         }
-        const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))) * a.scale_log2;
         if (__any(top > ref[nt] + kSlack)) {                 // (also where the reference is still -inf)
           float m = fmaxf(top, __shfl_xor(top, 16, kWave));
           m = fmaxf(m, __shfl_xor(m, 32, kWave));
@@ -792,7 +854,7 @@ __device__ __forceinline__ bool attend_unit(const AttendArgs& a, int kvh, int ch
         const float base = ref[nt] == -INFINITY ? 0.f : ref[nt];
         float e[8];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) e[r] = __builtin_amdgcn_exp2f(x[r] - base);
+        for (int r = 0; r < 8; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(x[r], a.scale_log2, -base));
         l[nt] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
         pb[nt] = pack8<DT>(e);
         float near[8];
@@ -800,14 +862,12 @@ __device__ __forceinline__ bool attend_unit(const AttendArgs& a, int kvh, int ch
 #pragma unroll
         for (int r = 0; r < 8; ++r) e[r] -= near[r];
         rest[nt] = pack8<DT>(e);
-      }
 #pragma unroll
-      for (int mt = 0; mt < D / 16; ++mt)
-#pragma unroll
-        for (int nt = 0; nt < ROWT; ++nt) {
+        for (int mt = 0; mt < D / 16; ++mt) {
           o[nt][mt] = mfma16x16x32<DT>(vt[mt], pb[nt], o[nt][mt]);
           o[nt][mt] = mfma16x16x32<DT>(vt[mt], rest[nt], o[nt][mt]);
         }
+      }
       if (st + kAttendStages < stages) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the stage has been read
         request(st + kAttendStages);
@@ -854,14 +914,30 @@ __global__ __launch_bounds__(kWave) void block_attention_kernel(AttendArgs a) {
   const uint32_t unit = blockIdx.x, tc = unit / (uint32_t)a.hkv;
   const int kvh = (int)(unit % (uint32_t)a.hkv), chunk = (int)(tc % (uint32_t)a.chunks), local = (int)(tc / (uint32_t)a.chunks);
   if constexpr (!SHARED) {
-    attend_unit<DT, D, ROWT, false>(a, kvh, chunk, a.first + local, 1, a.keys, a.chunk_keys, -1);
+    const int b = a.sequences[a.first + local];
+    if (b >= 0 && b < a.batch) attend_unit<DT, D, ROWT, false>(a, kvh, chunk, a.first + local, b, 1, a.keys, a.chunk_keys, -1);
   } else {
-    const int tokens = a.leads[kvh * a.tokens + local];      // (0: of no sequence, or in another's tile)
-    if (tokens == 0) return;
-    const int keys = a.counts[kvh * a.tokens + local] << a.page_shift;
-    for (int alone = -1; alone < tokens;) {
-      const bool apart = attend_unit<DT, D, ROWT, true>(a, kvh, chunk, a.first + local, tokens, keys, shared_chunk_keys(a, keys), alone);
-      alone = alone < 0 && !apart ? tokens : alone + 1;
+    // its first token, how many it has, their blocks; the tiles of the call
+    auto tile_of = [&](int m) {
+      const int4 v = a.tiles[m * a.hkv + kvh];
+      return make_int4(__builtin_amdgcn_readfirstlane(v.x), __builtin_amdgcn_readfirstlane(v.y), __builtin_amdgcn_readfirstlane(v.z),
+                       __builtin_amdgcn_readfirstlane(v.w));
+    };
+    int4 tile = tile_of(local);
+    if (tile.y == 0) return;
+    for (int m = local, alone = -1;;) {
+      const int t = a.first + tile.x, keys = tile.z << a.page_shift, chunks = min(tile_chunks(keys, tile.w * a.hkv), a.chunks);
+      if (chunk < chunks) {
+        if (chunk == 0 && (int)threadIdx.x < tile.y) a.parts[kvh * a.tokens + tile.x + threadIdx.x] = chunks;
+        const int each = ((keys + chunks - 1) / chunks + kAttendKeys - 1) / kAttendKeys * kAttendKeys;
+        const bool apart = attend_unit<DT, D, ROWT, true>(a, kvh, chunk, t, a.sequences[t], tile.y, keys, each, alone);
+        alone = alone < 0 && !apart ? tile.y : alone + 1;
+        if (alone < tile.y) continue;
+      }
+      alone = -1;
+      m += a.tiles_at_once;
+      if (m >= tile.w) return;
+      tile = tile_of(m);
     }
   }
 }
@@ -888,10 +964,7 @@ __global__ __launch_bounds__(256) void block_merge_kernel(AttendArgs a, int64_t 
   v2f mine = *(const v2f*)(ml + (int64_t)min(lane, a.chunks - 1) * a.group * 2);
   if (b < 0 || b >= a.batch) return;
   int chunks = a.chunks;
-  if (a.share) {
-    const int keys = a.counts[kvh * a.tokens + (t - a.first)] << a.page_shift, chunk_keys = shared_chunk_keys(a, keys);
-    chunks = max(1, (keys + chunk_keys - 1) / chunk_keys);
-  }
+  if (a.share) chunks = min(max(a.parts[kvh * a.tokens + (t - a.first)], 1), a.chunks);
   float top = lane < chunks ? mine[0] : -INFINITY;
   for (int c = lane + kWave; c < chunks; c += kWave) top = fmaxf(top, ml[(int64_t)c * a.group * 2]);
   top = wave_max(top);
@@ -935,7 +1008,7 @@ __global__ __launch_bounds__(256) void block_merge_kernel(AttendArgs a, int64_t 
 }
 
 // Tokens of a sequence that share a unit (1: none do), chunks of a unit's rows, tokens whose partial results are held at a time.
-struct AttendPlan { int share, chunk_keys, chunks; int64_t tokens; size_t part_o, part_ml, merged, counts, bytes; };
+struct AttendPlan { int share, chunk_keys, chunks; int64_t tokens; size_t part_o, part_ml, tiles, merged, parts, bytes; };
 static AttendPlan attend_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64_t hkv, int64_t head_dim, int64_t page_len, int64_t max_blocks, int64_t keep) {
   AttendPlan p{};
   const int64_t group = hq / hkv;
@@ -944,24 +1017,32 @@ static AttendPlan attend_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64
     while (p.share < 8 && 2 * p.share * group <= kShareRows) p.share *= 2;
   // rows of a unit: those of a token, or, of several, as many as lists that agree in most blocks have together
   const int64_t most = std::min(p.share * keep, std::max(max_blocks, keep)) * page_len, keys = p.share > 1 ? std::min(most, 2 * keep * page_len) : keep * page_len;
-  const int64_t units = std::max<int64_t>(1, n_tokens / p.share) * hkv;
-  int64_t per = ((int64_t)(0.65 * std::sqrt((double)units * (double)keys)) + kAttendKeys - 1) / kAttendKeys * kAttendKeys;
-  per = std::min<int64_t>(std::max<int64_t>(per, 64), p.share > 1 ? 256 : 384);
+  // (where several share: as many tiles as sequences, or as their tokens fill)
+  const int64_t units = (p.share > 1 ? std::max<int64_t>(std::min<int64_t>(n_tokens, batch), std::min<int64_t>(n_tokens, kTileTokens) / p.share) : n_tokens) * hkv;
+  int64_t per;
+  if (p.share > 1) {
+    const int64_t chunks = tile_chunks((int)keys, (int)units);
+    per = (keys + chunks - 1) / chunks;
+  } else {
+    per = ((int64_t)(0.65 * std::sqrt((double)units * (double)keys)) + kAttendKeys - 1) / kAttendKeys * kAttendKeys;
+    per = std::min<int64_t>(std::max<int64_t>(per, 64), 384);
+  }
   while (keys > per * 256) per *= 2;
   p.chunk_keys = (int)per;
   p.chunks = (int)((keys + per - 1) / per);
-  p.tokens = n_tokens;
-  if (p.chunks > 1) p.tokens = std::min<int64_t>(n_tokens, std::max<int64_t>(64, (1 << 20) / (hq * p.chunks)));      // half a gigabyte at 128 a head
+  p.tokens = p.share > 1 ? std::min<int64_t>(n_tokens, kTileTokens) : n_tokens;
+  if (p.chunks > 1) p.tokens = std::min<int64_t>(p.tokens, std::max<int64_t>(64, (1 << 20) / (hq * p.chunks)));      // half a gigabyte at 128 a head
   const size_t slots = (size_t)p.tokens * hq * p.chunks;
   if (p.chunks > 1) {
     p.part_o = align_up(slots * head_dim * sizeof(float), 256);
     p.part_ml = align_up(slots * 2 * sizeof(float), 256);
   }
   if (p.share > 1) {
+    p.tiles = align_up((size_t)p.tokens * hkv * sizeof(int4), 256);
     p.merged = align_up((size_t)p.tokens * hkv * keep * sizeof(int2), 256);
-    p.counts = align_up((size_t)p.tokens * hkv * sizeof(int32_t), 256);
+    p.parts = align_up((size_t)p.tokens * hkv * sizeof(int32_t), 256);
   }
-  p.bytes = 256 + p.part_o + p.part_ml + p.merged + 2 * p.counts;
+  p.bytes = 256 + p.part_o + p.part_ml + p.tiles + p.merged + p.parts;
   return p;
 }
 
@@ -977,14 +1058,15 @@ static void launch_scores(SelectArgs a, hipStream_t st) {
   const bool shared = a.tokens > a.batch;
   a.span = kScoreThreads / (D / 8) * (shared ? kSharedDepth : 8);
   a.spans = (int)((a.most + a.span - 1) / a.span);
-  const dim3 grid((unsigned)((int64_t)a.tokens * a.hkv * a.spans)), block(kScoreThreads);
+  a.tiles_at_once = tiles_at_once(a.tokens, a.batch, kScoreTokens);
+  const dim3 grid((unsigned)((int64_t)(shared ? a.tiles_at_once : a.tokens) * a.hkv * a.spans)), block(kScoreThreads);
   if (shared) hipLaunchKernelGGL((block_score_shared_kernel<DT, D>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((block_score_kernel<DT, D>), grid, block, 0, st, a);
 }
 
 template <int DT, int D>
 static void launch_attend_of(const AttendArgs& a, int64_t tokens, hipStream_t st) {
-  const dim3 grid((unsigned)(tokens * a.chunks * a.hkv)), block(kWave);
+  const dim3 grid((unsigned)((a.share ? a.tiles_at_once : tokens) * a.chunks * a.hkv)), block(kWave);
   if (a.share) {
     if (a.share * a.group <= 16) hipLaunchKernelGGL((block_attention_kernel<DT, D, 1, true>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((block_attention_kernel<DT, D, 2, true>), grid, block, 0, st, a);
@@ -1091,7 +1173,8 @@ extern "C" int subspec_select_blocks(const void* q, int64_t q_token_stride, int6
   a.batch = (int)batch; a.hkv = (int)n_kv_heads; a.group = (int)(n_q_heads / n_kv_heads);
   a.page_shift = block_shift_of(page_len); a.max_pages = (int)max_pages; a.keep = (int)keep; a.recent = (int)recent;
   a.last_row = (int)(std::min(max_kv, max_blocks * page_len) - 1);
-  const int64_t at_once = select_tokens(n_tokens, n_kv_heads, most);
+  int64_t at_once = select_tokens(n_tokens, n_kv_heads, most);
+  if (n_tokens > batch && most > keep) at_once = std::min<int64_t>(at_once, kTileTokens);
   hipStream_t st = (hipStream_t)stream;
   for (int64_t first = 0; first < n_tokens; first += at_once) {
     const int64_t some = std::min(at_once, n_tokens - first);
@@ -1154,9 +1237,9 @@ extern "C" int subspec_block_attention(const void* q, int64_t q_token_stride, in
   char* ws = (char*)workspace;
   a.part_o = (float*)ws; ws += p.part_o;
   a.part_ml = (float*)ws; ws += p.part_ml;
+  a.tiles = (int4*)ws; ws += p.tiles;
   a.merged = (int2*)ws; ws += p.merged;
-  a.counts = (int32_t*)ws; ws += p.counts;
-  a.leads = (int32_t*)ws;
+  a.parts = (int32_t*)ws;
   a.share = p.share > 1 ? p.share : 0;
   a.q_token = q_token_stride; a.q_head = q_head_stride; a.table_stride = table_stride; a.page_elems = page_len * n_kv_heads * head_dim;
   a.batch = (int)batch; a.hq = (int)n_q_heads; a.hkv = (int)n_kv_heads; a.group = (int)(n_q_heads / n_kv_heads);
@@ -1171,7 +1254,10 @@ extern "C" int subspec_block_attention(const void* q, int64_t q_token_stride, in
     const int64_t some = std::min(p.tokens, n_tokens - first);
     a.first = (int)first;
     a.tokens = (int)some;
-    if (a.share) hipLaunchKernelGGL(block_union_kernel, dim3((unsigned)(some * n_kv_heads)), dim3(kUnionThreads), 0, st, a);
+    if (a.share) {
+      a.tiles_at_once = tiles_at_once(some, batch, a.share);
+      hipLaunchKernelGGL(block_union_kernel, dim3((unsigned)(a.tiles_at_once * n_kv_heads)), dim3(kUnionThreads), 0, st, a);
+    }
     {
       DominantKernelTimer timer(st);
       if (dtype == SUBSPEC_BF16) {
