@@ -5,6 +5,7 @@
 // one page, block_table[sequence][j].  A token at position pos sees rows 0 .. pos, so blocks 0 .. c = pos / page_len, of which all but c
 // are full and hold nothing behind it.
 #include "paged.h"
+#include "sample.h"
 #include <algorithm>
 #include <cmath>
 
@@ -19,74 +20,98 @@ static int block_shift_of(int64_t page_len) {
 // ---------------------------------------------------------------------------------------------------------------- bounds
 // low_d = min over the page's rows of K_d, high_d = max, of every page whose last row is among the slots: the rows of a page are
 // written in order, so it is full then, and its bounds come from the page alone (nothing is read, changed and written back).
+// A wavefront takes a slice of 16 pieces (16 bytes each; 8 where a row has no more) of the pages whose last rows are among eight slots, several rows at a time with up
+// to sixteen requests a lane under way.  Its lanes meet through registers, so nobody waits for anybody, and a wavefront without such a page leaves.
+// As whole numbers that rise with the value: the bits of a negative value but its sign turned round.  A NaN is then above +infinity or below -infinity, so the
+// least and the largest say if there is one, and two values of either type take five instructions where a comparison in 32 bits that keeps a NaN takes sixteen.
+// Bound by the trips slots -> rows -> bounds: 61 slots 2.6 us, of which a launch is 2; 8191 rows of 8 heads of 128 in pages of 16 rows (18.9 MB) 5.6 (3.4 TB/s), of 1 row (50 MB)
+// 15.5, of 256 (16.4 MB) 14.6.  With a workgroup a slot, all of a page's pieces in it: 6.0, 7.5, 27 and 64; 4 / 16 slots a wavefront 8.8 / 4.8 for the second, but then sixteen
+// pages that fill up in one step follow each other.
 constexpr int kBoundsThreads = 256;
+constexpr int kBoundsSlots = 8;
+typedef short dec_s2 __attribute__((ext_vector_type(2)));
 struct BoundsArgs {
   const uint16_t* pool;
   uint16_t* bounds;              // [max_pages][n_kv_heads][2 (low, high)][head_dim]
   const int64_t* slots;
   int64_t n_slots, page_elems;
-  int n_tokens, per, page_shift, pieces, head_pieces;         // tokens of a workgroup; 16-byte pieces of a token's K, of a head's
+  int n_tokens, page_shift, pieces, head_pieces, slices, slices_shift, infinity;      // 16-byte pieces of a token's K, of a head's; slices of a workgroup, as a power of two
 };
-// a NaN stays: it is neither above nor below, and hides nothing
-__device__ __forceinline__ float lower_of(float a, float b) { return b < a || b != b ? b : a; }
-__device__ __forceinline__ float upper_of(float a, float b) { return b > a || b != b ? b : a; }
+__device__ __forceinline__ dec_s2 ordered(dec_s2 v) { return v ^ (v >> 15 & 0x7fff); }          // (and back)
 
-template <int DT>
+template <int LANES, int AT_ONCE>
 __global__ __launch_bounds__(kBoundsThreads) void page_bounds_kernel(BoundsArgs a) {
-  __shared__ __attribute__((aligned(16))) float side[kBoundsThreads][16];
-  const int tid = threadIdx.x, page_len = 1 << a.page_shift;
-  const int lanes = min(a.pieces, kBoundsThreads), groups = kBoundsThreads / lanes, group = tid / lanes, lane = tid % lanes;
-  // every wavefront looks the workgroup's slots over, together: one after the other they would be sixteen trips to memory
-  const int t = blockIdx.x * a.per + (tid & (kWave - 1));
-  const int64_t slot = (tid & (kWave - 1)) < a.per && t < a.n_tokens ? a.slots[t] : -1;
-  uint64_t last_rows = __ballot(slot >= 0 && slot < a.n_slots && (slot & (page_len - 1)) == page_len - 1);
-  for (; last_rows; last_rows &= last_rows - 1) {                                                // (the same in all wavefronts)
-    const int64_t page = __shfl((long long)slot, __ffsll((unsigned long long)last_rows) - 1, kWave) >> a.page_shift;
-    const dec_u4* rows = (const dec_u4*)(a.pool + page * 2 * a.page_elems);
-    dec_u4* out = (dec_u4*)(a.bounds + page * 2 * (a.page_elems >> a.page_shift));
-    for (int p0 = 0; p0 < a.pieces; p0 += lanes) {
-      const int piece = p0 + lane;
-      const bool mine = group < groups && piece < a.pieces;
-      float low[8], high[8];
+  constexpr int kRows = kWave / LANES;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, page_len = 1 << a.page_shift, row = lane / LANES;
+  const int slice = (blockIdx.y << a.slices_shift) + (wave & ((1 << a.slices_shift) - 1)), piece = slice * LANES + lane % LANES, from = min(piece, a.pieces - 1);
+  if (slice >= a.slices) return;
+  // a prompt's last rows come at equal distances: every XCD (each eighth workgroup) has neighbouring groups, or one of them would have all the work
+  const int64_t apart = (int64_t)gridDim.x * (kBoundsThreads / kWave >> a.slices_shift), block = (int64_t)(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
+  for (int64_t group = block * (kBoundsThreads / kWave >> a.slices_shift) + (wave >> a.slices_shift); group * kBoundsSlots < a.n_tokens; group += apart) {
+    const int64_t t = group * kBoundsSlots + lane;
+    const int64_t slot = lane < kBoundsSlots && t < a.n_tokens ? a.slots[t] : -1;
+    uint64_t last_rows = __ballot(slot >= 0 && slot < a.n_slots && (slot & (page_len - 1)) == page_len - 1);
+    for (; last_rows; last_rows &= last_rows - 1) {
+      const int64_t page = (int64_t)lane_u64((uint64_t)slot, __ffsll((unsigned long long)last_rows) - 1) >> a.page_shift;
+      const dec_u4* rows = (const dec_u4*)(a.pool + page * 2 * a.page_elems) + from;
+      dec_s2 low[4], high[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        low[e] = INFINITY;
-        high[e] = -INFINITY;
+      for (int e = 0; e < 4; ++e) {
+        low[e] = dec_s2{32767, 32767};
+        high[e] = dec_s2{-32768, -32768};
       }
-      if (mine) {
-#pragma unroll 8
-        for (int r = group; r < page_len; r += groups) {
-          float x[8];
-          unpack8<DT>(rows[(int64_t)r * a.pieces + piece], x);
+      for (int r0 = 0; r0 < page_len; r0 += kRows * AT_ONCE) {
+        dec_u4 raw[AT_ONCE];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            low[e] = lower_of(low[e], x[e]);
-            high[e] = upper_of(high[e], x[e]);
+        for (int k = 0; k < AT_ONCE; ++k) raw[k] = rows[(int64_t)min(r0 + k * kRows + row, page_len - 1) * a.pieces];       // (past the end: the last row again)
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const dec_s2 x = ordered(__builtin_bit_cast(dec_s2, (uint32_t)raw[k][e]));
+            low[e] = __builtin_elementwise_min(low[e], x);
+            high[e] = __builtin_elementwise_max(high[e], x);
           }
-        }
       }
-      if (groups > 1) {
+      if (page_len > 1) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          side[tid][e] = low[e];
-          side[tid][8 + e] = high[e];
-        }
-        __syncthreads();
-        if (group == 0)
-          for (int g = 1; g < groups; ++g)
+        for (int o = LANES; o < kWave; o <<= 1)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              low[e] = lower_of(low[e], side[g * lanes + lane][e]);
-              high[e] = upper_of(high[e], side[g * lanes + lane][8 + e]);
-            }
-        __syncthreads();
+          for (int e = 0; e < 4; ++e) {
+            low[e] = __builtin_elementwise_min(low[e], __builtin_bit_cast(dec_s2, __shfl_xor(__builtin_bit_cast(int, low[e]), o, kWave)));
+            high[e] = __builtin_elementwise_max(high[e], __builtin_bit_cast(dec_s2, __shfl_xor(__builtin_bit_cast(int, high[e]), o, kWave)));
+          }
       }
-      if (mine && group == 0) {
-        dec_u4* to = out + (piece / a.head_pieces) * 2 * a.head_pieces + piece % a.head_pieces;
-        to[0] = pack8<DT>(low);
-        to[a.head_pieces] = pack8<DT>(high);
+      if (piece < a.pieces && row < 2) {
+        dec_u4 out;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          dec_s2 v = ordered(row ? high[e] : low[e]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (high[e][i] > a.infinity || low[e][i] < ~a.infinity) v[i] = 0x7fff;                // (the order has -infinity at ~infinity)
+          out[e] = __builtin_bit_cast(uint32_t, v);
+        }
+        dec_u4* to = (dec_u4*)(a.bounds + page * 2 * (a.page_elems >> a.page_shift)) + (piece / a.head_pieces) * 2 * a.head_pieces + piece % a.head_pieces;
+        to[row * a.head_pieces] = out;
       }
     }
+  }
+}
+static void launch_bounds(BoundsArgs a, int lanes, hipStream_t st) {
+  a.slices = (a.pieces + lanes - 1) / lanes;
+  a.slices_shift = a.slices >= 4 ? 2 : a.slices >= 2 ? 1 : 0;
+  const int64_t groups = ((int64_t)a.n_tokens + kBoundsSlots - 1) / kBoundsSlots, of_block = kBoundsThreads / kWave >> a.slices_shift;
+  const dim3 grid((unsigned)std::min<int64_t>(((groups + of_block - 1) / of_block + 7) / 8 * 8, 1 << 16), (unsigned)((a.slices + (1 << a.slices_shift) - 1) >> a.slices_shift)), block(kBoundsThreads);
+  const int rows = (1 << a.page_shift) * lanes / kWave;      // of a lane
+  if (lanes == 8) {
+    if (rows <= 1) hipLaunchKernelGGL((page_bounds_kernel<8, 1>), grid, block, 0, st, a);
+    else if (rows < 16) hipLaunchKernelGGL((page_bounds_kernel<8, 4>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((page_bounds_kernel<8, 16>), grid, block, 0, st, a);
+  } else {
+    if (rows <= 1) hipLaunchKernelGGL((page_bounds_kernel<16, 1>), grid, block, 0, st, a);
+    else if (rows < 16) hipLaunchKernelGGL((page_bounds_kernel<16, 4>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((page_bounds_kernel<16, 16>), grid, block, 0, st, a);
   }
 }
 
@@ -1120,12 +1145,10 @@ extern "C" int subspec_kv_page_bounds(const void* kv_pool_layer, void* bounds, i
   a.n_slots = max_pages * page_len; a.page_elems = page_len * n_kv_heads * head_dim;
   a.n_tokens = (int)n_tokens; a.page_shift = block_shift_of(page_len);
   a.pieces = (int)(n_kv_heads * head_dim / 8); a.head_pieces = (int)(head_dim / 8);
-  a.per = n_tokens > 4096 ? 16 : 1;
+  a.infinity = dtype == SUBSPEC_BF16 ? 0x7f80 : 0x7c00;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)((n_tokens + a.per - 1) / a.per)), block(kBoundsThreads);
   DominantKernelTimer timer(st);
-  if (dtype == SUBSPEC_BF16) hipLaunchKernelGGL(page_bounds_kernel<SUBSPEC_BF16>, grid, block, 0, st, a);
-  else hipLaunchKernelGGL(page_bounds_kernel<SUBSPEC_F16>, grid, block, 0, st, a);
+  launch_bounds(a, a.pieces <= 8 ? 8 : 16, st);
   SUBSPEC_CHECK_HIP(hipGetLastError());
   return SUBSPEC_OK;
 }

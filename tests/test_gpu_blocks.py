@@ -42,6 +42,22 @@ def test_bounds(dtype, tokens, heads, D, page_len):
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0))
 
 
+@pytest.mark.parametrize("dtype,nans", [(torch.bfloat16, [0x7f81, 0xff81, 0x7fff, 0xffff]), (torch.float16, [0x7c01, 0xfc01, 0x7fff, 0xffff])])
+def test_bounds_of_every_nan_and_of_the_largest_numbers(dtype, nans):
+    """Every kind of NaN stays one, in both; infinities, the largest and the smallest numbers of either sign and the zeros are numbers like others."""
+    top = torch.finfo(dtype).max
+    pool = torch.randn(12, 2, 8, 1, 64, generator=torch.Generator().manual_seed(3)).to(dtype)
+    for page, bits in enumerate(nans):
+        pool.view(torch.int16)[page, 0, 3, 0, 5] = bits - (1 << 16) if bits >= 1 << 15 else bits
+    for page, values in ((4, [math.inf] * 8), (5, [-math.inf] * 8), (6, [math.inf, -math.inf] * 4), (7, [top, -top] * 4), (8, [-top] * 8),
+                         (9, [0.0, -0.0] * 4), (10, [2.0 ** -24 if dtype is torch.float16 else 2.0 ** -133, -1.0] * 4)):
+        pool[page, 0, :, 0, 9] = torch.tensor(values).to(dtype)
+    slots = torch.arange(12 * 8)
+    want = ok.page_bounds(torch.zeros(12, 1, 2, 64, dtype=dtype), pool, slots.tolist())
+    got = ops.kv_page_bounds_(torch.zeros(12, 1, 2, 64, dtype=dtype, device=DEV), pool.to(DEV), slots.to(DEV)).cpu()
+    assert got[:4, 0, :, 5].isnan().all() and torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0))
+
+
 def test_a_page_named_twice_and_nothing_at_all():
     pool = torch.randn(3, 2, 4, 2, 64, device=DEV).to(torch.bfloat16)
     bounds = torch.zeros(3, 2, 2, 64, device=DEV, dtype=torch.bfloat16)
