@@ -377,7 +377,8 @@ int subspec_kv_page_bounds(const void* kv_pool_layer, void* bounds, int dtype, i
 /* Blocks for every (token, KV head): the last `recent` that the token sees (its own among them), and of the others the keep - recent of largest
  *   s_j = sum over the KV head's query heads g and dimensions d of max(q_gd low_jd, q_gd high_jd)
  *       = sum_d low_jd sum_g min(q_gd, 0) + high_jd sum_g max(q_gd, 0),
- * which the heads' summed scores q_g . k of no key of the block exceed; in 64 bits, NaN as +infinity, of equal ones the lower block.  Where a token sees
+ * which the heads' summed scores q_g . k of no key of the block exceed; in 64 bits, NaN as +infinity, of equal ones the lower block.  (The second line is what is worked
+ * out: an infinite bound that meets a sum of 0 is NaN there, so such a block comes out ahead.)  Where a token sees
  * at most `keep` blocks it gets them all.  Only full blocks before its own are scored: no row behind the token has influence.
  *
  * sequences, positions   device int32 [n_tokens], as a plan leaves them: the token's row of block_table and its position.  A token whose sequence lies

@@ -186,7 +186,7 @@ struct SelectArgs {
   int32_t* blocks;               // [tokens][n_kv_heads][keep]
   double* scores;                // [token - first][n_kv_heads][most]
   int64_t q_token, q_head, table_stride, most;
-  int batch, first, tokens, hkv, group, page_shift, max_pages, keep, recent, last_row, span, spans, tiles_at_once;
+  int batch, first, tokens, hkv, group, page_shift, max_pages, keep, recent, last_row, span, spans, spans_at_once, tiles_at_once;
 };
 // Blocks that a token sees (0: none), and of these the first so many that compete.
 struct TokenBlocks { int seen, scored; };
@@ -198,6 +198,7 @@ __device__ __forceinline__ TokenBlocks token_blocks(const SelectArgs& a, int b, 
 }
 constexpr int kScoreTokens = 8;           // tokens of a sequence that share a reading of the bounds
 constexpr int kScoreThreads = 256;
+constexpr int kScoreBlocks = 1536;        // workgroups from which on they take several spans each, a third of these
 constexpr int kSharedDepth = 4;           // readings of a wavefront then (1 / 2 / 4: 20.4 / 15.2 / 10.5 us for 72 drafts)
 
 // a double from another lane of sixteen (a DPP control)
@@ -240,12 +241,13 @@ template <int DT, int D, int TOKENS, int THREADS, int DIMS, typename F>
 __device__ __forceinline__ void score_weights(const SelectArgs& a, int t, int tokens, int kvh, double* weight, F meanwhile) {
   constexpr int kTeam = TOKENS * D / DIMS, kTeams = THREADS / kTeam;
   const int team = threadIdx.x / kTeam, k = threadIdx.x / (D / DIMS) % TOKENS, d = threadIdx.x % (D / DIMS) * DIMS;
+  const int heads = k < tokens ? a.group : 0;                 // (a token that is not there has the weights 0)
   double up[DIMS], down[DIMS];
 #pragma unroll
   for (int e = 0; e < DIMS; ++e) up[e] = down[e] = 0.0;
   const uint16_t* q = a.q + (t + min(k, tokens - 1)) * a.q_token + (int64_t)kvh * a.group * a.q_head + d;
 #pragma unroll 4
-  for (int g = team; g < a.group; g += kTeams) {
+  for (int g = team; g < heads; g += kTeams) {
     const uint32_t* src = (const uint32_t*)(q + g * a.q_head);
 #pragma unroll
     for (int p = 0; p < DIMS / 2; ++p) {
@@ -339,29 +341,35 @@ __global__ __launch_bounds__(kScoreThreads) void block_score_kernel(SelectArgs a
 // The same for up to kScoreTokens neighbouring tokens of one sequence: the bounds are read and converted once for all, the weights come out of LDS again
 // for every block.  A token that has a neighbour of its sequence before it is left to the workgroup of the tile's first one.
 // (72 drafts of 16 sequences, 32 : 8 heads, up to 255 blocks: a conversion a token 17.4 us.)
-template <int DT, int D>
-__global__ __launch_bounds__(kScoreThreads) void block_score_shared_kernel(SelectArgs a) {
+// With MORE a workgroup goes on to the next spans, so that the weights are added up for several of them, and asks for their bounds while it looks at these.  Both fit
+// two wavefronts a SIMD; the loop costs registers, though, and where the spans fit at once nothing is gained: 128 tiles' 512 spans 9.0 us and 12.4, 504 tiles' 2016 of
+// two tokens each 26 and 17, 512 tiles' 16384 216 and 131.
+template <int DT, int D, bool MORE>
+__global__ __launch_bounds__(kScoreThreads, 2) void block_score_shared_kernel(SelectArgs a) {
   constexpr int kLanes = D / 8, kAtOnce = kWave / kLanes, kAtOnceTokens = 8 / kSharedDepth;            // (tokens that make eight sums)
   __shared__ __attribute__((aligned(16))) double weight[kScoreThreads / (D / 4) * 2 * D];
   const uint32_t unit = blockIdx.x;
-  const int kvh = (int)(unit % (uint32_t)a.hkv), span = (int)(unit / (uint32_t)a.hkv % (uint32_t)a.spans);
+  const int kvh = (int)(unit % (uint32_t)a.hkv), span = (int)(unit / (uint32_t)a.hkv % (uint32_t)a.spans_at_once);
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1), part = lane % kLanes, which = lane / kLanes;
-  for (int m = (int)(unit / (uint32_t)a.hkv / (uint32_t)a.spans);; m += a.tiles_at_once) {
+  for (int m = (int)(unit / (uint32_t)a.hkv / (uint32_t)a.spans_at_once);; m += a.tiles_at_once) {
     const TokenTile tile = token_tile(a.sequences, a.first, a.first + a.tokens, a.batch, kScoreTokens, m);
     if (!tile.tokens) return;
     const int t = tile.first, local = t - a.first;
     // a lane has a token's number of blocks
     const int mine = lane < tile.tokens ? token_blocks(a, tile.sequence, a.positions[t + lane]).scored : 0;
     const int most = (int)lanes_largest((uint32_t)mine);
-    const int j0 = span * a.span + wave * kAtOnce * kSharedDepth, j1 = min(j0 + kAtOnce * kSharedDepth, most);
-    if (span * a.span < most) {                               // (the whole workgroup)
+    const int first = span * a.span, step = a.spans_at_once * a.span;
+    if (first < most) {                                       // (the whole workgroup)
+      auto page_of = [&](int from) { return a.table[tile.sequence * a.table_stride + min(from + wave * kAtOnce * kSharedDepth + lane, most - 1)]; };
       dec_u4 low[kSharedDepth], high[kSharedDepth];
-      const int page = a.table[tile.sequence * a.table_stride + max(min(j0 + lane, j1 - 1), 0)];
+      int page = page_of(first);
       score_weights<DT, D, kScoreTokens, kScoreThreads, 4>(a, t, tile.tokens, kvh, weight, [&]() {
-        if (j0 < j1) load_bounds<D, kSharedDepth>(a, page, kvh, low, high);
+        load_bounds<D, kSharedDepth>(a, page, kvh, low, high);
+        if (MORE) page = page_of(first + step);
       });
-      double low_of[kSharedDepth][8], high_of[kSharedDepth][8];
-      if (j0 < j1) {
+      for (int from = first; from < most; from += step) {
+        const int j0 = from + wave * kAtOnce * kSharedDepth;
+        double low_of[kSharedDepth][8], high_of[kSharedDepth][8];
 #pragma unroll
         for (int i = 0; i < kSharedDepth; ++i) {
           float l[8], h[8];
@@ -373,33 +381,38 @@ __global__ __launch_bounds__(kScoreThreads) void block_score_shared_kernel(Selec
             high_of[i][e] = (double)h[e];
           }
         }
-      }
+        if (MORE && from + step < most) {
+          load_bounds<D, kSharedDepth>(a, page, kvh, low, high);
+          page = page_of(from + 2 * step);
+        }
 #pragma unroll
-      for (int k0 = 0; k0 < kScoreTokens; k0 += kAtOnceTokens) {
-        if (k0 >= tile.tokens || j0 >= j1) break;
-        double s[8], out[2];
+        for (int k0 = 0; k0 < kScoreTokens; k0 += kAtOnceTokens) {
+          if (k0 >= tile.tokens || j0 >= most) break;
+          double s[8], out[2];
 #pragma unroll
-        for (int k = 0; k < kAtOnceTokens; ++k) {
-          // (of a token that is not there: what the last one's queries gave once more, and nobody takes it)
-          const double* of = weight + (k0 + k) * 2 * D + part * 8;
+          for (int k = 0; k < kAtOnceTokens; ++k) {
+            // (a token that is not there has the weights 0, and nobody takes what comes of it)
+            const double* of = weight + (k0 + k) * 2 * D + part * 8;
 #pragma unroll
-          for (int i = 0; i < kSharedDepth; ++i) {
-            double above = 0.0, below = 0.0;                  // (two chains of sums: a wavefront has few others to wait beside)
+            for (int i = 0; i < kSharedDepth; ++i) {
+              double above = 0.0, below = 0.0;                // (two chains of sums: a wavefront has few others to wait beside)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              above = fma(of[e], high_of[i][e], above);
-              below = fma(of[D + e], low_of[i][e], below);
+              for (int e = 0; e < 8; ++e) {
+                above = fma(of[e], high_of[i][e], above);
+                below = fma(of[D + e], low_of[i][e], below);
+              }
+              s[k * kSharedDepth + i] = above + below;
             }
-            s[k * kSharedDepth + i] = above + below;
+          }
+          sum_eight<kLanes>(s, lane, out);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int v = 4 * i + part, k = k0 + v / kSharedDepth, j = j0 + v % kSharedDepth * kAtOnce + which;
+            const int n = __shfl(mine, k & 7, kWave);
+            if (part < 4 && j < n) a.scores[((int64_t)(local + k) * a.hkv + kvh) * a.most + j] = score_of(out[i]);
           }
         }
-        sum_eight<kLanes>(s, lane, out);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int v = 4 * i + part, k = k0 + v / kSharedDepth, j = j0 + v % kSharedDepth * kAtOnce + which;
-          const int n = __shfl(mine, k & 7, kWave);
-          if (part < 4 && j < min(j1, n)) a.scores[((int64_t)(local + k) * a.hkv + kvh) * a.most + j] = score_of(out[i]);
-        }
+        if (!MORE) break;
       }
     }
     if (m + a.tiles_at_once >= tile.all) return;
@@ -1084,8 +1097,12 @@ static void launch_scores(SelectArgs a, hipStream_t st) {
   a.span = kScoreThreads / (D / 8) * (shared ? kSharedDepth : 8);
   a.spans = (int)((a.most + a.span - 1) / a.span);
   a.tiles_at_once = tiles_at_once(a.tokens, a.batch, kScoreTokens);
-  const dim3 grid((unsigned)((int64_t)(shared ? a.tiles_at_once : a.tokens) * a.hkv * a.spans)), block(kScoreThreads);
-  if (shared) hipLaunchKernelGGL((block_score_shared_kernel<DT, D>), grid, block, 0, st, a);
+  const int64_t tiles = std::max<int64_t>(a.batch, a.tokens / kScoreTokens) * a.hkv;
+  const bool more = tiles * a.spans > kScoreBlocks;
+  a.spans_at_once = more ? (int)std::max<int64_t>(1, kScoreBlocks / 3 / tiles) : a.spans;
+  const dim3 grid((unsigned)((int64_t)(shared ? (int64_t)a.tiles_at_once * a.spans_at_once : (int64_t)a.tokens * a.spans) * a.hkv)), block(kScoreThreads);
+  if (shared && more) hipLaunchKernelGGL((block_score_shared_kernel<DT, D, true>), grid, block, 0, st, a);
+  else if (shared) hipLaunchKernelGGL((block_score_shared_kernel<DT, D, false>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((block_score_kernel<DT, D>), grid, block, 0, st, a);
 }
 

@@ -110,6 +110,21 @@ def test_select(dtype, case, values):
     assert got.tolist() == want
 
 
+@pytest.mark.parametrize("dtype,Hq,Hkv,D,rows,batch", [(torch.bfloat16, 16, 8, 128, 1100, 24), (torch.float16, 4, 4, 64, 2600, 30)])
+def test_select_where_a_workgroup_has_several_spans(dtype, Hq, Hkv, D, rows, batch):
+    """More drafts' blocks than fit at once: lists as of every token by itself."""
+    print("several spans", dtype, Hq, Hkv, D, rows, batch, flush=True)
+    g = torch.Generator().manual_seed(rows)
+    lens = [(rows - 7 * b, 1 + b % 5) for b in range(batch)]
+    table, seq, pos, pages = _maps(g, lens, 1)
+    q = torch.randn(len(seq), Hq, D, generator=g).to(dtype).to(DEV)
+    bounds = torch.randn(pages, Hkv, 2, D, generator=g).sort(2).values.to(dtype).to(DEV)
+    table, seq, pos = _i32(table), _i32(seq), _i32(pos)
+    got = ops.select_blocks(q, bounds, table, seq, pos, 1, 40, recent=3)
+    for t in range(len(seq)):
+        assert torch.equal(ops.select_blocks(q[t:t + 1], bounds, table, seq[t:t + 1], pos[t:t + 1], 1, 40, recent=3), got[t:t + 1]), t
+
+
 def test_select_with_infinities_and_nan():
     """A block whose score is NaN counts as +infinity; those behind the token's own are not looked at."""
     g = torch.Generator().manual_seed(3)
