@@ -381,7 +381,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_end_kernel(VerifyArgs a
         const bool some = left > 0.0;
         part += some ? w : 0;
         taken += some ? p : 0.0;
-        open |= fabs(left) <= kUnsure * m[e];
+        open |= fabs(left) < kUnsure * m[e];                  // (not where there is no mass: nothing is left of it)
       }
     }
     all = wave_sum_u64(all);
