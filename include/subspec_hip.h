@@ -457,7 +457,8 @@ int subspec_sample_filtered(const void* logits, int dtype, int64_t rows, int64_t
  *               the draft.  Entries below 0 and NaN count as 0.  A sequence's last row is not read
  * tokens        device int64 [n_rows]: a sequence's drafts that stay, its token, then -1; -1 in rows of no sequence, and for the token of
  *               a row without a logit above -inf
- * probs         device float [n_rows]: p_i at these tokens (0 beside -1);  accepted  device int32 [batch]: drafts that stay (0 without rows)
+ * probs         device float [n_rows]: p_i at these tokens (0 beside -1);  accepted  device int32 [batch]: drafts that stay (0 without rows).  Whether a draft stays, and
+ *               the token, are decided by masses in 64 bits; without filters the probs of drafts that stay come from a row's mass in 32 bits (within 2^-17 of it)
  * filtered      1 where any of the filters is given (a pointer, 0 < top_k < vocab, top_p < 1 or min_p > 0)
  * The outputs overlap no input.  Limits: n_rows <= 2^20, vocab <= 2^20, 1 <= batch <= SUBSPEC_MAX_BATCH.
  */

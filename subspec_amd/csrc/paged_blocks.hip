@@ -297,7 +297,7 @@ __device__ __forceinline__ void load_bounds(const SelectArgs& a, int page, int k
 __device__ __forceinline__ double score_of(double s) { return s != s ? INFINITY : s; }
 
 // A workgroup takes `span` blocks of (token, KV head), a wavefront a quarter of them: D / 8 lanes a block, all requests of a wavefront under way before
-// the first score; meanwhile the four of them add the query heads up.
+// the first score; meanwhile the four of them add the query heads up.  One token of 2048 blocks 4.9 us; 64 tokens, 193 MB, 38.9 (5.0 TB/s).
 template <int DT, int D>
 __global__ __launch_bounds__(kScoreThreads) void block_score_kernel(SelectArgs a) {
   constexpr int kLanes = D / 8, kAtOnce = kWave / kLanes, kDepth = 8;
@@ -339,8 +339,7 @@ __global__ __launch_bounds__(kScoreThreads) void block_score_kernel(SelectArgs a
 }
 
 // The same for up to kScoreTokens neighbouring tokens of one sequence: the bounds are read and converted once for all, the weights come out of LDS again
-// for every block.  A token that has a neighbour of its sequence before it is left to the workgroup of the tile's first one.
-// (72 drafts of 16 sequences, 32 : 8 heads, up to 255 blocks: a conversion a token 17.4 us.)
+// for every block.  (72 drafts of 16 sequences, 32 : 8 heads, up to 255 blocks: a conversion a token 17.4 us, this 9.2 to 10.2.)
 // With MORE a workgroup goes on to the next spans, so that the weights are added up for several of them, and asks for their bounds while it looks at these.  Both fit
 // two wavefronts a SIMD; the loop costs registers, though, and where the spans fit at once nothing is gained: 128 tiles' 512 spans 9.0 us and 12.4, 504 tiles' 2016 of
 // two tokens each 26 and 17, 512 tiles' 16384 216 and 131.
@@ -423,7 +422,7 @@ __global__ __launch_bounds__(kScoreThreads, 2) void block_score_shared_kernel(Se
 // ---------------------------------------------------------------------------------------------------------------- the best of them
 // The keep - recent blocks of largest score, equal ones from the lowest on, without sorting: the scores as ordered whole numbers, and the digits (eleven bits at
 // a time, from the first that differs) of the smallest that stays; the few entries that share them are ranked one by one.  What stays is a bit each, and the
-// bits in order are the list.
+// bits in order are the list.  2048 blocks: 6.2 us (its launch and loads alone 2.8).
 constexpr int kMostBlocks = 1 << 17;
 constexpr int kDigits = 2048;
 constexpr int kHeld = 8;                 // scores of a thread that stay in registers
@@ -599,7 +598,8 @@ __global__ __launch_bounds__(THREADS) void block_select_kernel(SelectArgs a) {
 // cache holds there never comes near a product.
 // Tokens of one sequence list much the same blocks, so where a call has more tokens than sequences up to eight of them share a unit (32 rows of a KV head): its
 // blocks are those that any of them lists, ascending, each with a bit a token (block_union_kernel), and a row sees a key by its token's bit and position.
-// 72 drafts of 16 sequences, 32 blocks of 64 rows each, 32 : 8 heads: a unit a token reads 600 MB, out of the caches, in 92 us.
+// 72 drafts of 16 sequences, 32 blocks of 64 rows each, 32 : 8 heads: a unit a token reads 600 MB, out of the caches, in 92 us; their union, 192 MB, takes 42 (4.6 TB/s).  64 tokens
+// by themselves, 134 MB: 26.7 (5.0 TB/s); one of 1024 rows: 5.5, five trips to memory and the launch.  A stage of 32 keys and 32 rows is 1.3 us of a wavefront's work.
 constexpr int kAttendKeys = 32;
 constexpr int kAttendStages = 2;
 constexpr int kAttendSegment = 512;        // keys whose row offsets are in LDS at a time
@@ -1230,7 +1230,7 @@ extern "C" int subspec_select_blocks(const void* q, int64_t q_token_stride, int6
         else launch_scores<SUBSPEC_F16, 64>(a, st);
       }
     }
-    // (up to 256 blocks 6.8 us with 256 threads and 9.0 with 512, 2048 blocks 8.6 and 7.6)
+    // (up to 255 blocks 5.4 us with 256 threads, a wave's steps fewer; 2048 blocks 6.2 with 512, two rounds of entries fewer: 6.8 and 9.0, 8.6 and 7.6 when these were compared)
     const dim3 lists((unsigned)(some * n_kv_heads));
     if (most <= 512) hipLaunchKernelGGL(block_select_kernel<256>, lists, dim3(256), 0, st, a);
     else hipLaunchKernelGGL(block_select_kernel<512>, lists, dim3(512), 0, st, a);
