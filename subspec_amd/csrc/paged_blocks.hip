@@ -630,9 +630,10 @@ struct AttendArgs {
 constexpr int kSharedKeys = 1024;
 constexpr int kUnitsAtOnce = 4 * 256;
 __host__ __device__ __forceinline__ int tile_chunks(int keys, int tiles) {
-  const int rounds = (int)(((int64_t)tiles * ((keys + kSharedKeys - 1) / kSharedKeys) + kUnitsAtOnce - 1) / kUnitsAtOnce);
+  const int64_t rounds = ((int64_t)tiles * ((keys + kSharedKeys - 1) / kSharedKeys) + kUnitsAtOnce - 1) / kUnitsAtOnce;
   const float least = fmaxf(64.f, 0.5f * sqrtf((float)tiles * (float)keys));
-  return max(1, min(max(rounds, 1) * kUnitsAtOnce / max(tiles, 1), (int)((float)keys / least)));
+  const int64_t chunks = rounds * kUnitsAtOnce / (tiles > 0 ? tiles : 1), most = (int64_t)((float)keys / least);
+  return (int)(chunks < most ? chunks > 0 ? chunks : 1 : most > 0 ? most : 1);
 }
 __device__ __forceinline__ int attend_last(const AttendArgs& a, int t) { return min(a.positions[t], a.last_row); }
 
@@ -1069,7 +1070,7 @@ static AttendPlan attend_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64
   p.chunk_keys = (int)per;
   p.chunks = (int)((keys + per - 1) / per);
   p.tokens = p.share > 1 ? std::min<int64_t>(n_tokens, kTileTokens) : n_tokens;
-  if (p.chunks > 1) p.tokens = std::min<int64_t>(p.tokens, std::max<int64_t>(64, (1 << 20) / (hq * p.chunks)));      // half a gigabyte at 128 a head
+  if (p.chunks > 1) p.tokens = std::min<int64_t>(p.tokens, std::max<int64_t>(8, (1 << 20) / (hq * p.chunks)));      // half a gigabyte at 128 a head
   const size_t slots = (size_t)p.tokens * hq * p.chunks;
   if (p.chunks > 1) {
     p.part_o = align_up(slots * head_dim * sizeof(float), 256);

@@ -342,6 +342,46 @@ def test_a_captured_step_and_another_stream():
         assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
 
 
+@pytest.mark.parametrize("Hq,Hkv,D", [(32, 8, 128), (8, 4, 64)])
+def test_a_replayed_graph_with_other_neighbours(Hq, Hkv, D):
+    """The tokens' sequences change between replays, from one run to a token each in turn (more tiles than a batch in order has), some of nobody: as the eager
+    calls, and as every token by itself up to the order of its sums."""
+    g = torch.Generator().manual_seed(21)
+    P, keep, rows, T = 8, 5, 330, 30
+    q, pool, table, _, _ = _cache(g, [(rows, 10)] * 3, P, Hq, Hkv, D, torch.bfloat16)
+    q, pool, table = q.to(DEV), pool.nan_to_num().to(DEV), _i32(table)
+    bounds = ops.kv_page_bounds_(torch.zeros(pool.shape[0], Hkv, 2, D, dtype=torch.bfloat16, device=DEV), pool, torch.arange(pool.shape[0] * P, device=DEV))
+    orders = [[0] * 30, [t % 3 for t in range(30)], [0] * 9 + [-1] * 3 + [1] * 17 + [2], [2] * 10 + [5] + [1, 1, 0, 0, 0, 1, 2, 2] * 2 + [-1] * 3, [-1] * 30,
+              [t // 10 for t in range(30)]]
+    seq, pos = _i32(orders[0]), _i32([rows - 1 - t for t in range(T)])
+    out = torch.empty(T, Hq * D, dtype=torch.bfloat16, device=DEV)
+
+    def step(out):
+        blocks = ops.select_blocks(q, bounds, table, seq, pos, P, keep)
+        return blocks, ops.block_attention(q, pool, table, blocks, seq, pos, out=out)
+
+    step(out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(out)
+    for turn, order in enumerate(orders + orders[::-1]):
+        seq.copy_(_i32(order))
+        pos.copy_(_i32([rows - 1 - (7 * t + turn) % 60 for t in range(T)]))
+        out.fill_(7.0)
+        graph.replay()
+        want = step(torch.full_like(out, 7.0))
+        assert torch.equal(held[0], want[0]) and torch.equal(out, want[1]), turn
+        nobody = torch.tensor([not 0 <= b < 3 for b in order], device=DEV)
+        assert out[nobody].eq(7.0).all() and held[0][nobody].eq(-1).all()
+        for t in range(0, T, 7):
+            if 0 <= order[t] < 3:
+                one = ops.select_blocks(q[t:t + 1], bounds, table, seq[t:t + 1], pos[t:t + 1], P, keep)
+                assert torch.equal(one[0], held[0][t]), (turn, t)
+                alone = ops.block_attention(q[t:t + 1], pool, table, one, seq[t:t + 1], pos[t:t + 1])[0]
+                # each is off from the formula by half a step of the result (2^-8 of it) and little else
+                assert (alone.float() - out[t].float()).abs().max() <= 2 * (2.0 ** -8 * 1.01 * float(alone.float().abs().max()) + 2.0 ** -14)
+
+
 def test_many_tokens_take_several_passes():
     """More partial results and scores than are held at a time: tokens go in passes, with the same results."""
     g = torch.Generator().manual_seed(13)
