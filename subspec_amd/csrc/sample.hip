@@ -139,19 +139,31 @@ struct Part {
     }
   }
 };
+// A thread's pieces of a part of a row, the first two asked for where this is made, before what has to be known of the row is (four or six: no faster).
+template <int DT, int THREADS>
+struct Pieces {
+  const Part<DT> part;
+  dec_u4 next[2];
+  __device__ __forceinline__ Pieces(const void* row, int i0, int i1) : part(row, i0, i1) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) next[u] = part.piece(threadIdx.x + u * THREADS);
+  }
+  // the piece of turn p, and one more asked for
+  __device__ __forceinline__ dec_u4 take(int p) {
+    const dec_u4 v = next[0];
+    next[0] = next[1];
+    next[1] = part.piece(p + 2 * THREADS);
+    return v;
+  }
+};
 // f(logit, index) for a part of a row, the next pieces asked for before the last are worked on.  One copy of f in the code (two for pairs of 16-bit
 // logits): it is long, and a slice takes few turns.
 template <int DT, int THREADS, typename F>
-__device__ __forceinline__ void each_entry(const void* row, int i0, int i1, F f) {
-  const Part<DT> part(row, i0, i1);
-  dec_u4 next[2];
-#pragma unroll
-  for (int u = 0; u < 2; ++u) next[u] = part.piece(threadIdx.x + u * THREADS);
+__device__ __forceinline__ void each_entry(Pieces<DT, THREADS>& pieces, F f) {
+  const Part<DT>& part = pieces.part;
 #pragma unroll 1
   for (int p = threadIdx.x; p < part.pieces; p += THREADS) {
-    dec_u4 v = next[0];
-    next[0] = next[1];
-    next[1] = part.piece(p + 2 * THREADS);
+    dec_u4 v = pieces.take(p);
 #pragma unroll 1
     for (int j = 0; j < 4; ++j) {
       const uint32_t bits = v[0];
@@ -197,12 +209,12 @@ __device__ __forceinline__ float part_top(const void* row, int i0, int i1) {
 
 // The bins of a part of a row, and the mass that min-p keeps of it (a thread's own, returned).  Counts are wanted with a top-k only.
 template <int DT, int THREADS>
-__device__ __forceinline__ uint64_t fill_bins(Hist& h, const void* row, int i0, int i1, int vocab, const RowTop& top, const RowRule& r) {
+__device__ __forceinline__ uint64_t fill_bins(Hist& h, Pieces<DT, THREADS>& pieces, int vocab, const RowTop& top, const RowRule& r) {
   const double least = r.min_p * (double)(1ull << kMassBits);
   const bool counted = r.k < vocab, sorted_out = r.min_p > 0.0;
   const Series series;
   uint64_t kept = 0;
-  each_entry<DT, THREADS>(row, i0, i1, [&](float l, int) {
+  each_entry<DT, THREADS>(pieces, [&](float l, int) {
     const float d = entry_distance(l, top, r);
     if (!(d < kReach)) return;
     const double m = entry_mass(l, top, r, series);
@@ -258,9 +270,10 @@ __device__ __forceinline__ bool in_ranges(const BinRanges& g, int b) {
 
 // The entries of those bins in a part of a row; *n counts them, `most` of them are kept.  Few are, so a piece is first looked over in 32 bits:
 // within a bin of one of the ranges, |top - l - centre| <= width, nine instructions an entry (a NaN, and infinities among them, passes).
-template <int DT, int THREADS>
-__device__ __forceinline__ void gather(uint64_t* keys, int most, int* n, const void* row, int i0, int i1, const RowTop& top, const RowRule& r,
+template <int DT, int THREADS, bool DRAW>
+__device__ __forceinline__ void gather(uint64_t* keys, int most, int* n, Pieces<DT, THREADS>& pieces, const RowTop& top, const RowRule& r,
                                        const BinRanges& g) {
+  if (!DRAW && !g.by_k && !g.by_p) return;                                // (uniform: nothing is looked for)
   float centre[3], width[3];
   const float bin = kReach / kBins / r.inv_t;                             // width of a bin in logits
 #pragma unroll
@@ -270,7 +283,7 @@ __device__ __forceinline__ void gather(uint64_t* keys, int most, int* n, const v
   }
   auto near = [&](float l) {
     const float x = top.value - l;
-    return !(fabsf(x - centre[0]) > width[0]) || !(fabsf(x - centre[1]) > width[1]) || !(fabsf(x - centre[2]) > width[2]);
+    return !(fabsf(x - centre[0]) > width[0]) || !(fabsf(x - centre[1]) > width[1]) || (DRAW && !(fabsf(x - centre[2]) > width[2]));
   };
   auto take = [&](float l, int i) {
     const float d = entry_distance(l, top, r);
@@ -279,15 +292,10 @@ __device__ __forceinline__ void gather(uint64_t* keys, int most, int* n, const v
     if (at < most) keys[at] = order_key<DT>(l, i);
   };
   constexpr int kVec = 16 / Elem<DT>::kBytes;
-  const Part<DT> part(row, i0, i1);
-  dec_u4 next[2];
-#pragma unroll
-  for (int u = 0; u < 2; ++u) next[u] = part.piece(threadIdx.x + u * THREADS);
+  const Part<DT>& part = pieces.part;
 #pragma unroll 1
   for (int p = threadIdx.x; p < part.pieces; p += THREADS) {
-    dec_u4 v = next[0];
-    next[0] = next[1];
-    next[1] = part.piece(p + 2 * THREADS);
+    const dec_u4 v = pieces.take(p);
     float x[kVec];
     if constexpr (DT == SUBSPEC_F32) {
 #pragma unroll
@@ -397,7 +405,8 @@ __device__ void draw_row(Search& s, const Hist& bins, const uint64_t* keys, int 
       if (n <= most) {
         for (int i = threadIdx.x; i < n; i += THREADS) f(keys[i]);
       } else {
-        each_entry<DT, THREADS>(row, 0, a.vocab, [&](float l, int i) {
+        Pieces<DT, THREADS> pieces(row, 0, a.vocab);
+        each_entry<DT, THREADS>(pieces, [&](float l, int i) {
           if (entry_distance(l, top, r) < kReach) f(order_key<DT>(l, i));
         });
       }
@@ -448,12 +457,14 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
     n = 0;
   }
   __syncthreads();
-  const uint64_t kept = wave_scan_u64(fill_bins<DT, kSampleThreads>(bins, row, 0, a.vocab, a.vocab, top, r));
+  Pieces<DT, kSampleThreads> first(row, 0, a.vocab);
+  const uint64_t kept = wave_scan_u64(fill_bins<DT, kSampleThreads>(bins, first, a.vocab, top, r));
   if ((threadIdx.x & (kWave - 1)) == kWave - 1) atomicAdd(&min_p_mass, (unsigned long long)kept);
   __syncthreads();
   scan_bins<kSampleThreads>(bins, s.wave_mass, s.wave_count);
   const BinRanges g = bin_ranges<DRAW>(bins, min_p_mass, r);
-  gather<DT, kSampleThreads>(keys, kCandidates, &n, row, 0, a.vocab, top, r, g);
+  Pieces<DT, kSampleThreads> again(row, 0, a.vocab);
+  gather<DT, kSampleThreads, DRAW>(keys, kCandidates, &n, again, top, r, g);
   __syncthreads();
   draw_row<DT, kSampleThreads, DRAW>(s, bins, keys, n, kCandidates, a, cuts, row_index, row, top, r, g.by_k, g.by_p, min_p_mass);
 }
@@ -499,12 +510,12 @@ __global__ __launch_bounds__(kSliceThreads) void sample_bins_kernel(SampleArgs a
   __shared__ float scratch[kSliceThreads / kWave];
   __shared__ unsigned long long min_p_mass;
   const int row_index = blockIdx.x / c.count, slice = blockIdx.x % c.count;
+  Pieces<DT, kSliceThreads> pieces(row_of<DT>(a, row_index), slice * c.length, min((slice + 1) * c.length, a.vocab));
   clear_hist<kSliceThreads>(h);
   if (threadIdx.x == 0) min_p_mass = 0;
   const RowRule r = row_rule(a, row_index);
   const RowTop top = row_top_of(row_top<kSliceThreads>(c, row_index, scratch), r);          // (its barriers also stand between the clearing and the sums)
-  const uint64_t kept = wave_scan_u64(fill_bins<DT, kSliceThreads>(h, row_of<DT>(a, row_index), slice * c.length,
-                                                                   min((slice + 1) * c.length, a.vocab), a.vocab, top, r));
+  const uint64_t kept = wave_scan_u64(fill_bins<DT, kSliceThreads>(h, pieces, a.vocab, top, r));
   if ((threadIdx.x & (kWave - 1)) == kWave - 1) atomicAdd(&min_p_mass, (unsigned long long)kept);
   __syncthreads();
   SliceRecord& out = c.slices[blockIdx.x];
@@ -523,6 +534,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_gather_kernel(SampleArgs
   __shared__ uint32_t wave_count[kSliceThreads / kWave];
   __shared__ int n;
   const int row_index = blockIdx.x / c.count, slice = blockIdx.x % c.count;
+  Pieces<DT, kSliceThreads> pieces(row_of<DT>(a, row_index), slice * c.length, min((slice + 1) * c.length, a.vocab));
   if (threadIdx.x == 0) n = 0;
   const RowRule r = row_rule(a, row_index);
   const SliceRecord* of = c.slices + (int64_t)row_index * c.count;
@@ -557,7 +569,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_gather_kernel(SampleArgs
   scan_bins<kSliceThreads>(h, wave_mass, wave_count);
   const BinRanges g = bin_ranges<DRAW>(h, kept, r);
   SliceRecord& out = c.slices[blockIdx.x];
-  gather<DT, kSliceThreads>(out.key, kSliceCandidates, &n, row_of<DT>(a, row_index), slice * c.length, min((slice + 1) * c.length, a.vocab), top, r, g);
+  gather<DT, kSliceThreads, DRAW>(out.key, kSliceCandidates, &n, pieces, top, r, g);
   if (slice == 0) {
     RowRecord& rec = c.rows[row_index];
     for (int i = threadIdx.x; i < kBins; i += kSliceThreads) {
