@@ -24,7 +24,7 @@ constexpr int kSampleThreads = 1024;      // of a workgroup that has a whole row
 constexpr int kSliceThreads = 512;        // ... a slice of one
 constexpr int kBins = 1024;
 constexpr int kCandidates = 4096;
-constexpr int kSliceCandidates = 1024;
+constexpr int kSliceCandidates = 2048;
 
 __device__ __forceinline__ int bin_of(float d) { return (int)(d * (0.999999f * kBins / kReach)); }      // (below kBins, rounding or not)
 
@@ -504,75 +504,67 @@ __global__ __launch_bounds__(kSliceThreads) void sample_top_kernel(SampleArgs a,
   if (threadIdx.x == 0) c.slices[blockIdx.x].top = top;
 }
 
-template <int DT>
-__global__ __launch_bounds__(kSliceThreads) void sample_bins_kernel(SampleArgs a, SliceArgs c) {
+template <int DT, int THREADS>
+__global__ __launch_bounds__(THREADS) void sample_bins_kernel(SampleArgs a, SliceArgs c) {
   __shared__ Hist h;
-  __shared__ float scratch[kSliceThreads / kWave];
+  __shared__ float scratch[THREADS / kWave];
   __shared__ unsigned long long min_p_mass;
   const int row_index = blockIdx.x / c.count, slice = blockIdx.x % c.count;
-  Pieces<DT, kSliceThreads> pieces(row_of<DT>(a, row_index), slice * c.length, min((slice + 1) * c.length, a.vocab));
-  clear_hist<kSliceThreads>(h);
+  Pieces<DT, THREADS> pieces(row_of<DT>(a, row_index), slice * c.length, min((slice + 1) * c.length, a.vocab));
+  clear_hist<THREADS>(h);
   if (threadIdx.x == 0) min_p_mass = 0;
   const RowRule r = row_rule(a, row_index);
-  const RowTop top = row_top_of(row_top<kSliceThreads>(c, row_index, scratch), r);          // (its barriers also stand between the clearing and the sums)
-  const uint64_t kept = wave_scan_u64(fill_bins<DT, kSliceThreads>(h, pieces, a.vocab, top, r));
+  const RowTop top = row_top_of(row_top<THREADS>(c, row_index, scratch), r);          // (its barriers also stand between the clearing and the sums)
+  const uint64_t kept = wave_scan_u64(fill_bins<DT, THREADS>(h, pieces, a.vocab, top, r));
   if ((threadIdx.x & (kWave - 1)) == kWave - 1) atomicAdd(&min_p_mass, (unsigned long long)kept);
   __syncthreads();
   SliceRecord& out = c.slices[blockIdx.x];
-  for (int i = threadIdx.x; i < kBins; i += kSliceThreads) {
+  for (int i = threadIdx.x; i < kBins; i += THREADS) {
     out.bins.mass[i] = h.mass[i];
     out.bins.count[i] = h.count[i];
   }
   if (threadIdx.x == 0) out.min_p_mass = min_p_mass;
 }
 
-template <int DT, bool DRAW>
-__global__ __launch_bounds__(kSliceThreads) void sample_gather_kernel(SampleArgs a, SliceArgs c) {
+template <int DT, bool DRAW, int THREADS>
+__global__ __launch_bounds__(THREADS) void sample_gather_kernel(SampleArgs a, SliceArgs c) {
   __shared__ Hist h;
-  __shared__ float scratch[kSliceThreads / kWave];
-  __shared__ uint64_t wave_mass[kSliceThreads / kWave];
-  __shared__ uint32_t wave_count[kSliceThreads / kWave];
+  __shared__ float scratch[THREADS / kWave];
+  __shared__ uint64_t wave_mass[THREADS / kWave];
+  __shared__ uint32_t wave_count[THREADS / kWave];
   __shared__ int n;
   const int row_index = blockIdx.x / c.count, slice = blockIdx.x % c.count;
-  Pieces<DT, kSliceThreads> pieces(row_of<DT>(a, row_index), slice * c.length, min((slice + 1) * c.length, a.vocab));
+  Pieces<DT, THREADS> pieces(row_of<DT>(a, row_index), slice * c.length, min((slice + 1) * c.length, a.vocab));
   if (threadIdx.x == 0) n = 0;
   const RowRule r = row_rule(a, row_index);
   const SliceRecord* of = c.slices + (int64_t)row_index * c.count;
   const int lane = threadIdx.x & (kWave - 1);
   uint64_t kept = lane < c.count ? of[lane].min_p_mass : 0;                                  // (at most 16 slices)
-  const RowTop top = row_top_of(row_top<kSliceThreads>(c, row_index, scratch), r);
+  const RowTop top = row_top_of(row_top<THREADS>(c, row_index, scratch), r);
   if (top.value == -INFINITY) return;                                             // (uniform) the last launch says so
-  static_assert(kBins == 2 * kSliceThreads, "a thread adds up two bins");
-  const int i2 = threadIdx.x * 2;
-  uint64_t m0 = 0, m1 = 0;
+  constexpr int kEach = kBins / THREADS;                  // bins that a thread adds up
+  typedef uint64_t Masses __attribute__((ext_vector_type(kEach)));
+  typedef uint32_t Counts __attribute__((ext_vector_type(kEach)));
+  const int first = threadIdx.x * kEach;
+  Masses m = 0;
 #pragma unroll 16
-  for (int j = 0; j < c.count; ++j) {
-    const ulonglong2 m = *(const ulonglong2*)&of[j].bins.mass[i2];
-    m0 += m.x;
-    m1 += m.y;
-  }
-  h.mass[i2] = m0;
-  h.mass[i2 + 1] = m1;
-  uint32_t k0 = 0, k1 = 0;
+  for (int j = 0; j < c.count; ++j) m += *(const Masses*)&of[j].bins.mass[first];
+  *(Masses*)&h.mass[first] = m;
+  Counts k = 0;
   if (r.k < a.vocab) {
 #pragma unroll 16
-    for (int j = 0; j < c.count; ++j) {
-      const uint2 k = *(const uint2*)&of[j].bins.count[i2];
-      k0 += k.x;
-      k1 += k.y;
-    }
+    for (int j = 0; j < c.count; ++j) k += *(const Counts*)&of[j].bins.count[first];
   }
-  h.count[i2] = k0;
-  h.count[i2 + 1] = k1;
+  *(Counts*)&h.count[first] = k;
   kept = __shfl((unsigned long long)wave_scan_u64(kept), kWave - 1, kWave);
   __syncthreads();
-  scan_bins<kSliceThreads>(h, wave_mass, wave_count);
+  scan_bins<THREADS>(h, wave_mass, wave_count);
   const BinRanges g = bin_ranges<DRAW>(h, kept, r);
   SliceRecord& out = c.slices[blockIdx.x];
-  gather<DT, kSliceThreads, DRAW>(out.key, kSliceCandidates, &n, pieces, top, r, g);
+  gather<DT, THREADS, DRAW>(out.key, kSliceCandidates, &n, pieces, top, r, g);
   if (slice == 0) {
     RowRecord& rec = c.rows[row_index];
-    for (int i = threadIdx.x; i < kBins; i += kSliceThreads) {
+    for (int i = threadIdx.x; i < kBins; i += THREADS) {
       rec.bins.mass[i] = h.mass[i];
       rec.bins.count[i] = h.count[i];
     }
@@ -621,9 +613,13 @@ __global__ __launch_bounds__(kSliceThreads) void sample_draw_kernel(SampleArgs a
 // each adds up the bins of all for itself.  1 / 4 / 8 / 16 / 32 slices, us (top-p 0.95, min-p 0.02): one row of 152064 fp32 92 53 41 34 32, 16 rows bf16
 // 87 53 45 39 45, 64 89 58 57 59 77, 128 93 75 81 88 124, 256 99 110 124 141 215; fp32, one row of 32000 31 28 27 26 27, 64 38 36 42 47 67; one of 16384
 // 21 23 24 23 -.
+// From 32 rows on slices of twice the threads, half as many, where that leaves as many threads: every workgroup of the second pass reads the bins of all its row's slices (63 rows of
+// 152064: 48 MB, now 12; bins 17.4 -> 15.8 us, the second pass 16.5 -> 13.3; 107 of 32000 12.3 -> 9.8 and 11.5 -> 10.8; 16 rows 8.9 -> 8.4 and 10.2 -> 11.1, 100 rows in two
+// instead of five 63.6 and 59.9).  From 171 rows on that is the whole row (170 rows in three slices 80, whole 84, 190 in two 100 and 86).
+static bool wide_slices(int64_t rows) { return rows >= 32 && 512 / rows == 2 * (256 / rows); }
 static int sample_slices(int64_t rows, int64_t vocab) {
-  if (vocab < 24576 || rows >= 192) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / rows, 16), vocab / (rows <= 8 ? 2048 : 8192)));
+  if (vocab < 24576) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((wide_slices(rows) ? 256 : 512) / rows, 16), vocab / (rows <= 8 ? 2048 : 8192)));
 }
 
 size_t row_search_workspace(int64_t rows, int64_t vocab) {
@@ -647,9 +643,11 @@ static void launch_row_search_of(const SampleArgs& a, int64_t rows, RowCut* cuts
   hipLaunchKernelGGL(sample_top_kernel<DT>, slices, dim3(kSliceThreads), 0, st, a, c);
   {
     DominantKernelTimer timer(st);
-    hipLaunchKernelGGL(sample_bins_kernel<DT>, slices, dim3(kSliceThreads), 0, st, a, c);
+    if (!wide_slices(rows)) hipLaunchKernelGGL((sample_bins_kernel<DT, kSliceThreads>), slices, dim3(kSliceThreads), 0, st, a, c);
+    else hipLaunchKernelGGL((sample_bins_kernel<DT, 2 * kSliceThreads>), slices, dim3(2 * kSliceThreads), 0, st, a, c);
   }
-  hipLaunchKernelGGL((sample_gather_kernel<DT, DRAW>), slices, dim3(kSliceThreads), 0, st, a, c);
+  if (!wide_slices(rows)) hipLaunchKernelGGL((sample_gather_kernel<DT, DRAW, kSliceThreads>), slices, dim3(kSliceThreads), 0, st, a, c);
+  else hipLaunchKernelGGL((sample_gather_kernel<DT, DRAW, 2 * kSliceThreads>), slices, dim3(2 * kSliceThreads), 0, st, a, c);
   hipLaunchKernelGGL((sample_draw_kernel<DT, DRAW>), grid, dim3(kSliceThreads), 0, st, a, c, cuts);
 }
 template <bool DRAW>
