@@ -10,7 +10,7 @@
 // max(m_j - q_j Z, 0) is rounded to such units again, so its sums are exact, no order of addition changes a token, and the token is the first in the
 // order of the vocabulary whose sum exceeds v times the whole.
 // 48 sequences of up to 8 drafts, 346 rows of 152064 bf16 (105 MB): the statistics of all rows 20.5 us (5.1 TB/s), acceptance and the end rows' masses 21, the draws 10.6; one sequence
-// of 4 drafts in fp32 4.0 + 6.0 + 4.3.  With filters the cuts of all rows come first (sample.hip): 63 rows' 50 us are most of 16 sequences' 63.
+// of 4 drafts in fp32 4.0 + 6.0 + 4.3.  With filters the cuts of all rows come first (sample.hip): 63 rows' 42 us are most of 16 sequences' 55.
 #include "sample.h"
 #include <algorithm>
 

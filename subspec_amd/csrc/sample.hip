@@ -10,10 +10,10 @@
 // exact and do not depend on the order in which wavefronts add them, 2^20 entries stay below 2^62, and what rounds to zero (less than 2^-43 of the
 // largest) is drawn with a probability below 2^-23 even if a million such entries are there.  In fp32 the sum over a flat row of 150000 entries is off
 // by more than the step between two of them.
-// One row of 152064 fp32: 30 us, four dependent launches of 3 + 8 + 11 + 8; 64 rows bf16 (19.5 MB): 58, the largest 6, the exponentials in 64 bits
-// 19, the sums of the slices' bins and the second pass 20, the search among the candidates 15.
+// One row of 152064 fp32: 28 us, four dependent launches of 3 + 7 + 10 + 8; 64 rows bf16 (19.5 MB): 50, the largest 6, the exponentials in 64 bits
+// 16, the sums of the slices' bins and the second pass 15, the search among the candidates 15.
 // A row of more candidates than kCandidates (or a slice's share of them) is searched by one workgroup, which reads it again for every ten bits of
-// every search: 152064 logits of deviation 2 at T = 3 and top-p 0.95 320 to 350 us (41 at T = 1), 64 such rows 400 to 455 (66); rows of equal logits
+// every search: 152064 logits of deviation 2 at T = 3 and top-p 0.95 46 us for one row (its slices hold them; 32 at T = 1), 363 for 64 (55); rows of equal logits
 // 0.65 to 1.3 ms, with a top-k of 70000 and a top-p 3.5.
 #include "sample.h"
 #include <algorithm>
