@@ -13,7 +13,7 @@
 // One row of 152064 fp32: 28 us, four dependent launches of 3 + 7 + 10 + 8; 64 rows bf16 (19.5 MB): 50, the largest 6, the exponentials in 64 bits
 // 16, the sums of the slices' bins and the second pass 15, the search among the candidates 15.
 // A row of more candidates than kCandidates (or a slice's share of them) is searched by one workgroup, which reads it again for every ten bits of
-// every search: 152064 logits of deviation 2 at T = 3 and top-p 0.95 46 us for one row (its slices hold them; 32 at T = 1), 363 for 64 (55); rows of equal logits
+// every search: 152064 logits of deviation 2 at T = 3 and top-p 0.95 310 us (32 at T = 1; a row of bf16 46), 64 rows of bf16 363 to 382 (55); rows of equal logits
 // 0.65 to 1.3 ms, with a top-k of 70000 and a top-p 3.5.
 #include "sample.h"
 #include <algorithm>
