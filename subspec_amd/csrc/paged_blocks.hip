@@ -20,36 +20,38 @@ static int block_shift_of(int64_t page_len) {
 // ---------------------------------------------------------------------------------------------------------------- bounds
 // low_d = min over the page's rows of K_d, high_d = max, of every page whose last row is among the slots: the rows of a page are
 // written in order, so it is full then, and its bounds come from the page alone (nothing is read, changed and written back).
-// A wavefront takes a slice of 16 pieces (16 bytes each; 8 where a row has no more) of the pages whose last rows are among eight slots, several rows at a time with up
+// A wavefront takes a slice of 16 pieces (16 bytes each; 8 where a row has no more) of the pages whose last rows are among up to eight slots (32 of long pages), several rows at a time with up
 // to sixteen requests a lane under way.  Its lanes meet through registers, so nobody waits for anybody, and a wavefront without such a page leaves.
 // As whole numbers that rise with the value: the bits of a negative value but its sign turned round.  A NaN is then above +infinity or below -infinity, so the
 // least and the largest say if there is one, and two values of either type take five instructions where a comparison in 32 bits that keeps a NaN takes sixteen.
-// Bound by the trips slots -> rows -> bounds: 61 slots 2.6 us, of which a launch is 2; 8191 rows of 8 heads of 128 in pages of 16 rows (18.9 MB) 5.6 (3.4 TB/s), of 1 row (50 MB)
-// 15.5, of 256 (16.4 MB) 14.6.  With a workgroup a slot, all of a page's pieces in it: 6.0, 7.5, 27 and 64; 4 / 16 slots a wavefront 8.8 / 4.8 for the second, but then sixteen
-// pages that fill up in one step follow each other.
+// Bound by the trips slots -> rows -> bounds: 61 slots 2.6 us, of which a launch is 2; 8191 rows of 8 heads of 128 in pages of 16 rows (18.9 MB) 6.2 (3.0 TB/s), of 1 row (50 MB)
+// 15.5, of 256 (16.4 MB) 7 to 8, 4000 rows in pages of 64 (8.4 MB) 4.1.  With a workgroup a slot, all of a page's pieces in it: 6.0, 7.5, 27, 64 and 33.
 constexpr int kBoundsThreads = 256;
-constexpr int kBoundsSlots = 8;
 typedef short dec_s2 __attribute__((ext_vector_type(2)));
 struct BoundsArgs {
   const uint16_t* pool;
   uint16_t* bounds;              // [max_pages][n_kv_heads][2 (low, high)][head_dim]
   const int64_t* slots;
   int64_t n_slots, page_elems;
-  int n_tokens, page_shift, pieces, head_pieces, slices, slices_shift, infinity;      // 16-byte pieces of a token's K, of a head's; slices of a workgroup, as a power of two
+  int n_tokens, page_shift, pieces, head_pieces, slices, slices_shift, infinity, per;      // slots of a wavefront; 16-byte pieces of a token's K, of a head's; slices of a workgroup, as a power of two
 };
 __device__ __forceinline__ dec_s2 ordered(dec_s2 v) { return v ^ (v >> 15 & 0x7fff); }          // (and back)
 
-template <int LANES, int AT_ONCE>
+// With SPLIT a workgroup's four wavefronts have the same slice and a quarter of the rows each, and meet through LDS.
+template <int LANES, int AT_ONCE, bool SPLIT>
 __global__ __launch_bounds__(kBoundsThreads) void page_bounds_kernel(BoundsArgs a) {
-  constexpr int kRows = kWave / LANES;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, page_len = 1 << a.page_shift, row = lane / LANES;
-  const int slice = (blockIdx.y << a.slices_shift) + (wave & ((1 << a.slices_shift) - 1)), piece = slice * LANES + lane % LANES, from = min(piece, a.pieces - 1);
+  constexpr int kWaves = kBoundsThreads / kWave, kRows = kWave / LANES * (SPLIT ? kWaves : 1);
+  __shared__ dec_s2 sides[SPLIT ? kWaves : 1][8][SPLIT ? LANES : 1];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, page_len = 1 << a.page_shift, half = lane / LANES;
+  const int row = half + (SPLIT ? wave * (kWave / LANES) : 0);
+  const int slice = SPLIT ? blockIdx.y : (blockIdx.y << a.slices_shift) + (wave & ((1 << a.slices_shift) - 1)), piece = slice * LANES + lane % LANES, from = min(piece, a.pieces - 1);
   if (slice >= a.slices) return;
   // a prompt's last rows come at equal distances: every XCD (each eighth workgroup) has neighbouring groups, or one of them would have all the work
-  const int64_t apart = (int64_t)gridDim.x * (kBoundsThreads / kWave >> a.slices_shift), block = (int64_t)(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
-  for (int64_t group = block * (kBoundsThreads / kWave >> a.slices_shift) + (wave >> a.slices_shift); group * kBoundsSlots < a.n_tokens; group += apart) {
-    const int64_t t = group * kBoundsSlots + lane;
-    const int64_t slot = lane < kBoundsSlots && t < a.n_tokens ? a.slots[t] : -1;
+  const int64_t of_block = SPLIT ? 1 : kWaves >> a.slices_shift;
+  const int64_t apart = (int64_t)gridDim.x * of_block, block = (int64_t)(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
+  for (int64_t group = block * of_block + (SPLIT ? 0 : wave >> a.slices_shift); group * a.per < a.n_tokens; group += apart) {
+    const int64_t t = group * a.per + lane;
+    const int64_t slot = lane < a.per && t < a.n_tokens ? a.slots[t] : -1;
     uint64_t last_rows = __ballot(slot >= 0 && slot < a.n_slots && (slot & (page_len - 1)) == page_len - 1);
     for (; last_rows; last_rows &= last_rows - 1) {
       const int64_t page = (int64_t)lane_u64((uint64_t)slot, __ffsll((unsigned long long)last_rows) - 1) >> a.page_shift;
@@ -82,37 +84,54 @@ __global__ __launch_bounds__(kBoundsThreads) void page_bounds_kernel(BoundsArgs 
             high[e] = __builtin_elementwise_max(high[e], __builtin_bit_cast(dec_s2, __shfl_xor(__builtin_bit_cast(int, high[e]), o, kWave)));
           }
       }
-      if (piece < a.pieces && row < 2) {
+      if constexpr (SPLIT) {                                 // (all four have the same slots)
+        if (half == 0)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            sides[wave][e][lane] = low[e];
+            sides[wave][4 + e][lane] = high[e];
+          }
+        __syncthreads();
+        if (wave == 0)
+#pragma unroll
+          for (int w = 1; w < kWaves; ++w)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              low[e] = __builtin_elementwise_min(low[e], sides[w][e][lane % LANES]);
+              high[e] = __builtin_elementwise_max(high[e], sides[w][4 + e][lane % LANES]);
+            }
+        __syncthreads();
+      }
+      if (piece < a.pieces && half < 2 && (!SPLIT || wave == 0)) {
         dec_u4 out;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          dec_s2 v = ordered(row ? high[e] : low[e]);
+          dec_s2 v = ordered(half ? high[e] : low[e]);
 #pragma unroll
           for (int i = 0; i < 2; ++i)
             if (high[e][i] > a.infinity || low[e][i] < ~a.infinity) v[i] = 0x7fff;                // (the order has -infinity at ~infinity)
           out[e] = __builtin_bit_cast(uint32_t, v);
         }
         dec_u4* to = (dec_u4*)(a.bounds + page * 2 * (a.page_elems >> a.page_shift)) + (piece / a.head_pieces) * 2 * a.head_pieces + piece % a.head_pieces;
-        to[row * a.head_pieces] = out;
+        to[half * a.head_pieces] = out;
       }
     }
   }
 }
-static void launch_bounds(BoundsArgs a, int lanes, hipStream_t st) {
-  a.slices = (a.pieces + lanes - 1) / lanes;
-  a.slices_shift = a.slices >= 4 ? 2 : a.slices >= 2 ? 1 : 0;
-  const int64_t groups = ((int64_t)a.n_tokens + kBoundsSlots - 1) / kBoundsSlots, of_block = kBoundsThreads / kWave >> a.slices_shift;
+template <int LANES>
+static void launch_bounds(BoundsArgs a, hipStream_t st) {
+  a.slices = (a.pieces + LANES - 1) / LANES;
+  const int rows = (1 << a.page_shift) * LANES / kWave;      // of a lane, where a wavefront has them all
+  const bool split = rows >= 16;
+  a.slices_shift = split ? 0 : a.slices >= 4 ? 2 : a.slices >= 2 ? 1 : 0;
+  // few slots a wavefront while there are few, whose pages may all fill up at once; of a prompt's many one in page_len is a last row
+  a.per = std::min(std::max(a.n_tokens / 64, 1), split ? 32 : 8);
+  const int64_t groups = ((int64_t)a.n_tokens + a.per - 1) / a.per, of_block = split ? 1 : kBoundsThreads / kWave >> a.slices_shift;
   const dim3 grid((unsigned)std::min<int64_t>(((groups + of_block - 1) / of_block + 7) / 8 * 8, 1 << 16), (unsigned)((a.slices + (1 << a.slices_shift) - 1) >> a.slices_shift)), block(kBoundsThreads);
-  const int rows = (1 << a.page_shift) * lanes / kWave;      // of a lane
-  if (lanes == 8) {
-    if (rows <= 1) hipLaunchKernelGGL((page_bounds_kernel<8, 1>), grid, block, 0, st, a);
-    else if (rows < 16) hipLaunchKernelGGL((page_bounds_kernel<8, 4>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((page_bounds_kernel<8, 16>), grid, block, 0, st, a);
-  } else {
-    if (rows <= 1) hipLaunchKernelGGL((page_bounds_kernel<16, 1>), grid, block, 0, st, a);
-    else if (rows < 16) hipLaunchKernelGGL((page_bounds_kernel<16, 4>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((page_bounds_kernel<16, 16>), grid, block, 0, st, a);
-  }
+  if (rows <= 1) hipLaunchKernelGGL((page_bounds_kernel<LANES, 1, false>), grid, block, 0, st, a);
+  else if (!split) hipLaunchKernelGGL((page_bounds_kernel<LANES, 4, false>), grid, block, 0, st, a);
+  else if (rows < 64) hipLaunchKernelGGL((page_bounds_kernel<LANES, 4, true>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((page_bounds_kernel<LANES, 16, true>), grid, block, 0, st, a);
 }
 
 // Sums up to each lane, and a wavefront's largest, by lanes that neighbour in a row of sixteen and the rows' last ones: a dozen instructions, where six exchanges
@@ -1166,7 +1185,8 @@ extern "C" int subspec_kv_page_bounds(const void* kv_pool_layer, void* bounds, i
   a.infinity = dtype == SUBSPEC_BF16 ? 0x7f80 : 0x7c00;
   hipStream_t st = (hipStream_t)stream;
   DominantKernelTimer timer(st);
-  launch_bounds(a, a.pieces <= 8 ? 8 : 16, st);
+  if (a.pieces <= 8) launch_bounds<8>(a, st);
+  else launch_bounds<16>(a, st);
   SUBSPEC_CHECK_HIP(hipGetLastError());
   return SUBSPEC_OK;
 }
