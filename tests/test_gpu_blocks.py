@@ -342,6 +342,31 @@ def test_a_captured_step_and_another_stream():
         assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
 
 
+@pytest.mark.parametrize("batch,Hq,Hkv,D,P,keep,rows", [(70, 8, 8, 64, 4, 150, 900), (66, 16, 8, 128, 8, 60, 700), (150, 16, 8, 64, 1, 300, 400)])
+def test_more_tiles_than_the_gpu_holds(batch, Hq, Hkv, D, P, keep, rows):
+    """So many drafts that a tile is one unit of more rows than are looked up at a time, or two: as the tokens get it when each is its sequence's only one."""
+    print("many tiles", batch, Hq, Hkv, D, P, keep, rows, flush=True)
+    g = torch.Generator(device=DEV).manual_seed(batch)
+    pages = -(-rows // P)
+    pool = torch.randn(batch * pages, 2, P, Hkv, D, generator=g, device=DEV).bfloat16()
+    table = torch.randperm(batch * pages, generator=g, device=DEV).int().view(batch, pages)
+    new = torch.tensor([1 + b % 4 for b in range(batch)], device=DEV)
+    seq = torch.repeat_interleave(torch.arange(batch, device=DEV), new).int()
+    T = seq.numel()
+    pos = (rows - 1 - torch.randint(0, 3 * P, (T,), generator=g, device=DEV)).int()
+    q = (torch.randn(T, Hq, D, generator=g, device=DEV) * 2).bfloat16()
+    want = torch.rand(batch, Hkv, pages, generator=g, device=DEV)[seq.long()] + 0.1 * torch.rand(T, Hkv, pages, generator=g, device=DEV)
+    blocks = want.topk(keep, -1).indices.int()
+    got = ops.block_attention(q, pool, table, blocks, seq, pos)
+    assert torch.equal(got, ops.block_attention(q, pool, table, blocks, seq, pos))
+    first = torch.cumsum(new, 0) - new
+    for k in range(4):
+        rows_of = first[new > k] + k
+        alone = ops.block_attention(q[rows_of], pool, table, blocks[rows_of], seq[rows_of].contiguous(), pos[rows_of].contiguous())
+        # each is off from the formula by half a step of the result (2^-8 of it) and little else
+        assert ((alone.float() - got[rows_of].float()).abs() <= 2 * (2.0 ** -8 * 1.01 * alone.float().abs() + 2.0 ** -12)).all()
+
+
 @pytest.mark.parametrize("Hq,Hkv,D", [(32, 8, 128), (8, 4, 64)])
 def test_a_replayed_graph_with_other_neighbours(Hq, Hkv, D):
     """The tokens' sequences change between replays, from one run to a token each in turn (more tiles than a batch in order has), some of nobody: as the eager
