@@ -210,20 +210,28 @@ template <int DT>
 __device__ RowCut row_from_slices(const VerifyArgs& a, int row, const RowRule& r) {
   const int lane = threadIdx.x % kRowLanes;
   const SliceStats* of = a.stats + (int64_t)row * a.slices;
+  // (a row of up to 262144 in one trip to memory)
+  constexpr int kHeld = 8;
+  SliceStats held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) held[i] = of[min(lane + i * kRowLanes, a.slices - 1)];
   float top = -INFINITY;
-#pragma unroll 4
-  for (int s = lane; s < a.slices; s += kRowLanes) top = fmaxf(top, of[s].top);
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) top = fmaxf(top, held[i].top);
+  for (int s = lane + kHeld * kRowLanes; s < a.slices; s += kRowLanes) top = fmaxf(top, of[s].top);
 #pragma unroll
   for (int o = kRowLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
   const float scale = (float)r.inv_t_log2e;
   float z = 0.f;
   int first = INT32_MAX;
-#pragma unroll 4
-  for (int s = lane; s < a.slices; s += kRowLanes) {
-    const SliceStats m = of[s];
+  auto add = [&](const SliceStats& m) {
     z = fmaf(m.sum, m.top == top ? 1.f : __builtin_amdgcn_exp2f(fmaxf((m.top - top) * scale, -200.f)), z);
     first = m.top == top ? min(first, m.first) : first;
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (lane + i * kRowLanes < a.slices) add(held[i]);
+  for (int s = lane + kHeld * kRowLanes; s < a.slices; s += kRowLanes) add(of[s]);
 #pragma unroll
   for (int o = kRowLanes / 2; o > 0; o >>= 1) {
     z += __shfl_xor(z, o, kWave);
