@@ -163,6 +163,9 @@ __device__ __forceinline__ uint64_t block_sum_u64(uint64_t v, uint64_t* scratch)
 // for the one row that a sequence ends with (and for a row whose draft the 32 bits leave undecided, see kUnsure).
 // A slice is a wavefront's, so nobody waits for anybody.
 constexpr int kSliceChunks = 4;
+// (l - top) / (T ln 2), from half of top and twice 1 / (T ln 2).  The difference comes first, and of halves: products of logits and 1 / T can be of any size (a mask
+// of -1e30, a T of 1e-20), and two of them leave nothing of it; so can the difference of two of the lowest and largest numbers.
+__device__ __forceinline__ float bits_below(float l, float half_top, float twice) { return fmaf(l, 0.5f, -half_top) * twice; }
 template <int DT>
 __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs a) {
   constexpr int ROUNDS = kSliceChunks, kLength = kSliceChunks * kChunk;
@@ -188,18 +191,16 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs
     first = wave_min_i(first);
     sum = wave_sum(sum);
   } else if (top > -INFINITY) {
-    // 2^((l - top) scale) = 2^(l scale - (top scale rounded)) 2^(what the rounding left out)
-    const float scale = (float)r.inv_t_log2e, base = top * scale, left = fmaf(top, scale, -base);
+    const float twice = 2.f * (float)r.inv_t_log2e, half = 0.5f * top;
 #pragma unroll
-    for (int e = 0; e < 8 * ROUNDS; ++e) sum += __builtin_amdgcn_exp2f(fmaf(x[e], scale, -base));
+    for (int e = 0; e < 8 * ROUNDS; ++e) sum += __builtin_amdgcn_exp2f(bits_below(x[e], half, twice));
     sum = wave_sum(sum);
     if (sum != sum) {                                                  // there is a NaN, which has no mass
       sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8 * ROUNDS; ++e) sum += x[e] != x[e] ? 0.f : __builtin_amdgcn_exp2f(fmaf(x[e], scale, -base));
+      for (int e = 0; e < 8 * ROUNDS; ++e) sum += x[e] != x[e] ? 0.f : __builtin_amdgcn_exp2f(bits_below(x[e], half, twice));
       sum = wave_sum(sum);
     }
-    sum *= __builtin_amdgcn_exp2f(-left);
   }
   if (lane == 0) a.stats[unit] = SliceStats{top, sum, first, 0};
 }
@@ -221,11 +222,11 @@ __device__ RowCut row_from_slices(const VerifyArgs& a, int row, const RowRule& r
   for (int s = lane + kHeld * kRowLanes; s < a.slices; s += kRowLanes) top = fmaxf(top, of[s].top);
 #pragma unroll
   for (int o = kRowLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
-  const float scale = (float)r.inv_t_log2e;
+  const float twice = 2.f * (float)r.inv_t_log2e, half = 0.5f * top;
   float z = 0.f;
   int first = INT32_MAX;
   auto add = [&](const SliceStats& m) {
-    z = fmaf(m.sum, m.top == top ? 1.f : __builtin_amdgcn_exp2f(fmaxf((m.top - top) * scale, -200.f)), z);
+    z = fmaf(m.sum, m.top == top ? 1.f : __builtin_amdgcn_exp2f(fmaxf(bits_below(m.top, half, twice), -200.f)), z);
     first = m.top == top ? min(first, m.first) : first;
   };
 #pragma unroll
@@ -262,7 +263,7 @@ __device__ uint64_t exact_mass(const VerifyArgs& a, int row, const RowCut& cut, 
 // What a draft leaves of an entry's mass
 __device__ __forceinline__ uint64_t rest_of(double m, float q, double z) { return whole(fmax(fma(-draft_prob(q), z, m), 0.0)); }
 // How far u q Z and m may be apart, relative to m, for 32 bits to say which is larger.  With d = (l - top) / (T ln 2) a term 2^d is off by 3 |d| 2^-24 ln 2
-// (the exponent's rounding, the factor's; a slice's largest logit against the row's) and 2^-23; 2^20 terms of a size below 2^-20 make no more than one, so by
+// (the difference's rounding, the product's, the factor's; what a slice's largest logit is below the row's is a part of d, with the same three) and 2^-23; 2^20 terms of a size below 2^-20 make no more than one, so by
 // 20 * 3 * 2^-24 * 0.7 on average; a lane adds 32 terms, a wavefront 64 sums in a tree, a row 512 of these, 32 a
 // lane: 2.5e-6 + 2^-23 + 74 * 2^-24 < 2^-17.
 constexpr double kUnsure = 0x1p-17;

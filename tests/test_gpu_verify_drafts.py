@@ -304,3 +304,83 @@ def test_numbers_at_the_border_in_32_bits(V):
     got = _run(case)
     _check(case, got)
     assert got["accepted"].tolist() == [int(side[:8].int().cumprod(0).sum()), int(side[9:13].int().cumprod(0).sum())]
+
+
+# ------------------------------------------------------------------------------------------------ masked vocabularies, small temperatures
+def _masked(g, rows, V, dtype, q_dtype, t, value, how, best):
+    """Logits of which ``how`` many are masked by a finite number, drafts that see the mask: drawn ones, or with ``best`` the rows' largest (which stay where p is 1)."""
+    logits, tokens, starts, u, v, _ = _case(g, rows, V, F32, None, t)
+    T = logits.shape[0]
+    open_ = torch.zeros(T, V, dtype=torch.bool)
+    if how == "slices":                                      # a row is looked at in slices of 2048: the odd ones, and what is left behind the last whole one
+        open_[:] = torch.arange(V) // 2048 % 2 == 0
+        open_[:, V // 2048 * 2048:] = V < 2048
+        open_[:, 5] = True
+    elif how == "all but three":
+        open_.scatter_(1, torch.randint(0, V, (T, 3), generator=g), True)
+    elif how == "nothing":
+        open_[:] = True
+    logits = torch.where(open_, logits, value).to(dtype)
+    probs = torch.softmax(((logits.double() - logits.double().amax(1, keepdim=True)) / max(t, 0.2)) + 0.3 * torch.randn(T, V, generator=g), -1).float()
+    drawn = logits.float().argmax(1) if best else torch.multinomial(probs, 1, generator=g)[:, 0]
+    return logits, torch.cat([drawn[-1:], drawn[:-1]]), starts, u, v, None if q_dtype is None else probs.to(q_dtype)
+
+
+def _both_ways(case, t):
+    """The call without filters, and with one that takes nothing away and so goes by masses in 64 bits alone: the formula's, both."""
+    want = ok.verify_drafts(*case, settings=lambda row: dict(temperature=t))
+    for settings in ({}, dict(min_p=1e-30)):
+        got = _run(case, temperature=t, **settings)
+        assert got["accepted"].tolist() == want[2] and got["tokens"].tolist() == want[0], (settings, got["accepted"].tolist(), want[2])
+        assert _near(got["probs"], want[1], bool(settings)), settings
+    return want
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("how", ["slices", "all but three", "all"])
+@pytest.mark.parametrize("value", [-1e4, -1e9, -1e10, -1e30, "lowest"])
+def test_vocabularies_masked_by_finite_numbers(dtype, how, value):
+    """A mask that is no infinity leaves slices of a row, or all of it, at one large negative number."""
+    value = torch.finfo(dtype).min if value == "lowest" else value
+    if value < torch.finfo(dtype).min:
+        pytest.skip("not a number of this type")
+    stays = 0
+    for V, rows in ((5000, [4, 3, 1, 5]), (2049, [6])):
+        for n, t in enumerate((0.2, 0.3, 0.5, 0.7, 1.0, 1.3, 1.5)):
+            g = torch.Generator().manual_seed(V + n)
+            for best in (False, True):
+                print("masked", dtype, how, value, V, t, best, flush=True)
+                stays += sum(_both_ways(_masked(g, rows, V, dtype, None if best else F32, t, value, how, best), t)[2])
+    assert stays > 20                                        # (most drafts stay, if anything is right)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("t", [1e-3, 1e-6, 1e-8, 1e-9, 1e-20, 1e-37, 1.2e-38, 30.0, 1e6, 1e30])
+def test_temperatures_of_any_size(dtype, t):
+    """Down to the smallest that is not greedy, where one entry has all unless others equal it, and up to those where all have the same."""
+    stays = 0
+    for V, rows in ((5000, [4, 3, 1, 5]), (2049, [6]), (7, [3, 2])):
+        g = torch.Generator().manual_seed(V)
+        for best in (False, True):
+            print("temperature", dtype, t, V, best, flush=True)
+            stays += sum(_both_ways(_masked(g, rows, V, dtype, None if best and t < 1 else F32, t, 0.0, "nothing", best), t)[2])
+    assert stays > 3
+
+
+def test_a_masked_row_beside_ordinary_ones():
+    """Rows of one call with temperatures of their own, some masked: nothing of one reaches another."""
+    g = torch.Generator().manual_seed(12)
+    rows, V = [5, 4, 6], 9000
+    T = sum(rows)
+    logits, tokens, starts, u, v, q = _masked(g, rows, V, F32, F32, 1.0, torch.finfo(F32).min, "slices", False)
+    plain = _case(g, rows, V, F32, F32)
+    some = torch.arange(T) % 3 == 1
+    logits[~some], q[~some] = plain[0][~some], plain[5][~some]
+    t = torch.tensor([1.0, 1e-9, 0.4, 0.0])[torch.arange(T) % 4]
+    drawn = logits.argmax(1)
+    case = (logits, torch.cat([drawn[-1:], drawn[:-1]]), starts, 0.02 * u, v, q)
+    want = ok.verify_drafts(*case, settings=lambda r: dict(temperature=float(t[r])))
+    assert want[2] == [4, 3, 5]
+    for settings in ({}, dict(min_p=1e-30)):
+        got = _run(case, temperature=t.to(DEV), **settings)
+        assert got["accepted"].tolist() == want[2] and got["tokens"].tolist() == want[0] and _near(got["probs"], want[1], bool(settings))
