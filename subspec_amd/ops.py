@@ -811,7 +811,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, query_starts: torc
     m_ptr, m = _per_row(min_p, rows, torch.float32, dev, "min_p", "verify_drafts")
     if t < 0 or p < 0 or m < 0 or k < 0:
         raise ValueError("verify_drafts: temperature, top_k, top_p and min_p must not be negative")
-    k = min(int(k), (1 << 31) - 1)
+    k, p, m = min(int(k), (1 << 31) - 1), ctypes.c_float(p).value, ctypes.c_float(m).value         # (as the library gets them: 0.99999999 is 1 and filters nothing)
     sizes = (rows, rows, batch)
     if out is None:
         o_tokens, o_probs, o_accepted = torch.empty(3 * rows + batch, dtype=torch.int32, device=dev).split_with_sizes((2 * rows, rows, batch))

@@ -384,3 +384,14 @@ def test_a_masked_row_beside_ordinary_ones():
     for settings in ({}, dict(min_p=1e-30)):
         got = _run(case, temperature=t.to(DEV), **settings)
         assert got["accepted"].tolist() == want[2] and got["tokens"].tolist() == want[0] and _near(got["probs"], want[1], bool(settings))
+
+
+@pytest.mark.parametrize("rows,V", [([4] * 25, 20000), ([5, 3], 300)])
+@pytest.mark.parametrize("settings", [dict(top_p=0.99999999), dict(min_p=1e-46), dict(top_p=1 - 2.0 ** -25, min_p=5e-46)])
+def test_settings_that_filter_nothing_once_they_are_32_bits(rows, V, settings):
+    """A number below 1, or above 0, that fp32 does not tell from it is no filter: the call without filters, which has a workspace of another size."""
+    case = _case(torch.Generator().manual_seed(V), rows, V, BF16, F32)
+    got, want = _run(case, **settings), _run(case)
+    assert all(torch.equal(got[name], want[name]) for name in want)
+    nearly = dict(top_p=1 - 2.0 ** -24) if "top_p" in settings else dict(min_p=1e-45)                    # the next number that is one
+    _check(case, _run(case, **nearly), lambda row: nearly, filtered=True)
