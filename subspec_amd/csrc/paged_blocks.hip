@@ -1104,9 +1104,9 @@ static AttendPlan attend_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64
   return p;
 }
 
-// Scores of so many tokens are held at a time (a quarter of a gigabyte)
+// Tokens of a pass: their scores are a quarter of a gigabyte, and their lists, a workgroup of up to 512 threads each, no more than a launch can have (below 2^32 threads).
 static int64_t select_tokens(int64_t n_tokens, int64_t hkv, int64_t most) {
-  const int64_t fit = std::max<int64_t>(kScoreTokens, (1 << 25) / (hkv * std::max<int64_t>(most, 1)) / kScoreTokens * kScoreTokens);
+  const int64_t fit = std::max<int64_t>(kScoreTokens, std::min((1 << 25) / (hkv * std::max<int64_t>(most, 1)), (1 << 22) / hkv) / kScoreTokens * kScoreTokens);
   return std::min(n_tokens, fit);
 }
 

@@ -662,3 +662,18 @@ def test_a_value_that_one_token_does_not_see_stays_out_of_its_sums(D, keep, P, w
     fine = torch.ones(D, dtype=torch.bool)
     fine[[3, 5]] = False
     assert torch.equal(got[hit][:, fine], clean[hit][:, fine])
+
+
+def test_select_for_a_million_tokens_of_32_heads():
+    """2^25 lists: more than one launch of a workgroup a list can have."""
+    T, H, D, P = 1 << 20, 32, 64, 16
+    q = torch.ones(1, H, D, dtype=torch.bfloat16, device=DEV).expand(T, H, D)
+    bounds = torch.zeros(3, H, 2, D, dtype=torch.bfloat16, device=DEV)
+    seq, pos = torch.arange(T, device=DEV).int() % 3 - 1, torch.arange(T, device=DEV).int() % 40
+    for keep, table in ((2, _i32([[0], [2]])), (1, _i32([[0], [1]])), (2, _i32([[0, 1], [2, 0]]))):
+        print("a million tokens", keep, table.tolist(), flush=True)
+        seen = torch.where(seq < 0, 0, (pos // P + 1).clamp(max=table.shape[1]))[:, None]
+        j = torch.arange(keep, device=DEV)
+        want = torch.where(j < seen, j, -1).int()
+        got = ops.select_blocks(q, bounds, table, seq, pos, P, keep, out=torch.full((T, H, keep), -7, dtype=torch.int32, device=DEV))
+        assert torch.equal(got, want[:, None].expand_as(got))
