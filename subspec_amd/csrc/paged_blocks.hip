@@ -1090,6 +1090,7 @@ static AttendPlan attend_plan(int64_t batch, int64_t n_tokens, int64_t hq, int64
   p.chunks = (int)((keys + per - 1) / per);
   p.tokens = p.share > 1 ? std::min<int64_t>(n_tokens, kTileTokens) : n_tokens;
   if (p.chunks > 1) p.tokens = std::min<int64_t>(p.tokens, std::max<int64_t>(8, (1 << 20) / (hq * p.chunks)));      // half a gigabyte at 128 a head
+  p.tokens = std::min<int64_t>(p.tokens, (1 << 25) / (p.chunks * hkv));        // (a launch has below 2^32 threads, a unit 64 of them)
   const size_t slots = (size_t)p.tokens * hq * p.chunks;
   if (p.chunks > 1) {
     p.part_o = align_up(slots * head_dim * sizeof(float), 256);
@@ -1308,8 +1309,6 @@ extern "C" int subspec_block_attention(const void* q, int64_t q_token_stride, in
   a.last_row = (int)(std::min<int64_t>(max_blocks * page_len, 1ll << 30) - 1);
   a.keys = (int)(keep * page_len); a.chunk_keys = p.chunk_keys; a.chunks = p.chunks;
   a.scale_log2 = scale * kLog2e;
-  if (p.tokens * p.chunks * n_kv_heads > INT32_MAX)
-    SUBSPEC_FAIL(SUBSPEC_ERR_LIMIT, "%s: too large (%lld tokens of %lld heads)", what, (long long)n_tokens, (long long)n_kv_heads);
   hipStream_t st = (hipStream_t)stream;
   for (int64_t first = 0; first < n_tokens; first += p.tokens) {
     const int64_t some = std::min(p.tokens, n_tokens - first);

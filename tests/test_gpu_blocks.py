@@ -677,3 +677,22 @@ def test_select_for_a_million_tokens_of_32_heads():
         want = torch.where(j < seen, j, -1).int()
         got = ops.select_blocks(q, bounds, table, seq, pos, P, keep, out=torch.full((T, H, keep), -7, dtype=torch.int32, device=DEV))
         assert torch.equal(got, want[:, None].expand_as(got))
+
+
+def test_attention_of_a_million_tokens_of_64_heads():
+    """2^26 units of a wavefront: more than one launch can have.  Every token attends to one row and gets its value."""
+    T, H, D, width = 1 << 20, 64, 64, 40000                  # (so many columns that no tokens share a unit)
+    pool = torch.randn(7, 2, 1, H, D, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).bfloat16()
+    q = torch.ones(1, H, D, dtype=torch.bfloat16, device=DEV).expand(T, H, D)
+    table = (torch.arange(width, device=DEV) % 7).int()[None]
+    seq = torch.where(torch.arange(T, device=DEV) % 1000 == 999, -1, 0).int()
+    pos = torch.full((T,), width - 1, dtype=torch.int32, device=DEV)
+    blocks = (torch.arange(T, device=DEV)[:, None] * 5 + torch.arange(H, device=DEV)).remainder(width).int()[:, :, None].contiguous()
+    out = torch.full((T, H * D), 7.0, dtype=torch.bfloat16, device=DEV)
+    print("a million tokens", flush=True)
+    ops.block_attention(q, pool, table, blocks, seq, pos, out=out)
+    step = 1 << 16
+    for t0 in range(0, T, step):
+        want = pool[(blocks[t0:t0 + step, :, 0] % 7).long(), 1, 0, torch.arange(H, device=DEV)]
+        want[seq[t0:t0 + step] < 0] = 7.0
+        assert torch.equal(out[t0:t0 + step].view(-1, H, D), want), t0
