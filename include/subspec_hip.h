@@ -460,7 +460,7 @@ int subspec_sample_filtered(const void* logits, int dtype, int64_t rows, int64_t
  * probs         device float [n_rows]: p_i at these tokens (0 beside -1);  accepted  device int32 [batch]: drafts that stay (0 without rows).  Whether a draft stays, and
  *               the token, are decided by masses in 64 bits; without filters the probs of drafts that stay come from a row's mass in 32 bits (within 2^-17 of it)
  * filtered      1 where any of the filters is given (a pointer, 0 < top_k < vocab, top_p < 1 or min_p > 0)
- * The outputs overlap no input.  Limits: n_rows <= 2^20, vocab <= 2^20, 1 <= batch <= SUBSPEC_MAX_BATCH.
+ * The outputs overlap no input.  Limits: n_rows <= 2^20, vocab <= 2^20, 1 <= batch <= SUBSPEC_MAX_BATCH; without filters n_rows * ceil(vocab / 2048) <= 2^26 - 4.
  */
 size_t subspec_verify_drafts_workspace(int64_t n_rows, int64_t batch, int64_t vocab, int filtered);
 

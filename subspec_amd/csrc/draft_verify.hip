@@ -597,7 +597,8 @@ extern "C" int subspec_verify_drafts(const void* logits, int dtype, int64_t n_ro
   if (!workspace || workspace_bytes < p.bytes)
     SUBSPEC_FAIL(SUBSPEC_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the %zu required", what, workspace_bytes, p.bytes);
   if ((uintptr_t)workspace % 16) SUBSPEC_FAIL(SUBSPEC_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
-  if (n_rows * p.slices > INT32_MAX || batch * p.end_slices >= INT32_MAX)
+  // (a launch has below 2^32 threads; the other ones, of a workgroup a row or an end row's slice, are far below)
+  if (!filtered && (n_rows * p.slices + kVerifyWaves - 1) / kVerifyWaves * kVerifyThreads > UINT32_MAX)
     SUBSPEC_FAIL(SUBSPEC_ERR_LIMIT, "%s: too large (%lld rows of %lld)", what, (long long)n_rows, (long long)vocab);
   VerifyArgs a{};
   a.s = SampleArgs{logits, uniforms, temperatures, top_ks, top_ps, min_ps, tokens, probs, row_stride, (int)vocab, top_k, temperature, top_p, min_p};

@@ -92,6 +92,12 @@ def test_verify_refuses(change, code):
     assert _verify(**change) == code and b"verify_drafts" in L.lib().subspec_last_error()
 
 
+@pytest.mark.parametrize("n,vocab", [(1 << 20, 1 << 20), (1 << 20, (1 << 17) - 1), (1 << 17, 1 << 20)])
+def test_verify_refuses_more_slices_than_a_launch_has_threads_for(n, vocab):
+    """A row without filters is looked at by a wavefront for every 2048 entries, and a launch has below 2^32 threads."""
+    assert _verify(n=n, vocab=vocab, stride=vocab, qs=vocab, ws_bytes=1 << 60) == -4 and b"verify_drafts: too large" in L.lib().subspec_last_error()
+
+
 def test_host_tensors_are_refused():
     q, pool, i32 = torch.zeros(1, 2, 64).bfloat16(), torch.zeros(2, 2, 4, 1, 64).bfloat16(), torch.zeros(1, dtype=torch.int32)
     bounds, table = torch.zeros(2, 1, 2, 64).bfloat16(), torch.zeros(1, 2, dtype=torch.int32)
