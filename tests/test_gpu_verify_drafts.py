@@ -336,14 +336,13 @@ def _both_ways(case, t):
     return want
 
 
-@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+MASKS = [(dtype, value) for dtype in (F32, BF16, F16) for value in (-1e4, -1e9, -1e10, -1e30, torch.finfo(dtype).min) if value >= torch.finfo(dtype).min]
+
+
 @pytest.mark.parametrize("how", ["slices", "all but three", "all"])
-@pytest.mark.parametrize("value", [-1e4, -1e9, -1e10, -1e30, "lowest"])
-def test_vocabularies_masked_by_finite_numbers(dtype, how, value):
+@pytest.mark.parametrize("dtype,value", MASKS)
+def test_vocabularies_masked_by_finite_numbers(dtype, value, how):
     """A mask that is no infinity leaves slices of a row, or all of it, at one large negative number."""
-    value = torch.finfo(dtype).min if value == "lowest" else value
-    if value < torch.finfo(dtype).min:
-        pytest.skip("not a number of this type")
     stays = 0
     for V, rows in ((5000, [4, 3, 1, 5]), (2049, [6])):
         for n, t in enumerate((0.2, 0.3, 0.5, 0.7, 1.0, 1.3, 1.5)):
