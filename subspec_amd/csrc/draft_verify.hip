@@ -6,11 +6,12 @@
 // draws (Y. Leviathan, M. Kalman, Y. Matias, "Fast inference from transformers via speculative decoding", 2023).  A draft without q is one
 // that nothing was drawn for: q_i(x_i) = 1.
 //
-// Masses are the whole numbers of a draw (2^-42 of the largest, see mass_series.h).  With m_j an entry's mass and Z the row's, the test is u q Z < m, and the rest
-// max(m_j - q_j Z, 0) is rounded to such units again, so its sums are exact, no order of addition changes a token, and the token is the first in the
-// order of the vocabulary whose sum exceeds v times the whole.
-// 48 sequences of up to 8 drafts, 346 rows of 152064 bf16 (105 MB): the statistics of all rows 20.5 us (5.1 TB/s), acceptance and the end rows' masses 21, the draws 10.6; one sequence
-// of 4 drafts in fp32 4.0 + 6.0 + 4.3.  With filters the cuts of all rows come first (sample.hip): 63 rows' 42 us are most of 16 sequences' 55.
+// Masses are the whole numbers of a draw (2^-42 of the largest, see mass_series.h).  With m_j an entry's mass and Z the row's, the test is u q Z < m, and of the
+// rest max(m_j - q_j Z, 0) the token is the first in the order of the vocabulary whose sum exceeds v times the whole.  The rest is whole numbers too, whose sums are exact: with
+// filters every entry's is rounded, without them that of 512 entries (from exact sums of masses and a sum of q in 64 bits and a fixed order, see kOpen below), and
+// within the 512 that the token falls to every entry's.
+// 48 sequences of up to 8 drafts, 346 rows of 152064 bf16 (105 MB): the statistics of all rows 20.5 us (5.1 TB/s), acceptance and the end rows' masses 20.6, the draws 10.4; one sequence
+// of 4 drafts in fp32 4.0 + 5.9 + 4.2.  With filters the cuts of all rows come first (sample.hip): 63 rows' 42 us are most of 16 sequences' 54.
 #include "sample.h"
 #include <algorithm>
 
@@ -164,7 +165,8 @@ __device__ __forceinline__ uint64_t block_sum_u64(uint64_t v, uint64_t* scratch)
 // A slice is a wavefront's, so nobody waits for anybody.
 constexpr int kSliceChunks = 4;
 // (l - top) / (T ln 2), from half of top and twice 1 / (T ln 2).  The difference comes first, and of halves: products of logits and 1 / T can be of any size (a mask
-// of -1e30, a T of 1e-20), and two of them leave nothing of it; so can the difference of two of the lowest and largest numbers.
+// of -1e30, a T of 1e-20), and two of them leave nothing of it; so can the difference of two of the lowest and largest numbers.  (Beside the row's way out of memory it costs
+// nothing: 20.5 us for 48 sequences' rows, as with one product less.)
 __device__ __forceinline__ float bits_below(float l, float half_top, float twice) { return fmaf(l, 0.5f, -half_top) * twice; }
 template <int DT>
 __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs a) {

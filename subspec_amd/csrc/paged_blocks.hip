@@ -24,8 +24,8 @@ static int block_shift_of(int64_t page_len) {
 // to sixteen requests a lane under way.  Its lanes meet through registers, so nobody waits for anybody, and a wavefront without such a page leaves.
 // As whole numbers that rise with the value: the bits of a negative value but its sign turned round.  A NaN is then above +infinity or below -infinity, so the
 // least and the largest say if there is one, and two values of either type take five instructions where a comparison in 32 bits that keeps a NaN takes sixteen.
-// Bound by the trips slots -> rows -> bounds: 61 slots 2.6 us, of which a launch is 2; 8191 rows of 8 heads of 128 in pages of 16 rows (18.9 MB) 6.2 (3.0 TB/s), of 1 row (50 MB)
-// 15.5, of 256 (16.4 MB) 7 to 8, 4000 rows in pages of 64 (8.4 MB) 4.1.  With a workgroup a slot, all of a page's pieces in it: 6.0, 7.5, 27, 64 and 33.
+// Bound by the trips slots -> rows -> bounds: 61 slots 2.6 to 3 us, of which a launch is 2; 8191 rows of 8 heads of 128 in pages of 16 rows (18.9 MB) 6.1 (3.1 TB/s), of 1 row (50 MB)
+// 15.4, of 256 (16.4 MB) 7 to 8.3, 4000 rows in pages of 64 (8.4 MB) 4.1 to 4.6.  With a workgroup a slot, all of a page's pieces in it: 6.0, 7.5, 27, 64 and 33.
 constexpr int kBoundsThreads = 256;
 typedef short dec_s2 __attribute__((ext_vector_type(2)));
 struct BoundsArgs {
@@ -316,7 +316,7 @@ __device__ __forceinline__ void load_bounds(const SelectArgs& a, int page, int k
 __device__ __forceinline__ double score_of(double s) { return s != s ? INFINITY : s; }
 
 // A workgroup takes `span` blocks of (token, KV head), a wavefront a quarter of them: D / 8 lanes a block, all requests of a wavefront under way before
-// the first score; meanwhile the four of them add the query heads up.  One token of 2048 blocks 4.9 us; 64 tokens, 193 MB, 38.9 (5.0 TB/s).
+// the first score; meanwhile the four of them add the query heads up.  One token of 2048 blocks 5.7 us (5.3 at best); 64 tokens, 193 MB, 39 (4.9 TB/s).
 template <int DT, int D>
 __global__ __launch_bounds__(kScoreThreads) void block_score_kernel(SelectArgs a) {
   constexpr int kLanes = D / 8, kAtOnce = kWave / kLanes, kDepth = 8;
@@ -618,7 +618,7 @@ __global__ __launch_bounds__(THREADS) void block_select_kernel(SelectArgs a) {
 // Tokens of one sequence list much the same blocks, so where a call has more tokens than sequences up to eight of them share a unit (32 rows of a KV head): its
 // blocks are those that any of them lists, ascending, each with a bit a token (block_union_kernel), and a row sees a key by its token's bit and position.
 // 72 drafts of 16 sequences, 32 blocks of 64 rows each, 32 : 8 heads: a unit a token reads 600 MB, out of the caches, in 92 us; their union, 192 MB, takes 42 (4.6 TB/s).  64 tokens
-// by themselves, 134 MB: 26.7 (5.0 TB/s); one of 1024 rows: 5.5, five trips to memory and the launch.  A stage of 32 keys and 32 rows is 1.3 us of a wavefront's work.
+// by themselves, 134 MB: 26.8 (5.0 TB/s); one of 1024 rows: 5.5, five trips to memory and the launch.  A stage of 32 keys and 32 rows is 1.3 us of a wavefront's work.
 constexpr int kAttendKeys = 32;
 constexpr int kAttendStages = 2;
 constexpr int kAttendSegment = 512;        // keys whose row offsets are in LDS at a time
